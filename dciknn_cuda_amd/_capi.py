@@ -20,6 +20,7 @@ APPEND_AUTO, APPEND_SORT, APPEND_MERGE = 0, 1, 2
 TRAVERSAL_AUTO, TRAVERSAL_STEP, TRAVERSAL_BATCH, TRAVERSAL_DENSE = 0, 1, 2, 3
 NOALLOC_SCRATCH_BYTES = 32 << 20
 NUM_TIMERS = 7
+F32, F16, BF16 = 0, 1, 2
 T_PROJECT, T_SEGSORT, T_QPROJECT, T_TRAVERSE, T_MERGE, T_BATCH, T_DENSE = range(7)
 
 # name -> (restype, argtypes); one line per declaration in include/dci_hip.h and include/dci_hip_debug.h
@@ -66,6 +67,26 @@ SIGNATURES = {
                                 _c.c_void_p, _c.c_void_p]),
     "dcih_segsort": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_void_p,
                                 _c.c_void_p, _c.c_void_p]),
+    "dcih_embed": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
+                              _c.c_int, _c.c_int64, _c.c_float, _c.c_void_p, _c.c_void_p]),
+    "dcih_embed_grad_work": (_c.c_int64, [_c.c_int64, _c.c_int]),
+    "dcih_embed_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
+                                   _c.c_int, _c.c_int64, _c.c_float, _c.c_int, _c.c_void_p, _c.c_int,
+                                   _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_logits_work": (_c.c_int64, [_c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
+    "dcih_token_logprobs": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
+                                       _c.c_int, _c.c_float, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+                                       _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_token_logprobs_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64,
+                                            _c.c_void_p, _c.c_int, _c.c_float, _c.c_void_p, _c.c_void_p,
+                                            _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_distill": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
+                                _c.c_int, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p,
+                                _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64,
+                                _c.c_void_p]),
+    "dcih_distill_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
+                                     _c.c_int, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p,
+                                     _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
 }
 
 _lib = None

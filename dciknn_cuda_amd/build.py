@@ -10,7 +10,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdci_hip.so")
-SOURCES = ["api.hip", "project.hip", "segsort.hip", "bucketsort.hip", "query.hip", "traverse_block.hip", "traverse_dense.hip", "exhaustive.hip", "rows8.hip", "bounds.hip", "confirm.hip", "nearest.hip"]
+SOURCES = ["api.hip", "project.hip", "segsort.hip", "bucketsort.hip", "query.hip", "traverse_block.hip", "traverse_dense.hip", "exhaustive.hip", "rows8.hip", "bounds.hip", "confirm.hip", "nearest.hip",
+           "embed.hip", "logits.hip", "token_api.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
@@ -48,6 +49,7 @@ def build_library(verbose=False):
 
 
 EXT = os.path.join(HERE, "_dci_cuda.so")
+EXT_SOURCES = ["_dci_cuda.cpp", "tokens_ext.cpp"]
 
 
 def build_extension(verbose=False):
@@ -59,22 +61,37 @@ def build_extension(verbose=False):
     if not os.path.exists(LIB):
         build_library(verbose)
     tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_dci_cuda",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-DPYBIND11_COMPILER_TYPE=\"_gcc\"",
-           "-DPYBIND11_STDLIB=\"_libstdcpp\"", "-DPYBIND11_BUILD_ABI=\"_cxxabi1011\"",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-Wno-deprecated-declarations"]
+    cxx = os.environ.get("CXX", "g++")
+    flags = ["-O2", "-std=c++17", "-fPIC",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_dci_cuda",
+             "-DTORCH_API_INCLUDE_EXTENSION_H", "-DPYBIND11_COMPILER_TYPE=\"_gcc\"",
+             "-DPYBIND11_STDLIB=\"_libstdcpp\"", "-DPYBIND11_BUILD_ABI=\"_cxxabi1011\"",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+             "-Wno-deprecated-declarations"]
     for inc in ce.include_paths() + ["/opt/rocm/include", sysconfig.get_paths()["include"]]:
-        cmd += ["-isystem", inc]
-    cmd += [os.path.join(CSRC, "_dci_cuda.cpp"), "-o", EXT,
-            "-L" + tlib, "-L" + HERE, "-ldci_hip", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
+        flags += ["-isystem", inc]
+
+    def compile_one(src):
+        obj = os.path.join(CSRC, os.path.splitext(src)[0] + ".o")
+        return obj, subprocess.run([cxx] + flags + ["-c", os.path.join(CSRC, src), "-o", obj],
+                                   capture_output=True, text=True)
+
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        results = list(ex.map(compile_one, EXT_SOURCES))
+    objs = [obj for obj, _ in results]
+    results.append((EXT, None))
+    if all(r is None or r.returncode == 0 for _, r in results):
+        link = [cxx, "-shared", "-fPIC"] + objs + [
+            "-o", EXT, "-L" + tlib, "-L" + HERE, "-ldci_hip", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
             "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("building _dci_cuda failed:\n%s" % r.stderr[-4000:])
-    if verbose and r.stderr.strip():
-        print(r.stderr[-2000:], file=sys.stderr)
+        results[-1] = (EXT, subprocess.run(link, capture_output=True, text=True))
+    for _, r in results:
+        if r is None:
+            continue
+        if r.returncode != 0:
+            raise RuntimeError("building _dci_cuda failed:\n%s" % r.stderr[-4000:])
+        if verbose and r.stderr.strip():
+            print(r.stderr[-2000:], file=sys.stderr)
     return EXT
 
 

@@ -137,6 +137,8 @@ uintptr_t dci_handle(py::handle capsule) { return reinterpret_cast<uintptr_t>(ho
 
 }  // namespace
 
+void bind_tokens(py::module_& m);      // tokens_ext.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("_dci_new", &dci_new, "Create new DCI instance. (HIP)", py::arg("dim"),
           py::arg("num_comp_indices"), py::arg("num_simp_indices"), py::arg("device_id"),
@@ -148,4 +150,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("_dci_free", &dci_free, "Free DCI. (HIP)");
     m.def("_dci_multi_query", &dci_multi_query, "Search on several DCI instances (one GPU: one instance). (HIP)");
     m.def("_dci_handle", &dci_handle, "Address of the libdci_hip handle.");
+    bind_tokens(m);
 }

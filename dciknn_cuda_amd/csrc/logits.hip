@@ -1,0 +1,489 @@
+// Operators on rows of logits z[row][0 .. vocab): log probabilities of given tokens with
+// entropies and best alternatives, the loss against a teacher's top logits, and the gradients
+// of both by the logits.
+//
+//   x_v = (z_v - max z) / T,  Z = sum_v exp x_v,  log p_v = x_v - log Z,
+//   H   = log Z - sum_v x_v exp(x_v) / Z
+//   d/dz_v (g log p_t + h H) = ( g ([v = t] - p_v) - h p_v (log p_v + H) ) / T
+//   q_j = softmax over a row's filled slots of t_j / T,  loss = sum_j q_j (log q_j - log p_{id_j})
+//   d/dz_v (w loss) = (w / T) (p_v - sum_{j: id_j = v} q_j)
+//
+// All of them are bound by memory: a row is read once for its statistics (max, sum and, for the
+// entropy, weighted sum are kept running per thread and joined at the end), and read and written
+// once more for a gradient.  Everything between is in 32 bits; a gradient is rounded once.
+#include <algorithm>
+
+#include "../../include/dci_hip.h"
+#include "token_common.h"
+
+namespace dcih {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int64_t kMaxGrid = 1 << 22; // workgroups of one launch (their threads are counted in 32 bits)
+constexpr int kTopRoom = 256;        // entries of a wavefront's candidate list: kMaxTop + 2 * 64 at least
+static_assert(kTopRoom >= kMaxTop + 2 * kWave && kTopRoom % kWave == 0, "room for two rounds of candidates");
+
+enum { kLogprobs = 0, kLogprobsTop = 1, kDistill = 2 };
+
+typedef unsigned long long u64;
+
+// One entry of a candidate list: larger logits first, ties to the lower index.
+__device__ inline u64 entry_of(float z, int index) {
+    return (u64)f2ord(z + 0.f) << 32 | (0xffffffffu - (uint32_t)index);      // (-0 and 0 tie)
+}
+__device__ inline float entry_logit(u64 e) { return ord2f((uint32_t)(e >> 32)); }
+__device__ inline int entry_index(u64 e) { return (int)(0xffffffffu - (uint32_t)e); }
+
+__device__ inline int lanes_below(u64 mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// What one lane wrote to the wavefront's own part of LDS the others may read after this.
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The k best entries a wavefront has met, in LDS of its own: entries are put behind one another
+// and cut back to the k best whenever another 64 might not fit, so that any order of the row and
+// any number of ties is taken.  An entry is 0 at no time (index 2^32 - 1 does not exist).
+struct WaveTop {
+    u64* buf;          // kTopRoom entries
+    int k, count = 0;
+    u64 least = 0;     // what an entry has to exceed
+
+    __device__ WaveTop(u64* b, int k_) : buf(b), k(k_) {}
+
+    __device__ void push(bool want, u64 e) {
+        const u64 mask = __ballot(want && e > least);
+        if (mask >> lane_id() & 1) buf[count + lanes_below(mask)] = e;
+        count += __popcll(mask);
+        if (count > kTopRoom - kWave) cut();
+    }
+    // Leaves the k best in order, best first.  Entries are all different: the rank of one is the
+    // number of larger ones.
+    __device__ void cut() {
+        wave_fence();
+        u64 mine[kTopRoom / kWave];
+        int rank[kTopRoom / kWave];
+#pragma unroll
+        for (int r = 0; r < kTopRoom / kWave; r++) {
+            const int i = r * kWave + lane_id();
+            mine[r] = i < count ? buf[i] : 0;
+            rank[r] = 0;
+        }
+        for (int i = 0; i < count; i++) {
+            const u64 e = buf[i];
+#pragma unroll
+            for (int r = 0; r < kTopRoom / kWave; r++) rank[r] += e > mine[r];
+        }
+        wave_fence();
+#pragma unroll
+        for (int r = 0; r < kTopRoom / kWave; r++)
+            if (mine[r] && rank[r] < k) buf[rank[r]] = mine[r];
+        wave_fence();
+        count = min(count, k);
+        if (count == k) least = buf[k - 1];
+    }
+};
+
+// The k-th largest (k = 1 .. 64) of the lanes' values, on every lane: a bitonic sort in registers.
+template <int SIZE, int STRIDE>
+__device__ inline void sort_step(uint32_t& v) {
+    const uint32_t o = lane_xor<STRIDE>(v);
+    const bool low = ((lane_id() & STRIDE) == 0) == ((lane_id() & SIZE) == 0 || SIZE == kWave);
+    v = low ? max(v, o) : min(v, o);
+    if constexpr (STRIDE > 1) sort_step<SIZE, STRIDE / 2>(v);
+}
+__device__ inline uint32_t kth_of_lanes(uint32_t v, int k) {
+    sort_step<2, 1>(v); sort_step<4, 2>(v); sort_step<8, 4>(v);
+    sort_step<16, 8>(v); sort_step<32, 16>(v); sort_step<64, 32>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, k - 1);
+}
+
+__device__ inline float teacher_at(const LogitArgs& a, int64_t i) {
+    switch (a.teacher_dtype) {
+        case DCIH_F32: return ((const float*)a.teacher)[i];
+        case DCIH_F16: return (float)((const _Float16*)a.teacher)[i];
+        default: return (float)((const __bf16*)a.teacher)[i];
+    }
+}
+
+// Whether a row of logits holds nothing but -inf.
+__device__ inline bool nothing_left(const Softmax& f) { return f.m == kNoLogit && f.s == 0.f; }
+
+// The maximum that is kept of a row: -inf for one without entries and for no other (one of nothing
+// but NaN keeps 0 beside its sum, NaN).
+__device__ inline float kept_max(const Softmax& f) { return nothing_left(f) ? kNoLogit : f.m == kNoLogit ? 0.f : f.m; }
+
+// One wavefront: what is returned of a row of log probabilities.  `best`: its `count` best entries
+// in order, count < k only where fewer entries are above -inf.
+template <class T>
+__device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& f, const u64* best, int count) {
+    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
+    const bool none = nothing_left(f);
+    const float log2s = log2_fast(f.s);
+    const float entropy = none ? 0.f : (log2s - f.a / f.s) * kLn2;
+    if (lane_id() == 0) {
+        const int64_t t = id_at(a.ids, a.wide_ids, row);
+        float lp = 0.f;
+        if (t >= a.vocab) lp = __builtin_nanf("");
+        else if (t >= 0) lp = none ? kNoLogit : (((float)z[t] - f.m) * a.c2 - log2s) * kLn2;
+        a.logprobs[row] = lp;
+        a.entropy[row] = entropy;
+        if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, entropy * kLog2e, 0.f);
+    }
+    const int k = a.top;
+    if (!k) return;
+    int32_t* ids = a.top_ids + row * k;
+    float* lps = a.top_logprobs + row * k;
+    if (lane_id() < count) {
+        const u64 e = best[lane_id()];
+        ids[lane_id()] = entry_index(e);
+        lps[lane_id()] = ((entry_logit(e) - f.m) * a.c2 - log2s) * kLn2;
+    }
+    // what is ruled out (or no number) follows in order of its index
+    const float rest = f.s != f.s ? f.s : kNoLogit;
+    for (int first = 0; count < k && first < a.vocab; first += kWave) {
+        const int i = first + lane_id();
+        const bool gone = i < a.vocab && !((float)z[i] > kNoLogit);
+        const u64 mask = __ballot(gone);
+        const int at = count + lanes_below(mask);
+        if (gone && at < k) {
+            ids[at] = i;
+            lps[at] = rest;
+        }
+        count += __popcll(mask);
+    }
+}
+
+// One wavefront: the loss of a row against its teacher.
+template <class T>
+__device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f) {
+    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
+    const int64_t at = row * a.slots;
+    Softmax t = Softmax::none();
+    bool wrong = false;
+    for (int j = lane_id(); j < a.slots; j += kWave) {
+        const int64_t id = id_at(a.ids, a.wide_ids, at + j);
+        float y[1] = {id < 0 ? kNoLogit : teacher_at(a, at + j)};
+        wrong |= id >= a.vocab && y[0] != kNoLogit;
+        t.add<1, false>(y, a.c2);
+    }
+    t.join_wave(a.c2);
+    wrong = __ballot(wrong) != 0;
+    const bool empty = nothing_left(t), none = nothing_left(f);
+    const float log2t = log2_fast(t.s);
+    float log2s = log2_fast(f.s);
+    float sum = 0.f;
+    for (int j = lane_id(); j < a.slots; j += kWave) {
+        const int64_t id = id_at(a.ids, a.wide_ids, at + j);
+        const float y = id < 0 ? kNoLogit : teacher_at(a, at + j);
+        if (y == kNoLogit || id >= a.vocab) continue;
+        const float logq = (y - t.m) * a.c2 - log2t;
+        const float q = exp2_fast(logq);
+        const float logp = none ? kNoLogit : ((float)z[id] - f.m) * a.c2 - log2s;
+        if (!(q == 0.f)) sum += q * (logq - logp);
+    }
+    sum = wave_sum(sum) * kLn2;
+    if (wrong || t.s != t.s) sum = log2s = __builtin_nanf("");
+    if (empty) sum = 0.f;
+    if (lane_id() == 0) {
+        a.losses[row] = sum;
+        if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, kept_max(t), log2t);
+    }
+}
+
+// Statistics of rows, each by `splits` workgroups.  Threads keep their own running statistics over
+// every 256th piece; a wavefront keeps its best entries, too.
+template <class T, int kMode, int U>
+__global__ __launch_bounds__(kThreads) void logit_stats_kernel(LogitArgs a) {
+    using P = Piece<T>;
+    __shared__ u64 s_top[kMode == kLogprobsTop ? kWaves * kTopRoom : 1];
+    __shared__ int s_count[kWaves];
+    __shared__ Softmax s_part[kWaves];
+    const int64_t row = a.first + blockIdx.x / (uint32_t)a.splits;
+    const int split = (int)(blockIdx.x % (uint32_t)a.splits);
+    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
+    const int tid = threadIdx.x, wave = tid / kWave;
+    const int end = min((a.vocab + P::kLen - 1) / P::kLen, (split + 1) * a.per_split);     // in pieces
+    Softmax f = Softmax::none();
+    WaveTop top(s_top + (kMode == kLogprobsTop ? wave * kTopRoom : 0), a.top);
+    bool first = true;
+    for (int base = split * a.per_split; base < end; base += kThreads * U) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = base + u * kThreads + tid;
+            if (i < end && (i + 1) * P::kLen <= a.vocab) raw[u] = P::load_once(z + (int64_t)i * P::kLen);
+            else raw[u] = P::load_part(z, i < end ? i * P::kLen : a.vocab, a.vocab, kNoLogit);
+        }
+        float x[U * P::kLen], most = kNoLogit;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float y[P::kLen];
+            P::unpack(raw[u], y);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) {
+                x[u * P::kLen + k] = y[k];
+                most = fmaxf(most, y[k]);
+            }
+        }
+        f.add<U * P::kLen, kMode != kDistill>(x, most, a.c2);
+        if constexpr (kMode == kLogprobsTop) {
+            // The k-th largest of the lanes' largest values has k entries at or above it: none
+            // below it is among the k best.
+            if (first) {
+                const uint32_t kth = kth_of_lanes(f2ord(most + 0.f), a.top);
+                top.least = (u64)kth << 32;
+                first = false;
+            }
+            const float bar = entry_logit(top.least);
+            if (__any(most >= bar && most > kNoLogit)) {
+                uint32_t left = 0;
+#pragma unroll
+                for (int k = 0; k < U * P::kLen; k++) left |= (x[k] >= bar && x[k] > kNoLogit ? 1u : 0u) << k;
+                while (__any(left != 0)) {
+                    const int k = left ? __builtin_ctz(left) : 0;
+                    const int i = (base + (k / P::kLen) * kThreads + tid) * P::kLen + k % P::kLen;
+                    const bool want = left != 0;
+                    top.push(want, want ? entry_of((float)z[i], i) : 0);
+                    left &= left - 1;
+                }
+            }
+        }
+    }
+    f.join_wave(a.c2);
+    if constexpr (kMode == kLogprobsTop) top.cut();
+    if (lane_id() == 0) {
+        s_part[wave] = f;
+        s_count[wave] = top.count;
+    }
+    __syncthreads();
+    if (wave) return;
+    f = s_part[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) f.join(s_part[w], a.c2);
+    if constexpr (kMode == kLogprobsTop) {
+        // the other wavefronts' entries behind the first one's own
+        top.count = s_count[0];
+        for (int w = 1; w < kWaves; w++)
+            top.push(lane_id() < s_count[w], lane_id() < s_count[w] ? s_top[w * kTopRoom + lane_id()] : 0);
+        top.cut();
+    }
+    if (a.splits > 1) {
+        const int64_t at = row * a.splits + split;
+        if (lane_id() == 0) a.part[at] = make_float4(f.m, f.s, f.a, 0.f);
+        if (kMode == kLogprobsTop && lane_id() < a.top)
+            a.part_top[at * a.top + lane_id()] = lane_id() < top.count ? top.buf[lane_id()] : 0;
+        return;
+    }
+    if constexpr (kMode == kDistill) finish_distill<T>(a, row, f);
+    else finish_logprobs<T>(a, row, f, top.buf, top.count);
+}
+
+// Joins the splits (up to 64) of a row: one wavefront each.
+template <class T, int kMode>
+__global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
+    __shared__ u64 s_top[kMode == kLogprobsTop ? kTopRoom : 1];
+    const int64_t row = a.first + blockIdx.x;
+    const int lane = lane_id();
+    Softmax f = Softmax::none();
+    if (lane < a.splits) {
+        const float4 p = a.part[row * a.splits + lane];
+        f.m = p.x; f.s = p.y; f.a = p.z;
+    }
+    f.join_wave(a.c2);
+    if constexpr (kMode == kDistill) {
+        finish_distill<T>(a, row, f);
+    } else {
+        WaveTop top(s_top, a.top);
+        if constexpr (kMode == kLogprobsTop) {
+            const u64* lists = a.part_top + (row * a.splits + min(lane, a.splits - 1)) * a.top;
+            // The lists are in order: with k lists or more, the k-th largest of their first entries bounds
+            // from below, and where no list has an entry above the bound at a place none has one behind it.
+            const u64 head = lane < a.splits ? lists[0] : 0;
+            const uint32_t kth = kth_of_lanes((uint32_t)(head >> 32), a.top);
+            if (a.top <= a.splits) top.least = (u64)kth << 32;
+            for (int p = 0; p < a.top; p++) {
+                const u64 e = lane < a.splits ? lists[p] : 0;
+                if (!__any(e > top.least)) break;
+                top.push(e != 0, e);
+            }
+            top.cut();
+        }
+        finish_logprobs<T>(a, row, f, top.buf, top.count);
+    }
+}
+
+// Gradients by the logits from a row's statistics, one tile of a row per workgroup.
+template <class T, int kMode, int U>
+__global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
+    using P = Piece<T>;
+    constexpr int kTile = kThreads * U * P::kLen;
+    constexpr int kOwn = kTeacherSlots / kThreads;
+    __shared__ int s_id[kMode == kDistill ? kTeacherSlots : 1];
+    __shared__ float s_q[kMode == kDistill ? kTeacherSlots : 1];
+    const int64_t row = a.first + blockIdx.x / (uint32_t)a.splits;
+    const int tile = (int)(blockIdx.x % (uint32_t)a.splits) * kTile, tid = threadIdx.x;
+    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
+    typename T::raw* dz = (typename T::raw*)a.grad + row * a.grad_stride;
+    const float4 st = a.stats[row];
+    // What a gradient is made of: dz = p (c0 + c1 log2 p) + at the target c2.
+    float c0, c1 = 0.f, at_target = 0.f;
+    int64_t target = -1;
+    bool zero = st.x == kNoLogit;
+    if constexpr (kMode == kDistill) {
+        c0 = (a.weights ? a.weights[row] : 1.f) * a.inv_t;
+        zero |= c0 == 0.f || st.z == kNoLogit;
+    } else {
+        target = id_at(a.ids, a.wide_ids, row);
+        const float g = a.grad_logprobs && target >= 0 ? a.grad_logprobs[row] * a.inv_t : 0.f;
+        const float h = a.grad_entropy ? a.grad_entropy[row] * a.inv_t : 0.f;
+        zero |= g == 0.f && h == 0.f;
+        c0 = -(g + h * st.z * kLn2);
+        c1 = -h * kLn2;
+        at_target = g;
+        if (target >= a.vocab && g != 0.f) c0 = __builtin_nanf("");
+    }
+    float own_z[kMode == kDistill ? kOwn : 1];
+    bool here = false;
+    if constexpr (kMode == kDistill) {
+        if (!zero) {
+#pragma unroll
+            for (int o = 0; o < kOwn; o++) {
+                const int j = o * kThreads + tid;
+                if (j >= a.slots) break;
+                const int64_t id = id_at(a.ids, a.wide_ids, row * a.slots + j);
+                const float y = teacher_at(a, row * a.slots + j);
+                const bool in = id >= tile && id < min(a.vocab, tile + kTile) && y != kNoLogit;
+                s_id[j] = in ? (int)id : -1;
+                s_q[j] = exp2_fast((y - st.z) * a.c2 - st.w);
+                if (in) own_z[o] = (float)z[id];       // before it is written over
+                here |= in;
+            }
+        }
+        here = __syncthreads_or(here);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = tile + (u * kThreads + tid) * P::kLen;
+        if (i >= a.vocab) continue;
+        const bool whole = i + P::kLen <= a.vocab;
+        float y[P::kLen];
+        if (zero) {
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) y[k] = 0.f;
+        } else {
+            P::unpack(whole ? P::load_once(z + i) : P::load_part(z, i, a.vocab, kNoLogit), y);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) {
+                const float x = (y[k] - st.x) * a.c2 - st.y;      // log2 p
+                const float p = exp2_fast(x);
+                if constexpr (kMode == kDistill) y[k] = p * c0;
+                else y[k] = p * __builtin_fmaf(c1, fmaxf(x, kFloor2), c0);
+            }
+            if (kMode != kDistill && target >= i && target < i + P::kLen) {
+#pragma unroll
+                for (int k = 0; k < P::kLen; k++) y[k] += i + k == target ? at_target : 0.f;
+            }
+        }
+        const u32x4 out = P::pack(y);
+        if (whole) P::store_once(dz + i, out);
+        else P::store_part(dz, i, a.vocab, out);
+    }
+    if constexpr (kMode == kDistill) {
+        if (!here) return;
+        __syncthreads();
+        // the teacher's tokens, each by the first of the slots that name it
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const int j = o * kThreads + tid;
+            if (j >= a.slots) break;
+            const int id = s_id[j];
+            if (id < 0) continue;
+            bool again = false;
+            for (int i = 0; i < j; i++) again |= s_id[i] == id;
+            if (again) continue;
+            float q = 0.f;
+            for (int i = j; i < a.slots; i++) q += s_id[i] == id ? s_q[i] : 0.f;
+            dz[id] = (typename T::raw)(c0 * (exp2_fast((own_z[o] - st.x) * a.c2 - st.y) - q));
+        }
+    }
+}
+
+template <class T, int kMode>
+int stats_of(LogitArgs a, hipStream_t s) {
+    constexpr int U = sizeof(typename T::raw) == 4 ? 4 : 2;
+    for (int64_t most = kMaxGrid / a.splits; a.first < a.n; a.first += most) {
+        const uint32_t rows = (uint32_t)std::min(most, a.n - a.first);
+        logit_stats_kernel<T, kMode, U><<<rows * a.splits, kThreads, 0, s>>>(a);
+        DCIH_HIP(hipGetLastError());
+        if (a.splits > 1) {
+            logit_join_kernel<T, kMode><<<rows, kWave, 0, s>>>(a);
+            DCIH_HIP(hipGetLastError());
+        }
+    }
+    return 0;
+}
+
+template <class T, int kMode>
+int grad_of(LogitArgs a, hipStream_t s) {
+    constexpr int U = 2, kTile = kThreads * U * Piece<T>::kLen;
+    a.splits = (a.vocab - 1) / kTile + 1;
+    for (int64_t most = std::max<int64_t>(1, kMaxGrid / a.splits); a.first < a.n; a.first += most) {
+        logit_grad_kernel<T, kMode, U><<<(uint32_t)std::min(most, a.n - a.first) * a.splits, kThreads, 0, s>>>(a);
+        DCIH_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+}  // namespace
+
+// Workgroups a row is split over: enough of them in all to fill the device, each with one
+// round of loads at least.
+int logit_splits(int64_t n, int vocab, int dtype) {
+    const int64_t pieces = ((int64_t)vocab * type_bytes(dtype) + 15) / 16;
+    const int64_t most = (pieces + kThreads - 1) / kThreads, want = (1024 + n - 1) / n;
+    return (int)(want < 1 ? 1 : want > most ? (most > kMaxSplits ? kMaxSplits : most) : want > kMaxSplits ? kMaxSplits : want);
+}
+
+int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
+    const int len = 16 / type_bytes(dtype), pieces = (int)(((int64_t)a.vocab + len - 1) / len);
+    a.per_split = (pieces + a.splits - 1) / a.splits;
+    if (distill) {
+        switch (dtype) {
+            case DCIH_F32: return stats_of<F32, kDistill>(a, s);
+            case DCIH_F16: return stats_of<F16, kDistill>(a, s);
+            default: return stats_of<BF16, kDistill>(a, s);
+        }
+    }
+    switch (dtype * 2 + (a.top > 0)) {
+        case DCIH_F32 * 2: return stats_of<F32, kLogprobs>(a, s);
+        case DCIH_F32 * 2 + 1: return stats_of<F32, kLogprobsTop>(a, s);
+        case DCIH_F16 * 2: return stats_of<F16, kLogprobs>(a, s);
+        case DCIH_F16 * 2 + 1: return stats_of<F16, kLogprobsTop>(a, s);
+        case DCIH_BF16 * 2: return stats_of<BF16, kLogprobs>(a, s);
+        default: return stats_of<BF16, kLogprobsTop>(a, s);
+    }
+}
+
+int logit_grad(const LogitArgs& a, int dtype, bool distill, hipStream_t s) {
+    if (distill) {
+        switch (dtype) {
+            case DCIH_F32: return grad_of<F32, kDistill>(a, s);
+            case DCIH_F16: return grad_of<F16, kDistill>(a, s);
+            default: return grad_of<BF16, kDistill>(a, s);
+        }
+    }
+    switch (dtype) {
+        case DCIH_F32: return grad_of<F32, kLogprobs>(a, s);
+        case DCIH_F16: return grad_of<F16, kLogprobs>(a, s);
+        default: return grad_of<BF16, kLogprobs>(a, s);
+    }
+}
+
+}  // namespace dcih

@@ -1,0 +1,196 @@
+// What the token operators share: element types, 16-byte pieces of rows that may start at any
+// element, ids of 4 or 8 bytes, the running
+// statistics of a softmax, and the launch interface.
+#pragma once
+
+#include "common.h"
+
+namespace dcih {
+
+// Element types as they stand in memory; values are computed with in 32 bits.
+struct F32 { using raw = float; };
+struct F16 { using raw = _Float16; };
+struct BF16 { using raw = __bf16; };
+
+// Bytes of an element of type code `dtype` (DCIH_F32, ..), 0 for no such type.
+inline int type_bytes(int dtype) { return dtype == 0 ? 4 : dtype == 1 || dtype == 2 ? 2 : 0; }
+
+// ---- what the entry points (token_api.hip) hand to embed.hip and logits.hip --------
+// Type codes are DCIH_F32, DCIH_F16, DCIH_BF16; ids are 4 or 8 bytes wide.
+
+constexpr int kMaxTop = 64;       // alternatives of a row
+constexpr int kTeacherSlots = 1024;   // slots of a teacher's row
+constexpr int kMaxSplits = 64;    // workgroups that share a row
+
+struct LogitArgs {
+    const void* z;                // logits: row r at z + r * stride (elements)
+    int64_t n, stride, first;     // `first`: the first row of a launch
+    int vocab;
+    float c2, inv_t;              // log2(e) / temperature, 1 / temperature
+    const void* ids;              // targets [n], or the teacher's ids [n][slots]
+    bool wide_ids;
+    int splits, per_split;        // workgroups of a row, 16-byte pieces of each
+    float4* stats;                // [n] (max, log2 sum, entropy / ln 2, -) or (max, log2 sum, teacher's max, teacher's log2 sum)
+    float4* part;                 // [n][splits] statistics of splits
+    unsigned long long* part_top; // [n][splits][top] their best entries
+    // log probabilities
+    int top;
+    float *logprobs, *entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+    // distillation
+    const void* teacher;          // [n][slots]
+    int teacher_dtype, slots;
+    float* losses;
+    // gradients
+    const float *grad_logprobs, *grad_entropy, *weights;
+    void* grad;
+    int64_t grad_stride;
+};
+int logit_splits(int64_t n, int vocab, int dtype);
+int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s);
+int logit_grad(const LogitArgs& a, int dtype, bool distill, hipStream_t s);
+
+struct EmbedArgs {
+    const void* rows;             // the table, or the gradients of the rows looked up
+    int64_t num_rows, stride;     // rows of the table; distance of rows in `rows` (elements)
+    int dim;
+    const void* ids;
+    bool wide_ids;
+    int64_t n;                    // ids
+    float scale;
+    void* out;                    // contiguous
+    bool accumulate;              // (gradient) added to what `out` holds
+    void* work;
+};
+int embed_rows(const EmbedArgs& a, int dtype, hipStream_t s);
+size_t embed_grad_bytes(int64_t n, int dim);
+int embed_grad(const EmbedArgs& a, int dtype, int out_dtype, hipStream_t s);
+
+#if defined(__HIPCC__)
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Sixteen bytes at any element's address: rows of odd lengths start on no boundary, and the
+// memory system takes such accesses (a wavefront's 1 KB then touches one line more).
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+template <class T> struct Piece {          // one 16-byte piece of a row
+    static constexpr int kLen = 16 / (int)sizeof(typename T::raw);
+    typedef typename T::raw vec __attribute__((ext_vector_type(kLen)));
+    typedef float fvec __attribute__((ext_vector_type(kLen)));
+
+    __device__ static u32x4 load(const typename T::raw* p) {
+        return *reinterpret_cast<const u32x4_any*>(p);
+    }
+    // Rows that are read or written once: not to displace what the caches hold.
+    __device__ static u32x4 load_once(const typename T::raw* p) {
+        return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+    }
+    // Elements [i, i + kLen) of a row of `len`, `fill` beyond its end.
+    __device__ static u32x4 load_part(const typename T::raw* row, int i, int len, float fill) {
+        vec v;
+#pragma unroll
+        for (int k = 0; k < kLen; k++) v[k] = i + k < len ? row[i + k] : (typename T::raw)fill;
+        return __builtin_bit_cast(u32x4, v);
+    }
+    __device__ static void unpack(u32x4 x, float (&z)[kLen]) {
+        const fvec f = __builtin_convertvector(__builtin_bit_cast(vec, x), fvec);
+#pragma unroll
+        for (int k = 0; k < kLen; k++) z[k] = f[k];
+    }
+    // Rounded to the nearest, ties to even.
+    __device__ static u32x4 pack(const float (&z)[kLen]) {
+        fvec f;
+#pragma unroll
+        for (int k = 0; k < kLen; k++) f[k] = z[k];
+        return __builtin_bit_cast(u32x4, __builtin_convertvector(f, vec));
+    }
+    __device__ static void store(typename T::raw* p, u32x4 x) { *reinterpret_cast<u32x4_any*>(p) = x; }
+    __device__ static void store_once(typename T::raw* p, u32x4 x) {
+        __builtin_nontemporal_store((u32x4_any)x, reinterpret_cast<u32x4_any*>(p));
+    }
+    __device__ static void store_part(typename T::raw* row, int i, int len, u32x4 x) {
+        const vec v = __builtin_bit_cast(vec, x);
+#pragma unroll
+        for (int k = 0; k < kLen; k++)
+            if (i + k < len) row[i + k] = v[k];
+    }
+};
+
+__device__ inline int64_t id_at(const void* ids, bool wide, int64_t i) {
+    return wide ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+}
+
+__device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32, 1 ulp
+__device__ inline float log2_fast(float x) { return __builtin_amdgcn_logf(x); }    // v_log_f32, 1 ulp
+
+constexpr float kNoLogit = -__builtin_huge_valf();
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kLog2e = 1.44269504088896341f;
+
+// Below 2^-256 nothing is left in 32 bits: exponents are cut off there wherever they are a
+// factor themselves, so that a ruled-out entry adds 0 * -256 and not 0 * -inf.
+constexpr float kFloor2 = -256.f;
+
+// Running statistics of a softmax over entries z at temperature T, exponents to the base 2
+// (c2 = log2(e) / T):  m = max z,  s = sum 2^((z - m) c2),  a = sum (z - m) c2 2^((z - m) c2).
+// The difference z - m is formed before the factor, so that the type's lowest value cannot
+// overflow.  With m = -inf nothing but -inf was seen and s = a = 0; a NaN or +inf leaves s = NaN.
+struct Softmax {
+    float m, s, a;
+
+    __device__ static Softmax none() { return Softmax{kNoLogit, 0.f, 0.f}; }
+
+    // The statistics of both parts.  (fmaxf(NaN, floor) = floor covers -inf - -inf.)
+    __device__ void join(const Softmax& o, float c2) {
+        const float top = fmaxf(m, o.m);
+        const float d1 = fmaxf((m - top) * c2, kFloor2), d2 = fmaxf((o.m - top) * c2, kFloor2);
+        const float f1 = exp2_fast(d1), f2 = exp2_fast(d2);
+        a = f1 * (a + d1 * s) + f2 * (o.a + d2 * o.s);
+        s = s * f1 + o.s * f2;
+        m = top;
+    }
+    // Adds N entries.
+    template <int N, bool kEntropy>
+    __device__ void add(const float (&z)[N], float c2) {
+        float top = z[0];
+#pragma unroll
+        for (int k = 1; k < N; k++) top = fmaxf(top, z[k]);
+        add<N, kEntropy>(z, top, c2);
+    }
+    // `top` is the largest of them.
+    template <int N, bool kEntropy>
+    __device__ void add(const float (&z)[N], float top, float c2) {
+        top = fmaxf(top, m);
+        const float ref = top == kNoLogit ? 0.f : top;
+        const float d = fmaxf((m - ref) * c2, kFloor2), f = exp2_fast(d);
+        if (kEntropy) a = f * (a + d * s);
+        s *= f;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float x = (z[k] - ref) * c2, e = exp2_fast(x);
+            s += e;
+            if (kEntropy) a = __builtin_fmaf(fmaxf(x, kFloor2), e, a);
+        }
+    }
+    template <int O> __device__ void join_lane(float c2) {
+        Softmax o;
+        o.m = lane_xor<O>(m); o.s = lane_xor<O>(s); o.a = lane_xor<O>(a);
+        join(o, c2);
+    }
+    // Over a wavefront; every lane gets the result.
+    __device__ void join_wave(float c2) {
+        join_lane<32>(c2); join_lane<16>(c2); join_lane<8>(c2);
+        join_lane<4>(c2); join_lane<2>(c2); join_lane<1>(c2);
+    }
+};
+
+__device__ inline float wave_max(float v) {
+    v = fmaxf(v, lane_xor<32>(v)); v = fmaxf(v, lane_xor<16>(v)); v = fmaxf(v, lane_xor<8>(v));
+    v = fmaxf(v, lane_xor<4>(v)); v = fmaxf(v, lane_xor<2>(v)); v = fmaxf(v, lane_xor<1>(v));
+    return v;
+}
+
+#endif  // __HIPCC__
+}  // namespace dcih

@@ -320,6 +320,87 @@ int dcih_project(const float* d_dirs, int num_indices, const float* d_rows,
 int dcih_segsort(const float* d_keys, int num_indices, int64_t num_points,
                  int block_size, float* d_skeys, int32_t* d_sids, void* stream);
 
+/*
+ * Operators of programs that train or serve a model on the rows and neighbours that an
+ * index holds and finds: the reference, a search engine alone, has no counterpart.  They need no
+ * handle, keep nothing between calls, allocate nothing and only enqueue work (they may be
+ * captured into a graph); where a workspace is asked for, the caller gives one of the
+ * size that the *_work function says, aligned to 16 bytes, to be used by nobody else until
+ * the stream has passed the call.
+ *
+ * Elements are of one of the three types below, computed with in 32 bits and rounded once (to the
+ * nearest, ties to even).  Ids are int32 or int64 (id_bytes 4 or 8), contiguous.  Rows have a
+ * distance of row_stride elements and may start at any element.  An id below 0 marks an empty slot, as
+ * dcih_query leaves them; an id beyond the table or the vocabulary is never accessed and gives
+ * NaN, as said with each operator.  Counts of rows and ids are below 2^31.
+ */
+enum { DCIH_F32 = 0, DCIH_F16 = 1, DCIH_BF16 = 2 };
+#define DCIH_MAX_VOCAB (1 << 28)
+
+/*
+ * d_out[i] = scale * d_table[ids[i]], contiguous rows of the table's type.  An empty slot's
+ * row is zeros, the row of an id beyond the table NaN.
+ */
+int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_t row_stride, const void* d_ids,
+               int id_bytes, int64_t num_ids, float scale, void* d_out, void* stream);
+
+/*
+ * The gradient of dcih_embed by the table: d_out[r] = scale * sum of d_grad[i] over the i
+ * with ids[i] = r, contiguous rows, of d_grad's type or DCIH_F32.  accumulate != 0 adds to what
+ * d_out holds (rows without an id are not touched), 0 writes every row.  Sums are
+ * formed in 32 bits in an order that depends on the ids alone: the same input gives the same
+ * bits.  Empty slots and ids beyond the table add nothing.
+ */
+int64_t dcih_embed_grad_work(int64_t num_ids, int dim);
+int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int64_t row_stride, const void* d_ids,
+                    int id_bytes, int64_t num_rows, float scale, int accumulate, void* d_out, int out_dtype,
+                    void* d_work, int64_t work_bytes, void* stream);
+
+/* Bytes of workspace of dcih_token_logprobs and (top = 0) dcih_distill. */
+int64_t dcih_logits_work(int64_t num_rows, int vocab, int dtype, int top);
+
+/*
+ * With p = softmax(logits / temperature) of a row: d_logprobs[i] = log p[target] (0 for a target
+ * below 0, NaN for one beyond the vocabulary), d_entropy[i] = -sum p log p, and the `top` (0 to
+ * 64) largest logits' indices and log p in descending order, [num_rows][top], equal ones by index, those of -inf
+ * or NaN last (both arrays may be NULL for top = 0).  A row of nothing but -inf has log p = -inf
+ * and entropy 0; one with NaN or +inf has NaN for both.  d_stats: NULL, or
+ * [num_rows][4] floats for dcih_token_logprobs_grad, aligned to 16 bytes.
+ */
+int dcih_token_logprobs(const void* d_logits, int dtype, int64_t num_rows, int vocab, int64_t row_stride, const void* d_targets,
+                        int id_bytes, float temperature, int top, float* d_logprobs, float* d_entropy, int32_t* d_top_ids,
+                        float* d_top_logprobs, float* d_stats, void* d_work, int64_t work_bytes, void* stream);
+
+/*
+ * The gradient by the logits of sum_i (d_grad_logprobs[i] * logprobs[i] + d_grad_entropy[i] *
+ * entropy[i]), either of them NULL for zeros, in the logits' type; d_grad may be d_logits itself (same stride)
+ * and must not overlap it otherwise.  A row whose two factors are 0 (or that is all -inf)
+ * has gradient 0 whatever it holds; a target beyond the vocabulary with a factor that is not 0 gives NaN.
+ */
+int dcih_token_logprobs_grad(const void* d_logits, int dtype, int64_t num_rows, int vocab, int64_t row_stride,
+                             const void* d_targets, int id_bytes, float temperature, const float* d_stats,
+                             const float* d_grad_logprobs, const float* d_grad_entropy, void* d_grad, int64_t grad_stride,
+                             void* stream);
+
+/*
+ * Distillation from a teacher's top logits.  d_ids and d_teacher are [num_rows][slots] (1 to
+ * 1024), the teacher's logits of any of the types; a slot with an id below 0 or a logit of -inf is empty, an
+ * id may stand in several slots.  With q = softmax(teacher / temperature) over a row's filled slots
+ * and p = softmax(logits / temperature): d_losses[i] = sum_j q_j (log q_j - log p[id_j]); 0 without filled slots;
+ * +inf where p is 0 at a filled slot; NaN for an id beyond the vocabulary.
+ * d_grad: NULL, or the gradient by the logits of sum_i d_weights[i] * d_losses[i] (d_weights NULL: ones),
+ * in the logits' type and in their place or apart as above; rows with weight 0, without filled slots or of
+ * nothing but -inf have gradient 0.  d_stats: NULL, or [num_rows][4] floats for dcih_distill_grad,
+ * which forms that gradient in a call of its own.
+ */
+int dcih_distill(const void* d_logits, int dtype, int64_t num_rows, int vocab, int64_t row_stride, const void* d_ids,
+                 int id_bytes, const void* d_teacher, int teacher_dtype, int slots, float temperature, float* d_losses,
+                 float* d_stats, const float* d_weights, void* d_grad, int64_t grad_stride, void* d_work, int64_t work_bytes,
+                 void* stream);
+int dcih_distill_grad(const void* d_logits, int dtype, int64_t num_rows, int vocab, int64_t row_stride, const void* d_ids,
+                      int id_bytes, const void* d_teacher, int teacher_dtype, int slots, float temperature,
+                      const float* d_stats, const float* d_weights, void* d_grad, int64_t grad_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
