@@ -69,7 +69,7 @@ SIGNATURES = {
                                 _c.c_void_p, _c.c_void_p]),
     "dcih_embed": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
                               _c.c_int, _c.c_int64, _c.c_float, _c.c_void_p, _c.c_void_p]),
-    "dcih_embed_grad_work": (_c.c_int64, [_c.c_int64, _c.c_int]),
+    "dcih_embed_grad_work": (_c.c_int64, [_c.c_int64, _c.c_int, _c.c_int64]),
     "dcih_embed_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
                                    _c.c_int, _c.c_int64, _c.c_float, _c.c_int, _c.c_void_p, _c.c_int,
                                    _c.c_void_p, _c.c_int64, _c.c_void_p]),

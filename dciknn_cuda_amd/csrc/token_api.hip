@@ -117,9 +117,9 @@ int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_
     return embed_rows(a, dtype, (hipStream_t)stream);
 }
 
-int64_t dcih_embed_grad_work(int64_t num_ids, int dim) {
-    if (num_ids < 0 || num_ids > kMaxCount || dim <= 0) return refuse("dcih_embed_grad_work", "bad size");
-    return (int64_t)embed_grad_bytes(num_ids, dim);
+int64_t dcih_embed_grad_work(int64_t num_ids, int dim, int64_t num_rows) {
+    if (num_ids < 0 || num_ids > kMaxCount || dim <= 0 || num_rows <= 0 || num_rows > kMaxCount) return refuse("dcih_embed_grad_work", "bad size");
+    return (int64_t)embed_grad_bytes(num_ids, dim, num_rows);
 }
 
 int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int64_t row_stride, const void* d_ids,
@@ -133,9 +133,9 @@ int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int
     if (num_ids) {
         if (const char* why = check_array(d_grad, dtype)) return refuse(who, why);
         if (const char* why = check_ids(d_ids, id_bytes)) return refuse(who, why);
-        if (!d_work || work_bytes < (int64_t)embed_grad_bytes(num_ids, dim)) return refuse(who, "workspace too small");
-        if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     }
+    if (!d_work || work_bytes < (int64_t)embed_grad_bytes(num_ids, dim, num_rows)) return refuse(who, "workspace too small");
+    if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     EmbedArgs a{};
     a.rows = d_grad;
     a.num_rows = num_rows;

@@ -64,7 +64,7 @@ struct EmbedArgs {
     void* work;
 };
 int embed_rows(const EmbedArgs& a, int dtype, hipStream_t s);
-size_t embed_grad_bytes(int64_t n, int dim);
+size_t embed_grad_bytes(int64_t n, int dim, int64_t num_rows);
 int embed_grad(const EmbedArgs& a, int dtype, int out_dtype, hipStream_t s);
 
 #if defined(__HIPCC__)

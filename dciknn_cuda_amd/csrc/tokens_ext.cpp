@@ -145,7 +145,7 @@ Tensor embed_grad(const Tensor& grad, const Tensor& ids_in, int64_t num_rows, do
     }
     c10::DeviceGuard guard(grad.device());
     if (!into) out = torch::empty({num_rows, r.len}, grad.options().requires_grad(false));
-    const Tensor work = bytes(dcih_embed_grad_work(r.n, (int)r.len), grad);
+    const Tensor work = bytes(dcih_embed_grad_work(r.n, (int)r.len, num_rows), grad);
     check(dcih_embed_grad(grad.data_ptr(), r.dtype, r.n, (int)r.len, r.stride, ids.data_ptr(), id_bytes(ids), num_rows,
                           (float)scale, into ? 1 : 0, out.data_ptr(), out.scalar_type() == torch::kFloat32 ? DCIH_F32 : r.dtype,
                           work.data_ptr(), work.numel(), stream_of(grad)));

@@ -351,7 +351,7 @@ int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_
  * formed in 32 bits in an order that depends on the ids alone: the same input gives the same
  * bits.  Empty slots and ids beyond the table add nothing.
  */
-int64_t dcih_embed_grad_work(int64_t num_ids, int dim);
+int64_t dcih_embed_grad_work(int64_t num_ids, int dim, int64_t num_rows);
 int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int64_t row_stride, const void* d_ids,
                     int id_bytes, int64_t num_rows, float scale, int accumulate, void* d_out, int out_dtype,
                     void* d_work, int64_t work_bytes, void* stream);

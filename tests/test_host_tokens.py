@@ -18,8 +18,9 @@ def test_entry_points_refuse(oracle):
         assert embed(**bad) == inval, bad
         assert lib.dcih_last_error().startswith(b"dcih_embed: ")
     assert embed(n=0, ids=None, out=None) == 0
-    need = lib.dcih_embed_grad_work(100, 8)
-    assert need > 0 and lib.dcih_embed_grad_work(-1, 8) == inval and lib.dcih_embed_grad_work(1, 0) == inval
+    need = lib.dcih_embed_grad_work(100, 8, 5)
+    assert need > 0 and lib.dcih_embed_grad_work(-1, 8, 5) == inval and lib.dcih_embed_grad_work(1, 0, 5) == inval
+    assert lib.dcih_embed_grad_work(1, 8, 0) == inval
     grad = lambda g=A, dtype=0, n=100, dim=8, stride=8, ids=A, width=8, rows=5, out=A, kind=0, work=A, size=need: lib.dcih_embed_grad(   # noqa: E731
         g, dtype, n, dim, stride, ids, width, rows, 1.0, 0, out, kind, work, size, None)
     for bad in (dict(g=None), dict(dtype=4), dict(n=-1), dict(dim=0), dict(stride=1), dict(ids=None), dict(width=1), dict(rows=0), dict(out=None),
