@@ -4,7 +4,7 @@
 //
 // Both are bound by memory.  The gradient's sums are formed without atomics on values, in the
 // order of the tokens whatever the schedule: the tokens are first grouped by their row (chunk_kernel,
-// bucket_kernel), then summed in pieces of up to kPiece tokens of one row (sum_kernel); the pieces of rows with more
+// bucket_kernel), then summed in pieces of up to 16 tokens of one row (sum_kernel); the pieces of rows with more
 // tokens than that are joined by a third launch (join_kernel).  Sums are in 32 bits, rounded once.
 #include "../../include/dci_hip.h"
 #include "token_common.h"
@@ -58,37 +58,46 @@ constexpr int kGroupThreads = 512, kGroupWaves = kGroupThreads / kWave;
 constexpr int kPerLane = kChunk / kGroupThreads;
 constexpr int kMinBucketBits = 8, kMaxBucketBits = 11;   // a bucket for each compute unit; what chunk_kernel counts on chip
 constexpr int kBins = 1024;                              // rows that bucket_kernel counts at a time
-constexpr int kPiece = 32;                               // tokens of a row that are summed by one group of lanes
+constexpr int kWide = 16;                                // pieces from which a row's sums are joined by groups
+constexpr int64_t kManySums = 1 << 20;                   // elements from which pieces of 16 tokens fill the device
 
 // The call's workspace.
 struct Work {
-    uint32_t* total;        // tokens with a row
+    uint32_t* total;        // [3]: tokens with a row; rows with more tokens than a piece, and than kWide pieces
     Placed* placed;         // [chunks][kChunk]: each chunk's tokens in order of (bucket, place)
     uint16_t* starts;       // [chunks][buckets + 1]: where a bucket's begin
     Token* tokens;          // [n] in the grouped order
-    unsigned long long* present;   // [buckets][words]: bit r mod 64 of word r / 64 for the r-th row of a bucket
+    uint32_t* common;       // [2][n / piece]: where the rows with more tokens than a piece, and than kWide pieces, begin
     float* part;            // [2 * windows][width]: see sum_kernel
     int64_t chunks, windows;
-    int bucket_bits, words, width;
+    int piece;              // tokens of a row that are summed by one group of lanes
+    int bucket_bits, width;
 };
+
+// Bucket b holds the rows r with r mod buckets = b: rows are often alike in their number of tokens where
+// they are near (with runs of 8 rows the commonest bucket took 30 us instead of 16 for 65536 tokens of text).
+__device__ inline uint32_t bucket_of(const Work& w, uint32_t row) { return row & ((1u << w.bucket_bits) - 1); }
+__device__ inline uint32_t bin_of(const Work& w, uint32_t row) { return row >> w.bucket_bits; }
+__device__ inline int64_t row_of(const Work& w, int64_t bucket, int64_t bin) { return (bin << w.bucket_bits) + bucket; }
+
 __host__ inline size_t lay_out(Work& w, void* mem, int64_t n, int dim, int64_t num_rows) {
     w.chunks = (n + kChunk - 1) / kChunk;
-    w.windows = (n + kPiece - 1) / kPiece;
+    w.piece = n * dim >= kManySums ? 16 : 8;
+    w.windows = (n + w.piece - 1) / w.piece;
     w.width = (dim + 7) & ~7;
     w.bucket_bits = kMinBucketBits;
     while (w.bucket_bits < kMaxBucketBits && num_rows > (int64_t)kBins << w.bucket_bits) w.bucket_bits++;
     const int64_t buckets = 1 << w.bucket_bits;
-    w.words = (int)(((num_rows + buckets - 1) / buckets + 63) / 64);
     size_t at = 0;
     auto take = [&](auto*& p, int64_t count) {
         p = (std::remove_reference_t<decltype(p)>)((char*)mem + at);
         at += (count * sizeof(*p) + 255) / 256 * 256;
     };
-    take(w.total, 1);
+    take(w.total, 3);
     take(w.placed, w.chunks * kChunk);
     take(w.starts, w.chunks * (buckets + 1));
     take(w.tokens, n);
-    take(w.present, buckets * w.words);
+    take(w.common, 2 * (n / w.piece));
     take(w.part, w.windows * 2 * w.width);
     return at;
 }
@@ -108,13 +117,14 @@ __device__ inline unsigned long long same_key(unsigned long long in, uint32_t ke
 }
 
 // Exclusive sums over the workgroup's threads of one value each, behind `before`; *all: the sum of all.
+template <int kWaves>
 __device__ inline uint32_t group_scan(uint32_t v, uint32_t before, uint32_t* s_wave, uint32_t* all) {
     const uint32_t upto = wave_scan_u32(v);
     __syncthreads();
     if (lane_id() == kWave - 1) s_wave[threadIdx.x / kWave] = upto;
     __syncthreads();
     uint32_t start = before + upto - v, sum = 0;
-    for (int w = 0; w < kGroupWaves; w++) {
+    for (int w = 0; w < kWaves; w++) {
         if (w < (int)threadIdx.x / kWave) start += s_wave[w];
         sum += s_wave[w];
     }
@@ -122,8 +132,7 @@ __device__ inline uint32_t group_scan(uint32_t v, uint32_t before, uint32_t* s_w
     return start;
 }
 
-// Grouping, first half.  Bucket b holds the rows r with r mod buckets = b (neighbouring rows, often alike in
-// their number of tokens, go to different ones).  A workgroup puts a chunk of the tokens in order
+// Grouping, first half.  A workgroup puts a chunk of the tokens in order
 // of their buckets, those of a bucket in their own order: a wavefront takes a run of them, counts
 // them by buckets as it goes, and the counts of the wavefronts before it give its places.
 __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, bool wide, int64_t n, int64_t num_rows, Work w) {
@@ -145,7 +154,7 @@ __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, b
     for (int j = 0; j < kPerLane; j++) {
         const bool real = id[j] >= 0 && id[j] < num_rows;
         if (!real) id[j] = -1;
-        const uint32_t bucket = (uint32_t)id[j] & (buckets - 1);
+        const uint32_t bucket = bucket_of(w, (uint32_t)id[j]);
         const unsigned long long same = same_key(__ballot(real), bucket, w.bucket_bits);
         if (real) {
             const uint32_t have = mine[bucket];
@@ -161,7 +170,7 @@ __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, b
         uint32_t len = 0, all;
         if (b < buckets)
             for (int v = 0; v < kGroupWaves; v++) len += s_count[v * buckets + b];
-        uint32_t start = group_scan(len, before, s_wave, &all);
+        uint32_t start = group_scan<kGroupWaves>(len, before, s_wave, &all);
         if (b < buckets) {
             starts[b] = (uint16_t)start;
             for (int v = 0; v < kGroupWaves; v++) {
@@ -172,113 +181,41 @@ __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, b
         }
         before += all;
     }
+    if (tid == 0 && blockIdx.x == 0) w.total[1] = w.total[2] = 0;
     if (tid == 0) starts[buckets] = (uint16_t)before;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPerLane; j++) {
         if (id[j] < 0) continue;
-        const uint32_t at = mine[(uint32_t)id[j] & (buckets - 1)] + rank[j];
+        const uint32_t at = mine[bucket_of(w, (uint32_t)id[j])] + rank[j];
         w.placed[base + at] = Placed{(uint32_t)id[j], (uint32_t)(base + (wave * kPerLane + j) * kWave + lane)};
     }
 }
 
-// Calls f(token, whether it is one) for a bucket's tokens in chunks [from, to), in order, by whole wavefronts.
+// Calls f(token, whether it is one) for a bucket's tokens in up to 64 chunks from `chunk` on, in order, by whole
+// wavefronts; a lane has the bounds [o0, o1) in one chunk.  The tokens are taken as one sequence, 64 at a
+// time whatever their chunks hold (by chunks, the commonest row of 65536 tokens of text cost 16 us, twice as much).
 template <class F>
-__device__ inline void for_tokens(const Work& w, int bucket, int64_t from, int64_t to, F f) {
-    const int lane = lane_id(), row = (1 << w.bucket_bits) + 1;
-    for (int64_t c0 = from; c0 < to; c0 += kWave) {
-        uint32_t o0 = 0, o1 = 0;
-        if (c0 + lane < to) {
-            o0 = w.starts[(c0 + lane) * row + bucket];
-            o1 = w.starts[(c0 + lane) * row + bucket + 1];
-        }
-        const int many = (int)min((int64_t)kWave, to - c0);
-        constexpr int kAhead = 4;
-        for (int j0 = 0; j0 < many; j0 += kAhead) {
-            Placed p[kAhead];
-            int first[kAhead], last[kAhead];
+__device__ inline void for_tokens(const Work& w, int64_t chunk, uint32_t o0, uint32_t o1, F f) {
+    constexpr int kAhead = 4;
+    const uint32_t upto = wave_scan_u32(o1 - o0), total = (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+    const uint32_t mine = upto - (o1 - o0);          // tokens in the lanes before
+    for (uint32_t t = 0; t < total; t += kAhead * kWave) {
+        Placed p[kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; j++) {
-                const int from_lane = min(j0 + j, many - 1);
-                first[j] = __builtin_amdgcn_readlane((int)o0, from_lane);
-                last[j] = j0 + j < many ? __builtin_amdgcn_readlane((int)o1, from_lane) : first[j];
-                p[j] = Placed{0, 0};
-                if (first[j] + lane < last[j]) p[j] = w.placed[(c0 + j0 + j) * kChunk + first[j] + lane];
-            }
+        for (int j = 0; j < kAhead; j++) {
+            const uint32_t at = t + j * kWave + lane_id();
+            int lane = 0;                            // the last one that starts at or before `at`: the one that holds it
 #pragma unroll
-            for (int j = 0; j < kAhead; j++) {
-                if (first[j] < last[j]) f(p[j], first[j] + lane < last[j]);
-                for (int t = first[j] + kWave; t < last[j]; t += kWave) {
-                    const bool real = t + lane < last[j];
-                    f(real ? w.placed[(c0 + j0 + j) * kChunk + t + lane] : Placed{0, 0}, real);
-                }
-            }
+            for (int step = kWave / 2; step; step /= 2)
+                if ((uint32_t)__shfl((int)mine, lane + step) <= at) lane += step;
+            const uint32_t first = (uint32_t)__shfl((int)o0, lane), before = (uint32_t)__shfl((int)mine, lane);
+            p[j] = Placed{0, 0};
+            if (at < total) p[j] = w.placed[(chunk + lane) * kChunk + first + (at - before)];
         }
-    }
-}
-
-// Second half: a workgroup takes a bucket, its wavefronts runs of the chunks.  What the chunks hold of the
-// buckets before it is where its part of the order starts; its rows are counted up to kBins at a time.
-__global__ __launch_bounds__(kGroupThreads) void bucket_kernel(int64_t num_rows, Work w) {
-    __shared__ uint32_t s_count[kGroupWaves][kBins];
-    __shared__ uint32_t s_start[kBins], s_len[kBins];
-    __shared__ uint32_t s_wave[kGroupWaves], s_before[kGroupWaves], s_total[kGroupWaves];
-    const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), bucket = blockIdx.x, buckets = 1 << w.bucket_bits;
-    const int64_t run = (w.chunks + kGroupWaves - 1) / kGroupWaves, from = min(w.chunks, wave * run), to = min(w.chunks, from + run);
-    uint32_t before = 0, total = 0;
-    for (int64_t c = from + lane; c < to; c += kWave) {
-        before += w.starts[c * (buckets + 1) + bucket];
-        total += w.starts[c * (buckets + 1) + buckets];
-    }
-    before = wave_sum_u32(before);
-    total = wave_sum_u32(total);
-    if (lane == 0) {
-        s_before[wave] = before;
-        s_total[wave] = total;
-    }
-    __syncthreads();
-    before = total = 0;
-    for (int v = 0; v < kGroupWaves; v++) {
-        before += s_before[v];
-        total += s_total[v];
-    }
-    if (bucket == 0 && tid == 0) *w.total = total;
-    const int64_t rows = (num_rows - bucket + buckets - 1) >> w.bucket_bits;       // of this bucket
-    for (int64_t bin0 = 0; bin0 < rows; bin0 += kBins) {
-        for (int i = tid; i < kGroupWaves * kBins; i += kGroupThreads) (&s_count[0][0])[i] = 0;
-        __syncthreads();
-        for_tokens(w, bucket, from, to, [&](Placed p, bool real) {
-            const uint32_t bin = (p.row >> w.bucket_bits) - (uint32_t)bin0;
-            if (real && bin < kBins) atomicAdd(&s_count[wave][bin], 1u);
-        });
-        __syncthreads();
-        for (int b0 = 0; b0 < kBins; b0 += kGroupThreads) {
-            const int b = b0 + tid;
-            uint32_t len = 0, all;
-            for (int v = 0; v < kGroupWaves; v++) {
-                const uint32_t c = s_count[v][b];
-                s_count[v][b] = len;
-                len += c;
-            }
-            s_start[b] = group_scan(len, before, s_wave, &all);
-            s_len[b] = len;
-            before += all;
-            const unsigned long long have = __ballot(len != 0);
-            const int64_t word = (bin0 + b) / kWave;
-            if (lane == 0 && word < w.words) w.present[(int64_t)bucket * w.words + word] = have;
-        }
-        __syncthreads();
-        for_tokens(w, bucket, from, to, [&](Placed p, bool real) {
-            const uint32_t bin = (p.row >> w.bucket_bits) - (uint32_t)bin0;
-            const bool mine = real && bin < kBins;
-            const unsigned long long same = same_key(__ballot(mine), bin, 10);       // 2^10 = kBins
-            if (mine) {
-                const uint32_t rank = s_count[wave][bin] + lanes_below(same);
-                if (lanes_below(same) == 0) s_count[wave][bin] = rank + __popcll(same);
-                w.tokens[s_start[bin] + rank] = Token{p.row, p.at, rank, s_len[bin]};
-            }
-        });
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (t + j * kWave < total) f(p[j], t + j * kWave + lane_id() < total);
     }
 }
 
@@ -301,7 +238,7 @@ __device__ inline void put_sums(const EmbedArgs& a, uint32_t row, int c, const f
 #pragma unroll
                 for (int k = 0; k < kStep; k++) y[k] = sum[j + k] * a.scale;
             }
-            P::store(out + c + j, P::pack(y));
+            P::store_once(out + c + j, P::pack(y));
         }
         return;
     }
@@ -320,38 +257,116 @@ __device__ inline void put_zeros(const EmbedArgs& a, int64_t row, int c) {
     const u32x4 none = {0, 0, 0, 0};
     if (c + N <= a.dim) {
 #pragma unroll
-        for (int j = 0; j < N; j += P::kLen) P::store(out + c + j, none);
+        for (int j = 0; j < N; j += P::kLen) P::store_once(out + c + j, none);
     } else {
         for (int k = c; k < a.dim; k++) out[k] = (typename O::raw)0.f;
     }
 }
 
-// `lanes` (a power of two up to 64) neighbouring lanes take one window of kPiece tokens in one slice of
-// the columns: they sum the pieces that START in the window, up to kPiece tokens of one row each.
-// Rows of up to kPiece tokens are one piece and final; the first piece of a longer one goes to
+// Second half of the grouping: a workgroup takes a bucket.  What the chunks hold of the buckets before it
+// is where its part of the order starts.  Half of its wavefronts read the bucket's tokens, in runs of the chunks, once to
+// count them by rows (up to kBins at a time) and once to put them into their places; the other half
+// meanwhile writes the rows without tokens, whose bytes hide the waits of the first.
+template <class O>
+__global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, Work w, int lanes) {
+    constexpr int kAllWaves = 2 * kGroupWaves;
+    __shared__ uint32_t s_count[kGroupWaves][kBins];
+    __shared__ uint32_t s_start[kBins], s_len[kBins];
+    __shared__ uint32_t s_wave[kAllWaves], s_before[kGroupWaves], s_total[kGroupWaves];
+    static_assert(kBins == 2 * kGroupThreads, "a thread per row");
+    const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), bucket = blockIdx.x, buckets = 1 << w.bucket_bits;
+    const bool reads = wave < kGroupWaves;
+    const int64_t run = (w.chunks + kGroupWaves - 1) / kGroupWaves;
+    const int64_t from = reads ? min(w.chunks, wave * run) : 0, to = reads ? min(w.chunks, from + run) : 0;
+    uint32_t before = 0, total = 0, o0 = 0, o1 = 0;
+    auto bounds = [&](int64_t c) {
+        o0 = c < to ? w.starts[c * (buckets + 1) + bucket] : 0;
+        o1 = c < to ? w.starts[c * (buckets + 1) + bucket + 1] : 0;
+    };
+    auto each_token = [&](auto f) {
+        for (int64_t c = from; c < to; c += kWave) {
+            if (run > kWave) bounds(c + lane);
+            for_tokens(w, c, o0, o1, f);
+        }
+    };
+    for (int64_t c = from + lane; c - lane < to; c += kWave) {
+        bounds(c);
+        before += o0;
+        if (bucket == 0 && c < to) total += w.starts[c * (buckets + 1) + buckets];
+    }
+    before = wave_sum_u32(before);
+    total = wave_sum_u32(total);
+    if (reads && lane == 0) {
+        s_before[wave] = before;
+        s_total[wave] = total;
+    }
+    __syncthreads();
+    before = total = 0;
+    for (int v = 0; v < kGroupWaves; v++) {
+        before += s_before[v];
+        total += s_total[v];
+    }
+    if (bucket == 0 && tid == 0) w.total[0] = total;
+    const int64_t rows = (a.num_rows - bucket + buckets - 1) >> w.bucket_bits;       // of this bucket
+    for (int64_t bin0 = 0; bin0 < rows; bin0 += kBins) {
+        for (int i = tid; i < kGroupWaves * kBins; i += 2 * kGroupThreads) (&s_count[0][0])[i] = 0;
+        __syncthreads();
+        each_token([&](Placed p, bool real) {
+            const uint32_t bin = bin_of(w, p.row) - (uint32_t)bin0;
+            if (real && bin < kBins) atomicAdd(&s_count[wave][bin], 1u);
+        });
+        __syncthreads();
+        uint32_t len = 0, all;
+        for (int v = 0; v < kGroupWaves; v++) {
+            const uint32_t c = s_count[v][tid];
+            s_count[v][tid] = len;
+            len += c;
+        }
+        const uint32_t start = group_scan<kAllWaves>(len, before, s_wave, &all);
+        before += all;
+        s_start[tid] = start;
+        s_len[tid] = len;
+        if (len > (uint32_t)w.piece) {      // (in any order)
+            const int wide = len > (uint32_t)(w.piece * kWide);
+            w.common[wide * (a.n / w.piece) + atomicAdd(&w.total[1 + wide], 1u)] = start;
+        }
+        __syncthreads();
+        if (reads) {
+            each_token([&](Placed p, bool real) {
+                const uint32_t bin = bin_of(w, p.row) - (uint32_t)bin0;
+                const bool mine = real && bin < kBins;
+                const unsigned long long same = same_key(__ballot(mine), bin, 10);       // 2^10 = kBins
+                if (mine) {
+                    const uint32_t rank = s_count[wave][bin] + lanes_below(same);
+                    if (lanes_below(same) == 0) s_count[wave][bin] = rank + __popcll(same);
+                    w.tokens[s_start[bin] + rank] = Token{p.row, p.at, rank, s_len[bin]};
+                }
+            });
+        } else if (!a.accumulate) {
+            const int64_t many = min((int64_t)kBins, rows - bin0);
+            const int id = tid - kGroupThreads;
+            for (int64_t r = id / lanes; r < many; r += kGroupThreads / lanes) {
+                if (s_len[r]) continue;
+                for (int c = id % lanes * Piece<O>::kLen; c < a.dim; c += lanes * Piece<O>::kLen)
+                    put_zeros<O, Piece<O>::kLen>(a, row_of(w, bucket, bin0 + r), c);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// `lanes` (a power of two up to 64) neighbouring lanes take one window of w.piece tokens in one slice of
+// the columns: they sum the pieces that START in the window, up to as many tokens of one row each.
+// Rows of up to w.piece tokens are one piece and final; the first piece of a longer one goes to
 // place 2 w + 1 of `part`, a later one to 2 w (a window w has at most one of each).
-//
-// Behind the windows' groups come those that write the rows without tokens: one takes the 64 rows
-// of a word of `present` in one slice.  Every row is written once, and these writes fill the gaps of the reads.
 template <class T, class O>
 __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int lanes, int slices, int64_t first) {
     using P = Piece<T>;
     constexpr int kAhead = 8;
     const int64_t unit = first + (int64_t)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
     const int64_t window = unit / slices, total = *w.total;
-    if (window >= w.windows) {
-        const int64_t word = window - w.windows;
-        const int c = ((int)(unit % slices) * lanes + threadIdx.x % lanes) * P::kLen;
-        if (a.accumulate || word >= (int64_t)w.words << w.bucket_bits || c >= a.dim) return;
-        const int64_t row0 = (word % w.words * 64 << w.bucket_bits) + word / w.words;
-        for (unsigned long long left = ~w.present[word]; left; left &= left - 1) {
-            const int64_t row = row0 + ((int64_t)__builtin_ctzll(left) << w.bucket_bits);
-            if (row >= a.num_rows) break;
-            put_zeros<O, P::kLen>(a, row, c);
-        }
-        return;
-    }
-    const int64_t begin = window * kPiece, end = min(total, begin + kPiece);
+    const int piece = w.piece;
+    const int64_t begin = window * piece, end = min(total, begin + piece);
     if (begin >= end) return;
     const int c = ((int)(unit % slices) * lanes + threadIdx.x % lanes) * P::kLen;
     if (c >= a.dim) return;
@@ -360,9 +375,9 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
     // the end of the piece of the window's last token
     const Token e0 = w.tokens[begin], e1 = w.tokens[end - 1];
     int64_t t = begin;
-    if (e0.rank % kPiece) t += min(kPiece - e0.rank % kPiece, e0.count - e0.rank);
+    if (e0.rank & (piece - 1)) t += min(piece - (e0.rank & (piece - 1)), e0.count - e0.rank);
     if (t >= end) return;
-    const int64_t stop = end - 1 + min(kPiece - e1.rank % kPiece, e1.count - e1.rank);
+    const int64_t stop = end - 1 + min(piece - (e1.rank & (piece - 1)), e1.count - e1.rank);
     float sum[P::kLen];
 #pragma unroll
     for (int k = 0; k < P::kLen; k++) sum[k] = 0.f;
@@ -374,7 +389,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const typename T::raw* row = (const typename T::raw*)a.rows + (int64_t)e[j].at * a.stride;
-            x[j] = whole ? P::load(row + c) : P::load_part(row, c, a.dim, 0.f);
+            x[j] = whole ? P::load_once(row + c) : P::load_part(row, c, a.dim, 0.f);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
@@ -383,12 +398,12 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
             P::unpack(x[j], y);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) sum[k] += y[k];
-            if (e[j].rank + 1 < e[j].count && (e[j].rank + 1) % kPiece) continue;
-            if (e[j].count <= kPiece) {
+            if (e[j].rank + 1 < e[j].count && (e[j].rank + 1) & (piece - 1)) continue;
+            if (e[j].count <= (uint32_t)piece) {
                 put_sums<O, P::kLen>(a, e[j].row, c, sum);
             } else {
-                const int64_t began = t + j - e[j].rank % kPiece;
-                float* part = w.part + (2 * (began / kPiece) + (e[j].rank < kPiece)) * w.width + c;
+                const int64_t began = t + j - (e[j].rank & (piece - 1));
+                float* part = w.part + (2 * (began / (uint32_t)piece) + (e[j].rank < (uint32_t)piece)) * w.width + c;
 #pragma unroll
                 for (int k = 0; k < P::kLen; k += 4)
                     *reinterpret_cast<float4*>(part + k) = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
@@ -399,50 +414,177 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
     }
 }
 
-// Rows of more than kPiece tokens: a workgroup looks for them among 256 tokens, and its wavefronts
-// add the pieces of each, every fourth one, in 256 columns.
-template <class O>
-__global__ __launch_bounds__(kThreads) void join_kernel(EmbedArgs a, Work w, int slices, int64_t first) {
-    constexpr int kWaves = kThreads / kWave;
-    __shared__ float s_sum[kWaves][kWave * 4];
-    __shared__ int s_found[kThreads / kPiece + 1];
-    __shared__ int s_n;
-    const int64_t unit = first + blockIdx.x, total = *w.total;
-    const int64_t base = unit / slices * kThreads;
-    if (base >= total) return;
-    const int c = (int)(unit % slices) * kWave * 4 + lane_id() * 4;
-    const int tid = threadIdx.x, wave = tid / kWave;
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    if (base + tid < total) {
-        const Token e = w.tokens[base + tid];
-        if (e.rank == 0 && e.count > kPiece) s_found[atomicAdd(&s_n, 1)] = tid;      // (in any order)
+// Rows of more tokens than a piece.  Up to kWide pieces: a thread adds the pieces of one in four columns.
+// More: sixteen groups of 16 lanes add every sixteenth piece of one in 64 columns.  (Sixteen groups for all
+// of them: 17 us for the 400 such rows of 65536 tokens of text, nearly all of it the waits of many small workgroups.)
+template <class O, bool kIsWide>
+__device__ void join_row(const EmbedArgs& a, const Work& w, uint32_t at, int slice, float4 (*s_sum)[16]) {
+    constexpr int kLanes = kIsWide ? 16 : kThreads, kGroups = kThreads / kLanes, kAhead = 8;
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, c = (slice * kLanes + lane) * 4;
+    const uint32_t window = at / (uint32_t)w.piece;
+    const Token e = w.tokens[at];
+    const int pieces = (int)((e.count + w.piece - 1) / (uint32_t)w.piece);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.dim) {
+        for (int p0 = group; p0 < pieces; p0 += kGroups * kAhead) {
+            float4 x[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                const int p = min(p0 + j * kGroups, pieces - 1);
+                x[j] = *reinterpret_cast<const float4*>(w.part + (2 * ((int64_t)window + p) + (p == 0)) * w.width + c);
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                if (p0 + j * kGroups >= pieces) break;
+                sum.x += x[j].x; sum.y += x[j].y; sum.z += x[j].z; sum.w += x[j].w;
+            }
+        }
     }
-    __syncthreads();
-    for (int f = 0; f < s_n; f++) {
-        const int64_t at = base + s_found[f], window = at / kPiece;
-        const Token e = w.tokens[at];
-        const int pieces = (int)((e.count + kPiece - 1) / kPiece);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < a.dim) {
-#pragma unroll 4
-            for (int p = wave; p < pieces; p += kWaves) {
-                const float4 x = *reinterpret_cast<const float4*>(w.part + (2 * (window + p) + (p == 0)) * w.width + c);
+    if (kIsWide) {
+        s_sum[group][lane % 16] = sum;
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int v = 1; v < kGroups; v++) {
+                const float4 x = s_sum[v][lane % 16];
                 sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
             }
         }
-        *reinterpret_cast<float4*>(&s_sum[wave][lane_id() * 4]) = sum;
-        __syncthreads();
-        if (wave == 0 && c < a.dim) {
-            float y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int v = 0; v < kWaves; v++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) y[k] += s_sum[v][lane_id() * 4 + k];
-            put_sums<O, 4>(a, e.row, c, y);
-        }
         __syncthreads();
     }
+    if (group == 0 && c < a.dim) {
+        const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+        put_sums<O, 4>(a, e.row, c, y);
+    }
+}
+template <class O>
+__global__ __launch_bounds__(kThreads) void join_kernel(EmbedArgs a, Work w, int wide_groups, int groups) {
+    __shared__ float4 s_sum[16][16];
+    int block = blockIdx.x;
+    const int wide_slices = (a.dim + 63) / 64, slices = (a.dim + kThreads * 4 - 1) / (kThreads * 4);
+    if (block < wide_groups * wide_slices) {
+        const uint32_t many = w.total[2];
+        for (uint32_t f = block / wide_slices; f < many; f += wide_groups)
+            join_row<O, true>(a, w, w.common[a.n / w.piece + f], block % wide_slices, s_sum);
+        return;
+    }
+    block -= wide_groups * wide_slices;
+    const uint32_t many = w.total[1];
+    for (uint32_t f = block / slices; f < many; f += groups)
+        join_row<O, false>(a, w, w.common[f], block % slices, s_sum);
+}
+
+// ---- few tokens --------------------------------------------------------------------------
+constexpr int kFew = 2048, kFewLanes = kFew / kGroupThreads;
+constexpr int kFewRows = 256;        // rows of a workgroup at most
+
+// Up to kFew tokens by one launch: a workgroup reads all ids, puts the tokens of its `rows` rows in
+// order of (row, place) in LDS and sums them in one slice of the columns.  `lanes` lanes are a group; each takes
+// the same share of the tokens, and the sum of a row that reaches over several shares is put together
+// by the group it starts in.
+template <class T, class O>
+__global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int rows, int lanes, int64_t first) {
+    using P = Piece<T>;
+    constexpr int kAhead = 8;
+    __shared__ uint32_t s_count[kGroupWaves * kFewRows], s_wave[kGroupWaves], s_start[kFewRows + 1];
+    __shared__ uint32_t s_token[kFew];                              // bin << 16 | place among all tokens
+    __shared__ float s_head[kGroupThreads * P::kLen];
+    const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+    const int64_t row0 = (first + blockIdx.x) * rows;
+    const int n = (int)a.n;
+    int bin[kFewLanes], rank[kFewLanes];
+#pragma unroll
+    for (int j = 0; j < kFewLanes; j++) {
+        const int i = (wave * kFewLanes + j) * kWave + lane;
+        const int64_t id = i < n ? id_at(a.ids, a.wide_ids, i) : -1;
+        bin[j] = id >= row0 && id < min(a.num_rows, row0 + rows) ? (int)(id - row0) : -1;
+    }
+    for (int i = tid; i < kGroupWaves * kFewRows; i += kGroupThreads) s_count[i] = 0;
+    __syncthreads();
+    uint32_t* mine = s_count + wave * kFewRows;
+#pragma unroll
+    for (int j = 0; j < kFewLanes; j++) {
+        const unsigned long long here = __ballot(bin[j] >= 0);
+        if (!here) continue;
+        const unsigned long long same = same_key(here, (uint32_t)bin[j], 8);         // 2^8 = kFewRows
+        if (bin[j] >= 0) {
+            const uint32_t have = mine[bin[j]];
+            rank[j] = have + lanes_below(same);
+            if (lanes_below(same) == 0) mine[bin[j]] = have + __popcll(same);
+        }
+    }
+    __syncthreads();
+    uint32_t len = 0, all;
+    if (tid < kFewRows)
+        for (int v = 0; v < kGroupWaves; v++) len += s_count[v * kFewRows + tid];
+    uint32_t start = group_scan<kGroupWaves>(len, 0, s_wave, &all);
+    if (tid < kFewRows) {
+        s_start[tid] = start;
+        for (int v = 0; v < kGroupWaves; v++) {
+            const uint32_t c = s_count[v * kFewRows + tid];
+            s_count[v * kFewRows + tid] = start;
+            start += c;
+        }
+        if (tid == kFewRows - 1) s_start[kFewRows] = start;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kFewLanes; j++)
+        if (bin[j] >= 0) s_token[mine[bin[j]] + rank[j]] = (uint32_t)bin[j] << 16 | (uint32_t)((wave * kFewLanes + j) * kWave + lane);
+    __syncthreads();
+    const int group = tid / lanes, groups = kGroupThreads / lanes, c = ((int)blockIdx.y * lanes + tid % lanes) * P::kLen;
+    const bool in = c < a.dim, whole = c + P::kLen <= a.dim;
+    // rows without tokens
+    if (in && !a.accumulate)
+        for (int r = group; r < rows && row0 + r < a.num_rows; r += groups)
+            if (s_start[r] == s_start[r + 1]) put_zeros<O, P::kLen>(a, row0 + r, c);
+    const int share = ((int)all + groups - 1) / groups;
+    const int from = min((int)all, group * share), to = min((int)all, from + share);
+    float sum[P::kLen];
+#pragma unroll
+    for (int k = 0; k < P::kLen; k++) sum[k] = 0.f;
+    for (int t = from; t < to; t += kAhead) {
+        uint32_t e[kAhead];
+        u32x4 x[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) e[j] = s_token[min(t + j, to - 1)];
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const typename T::raw* row = (const typename T::raw*)a.rows + (int64_t)(e[j] & 0xffff) * a.stride;
+            x[j] = u32x4{0, 0, 0, 0};
+            if (whole) x[j] = P::load(row + c);
+            else if (in) x[j] = P::load_part(row, c, a.dim, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            if (t + j >= to) break;
+            float y[P::kLen];
+            P::unpack(x[j], y);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) sum[k] += y[k];
+            const int r = (int)(e[j] >> 16), last = (int)s_start[r + 1] - 1;
+            if (t + j < last && t + j + 1 < to) continue;
+            // the row ends here, or the share
+            if ((int)s_start[r] < from) {
+#pragma unroll
+                for (int k = 0; k < P::kLen; k++) s_head[tid * P::kLen + k] = sum[k];
+            } else if (t + j == last) {
+                if (in) put_sums<O, P::kLen>(a, (uint32_t)(row0 + r), c, sum);
+            } else {
+                continue;                                          // the others' parts are to come
+            }
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) sum[k] = 0.f;
+        }
+    }
+    __syncthreads();
+    if (from >= to || !in) return;
+    const int r = (int)(s_token[to - 1] >> 16), end = (int)s_start[r + 1];
+    if ((int)s_start[r] < from || end <= to) return;
+    for (int g = group + 1; g * share < end; g++)
+#pragma unroll
+        for (int k = 0; k < P::kLen; k++) sum[k] += s_head[(g * lanes + tid % lanes) * P::kLen + k];
+    put_sums<O, P::kLen>(a, (uint32_t)(row0 + r), c, sum);
 }
 
 constexpr int64_t kMaxGrid = 1 << 22;     // workgroups of one launch (their threads are counted in 32 bits)
@@ -476,32 +618,42 @@ int room_for_counts() {
 }
 
 template <class T, class O>
-int grad(const EmbedArgs& a, hipStream_t s) {
-    Work w;
-    lay_out(w, a.work, a.n, a.dim, a.num_rows);
-    if (a.n) {
-        if (int rc = room_for_counts()) return rc;
-        chunk_kernel<<<(uint32_t)w.chunks, kGroupThreads, kGroupWaves * sizeof(uint32_t) << w.bucket_bits, s>>>(a.ids, a.wide_ids, a.n, a.num_rows, w);
+int grad_of_few(const EmbedArgs& a, hipStream_t s) {
+    const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, kWave);
+    // 512 workgroups fill the device
+    const int rows = (int)std::min<int64_t>(kFewRows, std::max<int64_t>(8, (a.num_rows + 511) / 512));
+    const int64_t blocks = (a.num_rows + rows - 1) / rows, slices = (pieces + lanes - 1) / lanes;
+    const int64_t most = std::max<int64_t>(1, kMaxGrid / slices);
+    for (int64_t first = 0; first < blocks; first += most) {
+        few_kernel<T, O><<<dim3((uint32_t)std::min(most, blocks - first), (uint32_t)slices), kGroupThreads, 0, s>>>(a, rows, lanes, first);
         DCIH_HIP(hipGetLastError());
     }
-    bucket_kernel<<<1u << w.bucket_bits, kGroupThreads, 0, s>>>(a.num_rows, w);
+    return 0;
+}
+
+template <class T, class O>
+int grad(const EmbedArgs& a, hipStream_t s) {
+    if (a.n <= kFew) return grad_of_few<T, O>(a, s);
+    Work w;
+    lay_out(w, a.work, a.n, a.dim, a.num_rows);
+    if (int rc = room_for_counts()) return rc;
+    chunk_kernel<<<(uint32_t)w.chunks, kGroupThreads, kGroupWaves * sizeof(uint32_t) << w.bucket_bits, s>>>(a.ids, a.wide_ids, a.n, a.num_rows, w);
+    DCIH_HIP(hipGetLastError());
+    bucket_kernel<O><<<1u << w.bucket_bits, 2 * kGroupThreads, 0, s>>>(a, w, lanes_for((a.dim + Piece<O>::kLen - 1) / Piece<O>::kLen, kWave));
     DCIH_HIP(hipGetLastError());
     const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, kWave);
-    int slices = (pieces + lanes - 1) / lanes;
-    const int per = kThreads / lanes;
-    int64_t units = (w.windows + (a.accumulate ? 0 : (int64_t)w.words << w.bucket_bits)) * slices;
+    const int slices = (pieces + lanes - 1) / lanes, per = kThreads / lanes;
+    const int64_t units = w.windows * slices;
     for (int64_t first = 0; first < units; first += kMaxGrid * per) {
         const int64_t groups = std::min(kMaxGrid, (units - first + per - 1) / per);
         sum_kernel<T, O><<<(uint32_t)groups, kThreads, 0, s>>>(a, w, lanes, slices, first);
         DCIH_HIP(hipGetLastError());
     }
-    if (a.n <= kPiece) return 0;
-    slices = (a.dim + kWave * 4 - 1) / (kWave * 4);
-    units = (a.n + kThreads - 1) / kThreads * slices;
-    for (int64_t first = 0; first < units; first += kMaxGrid) {
-        join_kernel<O><<<(uint32_t)std::min(kMaxGrid, units - first), kThreads, 0, s>>>(a, w, slices, first);
-        DCIH_HIP(hipGetLastError());
-    }
+    // groups of workgroups that fill the device, no more than there can be such rows
+    const int wide = (int)std::min<int64_t>(a.n / (w.piece * kWide + 1), 64), groups = (int)std::min<int64_t>(a.n / (w.piece + 1), 1024);
+    const int64_t blocks = (int64_t)wide * ((a.dim + 63) / 64) + (int64_t)groups * ((a.dim + kThreads * 4 - 1) / (kThreads * 4));
+    join_kernel<O><<<(uint32_t)blocks, kThreads, 0, s>>>(a, w, wide, groups);
+    DCIH_HIP(hipGetLastError());
     return 0;
 }
 
@@ -517,7 +669,7 @@ int embed_rows(const EmbedArgs& a, int dtype, hipStream_t s) {
 
 size_t embed_grad_bytes(int64_t n, int dim, int64_t num_rows) {
     Work w;
-    return lay_out(w, nullptr, n, dim, num_rows);
+    return n <= kFew ? 16 : lay_out(w, nullptr, n, dim, num_rows);
 }
 
 int embed_grad(const EmbedArgs& a, int dtype, int out_dtype, hipStream_t s) {

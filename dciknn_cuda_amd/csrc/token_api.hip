@@ -98,7 +98,7 @@ extern "C" {
 int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_t row_stride, const void* d_ids,
                int id_bytes, int64_t num_ids, float scale, void* d_out, void* stream) {
     const char* who = "dcih_embed";
-    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
+    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
         return refuse(who, "bad size");
     if (const char* why = check_array(d_table, dtype)) return refuse(who, why);
     if (!num_ids) return DCIH_OK;
@@ -118,7 +118,7 @@ int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_
 }
 
 int64_t dcih_embed_grad_work(int64_t num_ids, int dim, int64_t num_rows) {
-    if (num_ids < 0 || num_ids > kMaxCount || dim <= 0 || num_rows <= 0 || num_rows > kMaxCount) return refuse("dcih_embed_grad_work", "bad size");
+    if (num_ids < 0 || num_ids > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || num_rows <= 0 || num_rows > kMaxCount) return refuse("dcih_embed_grad_work", "bad size");
     return (int64_t)embed_grad_bytes(num_ids, dim, num_rows);
 }
 
@@ -126,7 +126,7 @@ int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int
                     int id_bytes, int64_t num_rows, float scale, int accumulate, void* d_out, int out_dtype,
                     void* d_work, int64_t work_bytes, void* stream) {
     const char* who = "dcih_embed_grad";
-    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
+    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
         return refuse(who, "bad size");
     if (const char* why = check_array(d_out, out_dtype)) return refuse(who, why);
     if (out_dtype != dtype && out_dtype != DCIH_F32) return refuse(who, "sums are of the gradient's type or of 32 bits");

@@ -115,7 +115,7 @@ bool wants_grad(const Tensor& t) { return torch::GradMode::is_enabled() && t.req
 Tensor embed_forward(const Tensor& table, const Tensor& ids_in, double scale) {
     const int dtype = type_code(table, "table");
     if (table.dim() != 2 || table.size(0) < 1 || table.size(1) < 1) bad_value("table must be [rows, dim]");
-    if (table.size(1) > 0x7fffffff || table.size(0) > 0x7fffffff) bad_value("table is too large");
+    if (table.size(1) > DCIH_MAX_DIM || table.size(0) > 0x7fffffff) bad_value("table is too large");
     const Rows r = rows_of(table, "table");
     const Tensor ids = ids_of(ids_in, table, "ids");
     if (ids.numel() > 0x7fffffff) bad_value("too many ids");
@@ -131,7 +131,8 @@ Tensor embed_grad(const Tensor& grad, const Tensor& ids_in, int64_t num_rows, do
     const Rows r = rows_of(grad, "grad");
     const Tensor ids = ids_of(ids_in, grad, "ids");
     if (leading(grad) != ids.sizes()) bad_value("grad must have one row for each id");
-    if (num_rows < 1 || num_rows > 0x7fffffff) bad_value("num_rows must be positive");
+    if (num_rows < 1 || num_rows > 0x7fffffff) bad_value("num_rows must be positive and below 2**31");
+    if (r.len > DCIH_MAX_DIM) bad_value("grad has rows that are too long");
     Tensor out;
     if (into) {
         out = *into;

@@ -335,7 +335,8 @@ int dcih_segsort(const float* d_keys, int num_indices, int64_t num_points,
  * NaN, as said with each operator.  Counts of rows and ids are below 2^31.
  */
 enum { DCIH_F32 = 0, DCIH_F16 = 1, DCIH_BF16 = 2 };
-#define DCIH_MAX_VOCAB (1 << 28)
+#define DCIH_MAX_VOCAB (1 << 28)   /* entries of a row of logits */
+#define DCIH_MAX_DIM (1 << 20)     /* elements of a row of a table */
 
 /*
  * d_out[i] = scale * d_table[ids[i]], contiguous rows of the table's type.  An empty slot's
