@@ -173,7 +173,7 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
         wrong |= id >= a.vocab && y[0] != kNoLogit;
         t.add<1, false>(y, a.c2);
     }
-    t.join_wave(a.c2);
+    t.join_wave<false>(a.c2);
     wrong = __ballot(wrong) != 0;
     const bool empty = nothing_left(t), none = nothing_left(f);
     const float log2t = log2_fast(t.s);
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void logit_stats_kernel(LogitArgs a) {
             }
         }
     }
-    f.join_wave(a.c2);
+    f.join_wave<kMode != kDistill>(a.c2);
     if constexpr (kMode == kLogprobsTop) top.cut();
     if (lane_id() == 0) {
         s_part[wave] = f;
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
         const float4 p = a.part[row * a.splits + lane];
         f.m = p.x; f.s = p.y; f.a = p.z;
     }
-    f.join_wave(a.c2);
+    f.join_wave<kMode != kDistill>(a.c2);
     if constexpr (kMode == kDistill) {
         finish_distill<T>(a, row, f);
     } else {
@@ -415,6 +415,199 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     }
 }
 
+// Loss and gradient of a row by one workgroup: the row is read once, kept in registers as it came
+// (NV pieces a thread) and written once.  A workgroup goes on to another row as soon as the gradient's
+// pieces leave: the next row's loads take their registers and travel beside the stores.  Memory
+// operations are waited for in their order and counted where their number is known, so there are no branches about
+// them: beyond the row's end a thread reads (and writes, the same values again) the last piece once more.
+template <class T, int kRowThreads, int NV>
+__global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) {
+    using P = Piece<T>;
+    using raw_t = typename T::raw;
+    constexpr int kRowWaves = kRowThreads / kWave, kOwn = kTeacherSlots / kRowThreads;
+    __shared__ int s_id[kTeacherSlots];
+    __shared__ float s_y[kTeacherSlots], s_q[kTeacherSlots];
+    __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
+    __shared__ float4 s_teacher;                         // max, log2 sum, whether there is one, whether its ids and logits are sound
+    const int tid = threadIdx.x, wave = tid / kWave;
+    // whole pieces, and behind them less than one whose elements a thread each takes
+    const int pieces = a.vocab / P::kLen, last = pieces * P::kLen + tid;
+    const uint32_t last_at = (uint32_t)min(last, a.vocab - 1) * (uint32_t)sizeof(raw_t);
+    auto row_of = [&](int64_t row) { return (const char*)a.z + row * a.stride * (int64_t)sizeof(raw_t); };
+    // (the thread's number is made to look new each time: the compiler would keep, and spill, an offset for every piece)
+    auto piece_of = [&](int u) {
+        int i = tid;
+        asm volatile("" : "+v"(i));
+        return i + u * kRowThreads;
+    };
+    auto at_piece = [&](int u, int most) { return (uint32_t)min(piece_of(u), most) * 16u; };
+    auto load = [&](const char* z, int u, int most) { return P::load_once((const raw_t*)(z + at_piece(u, most))); };
+    // a thread's slots: the id (-1: empty; vocab: beyond it), the teacher's logit and the student's there
+    uint32_t id_lo[kOwn], id_hi[kOwn];
+    uint16_t y_lo[kOwn], y_hi[kOwn];
+    raw_t there[kOwn];
+    const int id_size = a.wide_ids ? 8 : 4, y_size = a.teacher_dtype == DCIH_F32 ? 4 : 2;
+    auto load_slots = [&](int64_t row) {
+        const char* ids = (const char*)a.ids + row * a.slots * id_size;
+        const char* ys = (const char*)a.teacher + row * a.slots * y_size;
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const uint32_t j = (uint32_t)min(o * kRowThreads + tid, a.slots - 1);
+            id_lo[o] = *(const uint32_t*)(ids + j * id_size);
+            id_hi[o] = *(const uint32_t*)(ids + (j + 1) * id_size - 4);
+            y_lo[o] = *(const uint16_t*)(ys + j * y_size);
+            y_hi[o] = *(const uint16_t*)(ys + (j + 1) * y_size - 2);
+        }
+    };
+    auto id_of = [&](int o) {
+        const int64_t id = a.wide_ids ? (int64_t)((uint64_t)id_hi[o] << 32 | id_lo[o]) : (int64_t)(int32_t)id_lo[o];
+        return o * kRowThreads + tid >= a.slots || id < 0 ? -1 : (int)min(id, (int64_t)a.vocab);
+    };
+    auto y_of = [&](int o) {
+        const float y = a.teacher_dtype == DCIH_F16 ? (float)__builtin_bit_cast(_Float16, y_lo[o])
+                                                    : __builtin_bit_cast(float, (uint32_t)y_hi[o] << 16 | (y_size == 4 ? y_lo[o] : 0));
+        return id_of(o) < 0 ? kNoLogit : y;
+    };
+    auto load_there = [&](const char* z) {
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            asm volatile("" : "+v"(id_lo[o]), "+v"(id_hi[o]));         // (not to be waited for before this place)
+            const int id = id_of(o);
+            there[o] = ((const raw_t*)z)[id >= 0 && id < a.vocab ? id : 0];
+        }
+    };
+    int64_t row = blockIdx.x;
+    const char* z = row_of(row);
+    u32x4 raw[NV];
+    load_slots(row);
+    raw_t raw_last = *(const raw_t*)(z + last_at);
+    load_there(z);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < NV; u++) raw[u] = load(z, u, pieces - 1);
+    while (true) {
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const float y = y_of(o);
+            s_id[o * kRowThreads + tid] = y == kNoLogit ? -1 : id_of(o);
+            s_y[o * kRowThreads + tid] = y;
+        }
+        __syncthreads();
+        if (wave == 0) {      // while the row arrives
+            Softmax t = Softmax::none();
+            bool wrong = false;
+            for (int j = lane_id(); j < a.slots; j += kWave) {
+                const float y[1] = {s_y[j]};
+                wrong |= s_id[j] == a.vocab;
+                t.add<1, false>(y, a.c2);
+            }
+            t.join_wave<false>(a.c2);
+            wrong = __ballot(wrong) != 0 || t.s != t.s;
+            if (lane_id() == 0) s_teacher = make_float4(kept_max(t), log2_fast(t.s), nothing_left(t) ? 0.f : 1.f, wrong ? 1.f : 0.f);
+        }
+        Softmax f = Softmax::none();
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            float x[P::kLen];
+            const u32x4 none = P::filled(kNoLogit);
+            const bool in = piece_of(u) < pieces;
+            u32x4 piece = raw[u];
+#pragma unroll
+            for (int k = 0; k < 4; k++) piece[k] = in ? piece[k] : none[k];
+            P::unpack(piece, x);
+            f.add<P::kLen, false>(x, a.c2);
+            __builtin_amdgcn_sched_barrier(0);           // (one piece unpacked at a time)
+        }
+        {
+            const float x[1] = {last < a.vocab ? (float)raw_last : kNoLogit};
+            f.add<1, false>(x, a.c2);
+        }
+        f.join_wave<false>(a.c2);
+        if (lane_id() == 0) {
+            s_max[wave] = f.m;
+            s_sum[wave] = f.s;
+        }
+        __syncthreads();
+        f = Softmax::none();
+        if (lane_id() < kRowWaves) {
+            f.m = s_max[lane_id()];
+            f.s = s_sum[lane_id()];
+        }
+        f.join_wave<false>(a.c2);
+        const float4 t = s_teacher;
+        const bool none = nothing_left(f), empty = t.z == 0.f;
+        const float m = kept_max(f), log2s = !empty && t.w != 0.f ? __builtin_nanf("") : log2_fast(f.s);
+        // (read through the scalar cache: no vector load to wait for)
+        const float weight = a.weights ? ((const __attribute__((address_space(4))) float*)a.weights)[row] : 1.f;
+        const float w = none || empty ? 0.f : weight * a.inv_t;
+        char* dz = (char*)a.grad + row * a.grad_stride * (int64_t)sizeof(raw_t);
+        auto gradient = [&](float x) { return w == 0.f ? 0.f : w * exp2_fast((x - m) * a.c2 - log2s); };
+        auto put = [&](int u) {
+            asm volatile("" : "+v"(raw[u]));             // (keeps the pieces packed: not the 32-bit values of the sums)
+            float x[P::kLen];
+            P::unpack(raw[u], x);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) x[k] = gradient(x[k]);
+            P::store_once((raw_t*)(dz + at_piece(u, pieces - 1)), P::pack(x));
+        };
+        // (without a next row one piece of this one is read instead, by all)
+        const bool more = row + gridDim.x < a.n;
+        const int64_t next = more ? row + gridDim.x : row;
+        const int most = more ? pieces - 1 : 0;
+        const raw_t was_last = raw_last;
+        float zy[kOwn];
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) zy[o] = (float)there[o];
+        z = row_of(next);
+        load_slots(next);
+        raw_last = *(const raw_t*)(z + last_at);
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            put(u);
+            raw[u] = load(z, u, most);
+            if (u == (NV - 1) / 4) load_there(z);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (last < a.vocab) ((raw_t*)dz)[last] = (raw_t)gradient((float)was_last);
+        // the teacher's part: the loss, and its tokens, each by the first of the slots that name it
+        float loss = 0.f, q[kOwn];
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const int j = o * kRowThreads + tid;
+            const float q2 = (s_y[j] - t.x) * a.c2 - t.y;
+            const float logp = none ? kNoLogit : (zy[o] - m) * a.c2 - log2s;
+            q[o] = s_id[j] < 0 ? 0.f : exp2_fast(q2);
+            if (!(q[o] == 0.f)) loss += q[o] * (q2 - logp);
+            s_q[j] = q[o];
+        }
+        loss = wave_sum(loss);
+        if (lane_id() == 0) s_sum[wave] = loss;
+        __syncthreads();
+        if (tid == 0) {
+            loss = 0.f;
+            for (int v = 0; v < kRowWaves; v++) loss += s_sum[v];
+            a.losses[row] = empty ? 0.f : t.w != 0.f ? __builtin_nanf("") : loss * kLn2;
+            if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
+        }
+        if (w != 0.f) {
+#pragma unroll
+            for (int o = 0; o < kOwn; o++) {
+                const int j = o * kRowThreads + tid, token = s_id[j];
+                if (token < 0 || token >= a.vocab) continue;
+                bool again = false;
+                for (int i = 0; i < j; i++) again |= s_id[i] == token;
+                if (again) continue;
+                float sum = q[o];
+                for (int i = j + 1; i < a.slots; i++) sum += s_id[i] == token ? s_q[i] : 0.f;
+                ((raw_t*)dz)[token] = (raw_t)(w * (exp2_fast((zy[o] - m) * a.c2 - log2s) - sum));
+            }
+        }
+        __syncthreads();
+        if (!more) return;
+        row = next;
+    }
+}
+
 template <class T, int kMode>
 int stats_of(LogitArgs a, hipStream_t s) {
     constexpr int U = sizeof(typename T::raw) == 4 ? 4 : 2;
@@ -428,6 +621,29 @@ int stats_of(LogitArgs a, hipStream_t s) {
         }
     }
     return 0;
+}
+
+template <class T, int kRowThreads, int NV>
+int distill_rows_by(const LogitArgs& a, int per_unit, hipStream_t s) {
+    const uint32_t groups = (uint32_t)std::min<int64_t>(a.n, 256 * per_unit);
+    distill_rows_kernel<T, kRowThreads, NV><<<groups, kRowThreads, 0, s>>>(a);
+    DCIH_HIP(hipGetLastError());
+    return 0;
+}
+
+constexpr int kMostPieces = 16 * 1024;       // of a row in registers
+
+template <class T>
+int distill_rows_of(const LogitArgs& a, hipStream_t s) {
+    const int pieces = a.vocab / Piece<T>::kLen;
+    if (pieces <= 2 * 256) return distill_rows_by<T, 256, 2>(a, 6, s);
+    if (pieces <= 4 * 512) return distill_rows_by<T, 512, 4>(a, 3, s);
+    if (pieces <= 8 * 512) return distill_rows_by<T, 512, 8>(a, 2, s);
+    if (pieces <= 6 * 1024) return distill_rows_by<T, 1024, 6>(a, 1, s);
+    if (pieces <= 8 * 1024) return distill_rows_by<T, 1024, 8>(a, 1, s);
+    if (pieces <= 10 * 1024) return distill_rows_by<T, 1024, 10>(a, 1, s);
+    if (pieces <= 13 * 1024) return distill_rows_by<T, 1024, 13>(a, 1, s);
+    return distill_rows_by<T, 1024, 16>(a, 1, s);
 }
 
 template <class T, int kMode>
@@ -468,6 +684,20 @@ int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
         case DCIH_F16 * 2 + 1: return stats_of<F16, kLogprobsTop>(a, s);
         case DCIH_BF16 * 2: return stats_of<BF16, kLogprobs>(a, s);
         default: return stats_of<BF16, kLogprobsTop>(a, s);
+    }
+}
+
+// Enough rows that a workgroup each fills the device, and rows that fit one.
+bool distill_by_rows(const LogitArgs& a, int dtype) {
+    const int pieces = a.vocab / (16 / type_bytes(dtype));
+    return a.n >= 192 && pieces >= 1 && pieces <= kMostPieces;
+}
+
+int distill_rows(const LogitArgs& a, int dtype, hipStream_t s) {
+    switch (dtype) {
+        case DCIH_F32: return distill_rows_of<F32>(a, s);
+        case DCIH_F16: return distill_rows_of<F16>(a, s);
+        default: return distill_rows_of<BF16>(a, s);
     }
 }
 

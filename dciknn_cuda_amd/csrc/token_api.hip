@@ -220,6 +220,10 @@ int dcih_distill(const void* d_logits, int dtype, int64_t num_rows, int vocab, i
     a.weights = d_weights;
     a.grad = d_grad;
     a.grad_stride = grad_stride;
+    if (d_grad && distill_by_rows(a, dtype)) {
+        a.stats = (float4*)d_stats;
+        return distill_rows(a, dtype, (hipStream_t)stream);
+    }
     if (int rc = logit_stats(a, dtype, true, (hipStream_t)stream)) return rc;
     return d_grad ? logit_grad(a, dtype, true, (hipStream_t)stream) : DCIH_OK;
 }

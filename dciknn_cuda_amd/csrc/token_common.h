@@ -50,6 +50,8 @@ struct LogitArgs {
 int logit_splits(int64_t n, int vocab, int dtype);
 int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s);
 int logit_grad(const LogitArgs& a, int dtype, bool distill, hipStream_t s);
+bool distill_by_rows(const LogitArgs& a, int dtype);                             // loss and gradient by one workgroup a row
+int distill_rows(const LogitArgs& a, int dtype, hipStream_t s);
 
 struct EmbedArgs {
     const void* rows;             // the table, or the gradients of the rows looked up
@@ -93,6 +95,12 @@ template <class T> struct Piece {          // one 16-byte piece of a row
         for (int k = 0; k < kLen; k++) v[k] = i + k < len ? row[i + k] : (typename T::raw)fill;
         return __builtin_bit_cast(u32x4, v);
     }
+    __device__ static u32x4 filled(float y) {
+        vec v;
+#pragma unroll
+        for (int k = 0; k < kLen; k++) v[k] = (typename T::raw)y;
+        return __builtin_bit_cast(u32x4, v);
+    }
     __device__ static void unpack(u32x4 x, float (&z)[kLen]) {
         const fvec f = __builtin_convertvector(__builtin_bit_cast(vec, x), fvec);
 #pragma unroll
@@ -131,6 +139,12 @@ constexpr float kLog2e = 1.44269504088896341f;
 // Below 2^-256 nothing is left in 32 bits: exponents are cut off there wherever they are a
 // factor themselves, so that a ruled-out entry adds 0 * -256 and not 0 * -inf.
 constexpr float kFloor2 = -256.f;
+
+__device__ inline float wave_max(float v) {
+    v = fmaxf(v, lane_xor<32>(v)); v = fmaxf(v, lane_xor<16>(v)); v = fmaxf(v, lane_xor<8>(v));
+    v = fmaxf(v, lane_xor<4>(v)); v = fmaxf(v, lane_xor<2>(v)); v = fmaxf(v, lane_xor<1>(v));
+    return v;
+}
 
 // Running statistics of a softmax over entries z at temperature T, exponents to the base 2
 // (c2 = log2(e) / T):  m = max z,  s = sum 2^((z - m) c2),  a = sum (z - m) c2 2^((z - m) c2).
@@ -174,23 +188,15 @@ struct Softmax {
             if (kEntropy) a = __builtin_fmaf(fmaxf(x, kFloor2), e, a);
         }
     }
-    template <int O> __device__ void join_lane(float c2) {
-        Softmax o;
-        o.m = lane_xor<O>(m); o.s = lane_xor<O>(s); o.a = lane_xor<O>(a);
-        join(o, c2);
-    }
     // Over a wavefront; every lane gets the result.
+    template <bool kEntropy>
     __device__ void join_wave(float c2) {
-        join_lane<32>(c2); join_lane<16>(c2); join_lane<8>(c2);
-        join_lane<4>(c2); join_lane<2>(c2); join_lane<1>(c2);
+        const float top = wave_max(m), d = fmaxf((m - top) * c2, kFloor2), f = exp2_fast(d);
+        if (kEntropy) a = wave_sum(f * (a + d * s));
+        s = wave_sum(s * f);
+        m = top;
     }
 };
-
-__device__ inline float wave_max(float v) {
-    v = fmaxf(v, lane_xor<32>(v)); v = fmaxf(v, lane_xor<16>(v)); v = fmaxf(v, lane_xor<8>(v));
-    v = fmaxf(v, lane_xor<4>(v)); v = fmaxf(v, lane_xor<2>(v)); v = fmaxf(v, lane_xor<1>(v));
-    return v;
-}
 
 #endif  // __HIPCC__
 }  // namespace dcih
