@@ -20,8 +20,8 @@ namespace dcih {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int64_t kMaxGrid = 1 << 22; // workgroups of one launch (their threads are counted in 32 bits)
+constexpr int kTopSlack = 8;         // entries beyond the k best that a wavefront gathers before it drops them
 constexpr int kTopRoom = 256;        // entries of a wavefront's candidate list: kMaxTop + 2 * 64 at least
 static_assert(kTopRoom >= kMaxTop + 2 * kWave && kTopRoom % kWave == 0, "room for two rounds of candidates");
 
@@ -67,6 +67,24 @@ struct WaveTop {
     // number of larger ones.
     __device__ void cut() {
         wave_fence();
+        if (count <= kWave) {      // nearly always
+            const u64 mine = lane_id() < count ? buf[lane_id()] : 0;
+            int rank = 0;
+            for (int i = 0; i < count; i++) {
+                const u64 e = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 |
+                              (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+                rank += e > mine;
+            }
+            wave_fence();
+            if (mine && rank < k) buf[rank] = mine;
+        } else {
+            cut_many();
+        }
+        wave_fence();
+        count = min(count, k);
+        if (count == k) least = max(least, buf[k - 1]);
+    }
+    __device__ void cut_many() {
         u64 mine[kTopRoom / kWave];
         int rank[kTopRoom / kWave];
 #pragma unroll
@@ -84,9 +102,6 @@ struct WaveTop {
 #pragma unroll
         for (int r = 0; r < kTopRoom / kWave; r++)
             if (mine[r] && rank[r] < k) buf[rank[r]] = mine[r];
-        wave_fence();
-        count = min(count, k);
-        if (count == k) least = buf[k - 1];
     }
 };
 
@@ -198,30 +213,37 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
 }
 
 // Statistics of rows, each by `splits` workgroups.  Threads keep their own running statistics over
-// every 256th piece; a wavefront keeps its best entries, too.
-template <class T, int kMode, int U>
-__global__ __launch_bounds__(kThreads) void logit_stats_kernel(LogitArgs a) {
+// every kRowThreads-th piece; a wavefront keeps its best entries, too, and what one of them
+// finds to be the least that can still be among the best bounds the others' as well.
+template <class T, int kMode, int kRowThreads, int U>
+__global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     using P = Piece<T>;
-    __shared__ u64 s_top[kMode == kLogprobsTop ? kWaves * kTopRoom : 1];
+    constexpr int kWaves = kRowThreads / kWave, N = U * P::kLen;
+    constexpr bool kTop = kMode == kLogprobsTop;
+    __shared__ u64 s_top[kTop ? kWaves * kTopRoom : 1];
+    __shared__ u64 s_least;
     __shared__ int s_count[kWaves];
     __shared__ Softmax s_part[kWaves];
-    const int64_t row = a.first + blockIdx.x / (uint32_t)a.splits;
+    const int64_t at_row = a.first + blockIdx.x / (uint32_t)a.splits;
     const int split = (int)(blockIdx.x % (uint32_t)a.splits);
-    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
+    const Row<T> row(a.z, at_row, a.stride, a.vocab);
     const int tid = threadIdx.x, wave = tid / kWave;
-    const int end = min((a.vocab + P::kLen - 1) / P::kLen, (split + 1) * a.per_split);     // in pieces
+    const int end = min(row.pieces + 1, (split + 1) * a.per_split);
     Softmax f = Softmax::none();
-    WaveTop top(s_top + (kMode == kLogprobsTop ? wave * kTopRoom : 0), a.top);
+    WaveTop top(s_top + (kTop ? wave * kTopRoom : 0), a.top);
+    if (kTop && kWaves > 1) {
+        if (tid == 0) s_least = 0;
+        __syncthreads();
+    }
     bool first = true;
-    for (int base = split * a.per_split; base < end; base += kThreads * U) {
+    for (int base = split * a.per_split; base < end; base += kRowThreads * U) {
         u32x4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int i = base + u * kThreads + tid;
-            if (i < end && (i + 1) * P::kLen <= a.vocab) raw[u] = P::load_once(z + (int64_t)i * P::kLen);
-            else raw[u] = P::load_part(z, i < end ? i * P::kLen : a.vocab, a.vocab, kNoLogit);
+            const int i = base + u * kRowThreads + tid;
+            raw[u] = row.load(i < end ? i : row.pieces + 1);
         }
-        float x[U * P::kLen], most = kNoLogit;
+        float x[N], most = kNoLogit;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float y[P::kLen];
@@ -232,57 +254,60 @@ __global__ __launch_bounds__(kThreads) void logit_stats_kernel(LogitArgs a) {
                 most = fmaxf(most, y[k]);
             }
         }
-        f.add<U * P::kLen, kMode != kDistill>(x, most, a.c2);
-        if constexpr (kMode == kLogprobsTop) {
+        if constexpr (kTop) {
+            if (kWaves > 1) top.least = max(top.least, __hip_atomic_load(&s_least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
             // The k-th largest of the lanes' largest values has k entries at or above it: none
             // below it is among the k best.
-            if (first) {
-                const uint32_t kth = kth_of_lanes(f2ord(most + 0.f), a.top);
-                top.least = (u64)kth << 32;
-                first = false;
-            }
-            const float bar = entry_logit(top.least);
-            if (__any(most >= bar && most > kNoLogit)) {
+            if (first) top.least = max(top.least, (u64)kth_of_lanes(f2ord(most + 0.f), a.top) << 32);
+            first = false;
+            const float bar = fmaxf(entry_logit(top.least), -__FLT_MAX__);
+            if (__any(most >= bar)) {
                 uint32_t left = 0;
 #pragma unroll
-                for (int k = 0; k < U * P::kLen; k++) left |= (x[k] >= bar && x[k] > kNoLogit ? 1u : 0u) << k;
+                for (int k = 0; k < N; k++) left |= x[k] >= bar ? 1u << k : 0;
                 while (__any(left != 0)) {
-                    const int k = left ? __builtin_ctz(left) : 0;
-                    const int i = (base + (k / P::kLen) * kThreads + tid) * P::kLen + k % P::kLen;
-                    const bool want = left != 0;
-                    top.push(want, want ? entry_of((float)z[i], i) : 0);
+                    const int at = left ? __builtin_ctz(left) : 0;
+                    float z = x[0];
+#pragma unroll
+                    for (int k = 1; k < N; k++) z = at == k ? x[k] : z;
+                    top.push(left != 0, entry_of(z, (base + at / P::kLen * kRowThreads + tid) * P::kLen + at % P::kLen));
                     left &= left - 1;
                 }
+                // more than a few beyond the k best: what is best of them bounds what comes
+                if (top.count > a.top + kTopSlack) top.cut();
+                if (kWaves > 1 && lane_id() == 0) atomicMax(&s_least, top.least);
             }
         }
+        f.add<N, kMode != kDistill>(x, most, a.c2);
     }
     f.join_wave<kMode != kDistill>(a.c2);
-    if constexpr (kMode == kLogprobsTop) top.cut();
-    if (lane_id() == 0) {
-        s_part[wave] = f;
-        s_count[wave] = top.count;
-    }
-    __syncthreads();
-    if (wave) return;
-    f = s_part[0];
+    if constexpr (kTop) top.cut();
+    if constexpr (kWaves > 1) {
+        if (lane_id() == 0) {
+            s_part[wave] = f;
+            s_count[wave] = top.count;
+        }
+        __syncthreads();
+        if (wave) return;
+        f = s_part[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; w++) f.join(s_part[w], a.c2);
-    if constexpr (kMode == kLogprobsTop) {
-        // the other wavefronts' entries behind the first one's own
-        top.count = s_count[0];
-        for (int w = 1; w < kWaves; w++)
-            top.push(lane_id() < s_count[w], lane_id() < s_count[w] ? s_top[w * kTopRoom + lane_id()] : 0);
-        top.cut();
+        for (int w = 1; w < kWaves; w++) f.join(s_part[w], a.c2);
+        if constexpr (kTop) {
+            // the other wavefronts' entries behind the first one's own, the one that is the bound among them
+            top.least = 0;
+            for (int w = 1; w < kWaves; w++)
+                top.push(lane_id() < s_count[w], lane_id() < s_count[w] ? s_top[w * kTopRoom + lane_id()] : 0);
+            top.cut();
+        }
     }
     if (a.splits > 1) {
-        const int64_t at = row * a.splits + split;
+        const int64_t at = at_row * a.splits + split;
         if (lane_id() == 0) a.part[at] = make_float4(f.m, f.s, f.a, 0.f);
-        if (kMode == kLogprobsTop && lane_id() < a.top)
-            a.part_top[at * a.top + lane_id()] = lane_id() < top.count ? top.buf[lane_id()] : 0;
+        if (kTop && lane_id() < a.top) a.part_top[at * a.top + lane_id()] = lane_id() < top.count ? top.buf[lane_id()] : 0;
         return;
     }
-    if constexpr (kMode == kDistill) finish_distill<T>(a, row, f);
-    else finish_logprobs<T>(a, row, f, top.buf, top.count);
+    if constexpr (kMode == kDistill) finish_distill<T>(a, at_row, f);
+    else finish_logprobs<T>(a, at_row, f, top.buf, top.count);
 }
 
 // Joins the splits (up to 64) of a row: one wavefront each.
@@ -323,26 +348,26 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
 template <class T, int kMode, int U>
 __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     using P = Piece<T>;
-    constexpr int kTile = kThreads * U * P::kLen;
+    constexpr int kTile = kThreads * U;                  // pieces
     constexpr int kOwn = kTeacherSlots / kThreads;
     __shared__ int s_id[kMode == kDistill ? kTeacherSlots : 1];
     __shared__ float s_q[kMode == kDistill ? kTeacherSlots : 1];
-    const int64_t row = a.first + blockIdx.x / (uint32_t)a.splits;
+    const int64_t at_row = a.first + blockIdx.x / (uint32_t)a.splits;
     const int tile = (int)(blockIdx.x % (uint32_t)a.splits) * kTile, tid = threadIdx.x;
-    const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
-    typename T::raw* dz = (typename T::raw*)a.grad + row * a.grad_stride;
-    const float4 st = a.stats[row];
+    const Row<T> row(a.z, at_row, a.stride, a.vocab);
+    typename T::raw* dz = (typename T::raw*)a.grad + at_row * a.grad_stride;
+    const float4 st = a.stats[at_row];
     // What a gradient is made of: dz = p (c0 + c1 log2 p) + at the target c2.
     float c0, c1 = 0.f, at_target = 0.f;
     int64_t target = -1;
     bool zero = st.x == kNoLogit;
     if constexpr (kMode == kDistill) {
-        c0 = (a.weights ? a.weights[row] : 1.f) * a.inv_t;
+        c0 = (a.weights ? a.weights[at_row] : 1.f) * a.inv_t;
         zero |= c0 == 0.f || st.z == kNoLogit;
     } else {
-        target = id_at(a.ids, a.wide_ids, row);
-        const float g = a.grad_logprobs && target >= 0 ? a.grad_logprobs[row] * a.inv_t : 0.f;
-        const float h = a.grad_entropy ? a.grad_entropy[row] * a.inv_t : 0.f;
+        target = id_at(a.ids, a.wide_ids, at_row);
+        const float g = a.grad_logprobs && target >= 0 ? a.grad_logprobs[at_row] * a.inv_t : 0.f;
+        const float h = a.grad_entropy ? a.grad_entropy[at_row] * a.inv_t : 0.f;
         zero |= g == 0.f && h == 0.f;
         c0 = -(g + h * st.z * kLn2);
         c1 = -h * kLn2;
@@ -357,12 +382,12 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
             for (int o = 0; o < kOwn; o++) {
                 const int j = o * kThreads + tid;
                 if (j >= a.slots) break;
-                const int64_t id = id_at(a.ids, a.wide_ids, row * a.slots + j);
-                const float y = teacher_at(a, row * a.slots + j);
-                const bool in = id >= tile && id < min(a.vocab, tile + kTile) && y != kNoLogit;
+                const int64_t id = id_at(a.ids, a.wide_ids, at_row * a.slots + j);
+                const float y = teacher_at(a, at_row * a.slots + j);
+                const bool in = id >= 0 && id < a.vocab && id / P::kLen >= tile && id / P::kLen < tile + kTile && y != kNoLogit;
                 s_id[j] = in ? (int)id : -1;
                 s_q[j] = exp2_fast((y - st.z) * a.c2 - st.w);
-                if (in) own_z[o] = (float)z[id];       // before it is written over
+                if (in) own_z[o] = (float)row.z[id];       // before it is written over
                 here |= in;
             }
         }
@@ -370,15 +395,14 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int i = tile + (u * kThreads + tid) * P::kLen;
-        if (i >= a.vocab) continue;
-        const bool whole = i + P::kLen <= a.vocab;
+        const int i = tile + u * kThreads + tid;
+        if (i > row.pieces) continue;
         float y[P::kLen];
         if (zero) {
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) y[k] = 0.f;
         } else {
-            P::unpack(whole ? P::load_once(z + i) : P::load_part(z, i, a.vocab, kNoLogit), y);
+            P::unpack(row.load(i), y);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) {
                 const float x = (y[k] - st.x) * a.c2 - st.y;      // log2 p
@@ -386,14 +410,12 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
                 if constexpr (kMode == kDistill) y[k] = p * c0;
                 else y[k] = p * __builtin_fmaf(c1, fmaxf(x, kFloor2), c0);
             }
-            if (kMode != kDistill && target >= i && target < i + P::kLen) {
+            if (kMode != kDistill && target / P::kLen == i) {
 #pragma unroll
-                for (int k = 0; k < P::kLen; k++) y[k] += i + k == target ? at_target : 0.f;
+                for (int k = 0; k < P::kLen; k++) y[k] += i * P::kLen + k == target ? at_target : 0.f;
             }
         }
-        const u32x4 out = P::pack(y);
-        if (whole) P::store_once(dz + i, out);
-        else P::store_part(dz, i, a.vocab, out);
+        row.store(dz, i, P::pack(y));
     }
     if constexpr (kMode == kDistill) {
         if (!here) return;
@@ -608,12 +630,12 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
     }
 }
 
-template <class T, int kMode>
-int stats_of(LogitArgs a, hipStream_t s) {
+template <class T, int kMode, int kRowThreads>
+int stats_by(LogitArgs a, hipStream_t s) {
     constexpr int U = sizeof(typename T::raw) == 4 ? 4 : 2;
     for (int64_t most = kMaxGrid / a.splits; a.first < a.n; a.first += most) {
         const uint32_t rows = (uint32_t)std::min(most, a.n - a.first);
-        logit_stats_kernel<T, kMode, U><<<rows * a.splits, kThreads, 0, s>>>(a);
+        logit_stats_kernel<T, kMode, kRowThreads, U><<<rows * a.splits, kRowThreads, 0, s>>>(a);
         DCIH_HIP(hipGetLastError());
         if (a.splits > 1) {
             logit_join_kernel<T, kMode><<<rows, kWave, 0, s>>>(a);
@@ -621,6 +643,11 @@ int stats_of(LogitArgs a, hipStream_t s) {
         }
     }
     return 0;
+}
+
+template <class T, int kMode>
+int stats_of(const LogitArgs& a, hipStream_t s) {
+    return stats_by<T, kMode, kThreads>(a, s);
 }
 
 template <class T, int kRowThreads, int NV>
@@ -648,8 +675,8 @@ int distill_rows_of(const LogitArgs& a, hipStream_t s) {
 
 template <class T, int kMode>
 int grad_of(LogitArgs a, hipStream_t s) {
-    constexpr int U = 2, kTile = kThreads * U * Piece<T>::kLen;
-    a.splits = (a.vocab - 1) / kTile + 1;
+    constexpr int U = 2, kTile = kThreads * U * Piece<T>::kLen;      // elements
+    a.splits = a.vocab / kTile + 1;           // (what is left of a row is a piece more)
     for (int64_t most = std::max<int64_t>(1, kMaxGrid / a.splits); a.first < a.n; a.first += most) {
         logit_grad_kernel<T, kMode, U><<<(uint32_t)std::min(most, a.n - a.first) * a.splits, kThreads, 0, s>>>(a);
         DCIH_HIP(hipGetLastError());
@@ -668,7 +695,7 @@ int logit_splits(int64_t n, int vocab, int dtype) {
 }
 
 int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
-    const int len = 16 / type_bytes(dtype), pieces = (int)(((int64_t)a.vocab + len - 1) / len);
+    const int len = 16 / type_bytes(dtype), pieces = a.vocab / len + 1;
     a.per_split = (pieces + a.splits - 1) / a.splits;
     if (distill) {
         switch (dtype) {

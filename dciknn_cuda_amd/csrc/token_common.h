@@ -125,6 +125,39 @@ template <class T> struct Piece {          // one 16-byte piece of a row
     }
 };
 
+// A row of logits as whole 16-byte pieces and, as one more, what is left behind them.
+template <class T> struct Row {
+    using raw_t = typename T::raw;
+    static constexpr int kLen = Piece<T>::kLen;
+    const raw_t* z;
+    int pieces, len;
+    bool odd;           // elements of two bytes that start within a word
+    __device__ Row(const void* logits, int64_t row, int64_t stride, int len_) : z((const raw_t*)logits + row * stride), len(len_) {
+        pieces = len / kLen;
+        odd = sizeof(raw_t) == 2 && ((uintptr_t)z & 2);
+    }
+    // Piece `piece`, what is left for the one behind the last, -inf beyond the row.
+    __device__ u32x4 load(int piece) const {
+        if (piece < pieces) {
+            const raw_t* p = z + (int64_t)piece * kLen;
+            if (sizeof(raw_t) == 4 || !odd) return Piece<T>::load_once(p);
+            // by whole words, shifted (a large row by accesses within words: 4.9 TB/s instead of 6.0); the first
+            // and the last word are shared with what stands beside the piece
+            const uint32_t* w = (const uint32_t*)(p - 1);
+            const u32x4 x = __builtin_nontemporal_load((const u32x4_any*)w);
+            const uint32_t next = w[4];
+            return u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
+                         __builtin_amdgcn_alignbit(x[3], x[2], 16), __builtin_amdgcn_alignbit(next, x[3], 16)};
+        }
+        return Piece<T>::load_part(z, piece == pieces ? pieces * kLen : len, len, -__builtin_huge_valf());
+    }
+    // To the same place of another row.
+    __device__ void store(raw_t* to, int piece, u32x4 x) const {
+        if (piece < pieces) Piece<T>::store_once(to + (int64_t)piece * kLen, x);
+        else Piece<T>::store_part(to, pieces * kLen, len, x);
+    }
+};
+
 __device__ inline int64_t id_at(const void* ids, bool wide, int64_t i) {
     return wide ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
 }
