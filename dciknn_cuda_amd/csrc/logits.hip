@@ -21,15 +21,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int64_t kMaxGrid = 1 << 22; // workgroups of one launch (their threads are counted in 32 bits)
-constexpr int kTopSlack = 8;         // entries beyond the k best that a wavefront gathers before it drops them
-constexpr int kTopRoom = 256;        // entries of a wavefront's candidate list: kMaxTop + 2 * 64 at least
-static_assert(kTopRoom >= kMaxTop + 2 * kWave && kTopRoom % kWave == 0, "room for two rounds of candidates");
+constexpr int kTopWait = 8;          // candidates that a wavefront gathers before it puts them in order
+constexpr int kTopRoom = 320;        // room for candidates: those and four rounds of 64
+static_assert(kTopRoom >= kTopWait + 4 * kWave, "room for four rounds of candidates");
 
 enum { kLogprobs = 0, kLogprobsTop = 1, kDistill = 2 };
 
 typedef unsigned long long u64;
 
-// One entry of a candidate list: larger logits first, ties to the lower index.
+// One entry of a candidate list: larger logits first, ties to the lower index (of an element or a piece).
 __device__ inline u64 entry_of(float z, int index) {
     return (u64)f2ord(z + 0.f) << 32 | (0xffffffffu - (uint32_t)index);      // (-0 and 0 tie)
 }
@@ -47,77 +47,69 @@ __device__ inline void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// The k best entries a wavefront has met, in LDS of its own: entries are put behind one another
-// and cut back to the k best whenever another 64 might not fit, so that any order of the row and
-// any number of ties is taken.  An entry is 0 at no time (index 2^32 - 1 does not exist).
+// One step of a bitonic sort over the lanes, larger ones first: towards runs of SIZE.
+template <int SIZE, int STRIDE, class V>
+__device__ inline void sort_step(V& v) {
+    const V o = lane_xor<STRIDE>(v);
+    const bool larger = ((lane_id() & STRIDE) == 0) == (SIZE == kWave || (lane_id() & SIZE) == 0);
+    v = (o > v) == larger ? o : v;
+}
+template <int SIZE, int STRIDE, class V>
+__device__ inline void sort_steps(V& v) {
+    sort_step<SIZE, STRIDE>(v);
+    if constexpr (STRIDE > 1) sort_steps<SIZE, STRIDE / 2>(v);
+}
+
+// The k-th largest (k = 1 .. 64) of the lanes' values, on every lane.
+__device__ inline uint32_t kth_of_lanes(uint32_t v, int k) {
+    sort_steps<2, 1>(v); sort_steps<4, 2>(v); sort_steps<8, 4>(v);
+    sort_steps<16, 8>(v); sort_steps<32, 16>(v); sort_steps<64, 32>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, k - 1);
+}
+__device__ inline u64 of_lane(u64 v, int lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// The k best pieces a wavefront has met, or elements: lane i holds the i-th best of them.  Candidates wait in
+// LDS until there are more than a few, after four rounds of up to 64 at the latest, so that any order of
+// the row and any number of ties is taken.  No entry is 0 (index 2^32 - 1 does not exist).
 struct WaveTop {
-    u64* buf;          // kTopRoom entries
-    int k, count = 0;
+    u64* wait;         // kTopRoom entries
+    int k, count = 0;  // of those that wait
+    u64 best = 0;
     u64 least = 0;     // what an entry has to exceed
 
-    __device__ WaveTop(u64* b, int k_) : buf(b), k(k_) {}
+    __device__ WaveTop(u64* b, int k_) : wait(b), k(k_) {}
 
     __device__ void push(bool want, u64 e) {
         const u64 mask = __ballot(want && e > least);
-        if (mask >> lane_id() & 1) buf[count + lanes_below(mask)] = e;
+        if (mask >> lane_id() & 1) wait[count + lanes_below(mask)] = e;
         count += __popcll(mask);
-        if (count > kTopRoom - kWave) cut();
     }
-    // Leaves the k best in order, best first.  Entries are all different: the rank of one is the
-    // number of larger ones.
-    __device__ void cut() {
+    // `other`: another list, its best on the last lane.
+    __device__ void merge_reversed(u64 other) {
+        best = best > other ? best : other;        // the best 64 of both, rising and falling
+        sort_steps<kWave, kWave / 2>(best);
+    }
+    __device__ void settle() {
         wave_fence();
-        if (count <= kWave) {      // nearly always
-            const u64 mine = lane_id() < count ? buf[lane_id()] : 0;
-            int rank = 0;
-            for (int i = 0; i < count; i++) {
-                const u64 e = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 |
-                              (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-                rank += e > mine;
+        for (int first = 0; first < count; first += kWave) {
+            u64 e = first + lane_id() < count ? wait[first + lane_id()] : 0;
+            sort_steps<2, 1>(e); sort_steps<4, 2>(e); sort_steps<8, 4>(e);
+            if (count - first > 8) {               // (the other lanes hold nothing)
+                sort_steps<16, 8>(e); sort_steps<32, 16>(e); sort_steps<64, 32>(e);
             }
-            wave_fence();
-            if (mine && rank < k) buf[rank] = mine;
-        } else {
-            cut_many();
+            merge_reversed(__shfl(e, kWave - 1 - lane_id()));
         }
         wave_fence();
-        count = min(count, k);
-        if (count == k) least = max(least, buf[k - 1]);
+        count = 0;
+        least = max(least, of_lane(best, k - 1));
     }
-    __device__ void cut_many() {
-        u64 mine[kTopRoom / kWave];
-        int rank[kTopRoom / kWave];
-#pragma unroll
-        for (int r = 0; r < kTopRoom / kWave; r++) {
-            const int i = r * kWave + lane_id();
-            mine[r] = i < count ? buf[i] : 0;
-            rank[r] = 0;
-        }
-        for (int i = 0; i < count; i++) {
-            const u64 e = buf[i];
-#pragma unroll
-            for (int r = 0; r < kTopRoom / kWave; r++) rank[r] += e > mine[r];
-        }
-        wave_fence();
-#pragma unroll
-        for (int r = 0; r < kTopRoom / kWave; r++)
-            if (mine[r] && rank[r] < k) buf[rank[r]] = mine[r];
+    __device__ void tidy() {
+        if (count > kTopWait) settle();
     }
+    __device__ int held() const { return min(k, (int)__popcll(__ballot(best != 0))); }
 };
-
-// The k-th largest (k = 1 .. 64) of the lanes' values, on every lane: a bitonic sort in registers.
-template <int SIZE, int STRIDE>
-__device__ inline void sort_step(uint32_t& v) {
-    const uint32_t o = lane_xor<STRIDE>(v);
-    const bool low = ((lane_id() & STRIDE) == 0) == ((lane_id() & SIZE) == 0 || SIZE == kWave);
-    v = low ? max(v, o) : min(v, o);
-    if constexpr (STRIDE > 1) sort_step<SIZE, STRIDE / 2>(v);
-}
-__device__ inline uint32_t kth_of_lanes(uint32_t v, int k) {
-    sort_step<2, 1>(v); sort_step<4, 2>(v); sort_step<8, 4>(v);
-    sort_step<16, 8>(v); sort_step<32, 16>(v); sort_step<64, 32>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, k - 1);
-}
 
 __device__ inline float teacher_at(const LogitArgs& a, int64_t i) {
     switch (a.teacher_dtype) {
@@ -134,29 +126,48 @@ __device__ inline bool nothing_left(const Softmax& f) { return f.m == kNoLogit &
 // but NaN keeps 0 beside its sum, NaN).
 __device__ inline float kept_max(const Softmax& f) { return nothing_left(f) ? kNoLogit : f.m == kNoLogit ? 0.f : f.m; }
 
-// One wavefront: what is returned of a row of log probabilities.  `best`: its `count` best entries
-// in order, count < k only where fewer entries are above -inf.
+// From the k best pieces of a row by their largest elements (the k best elements are in them: every piece
+// before an element's own holds a better one) to its k best elements.  Fewer than k: all that are above -inf.
 template <class T>
-__device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& f, const u64* best, int count) {
+__device__ void best_of_pieces(const LogitArgs& a, int64_t row, WaveTop& top) {
+    using P = Piece<T>;
+    const bool have = lane_id() < top.k && top.best;
+    const int piece = have ? entry_index(top.best) : 0;
+    const u64 last = of_lane(top.best, top.k - 1);
+    const float bar = last ? entry_logit(last) : -__FLT_MAX__;
+    float x[P::kLen];
+    P::unpack(Row<T>(a.z, row, a.stride, a.vocab).load(piece), x);
+    top.best = top.least = 0;
+#pragma unroll
+    for (int k = 0; k < P::kLen; k++) {
+        top.push(have && x[k] >= bar, entry_of(x[k], piece * P::kLen + k));
+        if (k % 4 == 3) top.settle();
+    }
+}
+
+// One wavefront: what is returned of a row of log probabilities.  `top`: its best pieces.
+template <class T>
+__device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& f, WaveTop& top, int64_t t, float z_t) {
     const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
     const bool none = nothing_left(f);
     const float log2s = log2_fast(f.s);
     const float entropy = none ? 0.f : (log2s - f.a / f.s) * kLn2;
     if (lane_id() == 0) {
-        const int64_t t = id_at(a.ids, a.wide_ids, row);
         float lp = 0.f;
         if (t >= a.vocab) lp = __builtin_nanf("");
-        else if (t >= 0) lp = none ? kNoLogit : (((float)z[t] - f.m) * a.c2 - log2s) * kLn2;
+        else if (t >= 0) lp = none ? kNoLogit : ((z_t - f.m) * a.c2 - log2s) * kLn2;
         a.logprobs[row] = lp;
         a.entropy[row] = entropy;
         if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, entropy * kLog2e, 0.f);
     }
     const int k = a.top;
     if (!k) return;
+    best_of_pieces<T>(a, row, top);
+    int count = top.held();
     int32_t* ids = a.top_ids + row * k;
     float* lps = a.top_logprobs + row * k;
     if (lane_id() < count) {
-        const u64 e = best[lane_id()];
+        const u64 e = top.best;
         ids[lane_id()] = entry_index(e);
         lps[lane_id()] = ((entry_logit(e) - f.m) * a.c2 - log2s) * kLn2;
     }
@@ -213,8 +224,9 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
 }
 
 // Statistics of rows, each by `splits` workgroups.  Threads keep their own running statistics over
-// every kRowThreads-th piece; a wavefront keeps its best entries, too, and what one of them
-// finds to be the least that can still be among the best bounds the others' as well.
+// every kRowThreads-th piece; a wavefront keeps its best pieces, too, and what one of them
+// finds to be the least that can still be among the best bounds the others' as well.  (Keeping elements
+// instead of pieces doubled the arithmetic, which is what bounds this kernel with alternatives: 115 us instead of TOPNEW.)
 template <class T, int kMode, int kRowThreads, int U>
 __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -222,13 +234,19 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     constexpr bool kTop = kMode == kLogprobsTop;
     __shared__ u64 s_top[kTop ? kWaves * kTopRoom : 1];
     __shared__ u64 s_least;
-    __shared__ int s_count[kWaves];
     __shared__ Softmax s_part[kWaves];
     const int64_t at_row = a.first + blockIdx.x / (uint32_t)a.splits;
     const int split = (int)(blockIdx.x % (uint32_t)a.splits);
     const Row<T> row(a.z, at_row, a.stride, a.vocab);
     const int tid = threadIdx.x, wave = tid / kWave;
     const int end = min(row.pieces + 1, (split + 1) * a.per_split);
+    // the target's logit, asked for before the row
+    int64_t t = -1;
+    float z_t = 0.f;
+    if (kMode != kDistill && a.splits == 1) {
+        t = id_at(a.ids, a.wide_ids, at_row);
+        if (t >= 0 && t < a.vocab) z_t = (float)row.z[t];
+    }
     Softmax f = Softmax::none();
     WaveTop top(s_top + (kTop ? wave * kTopRoom : 0), a.top);
     if (kTop && kWaves > 1) {
@@ -238,76 +256,67 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     bool first = true;
     for (int base = split * a.per_split; base < end; base += kRowThreads * U) {
         u32x4 raw[U];
+        if (base + kRowThreads * U <= min(end, row.pieces)) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = base + u * kRowThreads + tid;
-            raw[u] = row.load(i < end ? i : row.pieces + 1);
+            for (int u = 0; u < U; u++) raw[u] = row.load_whole(base + u * kRowThreads + tid);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = base + u * kRowThreads + tid;
+                raw[u] = row.load(i < end ? i : row.pieces + 1);
+            }
         }
-        float x[N], most = kNoLogit;
+        float x[N], most = kNoLogit, largest[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float y[P::kLen];
             P::unpack(raw[u], y);
+            largest[u] = y[0];
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) {
                 x[u * P::kLen + k] = y[k];
-                most = fmaxf(most, y[k]);
+                largest[u] = fmaxf(largest[u], y[k]);
             }
+            most = fmaxf(most, largest[u]);
         }
         if constexpr (kTop) {
             if (kWaves > 1) top.least = max(top.least, __hip_atomic_load(&s_least, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-            // The k-th largest of the lanes' largest values has k entries at or above it: none
+            // The k-th largest of the lanes' largest values has k pieces at or above it: none
             // below it is among the k best.
             if (first) top.least = max(top.least, (u64)kth_of_lanes(f2ord(most + 0.f), a.top) << 32);
             first = false;
             const float bar = fmaxf(entry_logit(top.least), -__FLT_MAX__);
             if (__any(most >= bar)) {
-                uint32_t left = 0;
 #pragma unroll
-                for (int k = 0; k < N; k++) left |= x[k] >= bar ? 1u << k : 0;
-                while (__any(left != 0)) {
-                    const int at = left ? __builtin_ctz(left) : 0;
-                    float z = x[0];
-#pragma unroll
-                    for (int k = 1; k < N; k++) z = at == k ? x[k] : z;
-                    top.push(left != 0, entry_of(z, (base + at / P::kLen * kRowThreads + tid) * P::kLen + at % P::kLen));
-                    left &= left - 1;
-                }
-                // more than a few beyond the k best: what is best of them bounds what comes
-                if (top.count > a.top + kTopSlack) top.cut();
+                for (int u = 0; u < U; u++) top.push(largest[u] >= bar, entry_of(largest[u], base + u * kRowThreads + tid));
+                top.tidy();           // (what is best of them bounds what comes)
                 if (kWaves > 1 && lane_id() == 0) atomicMax(&s_least, top.least);
             }
         }
         f.add<N, kMode != kDistill>(x, most, a.c2);
     }
     f.join_wave<kMode != kDistill>(a.c2);
-    if constexpr (kTop) top.cut();
+    if constexpr (kTop) top.settle();
     if constexpr (kWaves > 1) {
-        if (lane_id() == 0) {
-            s_part[wave] = f;
-            s_count[wave] = top.count;
-        }
+        if (lane_id() == 0) s_part[wave] = f;
+        if constexpr (kTop) s_top[wave * kTopRoom + lane_id()] = top.best;
         __syncthreads();
         if (wave) return;
         f = s_part[0];
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) f.join(s_part[w], a.c2);
-        if constexpr (kTop) {
-            // the other wavefronts' entries behind the first one's own, the one that is the bound among them
-            top.least = 0;
-            for (int w = 1; w < kWaves; w++)
-                top.push(lane_id() < s_count[w], lane_id() < s_count[w] ? s_top[w * kTopRoom + lane_id()] : 0);
-            top.cut();
+        for (int w = 1; w < kWaves; w++) {
+            f.join(s_part[w], a.c2);
+            if constexpr (kTop) top.merge_reversed(s_top[w * kTopRoom + kWave - 1 - lane_id()]);
         }
     }
     if (a.splits > 1) {
         const int64_t at = at_row * a.splits + split;
         if (lane_id() == 0) a.part[at] = make_float4(f.m, f.s, f.a, 0.f);
-        if (kTop && lane_id() < a.top) a.part_top[at * a.top + lane_id()] = lane_id() < top.count ? top.buf[lane_id()] : 0;
+        if (kTop && lane_id() < a.top) a.part_top[at * a.top + lane_id()] = top.best;
         return;
     }
     if constexpr (kMode == kDistill) finish_distill<T>(a, at_row, f);
-    else finish_logprobs<T>(a, at_row, f, top.buf, top.count);
+    else finish_logprobs<T>(a, at_row, f, top, t, z_t);
 }
 
 // Joins the splits (up to 64) of a row: one wavefront each.
@@ -316,6 +325,12 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
     __shared__ u64 s_top[kMode == kLogprobsTop ? kTopRoom : 1];
     const int64_t row = a.first + blockIdx.x;
     const int lane = lane_id();
+    int64_t t = -1;
+    float z_t = 0.f;
+    if (kMode != kDistill) {
+        t = id_at(a.ids, a.wide_ids, row);
+        if (t >= 0 && t < a.vocab) z_t = (float)((const typename T::raw*)a.z + row * a.stride)[t];
+    }
     Softmax f = Softmax::none();
     if (lane < a.splits) {
         const float4 p = a.part[row * a.splits + lane];
@@ -337,10 +352,11 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
                 const u64 e = lane < a.splits ? lists[p] : 0;
                 if (!__any(e > top.least)) break;
                 top.push(e != 0, e);
+                if (top.count > kTopRoom - kWave) top.settle();
             }
-            top.cut();
+            top.settle();
         }
-        finish_logprobs<T>(a, row, f, top.buf, top.count);
+        finish_logprobs<T>(a, row, f, top, t, z_t);
     }
 }
 
@@ -632,7 +648,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
 
 template <class T, int kMode, int kRowThreads>
 int stats_by(LogitArgs a, hipStream_t s) {
-    constexpr int U = sizeof(typename T::raw) == 4 ? 4 : 2;
+    constexpr int U = sizeof(typename T::raw) == 4 || kRowThreads == kWave ? 4 : 2;      // loads in flight
     for (int64_t most = kMaxGrid / a.splits; a.first < a.n; a.first += most) {
         const uint32_t rows = (uint32_t)std::min(most, a.n - a.first);
         logit_stats_kernel<T, kMode, kRowThreads, U><<<rows * a.splits, kRowThreads, 0, s>>>(a);
@@ -645,9 +661,11 @@ int stats_by(LogitArgs a, hipStream_t s) {
     return 0;
 }
 
+// With rows enough that one wavefront each fills the device, one takes a row: nothing is to be joined.
+// (4096 x 50001 f16, five alternatives: TOPNEW us, 107 by four.)
 template <class T, int kMode>
 int stats_of(const LogitArgs& a, hipStream_t s) {
-    return stats_by<T, kMode, kThreads>(a, s);
+    return a.n >= 4096 ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
 }
 
 template <class T, int kRowThreads, int NV>

@@ -32,7 +32,7 @@ struct LogitArgs {
     int splits, per_split;        // workgroups of a row, 16-byte pieces of each
     float4* stats;                // [n] (max, log2 sum, entropy / ln 2, -) or (max, log2 sum, teacher's max, teacher's log2 sum)
     float4* part;                 // [n][splits] statistics of splits
-    unsigned long long* part_top; // [n][splits][top] their best entries
+    unsigned long long* part_top; // [n][splits][top] their best pieces
     // log probabilities
     int top;
     float *logprobs, *entropy;
@@ -136,19 +136,20 @@ template <class T> struct Row {
         pieces = len / kLen;
         odd = sizeof(raw_t) == 2 && ((uintptr_t)z & 2);
     }
-    // Piece `piece`, what is left for the one behind the last, -inf beyond the row.
+    __device__ u32x4 load_whole(int piece) const {
+        const raw_t* p = z + (int64_t)piece * kLen;
+        if (sizeof(raw_t) == 4 || !odd) return Piece<T>::load_once(p);
+        // by whole words, shifted (a large row by accesses within words: 4.9 TB/s instead of 6.0); the first
+        // and the last word are shared with what stands beside the piece
+        const uint32_t* w = (const uint32_t*)(p - 1);
+        const u32x4 x = __builtin_nontemporal_load((const u32x4_any*)w);
+        const uint32_t next = w[4];
+        return u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
+                     __builtin_amdgcn_alignbit(x[3], x[2], 16), __builtin_amdgcn_alignbit(next, x[3], 16)};
+    }
+    // Any piece: what is left for the one behind the whole ones, -inf beyond the row.
     __device__ u32x4 load(int piece) const {
-        if (piece < pieces) {
-            const raw_t* p = z + (int64_t)piece * kLen;
-            if (sizeof(raw_t) == 4 || !odd) return Piece<T>::load_once(p);
-            // by whole words, shifted (a large row by accesses within words: 4.9 TB/s instead of 6.0); the first
-            // and the last word are shared with what stands beside the piece
-            const uint32_t* w = (const uint32_t*)(p - 1);
-            const u32x4 x = __builtin_nontemporal_load((const u32x4_any*)w);
-            const uint32_t next = w[4];
-            return u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
-                         __builtin_amdgcn_alignbit(x[3], x[2], 16), __builtin_amdgcn_alignbit(next, x[3], 16)};
-        }
+        if (piece < pieces) return load_whole(piece);
         return Piece<T>::load_part(z, piece == pieces ? pieces * kLen : len, len, -__builtin_huge_valf());
     }
     // To the same place of another row.
