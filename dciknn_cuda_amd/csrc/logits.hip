@@ -240,13 +240,7 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     const Row<T> row(a.z, at_row, a.stride, a.vocab);
     const int tid = threadIdx.x, wave = tid / kWave;
     const int end = min(row.pieces + 1, (split + 1) * a.per_split);
-    // the target's logit, asked for before the row
-    int64_t t = -1;
-    float z_t = 0.f;
-    if (kMode != kDistill && a.splits == 1) {
-        t = id_at(a.ids, a.wide_ids, at_row);
-        if (t >= 0 && t < a.vocab) z_t = (float)row.z[t];
-    }
+    const int64_t t = kMode == kDistill ? -1 : id_of_all(a.ids, a.wide_ids, at_row);
     Softmax f = Softmax::none();
     WaveTop top(s_top + (kTop ? wave * kTopRoom : 0), a.top);
     if (kTop && kWaves > 1) {
@@ -257,8 +251,7 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
     for (int base = split * a.per_split; base < end; base += kRowThreads * U) {
         u32x4 raw[U];
         if (base + kRowThreads * U <= min(end, row.pieces)) {
-#pragma unroll
-            for (int u = 0; u < U; u++) raw[u] = row.load_whole(base + u * kRowThreads + tid);
+            row.load_runs(base + tid, kRowThreads, raw);
         } else {
 #pragma unroll
             for (int u = 0; u < U; u++) {
@@ -288,13 +281,16 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
             const float bar = fmaxf(entry_logit(top.least), -__FLT_MAX__);
             if (__any(most >= bar)) {
 #pragma unroll
-                for (int u = 0; u < U; u++) top.push(largest[u] >= bar, entry_of(largest[u], base + u * kRowThreads + tid));
+                for (int u = 0; u < U; u++)
+                    if (__any(largest[u] >= bar)) top.push(largest[u] >= bar, entry_of(largest[u], base + u * kRowThreads + tid));
                 top.tidy();           // (what is best of them bounds what comes)
                 if (kWaves > 1 && lane_id() == 0) atomicMax(&s_least, top.least);
             }
         }
         f.add<N, kMode != kDistill>(x, most, a.c2);
     }
+    // (asked for now, used at the end)
+    const typename T::raw z_t = kMode != kDistill && a.splits == 1 ? row.z[t >= 0 && t < a.vocab ? t : 0] : (typename T::raw)0.f;
     f.join_wave<kMode != kDistill>(a.c2);
     if constexpr (kTop) top.settle();
     if constexpr (kWaves > 1) {
@@ -316,7 +312,7 @@ __global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
         return;
     }
     if constexpr (kMode == kDistill) finish_distill<T>(a, at_row, f);
-    else finish_logprobs<T>(a, at_row, f, top, t, z_t);
+    else finish_logprobs<T>(a, at_row, f, top, t, (float)z_t);
 }
 
 // Joins the splits (up to 64) of a row: one wavefront each.
@@ -325,17 +321,13 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
     __shared__ u64 s_top[kMode == kLogprobsTop ? kTopRoom : 1];
     const int64_t row = a.first + blockIdx.x;
     const int lane = lane_id();
-    int64_t t = -1;
-    float z_t = 0.f;
-    if (kMode != kDistill) {
-        t = id_at(a.ids, a.wide_ids, row);
-        if (t >= 0 && t < a.vocab) z_t = (float)((const typename T::raw*)a.z + row * a.stride)[t];
-    }
+    const int64_t t = kMode == kDistill ? -1 : id_of_all(a.ids, a.wide_ids, row);
     Softmax f = Softmax::none();
     if (lane < a.splits) {
         const float4 p = a.part[row * a.splits + lane];
         f.m = p.x; f.s = p.y; f.a = p.z;
     }
+    const typename T::raw z_t = kMode == kDistill ? (typename T::raw)0.f : ((const typename T::raw*)a.z + row * a.stride)[t >= 0 && t < a.vocab ? t : 0];
     f.join_wave<kMode != kDistill>(a.c2);
     if constexpr (kMode == kDistill) {
         finish_distill<T>(a, row, f);
@@ -356,7 +348,7 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
             }
             top.settle();
         }
-        finish_logprobs<T>(a, row, f, top, t, z_t);
+        finish_logprobs<T>(a, row, f, top, t, (float)z_t);
     }
 }
 
@@ -579,7 +571,8 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         const float weight = a.weights ? ((const __attribute__((address_space(4))) float*)a.weights)[row] : 1.f;
         const float w = none || empty ? 0.f : weight * a.inv_t;
         char* dz = (char*)a.grad + row * a.grad_stride * (int64_t)sizeof(raw_t);
-        auto gradient = [&](float x) { return w == 0.f ? 0.f : w * exp2_fast((x - m) * a.c2 - log2s); };
+        const float share = w * exp2_fast(-log2s);           // the row's factor / the sum of the powers
+        auto gradient = [&](float x) { return w == 0.f ? 0.f : share * exp2_fast((x - m) * a.c2); };
         auto put = [&](int u) {
             asm volatile("" : "+v"(raw[u]));             // (keeps the pieces packed: not the 32-bit values of the sums)
             float x[P::kLen];
@@ -637,7 +630,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
                 if (again) continue;
                 float sum = q[o];
                 for (int i = j + 1; i < a.slots; i++) sum += s_id[i] == token ? s_q[i] : 0.f;
-                ((raw_t*)dz)[token] = (raw_t)(w * (exp2_fast((zy[o] - m) * a.c2 - log2s) - sum));
+                ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy[o] - m) * a.c2) - w * sum);
             }
         }
         __syncthreads();
@@ -665,7 +658,7 @@ int stats_by(LogitArgs a, hipStream_t s) {
 // (4096 x 50001 f16, five alternatives: TOPNEW us, 107 by four.)
 template <class T, int kMode>
 int stats_of(const LogitArgs& a, hipStream_t s) {
-    return a.n >= 4096 ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
+    return a.n >= 4096 && a.vocab >= 2048 ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
 }
 
 template <class T, int kRowThreads, int NV>

@@ -136,20 +136,34 @@ template <class T> struct Row {
         pieces = len / kLen;
         odd = sizeof(raw_t) == 2 && ((uintptr_t)z & 2);
     }
-    __device__ u32x4 load_whole(int piece) const {
-        const raw_t* p = z + (int64_t)piece * kLen;
-        if (sizeof(raw_t) == 4 || !odd) return Piece<T>::load_once(p);
-        // by whole words, shifted (a large row by accesses within words: 4.9 TB/s instead of 6.0); the first
-        // and the last word are shared with what stands beside the piece
-        const uint32_t* w = (const uint32_t*)(p - 1);
-        const u32x4 x = __builtin_nontemporal_load((const u32x4_any*)w);
-        const uint32_t next = w[4];
-        return u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
-                     __builtin_amdgcn_alignbit(x[3], x[2], 16), __builtin_amdgcn_alignbit(next, x[3], 16)};
+    // Whole pieces piece, piece + step, .. of each lane, one behind that of the lane before.  Rows within words are
+    // read by whole words (by accesses within words: 4.9 TB/s instead of 6.0) and shifted; the first and the
+    // last word of a run are shared with what stands beside it.
+    template <int U> __device__ void load_runs(int piece, int step, u32x4 (&raw)[U]) const {
+        if (sizeof(raw_t) == 4 || !odd) {
+#pragma unroll
+            for (int u = 0; u < U; u++) raw[u] = Piece<T>::load_once(z + (int64_t)(piece + u * step) * kLen);
+            return;
+        }
+        const uint32_t* w = (const uint32_t*)(z - 1);
+        const int behind = __builtin_amdgcn_readfirstlane(piece) + kWave;        // the piece behind the last lane's
+        uint32_t last[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            raw[u] = __builtin_nontemporal_load((const u32x4_any*)(w + (int64_t)(piece + u * step) * 4));
+            last[u] = w[(int64_t)(behind + u * step) * 4];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u32x4 x = raw[u];
+            const uint32_t next = (uint32_t)__builtin_amdgcn_update_dpp((int)last[u], (int)x[0], 0x130, 0xf, 0xf, false);      // wave_shl:1
+            raw[u] = u32x4{__builtin_amdgcn_alignbit(x[1], x[0], 16), __builtin_amdgcn_alignbit(x[2], x[1], 16),
+                           __builtin_amdgcn_alignbit(x[3], x[2], 16), __builtin_amdgcn_alignbit(next, x[3], 16)};
+        }
     }
     // Any piece: what is left for the one behind the whole ones, -inf beyond the row.
     __device__ u32x4 load(int piece) const {
-        if (piece < pieces) return load_whole(piece);
+        if (piece < pieces) return Piece<T>::load_once(z + (int64_t)piece * kLen);
         return Piece<T>::load_part(z, piece == pieces ? pieces * kLen : len, len, -__builtin_huge_valf());
     }
     // To the same place of another row.
@@ -161,6 +175,11 @@ template <class T> struct Row {
 
 __device__ inline int64_t id_at(const void* ids, bool wide, int64_t i) {
     return wide ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+}
+
+// The same for an index that all lanes share and ids that the kernel does not write: through the scalar cache.
+__device__ inline int64_t id_of_all(const void* ids, bool wide, int64_t i) {
+    return wide ? ((const __attribute__((address_space(4))) int64_t*)ids)[i] : (int64_t)((const __attribute__((address_space(4))) int32_t*)ids)[i];
 }
 
 __device__ inline float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32, 1 ulp
