@@ -225,10 +225,10 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
 
 // Statistics of rows, each by `splits` workgroups.  Threads keep their own running statistics over
 // every kRowThreads-th piece; a wavefront keeps its best pieces, too, and what one of them
-// finds to be the least that can still be among the best bounds the others' as well.  (Keeping elements
-// instead of pieces doubled the arithmetic, which is what bounds this kernel with alternatives: 115 us instead of TOPNEW.)
+// finds to be the least that can still be among the best bounds the others' as well.  (Keeping
+// elements instead of pieces doubled the arithmetic, which is what bounds this kernel with alternatives.)
 template <class T, int kMode, int kRowThreads, int U>
-__global__ __launch_bounds__(kRowThreads) void logit_stats_kernel(LogitArgs a) {
+__global__ __launch_bounds__(kRowThreads, 8) void logit_stats_kernel(LogitArgs a) {
     using P = Piece<T>;
     constexpr int kWaves = kRowThreads / kWave, N = U * P::kLen;
     constexpr bool kTop = kMode == kLogprobsTop;
@@ -337,14 +337,19 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
             const u64* lists = a.part_top + (row * a.splits + min(lane, a.splits - 1)) * a.top;
             // The lists are in order: with k lists or more, the k-th largest of their first entries bounds
             // from below, and where no list has an entry above the bound at a place none has one behind it.
-            const u64 head = lane < a.splits ? lists[0] : 0;
-            const uint32_t kth = kth_of_lanes((uint32_t)(head >> 32), a.top);
-            if (a.top <= a.splits) top.least = (u64)kth << 32;
-            for (int p = 0; p < a.top; p++) {
-                const u64 e = lane < a.splits ? lists[p] : 0;
-                if (!__any(e > top.least)) break;
-                top.push(e != 0, e);
-                if (top.count > kTopRoom - kWave) top.settle();
+            constexpr int kAhead = 4;
+            u64 e[kAhead];
+            for (int p = 0; p < a.top; p += kAhead) {
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) e[j] = lane < a.splits && p + j < a.top ? lists[p + j] : 0;
+                if (p == 0) {
+                    const uint32_t kth = kth_of_lanes((uint32_t)(e[0] >> 32), a.top);
+                    if (a.top <= a.splits) top.least = (u64)kth << 32;
+                }
+                if (!__any(e[0] > top.least)) break;
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) top.push(e[j] != 0, e[j]);
+                if (top.count > kTopRoom - kAhead * kWave) top.settle();
             }
             top.settle();
         }
@@ -454,16 +459,27 @@ template <class T, int kRowThreads, int NV>
 __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) {
     using P = Piece<T>;
     using raw_t = typename T::raw;
-    constexpr int kRowWaves = kRowThreads / kWave, kOwn = kTeacherSlots / kRowThreads;
-    __shared__ int s_id[kTeacherSlots];
-    __shared__ float s_y[kTeacherSlots], s_q[kTeacherSlots];
+    constexpr int kRowWaves = kRowThreads / kWave;
+    __shared__ int s_id[kRowThreads];
+    __shared__ float s_y[kRowThreads], s_q[kRowThreads];
     __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
     __shared__ float4 s_teacher;                         // max, log2 sum, whether there is one, whether its ids and logits are sound
     const int tid = threadIdx.x, wave = tid / kWave;
-    // whole pieces, and behind them less than one whose elements a thread each takes
-    const int pieces = a.vocab / P::kLen, last = pieces * P::kLen + tid;
-    const uint32_t last_at = (uint32_t)min(last, a.vocab - 1) * (uint32_t)sizeof(raw_t);
-    auto row_of = [&](int64_t row) { return (const char*)a.z + row * a.stride * (int64_t)sizeof(raw_t); };
+    // A row is whole pieces from its first whole word on and, at both ends, up to a piece of elements that a
+    // thread each takes.
+    struct Place {
+        const char* z;
+        int head, pieces;
+        __device__ int end(int tid) const { return tid < head ? tid : pieces * P::kLen + tid; }
+    };
+    auto place_of = [&](int64_t row) {
+        Place p;
+        p.z = (const char*)a.z + row * a.stride * (int64_t)sizeof(raw_t);
+        p.head = sizeof(raw_t) == 2 && ((uintptr_t)p.z & 2) ? 1 : 0;
+        p.pieces = (a.vocab - p.head) / P::kLen;
+        return p;
+    };
+    auto load_end = [&](const Place& p) { return ((const raw_t*)p.z)[min(p.end(tid), a.vocab - 1)]; };
     // (the thread's number is made to look new each time: the compiler would keep, and spill, an offset for every piece)
     auto piece_of = [&](int u) {
         int i = tid;
@@ -471,57 +487,47 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         return i + u * kRowThreads;
     };
     auto at_piece = [&](int u, int most) { return (uint32_t)min(piece_of(u), most) * 16u; };
-    auto load = [&](const char* z, int u, int most) { return P::load_once((const raw_t*)(z + at_piece(u, most))); };
-    // a thread's slots: the id (-1: empty; vocab: beyond it), the teacher's logit and the student's there
-    uint32_t id_lo[kOwn], id_hi[kOwn];
-    uint16_t y_lo[kOwn], y_hi[kOwn];
-    raw_t there[kOwn];
+    auto load = [&](const Place& p, int u, int most) { return P::load_once((const raw_t*)(p.z + p.head * sizeof(raw_t) + at_piece(u, most))); };
+    // a thread's slot: the id (-1: empty; vocab: beyond it), the teacher's logit and the student's there
+    uint32_t id_lo, id_hi;
+    uint16_t y_lo, y_hi;
+    raw_t there;
     const int id_size = a.wide_ids ? 8 : 4, y_size = a.teacher_dtype == DCIH_F32 ? 4 : 2;
     auto load_slots = [&](int64_t row) {
-        const char* ids = (const char*)a.ids + row * a.slots * id_size;
-        const char* ys = (const char*)a.teacher + row * a.slots * y_size;
-#pragma unroll
-        for (int o = 0; o < kOwn; o++) {
-            const uint32_t j = (uint32_t)min(o * kRowThreads + tid, a.slots - 1);
-            id_lo[o] = *(const uint32_t*)(ids + j * id_size);
-            id_hi[o] = *(const uint32_t*)(ids + (j + 1) * id_size - 4);
-            y_lo[o] = *(const uint16_t*)(ys + j * y_size);
-            y_hi[o] = *(const uint16_t*)(ys + (j + 1) * y_size - 2);
-        }
+        const uint32_t j = (uint32_t)min(tid, a.slots - 1);
+        const char* id = (const char*)a.ids + row * a.slots * id_size + j * id_size;
+        const char* y = (const char*)a.teacher + row * a.slots * y_size + j * y_size;
+        id_lo = *(const uint32_t*)id;
+        id_hi = *(const uint32_t*)(id + id_size - 4);
+        y_lo = *(const uint16_t*)y;
+        y_hi = *(const uint16_t*)(y + y_size - 2);
     };
-    auto id_of = [&](int o) {
-        const int64_t id = a.wide_ids ? (int64_t)((uint64_t)id_hi[o] << 32 | id_lo[o]) : (int64_t)(int32_t)id_lo[o];
-        return o * kRowThreads + tid >= a.slots || id < 0 ? -1 : (int)min(id, (int64_t)a.vocab);
+    auto id_of = [&]() {
+        const int64_t id = a.wide_ids ? (int64_t)((uint64_t)id_hi << 32 | id_lo) : (int64_t)(int32_t)id_lo;
+        return tid >= a.slots || id < 0 ? -1 : (int)min(id, (int64_t)a.vocab);
     };
-    auto y_of = [&](int o) {
-        const float y = a.teacher_dtype == DCIH_F16 ? (float)__builtin_bit_cast(_Float16, y_lo[o])
-                                                    : __builtin_bit_cast(float, (uint32_t)y_hi[o] << 16 | (y_size == 4 ? y_lo[o] : 0));
-        return id_of(o) < 0 ? kNoLogit : y;
+    auto y_of = [&]() {
+        const float y = a.teacher_dtype == DCIH_F16 ? (float)__builtin_bit_cast(_Float16, y_lo)
+                                                    : __builtin_bit_cast(float, (uint32_t)y_hi << 16 | (y_size == 4 ? y_lo : 0));
+        return id_of() < 0 ? kNoLogit : y;
     };
     auto load_there = [&](const char* z) {
-#pragma unroll
-        for (int o = 0; o < kOwn; o++) {
-            asm volatile("" : "+v"(id_lo[o]), "+v"(id_hi[o]));         // (not to be waited for before this place)
-            const int id = id_of(o);
-            there[o] = ((const raw_t*)z)[id >= 0 && id < a.vocab ? id : 0];
-        }
+        asm volatile("" : "+v"(id_lo), "+v"(id_hi));         // (not to be waited for before this place)
+        const int id = id_of();
+        there = ((const raw_t*)z)[id >= 0 && id < a.vocab ? id : 0];
     };
     int64_t row = blockIdx.x;
-    const char* z = row_of(row);
+    Place now = place_of(row);
     u32x4 raw[NV];
     load_slots(row);
-    raw_t raw_last = *(const raw_t*)(z + last_at);
-    load_there(z);
+    raw_t raw_end = load_end(now);
+    load_there(now.z);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < NV; u++) raw[u] = load(z, u, pieces - 1);
+    for (int u = 0; u < NV; u++) raw[u] = load(now, u, now.pieces - 1);
     while (true) {
-#pragma unroll
-        for (int o = 0; o < kOwn; o++) {
-            const float y = y_of(o);
-            s_id[o * kRowThreads + tid] = y == kNoLogit ? -1 : id_of(o);
-            s_y[o * kRowThreads + tid] = y;
-        }
+        s_id[tid] = y_of() == kNoLogit ? -1 : id_of();
+        s_y[tid] = y_of();
         __syncthreads();
         if (wave == 0) {      // while the row arrives
             Softmax t = Softmax::none();
@@ -540,7 +546,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         for (int u = 0; u < NV; u++) {
             float x[P::kLen];
             const u32x4 none = P::filled(kNoLogit);
-            const bool in = piece_of(u) < pieces;
+            const bool in = piece_of(u) < now.pieces;
             u32x4 piece = raw[u];
 #pragma unroll
             for (int k = 0; k < 4; k++) piece[k] = in ? piece[k] : none[k];
@@ -549,7 +555,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             __builtin_amdgcn_sched_barrier(0);           // (one piece unpacked at a time)
         }
         {
-            const float x[1] = {last < a.vocab ? (float)raw_last : kNoLogit};
+            const float x[1] = {now.end(tid) < a.vocab ? (float)raw_end : kNoLogit};
             f.add<1, false>(x, a.c2);
         }
         f.join_wave<false>(a.c2);
@@ -579,38 +585,31 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             P::unpack(raw[u], x);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) x[k] = gradient(x[k]);
-            P::store_once((raw_t*)(dz + at_piece(u, pieces - 1)), P::pack(x));
+            P::store_once((raw_t*)(dz + now.head * sizeof(raw_t) + at_piece(u, now.pieces - 1)), P::pack(x));
         };
         // (without a next row one piece of this one is read instead, by all)
         const bool more = row + gridDim.x < a.n;
         const int64_t next = more ? row + gridDim.x : row;
-        const int most = more ? pieces - 1 : 0;
-        const raw_t was_last = raw_last;
-        float zy[kOwn];
-#pragma unroll
-        for (int o = 0; o < kOwn; o++) zy[o] = (float)there[o];
-        z = row_of(next);
+        const Place then = place_of(next);
+        const int most = more ? then.pieces - 1 : 0;
+        const raw_t was_end = raw_end;
+        const float zy = (float)there;
         load_slots(next);
-        raw_last = *(const raw_t*)(z + last_at);
+        raw_end = load_end(then);
 #pragma unroll
         for (int u = 0; u < NV; u++) {
             put(u);
-            raw[u] = load(z, u, most);
-            if (u == (NV - 1) / 4) load_there(z);
+            raw[u] = load(then, u, most);
+            if (u == (NV - 1) / 4) load_there(then.z);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (last < a.vocab) ((raw_t*)dz)[last] = (raw_t)gradient((float)was_last);
+        if (now.end(tid) < a.vocab) ((raw_t*)dz)[now.end(tid)] = (raw_t)gradient((float)was_end);
         // the teacher's part: the loss, and its tokens, each by the first of the slots that name it
-        float loss = 0.f, q[kOwn];
-#pragma unroll
-        for (int o = 0; o < kOwn; o++) {
-            const int j = o * kRowThreads + tid;
-            const float q2 = (s_y[j] - t.x) * a.c2 - t.y;
-            const float logp = none ? kNoLogit : (zy[o] - m) * a.c2 - log2s;
-            q[o] = s_id[j] < 0 ? 0.f : exp2_fast(q2);
-            if (!(q[o] == 0.f)) loss += q[o] * (q2 - logp);
-            s_q[j] = q[o];
-        }
+        const int token = s_id[tid];
+        const float q2 = (s_y[tid] - t.x) * a.c2 - t.y, q = token < 0 ? 0.f : exp2_fast(q2);
+        const float logp = none ? kNoLogit : (zy - m) * a.c2 - log2s;
+        float loss = q == 0.f ? 0.f : q * (q2 - logp);
+        s_q[tid] = q;
         loss = wave_sum(loss);
         if (lane_id() == 0) s_sum[wave] = loss;
         __syncthreads();
@@ -620,22 +619,19 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             a.losses[row] = empty ? 0.f : t.w != 0.f ? __builtin_nanf("") : loss * kLn2;
             if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
         }
-        if (w != 0.f) {
-#pragma unroll
-            for (int o = 0; o < kOwn; o++) {
-                const int j = o * kRowThreads + tid, token = s_id[j];
-                if (token < 0 || token >= a.vocab) continue;
-                bool again = false;
-                for (int i = 0; i < j; i++) again |= s_id[i] == token;
-                if (again) continue;
-                float sum = q[o];
-                for (int i = j + 1; i < a.slots; i++) sum += s_id[i] == token ? s_q[i] : 0.f;
-                ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy[o] - m) * a.c2) - w * sum);
+        if (w != 0.f && token >= 0 && token < a.vocab) {
+            bool again = false;
+            for (int i = 0; i < tid; i++) again |= s_id[i] == token;
+            if (!again) {
+                float sum = q;
+                for (int i = tid + 1; i < a.slots; i++) sum += s_id[i] == token ? s_q[i] : 0.f;
+                ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy - m) * a.c2) - w * sum);
             }
         }
         __syncthreads();
         if (!more) return;
         row = next;
+        now = then;
     }
 }
 
@@ -654,11 +650,12 @@ int stats_by(LogitArgs a, hipStream_t s) {
     return 0;
 }
 
-// With rows enough that one wavefront each fills the device, one takes a row: nothing is to be joined.
-// (4096 x 50001 f16, five alternatives: TOPNEW us, 107 by four.)
+// With rows enough that one wavefront each fills the device, or too short for more, one takes a row:
+// nothing is to be joined.
 template <class T, int kMode>
 int stats_of(const LogitArgs& a, hipStream_t s) {
-    return a.n >= 4096 && a.vocab >= 2048 ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
+    const bool few = a.vocab <= 4 * kWave * Piece<T>::kLen;
+    return a.splits == 1 && (a.n >= 4096 || few) ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
 }
 
 template <class T, int kRowThreads, int NV>
@@ -671,13 +668,22 @@ int distill_rows_by(const LogitArgs& a, int per_unit, hipStream_t s) {
 
 constexpr int kMostPieces = 16 * 1024;       // of a row in registers
 
+// The fewest threads that hold a row in 16 pieces each and a slot each: several rows are on a compute unit then,
+// and one's sums run while others' bytes travel.  Fewer pieces where they do.
 template <class T>
 int distill_rows_of(const LogitArgs& a, hipStream_t s) {
     const int pieces = a.vocab / Piece<T>::kLen;
-    if (pieces <= 2 * 256) return distill_rows_by<T, 256, 2>(a, 6, s);
-    if (pieces <= 4 * 512) return distill_rows_by<T, 512, 4>(a, 3, s);
-    if (pieces <= 8 * 512) return distill_rows_by<T, 512, 8>(a, 2, s);
-    if (pieces <= 6 * 1024) return distill_rows_by<T, 1024, 6>(a, 1, s);
+    if (a.slots <= 256) {
+        if (pieces <= 4 * 256) return distill_rows_by<T, 256, 4>(a, 6, s);
+        if (pieces <= 8 * 256) return distill_rows_by<T, 256, 8>(a, 5, s);
+        if (pieces <= 16 * 256) return distill_rows_by<T, 256, 16>(a, 4, s);
+    }
+    if (a.slots <= 512) {
+        if (pieces <= 8 * 512) return distill_rows_by<T, 512, 8>(a, 2, s);
+        if (pieces <= 13 * 512) return distill_rows_by<T, 512, 13>(a, 2, s);
+        if (pieces <= 16 * 512) return distill_rows_by<T, 512, 16>(a, 2, s);
+    }
+    if (pieces <= 4 * 1024) return distill_rows_by<T, 1024, 4>(a, 1, s);
     if (pieces <= 8 * 1024) return distill_rows_by<T, 1024, 8>(a, 1, s);
     if (pieces <= 10 * 1024) return distill_rows_by<T, 1024, 10>(a, 1, s);
     if (pieces <= 13 * 1024) return distill_rows_by<T, 1024, 13>(a, 1, s);
@@ -727,8 +733,8 @@ int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
 
 // Enough rows that a workgroup each fills the device, and rows that fit one.
 bool distill_by_rows(const LogitArgs& a, int dtype) {
-    const int pieces = a.vocab / (16 / type_bytes(dtype));
-    return a.n >= 192 && pieces >= 1 && pieces <= kMostPieces;
+    const int len = 16 / type_bytes(dtype);
+    return a.n >= 192 && a.vocab > len && a.vocab / len <= kMostPieces;
 }
 
 int distill_rows(const LogitArgs& a, int dtype, hipStream_t s) {
