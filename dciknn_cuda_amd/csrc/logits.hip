@@ -22,8 +22,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int64_t kMaxGrid = 1 << 22; // workgroups of one launch (their threads are counted in 32 bits)
 constexpr int kTopWait = 8;          // candidates that a wavefront gathers before it puts them in order
-constexpr int kTopRoom = 320;        // room for candidates: those and four rounds of 64
-static_assert(kTopRoom >= kTopWait + 4 * kWave, "room for four rounds of candidates");
+constexpr int kTopRoom = 520;        // room for candidates: those and eight rounds of 64
+static_assert(kTopRoom >= kTopWait + 8 * kWave, "room for eight rounds of candidates");
 
 enum { kLogprobs = 0, kLogprobsTop = 1, kDistill = 2 };
 
@@ -71,7 +71,7 @@ __device__ inline u64 of_lane(u64 v, int lane) {
 }
 
 // The k best pieces a wavefront has met, or elements: lane i holds the i-th best of them.  Candidates wait in
-// LDS until there are more than a few, after four rounds of up to 64 at the latest, so that any order of
+// LDS until there are more than a few, after eight rounds of up to 64 at the latest, so that any order of
 // the row and any number of ties is taken.  No entry is 0 (index 2^32 - 1 does not exist).
 struct WaveTop {
     u64* wait;         // kTopRoom entries
@@ -139,10 +139,8 @@ __device__ void best_of_pieces(const LogitArgs& a, int64_t row, WaveTop& top) {
     P::unpack(Row<T>(a.z, row, a.stride, a.vocab).load(piece), x);
     top.best = top.least = 0;
 #pragma unroll
-    for (int k = 0; k < P::kLen; k++) {
-        top.push(have && x[k] >= bar, entry_of(x[k], piece * P::kLen + k));
-        if (k % 4 == 3) top.settle();
-    }
+    for (int k = 0; k < P::kLen; k++) top.push(have && x[k] >= bar, entry_of(x[k], piece * P::kLen + k));
+    top.settle();
 }
 
 // One wavefront: what is returned of a row of log probabilities.  `top`: its best pieces.
@@ -337,7 +335,7 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
             const u64* lists = a.part_top + (row * a.splits + min(lane, a.splits - 1)) * a.top;
             // The lists are in order: with k lists or more, the k-th largest of their first entries bounds
             // from below, and where no list has an entry above the bound at a place none has one behind it.
-            constexpr int kAhead = 4;
+            constexpr int kAhead = 8;
             u64 e[kAhead];
             for (int p = 0; p < a.top; p += kAhead) {
 #pragma unroll
@@ -349,12 +347,31 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
                 if (!__any(e[0] > top.least)) break;
 #pragma unroll
                 for (int j = 0; j < kAhead; j++) top.push(e[j] != 0, e[j]);
-                if (top.count > kTopRoom - kAhead * kWave) top.settle();
+                top.settle();
             }
             top.settle();
         }
         finish_logprobs<T>(a, row, f, top, t, (float)z_t);
     }
+}
+
+// What the slots that name `token` add up to, in their order, where `slot` is the first of them; -1 where it is not.
+// (A NaN stays one.)  `fours`: slots by fours, those beyond the last named by no token.
+__device__ inline float slots_of_token(const int* s_id, const float* s_q, int fours, int token, int slot) {
+    float sum = 0.f;
+    bool again = false;
+#pragma unroll 4
+    for (int i = 0; i < fours; i++) {
+        const int4 id = reinterpret_cast<const int4*>(s_id)[i];
+        const float4 q = reinterpret_cast<const float4*>(s_q)[i];
+        again |= (id.x == token && i * 4 < slot) || (id.y == token && i * 4 + 1 < slot) || (id.z == token && i * 4 + 2 < slot) ||
+                 (id.w == token && i * 4 + 3 < slot);
+        sum += id.x == token ? q.x : 0.f;
+        sum += id.y == token ? q.y : 0.f;
+        sum += id.z == token ? q.z : 0.f;
+        sum += id.w == token ? q.w : 0.f;
+    }
+    return again ? -1.f : sum;
 }
 
 // Gradients by the logits from a row's statistics, one tile of a row per workgroup.
@@ -363,8 +380,8 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     using P = Piece<T>;
     constexpr int kTile = kThreads * U;                  // pieces
     constexpr int kOwn = kTeacherSlots / kThreads;
-    __shared__ int s_id[kMode == kDistill ? kTeacherSlots : 1];
-    __shared__ float s_q[kMode == kDistill ? kTeacherSlots : 1];
+    __shared__ alignas(16) int s_id[kMode == kDistill ? kTeacherSlots : 1];
+    __shared__ alignas(16) float s_q[kMode == kDistill ? kTeacherSlots : 1];
     const int64_t at_row = a.first + blockIdx.x / (uint32_t)a.splits;
     const int tile = (int)(blockIdx.x % (uint32_t)a.splits) * kTile, tid = threadIdx.x;
     const Row<T> row(a.z, at_row, a.stride, a.vocab);
@@ -391,6 +408,8 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     bool here = false;
     if constexpr (kMode == kDistill) {
         if (!zero) {
+            if (tid < 4) s_id[(a.slots - 1) / 4 * 4 + tid] = -1;       // (those beyond the last)
+            __syncthreads();
 #pragma unroll
             for (int o = 0; o < kOwn; o++) {
                 const int j = o * kThreads + tid;
@@ -440,11 +459,8 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
             if (j >= a.slots) break;
             const int id = s_id[j];
             if (id < 0) continue;
-            bool again = false;
-            for (int i = 0; i < j; i++) again |= s_id[i] == id;
-            if (again) continue;
-            float q = 0.f;
-            for (int i = j; i < a.slots; i++) q += s_id[i] == id ? s_q[i] : 0.f;
+            const float q = slots_of_token(s_id, s_q, (a.slots + 3) / 4, id, j);
+            if (q < 0.f) continue;
             dz[id] = (typename T::raw)(c0 * (exp2_fast((own_z[o] - st.x) * a.c2 - st.y) - q));
         }
     }
@@ -460,26 +476,17 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
     using P = Piece<T>;
     using raw_t = typename T::raw;
     constexpr int kRowWaves = kRowThreads / kWave;
-    __shared__ int s_id[kRowThreads];
-    __shared__ float s_y[kRowThreads], s_q[kRowThreads];
+    __shared__ alignas(16) int s_id[kRowThreads];
+    __shared__ alignas(16) float s_q[kRowThreads];
+    __shared__ float s_y[kRowThreads];
     __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
     __shared__ float4 s_teacher;                         // max, log2 sum, whether there is one, whether its ids and logits are sound
     const int tid = threadIdx.x, wave = tid / kWave;
-    // A row is whole pieces from its first whole word on and, at both ends, up to a piece of elements that a
-    // thread each takes.
-    struct Place {
-        const char* z;
-        int head, pieces;
-        __device__ int end(int tid) const { return tid < head ? tid : pieces * P::kLen + tid; }
-    };
-    auto place_of = [&](int64_t row) {
-        Place p;
-        p.z = (const char*)a.z + row * a.stride * (int64_t)sizeof(raw_t);
-        p.head = sizeof(raw_t) == 2 && ((uintptr_t)p.z & 2) ? 1 : 0;
-        p.pieces = (a.vocab - p.head) / P::kLen;
-        return p;
-    };
-    auto load_end = [&](const Place& p) { return ((const raw_t*)p.z)[min(p.end(tid), a.vocab - 1)]; };
+    // whole pieces, and behind them less than one whose elements a thread each takes
+    const int pieces = a.vocab / P::kLen, end = pieces * P::kLen + tid;
+    const uint32_t end_at = (uint32_t)min(end, a.vocab - 1) * (uint32_t)sizeof(raw_t);
+    auto row_of = [&](int64_t row) { return (const char*)a.z + row * a.stride * (int64_t)sizeof(raw_t); };
+    auto load_end = [&](const char* z) { return *(const raw_t*)(z + end_at); };
     // (the thread's number is made to look new each time: the compiler would keep, and spill, an offset for every piece)
     auto piece_of = [&](int u) {
         int i = tid;
@@ -487,7 +494,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         return i + u * kRowThreads;
     };
     auto at_piece = [&](int u, int most) { return (uint32_t)min(piece_of(u), most) * 16u; };
-    auto load = [&](const Place& p, int u, int most) { return P::load_once((const raw_t*)(p.z + p.head * sizeof(raw_t) + at_piece(u, most))); };
+    auto load = [&](const char* z, int u, int most) { return P::load_once((const raw_t*)(z + at_piece(u, most))); };
     // a thread's slot: the id (-1: empty; vocab: beyond it), the teacher's logit and the student's there
     uint32_t id_lo, id_hi;
     uint16_t y_lo, y_hi;
@@ -517,14 +524,14 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         there = ((const raw_t*)z)[id >= 0 && id < a.vocab ? id : 0];
     };
     int64_t row = blockIdx.x;
-    Place now = place_of(row);
+    const char* z = row_of(row);
     u32x4 raw[NV];
     load_slots(row);
-    raw_t raw_end = load_end(now);
-    load_there(now.z);
+    raw_t raw_end = load_end(z);
+    load_there(z);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < NV; u++) raw[u] = load(now, u, now.pieces - 1);
+    for (int u = 0; u < NV; u++) raw[u] = load(z, u, pieces - 1);
     while (true) {
         s_id[tid] = y_of() == kNoLogit ? -1 : id_of();
         s_y[tid] = y_of();
@@ -546,7 +553,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         for (int u = 0; u < NV; u++) {
             float x[P::kLen];
             const u32x4 none = P::filled(kNoLogit);
-            const bool in = piece_of(u) < now.pieces;
+            const bool in = piece_of(u) < pieces;
             u32x4 piece = raw[u];
 #pragma unroll
             for (int k = 0; k < 4; k++) piece[k] = in ? piece[k] : none[k];
@@ -555,7 +562,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             __builtin_amdgcn_sched_barrier(0);           // (one piece unpacked at a time)
         }
         {
-            const float x[1] = {now.end(tid) < a.vocab ? (float)raw_end : kNoLogit};
+            const float x[1] = {end < a.vocab ? (float)raw_end : kNoLogit};
             f.add<1, false>(x, a.c2);
         }
         f.join_wave<false>(a.c2);
@@ -585,25 +592,25 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             P::unpack(raw[u], x);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) x[k] = gradient(x[k]);
-            P::store_once((raw_t*)(dz + now.head * sizeof(raw_t) + at_piece(u, now.pieces - 1)), P::pack(x));
+            P::store_once((raw_t*)(dz + at_piece(u, pieces - 1)), P::pack(x));
         };
         // (without a next row one piece of this one is read instead, by all)
         const bool more = row + gridDim.x < a.n;
         const int64_t next = more ? row + gridDim.x : row;
-        const Place then = place_of(next);
-        const int most = more ? then.pieces - 1 : 0;
+        const int most = more ? pieces - 1 : 0;
+        z = row_of(next);
         const raw_t was_end = raw_end;
         const float zy = (float)there;
         load_slots(next);
-        raw_end = load_end(then);
+        raw_end = load_end(z);
 #pragma unroll
         for (int u = 0; u < NV; u++) {
             put(u);
-            raw[u] = load(then, u, most);
-            if (u == (NV - 1) / 4) load_there(then.z);
+            raw[u] = load(z, u, most);
+            if (u == (NV - 1) / 4) load_there(z);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (now.end(tid) < a.vocab) ((raw_t*)dz)[now.end(tid)] = (raw_t)gradient((float)was_end);
+        if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)gradient((float)was_end);
         // the teacher's part: the loss, and its tokens, each by the first of the slots that name it
         const int token = s_id[tid];
         const float q2 = (s_y[tid] - t.x) * a.c2 - t.y, q = token < 0 ? 0.f : exp2_fast(q2);
@@ -620,18 +627,12 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
         }
         if (w != 0.f && token >= 0 && token < a.vocab) {
-            bool again = false;
-            for (int i = 0; i < tid; i++) again |= s_id[i] == token;
-            if (!again) {
-                float sum = q;
-                for (int i = tid + 1; i < a.slots; i++) sum += s_id[i] == token ? s_q[i] : 0.f;
-                ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy - m) * a.c2) - w * sum);
-            }
+            const float sum = slots_of_token(s_id, s_q, (a.slots + 3) / 4, token, tid);
+            if (!(sum < 0.f)) ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy - m) * a.c2) - w * sum);
         }
         __syncthreads();
         if (!more) return;
         row = next;
-        now = then;
     }
 }
 
@@ -673,6 +674,11 @@ constexpr int kMostPieces = 16 * 1024;       // of a row in registers
 template <class T>
 int distill_rows_of(const LogitArgs& a, hipStream_t s) {
     const int pieces = a.vocab / Piece<T>::kLen;
+    if (a.slots <= 64) {
+        if (pieces <= 4 * 64) return distill_rows_by<T, 64, 4>(a, 24, s);
+        if (pieces <= 8 * 64) return distill_rows_by<T, 64, 8>(a, 20, s);
+        if (pieces <= 16 * 64) return distill_rows_by<T, 64, 16>(a, 16, s);
+    }
     if (a.slots <= 256) {
         if (pieces <= 4 * 256) return distill_rows_by<T, 256, 4>(a, 6, s);
         if (pieces <= 8 * 256) return distill_rows_by<T, 256, 8>(a, 5, s);
@@ -731,10 +737,12 @@ int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
     }
 }
 
-// Enough rows that a workgroup each fills the device, and rows that fit one.
+// Rows that fit a workgroup's registers, by one workgroup each; where they are long, only if there are enough of
+// them: one of 131072 bf16 takes 22 us by one workgroup and 13 by three launches over the device, 64 25 and 24, 128 27
+// and 33; one of 32000 takes 11 and 13.
 bool distill_by_rows(const LogitArgs& a, int dtype) {
-    const int len = 16 / type_bytes(dtype);
-    return a.n >= 192 && a.vocab > len && a.vocab / len <= kMostPieces;
+    const int len = 16 / type_bytes(dtype), pieces = a.vocab / len;
+    return pieces >= 1 && pieces <= kMostPieces && (pieces <= 4096 || a.n >= 96);
 }
 
 int distill_rows(const LogitArgs& a, int dtype, hipStream_t s) {

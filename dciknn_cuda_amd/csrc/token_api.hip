@@ -1,6 +1,6 @@
 // The entry points of include/dci_hip.h that work on tokens: checks of the arguments, the caller's
 // workspace laid out, launches.  No handle, no state; nothing here allocates, waits or throws.
-#include <cmath>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/dci_hip.h"
@@ -24,6 +24,12 @@ const char* check_ids(const void* p, int id_bytes) {
     if (id_bytes != 4 && id_bytes != 8) return "ids are of 4 or 8 bytes";
     if (!p) return "null ids";
     return aligned(p, id_bytes) ? nullptr : "ids not aligned to their size";
+}
+
+bool all_aligned(std::initializer_list<const void*> arrays) {
+    for (const void* p : arrays)
+        if (!aligned(p, 4)) return false;
+    return true;
 }
 
 int refuse(const char* who, const char* why) { return fail(DCIH_EINVAL, std::string(who) + ": " + why); }
@@ -168,6 +174,7 @@ int dcih_token_logprobs(const void* d_logits, int dtype, int64_t num_rows, int v
     if (const char* why = check_ids(d_targets, id_bytes)) return refuse(who, why);
     if (!d_logprobs || !d_entropy || (top && (!d_top_ids || !d_top_logprobs))) return refuse(who, "null array");
     if (d_stats && !aligned(d_stats, 16)) return refuse(who, "statistics not aligned to 16 bytes");
+    if (!all_aligned({d_logprobs, d_entropy, d_top_ids, d_top_logprobs})) return refuse(who, "results not aligned to their elements");
     LogitArgs a = logit_args(d_logits, dtype, num_rows, vocab, row_stride, temperature, d_targets, id_bytes);
     if (const char* why = lay_out(a, top, false, d_work, work_bytes)) return refuse(who, why);
     a.top = top;
@@ -190,6 +197,7 @@ int dcih_token_logprobs_grad(const void* d_logits, int dtype, int64_t num_rows, 
     if (!d_stats || !aligned(d_stats, 16)) return refuse(who, "statistics missing or not aligned to 16 bytes");
     if (const char* why = check_grad(d_logits, d_grad, dtype, num_rows, vocab, row_stride, grad_stride)) return refuse(who, why);
     LogitArgs a = logit_args(d_logits, dtype, num_rows, vocab, row_stride, temperature, d_targets, id_bytes);
+    if (!all_aligned({d_grad_logprobs, d_grad_entropy})) return refuse(who, "factors not aligned to their elements");
     a.stats = (float4*)d_stats;
     a.grad_logprobs = d_grad_logprobs;
     a.grad_entropy = d_grad_entropy;
@@ -207,6 +215,7 @@ int dcih_distill(const void* d_logits, int dtype, int64_t num_rows, int vocab, i
     if (!num_rows) return DCIH_OK;
     if (const char* why = check_teacher(d_teacher, teacher_dtype, slots, d_ids, id_bytes)) return refuse(who, why);
     if (!d_losses) return refuse(who, "null array");
+    if (!all_aligned({d_losses, d_weights})) return refuse(who, "losses or weights not aligned to their elements");
     if (d_stats && !aligned(d_stats, 16)) return refuse(who, "statistics not aligned to 16 bytes");
     if (d_grad)
         if (const char* why = check_grad(d_logits, d_grad, dtype, num_rows, vocab, row_stride, grad_stride)) return refuse(who, why);
@@ -241,6 +250,7 @@ int dcih_distill_grad(const void* d_logits, int dtype, int64_t num_rows, int voc
     a.stats = (float4*)d_stats;
     a.teacher = d_teacher;
     a.teacher_dtype = teacher_dtype;
+    if (!all_aligned({d_weights})) return refuse(who, "weights not aligned to their elements");
     a.slots = slots;
     a.weights = d_weights;
     a.grad = d_grad;

@@ -145,7 +145,9 @@ template <class T> struct Row {
             for (int u = 0; u < U; u++) raw[u] = Piece<T>::load_once(z + (int64_t)(piece + u * step) * kLen);
             return;
         }
-        const uint32_t* w = (const uint32_t*)(z - 1);
+        // (rounded down as a number: a scalar load drops the low bits of its base and of its offset each, so a base of
+        // z - 1 with the odd z in a register would miss by a word)
+        const uint32_t* w = (const uint32_t*)((uintptr_t)z & ~(uintptr_t)3);
         const int behind = __builtin_amdgcn_readfirstlane(piece) + kWave;        // the piece behind the last lane's
         uint32_t last[U];
 #pragma unroll

@@ -153,6 +153,26 @@ def test_lookup_gradient_by_autograd(gpu):
         torch.autograd.grad(gpu.embed(table, ids), table, torch.ones_like(x).requires_grad_(), create_graph=True)
 
 
+@pytest.mark.parametrize("n,v,d,dtype", [(2048, 5, 40, "bf16"), (2049, 5, 40, "bf16"), (4097, 300_000, 24, "f32"), (70_000, 20_000, 40, "f16"),
+                                         (5000, 2_200_000, 4, "f32"), (200_000, 3, 8, "f32"), (9000, 70, 1030, "f16"), (2500, 3_000_000, 3, "bf16")])
+def test_lookup_gradient_of_many_tokens(gpu, n, v, d, dtype):
+    """Tokens in chunks and buckets, more rows than a bucket counts at a time, every seventh token of one row."""
+    r = gen(n)
+    ids = np.where(np.arange(n) % 7 == 3, v // 2, r.integers(-1, v + 1, n))
+    d_ids, grad = on_gpu(ids, torch.int64), on_gpu(r.normal(size=(n, d)).astype(np.float32), TYPES[dtype])
+    got = gpu.embed_grad(grad, d_ids, v, 0.5)
+    valid = (d_ids >= 0) & (d_ids < v)
+    want = torch.zeros(v, d, dtype=torch.float64, device="cuda").index_add_(0, d_ids[valid], grad[valid].double() * 0.5)
+    size = torch.zeros(v, d, dtype=torch.float64, device="cuda").index_add_(0, d_ids[valid], grad[valid].double().abs() * 0.5)
+    count = torch.bincount(d_ids[valid], minlength=v).double()[:, None]
+    far = (got.double() - want).abs() - HALF_UNIT[dtype] * want.abs() * 1.01 - LEAST[dtype] - (count + 2) * 2.0 ** -24 * size
+    assert (far <= 0).all() and torch.equal(got, gpu.embed_grad(grad, d_ids.int(), v, 0.5))
+    base = torch.randn(v, d, device="cuda")
+    into = gpu.embed_grad(grad, d_ids, v, 0.5, out=base.clone())
+    far = (into.double() - want - base.double()).abs() - ((count + 3) * 2.0 ** -24) * (size + base.double().abs())
+    assert (far <= 0).all() and torch.equal(into[count[:, 0] == 0], base[count[:, 0] == 0])
+
+
 def test_many_tokens_of_few_rows(gpu):
     n, d = 131_072, 24
     ids = torch.zeros(n, dtype=torch.int64, device="cuda")
@@ -300,6 +320,41 @@ def test_distillation(gpu, dtype, n, v, k, spread):
     z.requires_grad_()
     dz, = torch.autograd.grad(gpu.distill_loss(z, d_ids, d_teacher, 1.5), z, d_w)
     near(dz, ref, size, dtype)
+
+
+# Rows that a workgroup holds, by every number of threads and pieces, more rows than workgroups, rows just too long.
+@pytest.mark.parametrize("n,v,k,dtype", [
+    (5, 8, 3, "f16"), (5, 9, 3, "bf16"), (3, 4, 2, "f32"), (40, 2047, 64, "f16"), (40, 4100, 64, "bf16"), (40, 8191, 64, "f16"), (40, 8190, 65, "bf16"),
+    (40, 16_000, 100, "f16"), (40, 32_767, 256, "bf16"), (40, 16_383, 100, "f32"), (40, 20_000, 300, "f16"), (97, 50_001, 512, "f16"),
+    (97, 65_533, 10, "bf16"), (40, 30_000, 600, "f16"), (97, 60_000, 1024, "bf16"), (97, 81_917, 64, "f16"), (97, 106_001, 64, "bf16"),
+    (97, 131_072, 64, "bf16"), (97, 65_536, 64, "f32"), (97, 131_080, 64, "bf16"), (300, 66_001, 20, "f16"), (6200, 40, 5, "f32"), (1100, 9000, 70, "f16")])
+def test_distillation_by_rows(gpu, n, v, k, dtype):
+    r = gen(n + v + k)
+    z = on_gpu((r.normal(size=(n, v)) * 2).astype(np.float32), TYPES[dtype])
+    ids, teacher = _teacher(r, n, v, k, max(2, v // 3))
+    weights = np.where(r.random(n) < 0.1, 0.0, r.normal(size=n))
+    d_teacher, d_w = on_gpu(teacher, torch.float32), on_gpu(weights, torch.float32)
+    want, ref, size = O.distill(f64(z), ids, f64(d_teacher), 0.7, f64(d_w))
+    losses, grad = gpu.distill_step(z, on_gpu(ids, torch.int64), d_teacher, d_w, 0.7)
+    near_abs(losses, want, 2 * SUM)
+    near(grad, ref, size, dtype)
+    assert torch.equal(gpu.distill_step(z, on_gpu(ids, torch.int32), d_teacher, d_w, 0.7, out=z)[1], grad) and torch.equal(z, grad)
+
+
+# One wavefront a row: enough rows, or short ones.
+@pytest.mark.parametrize("n,v,dtype", [(4100, 801, "f16"), (4096, 2049, "bf16"), (4097, 1500, "f32"), (2000, 2047, "bf16"), (1500, 1024, "f32"), (5000, 4111, "f16")])
+def test_token_logprobs_by_wavefronts(gpu, n, v, dtype):
+    r = gen(n + v)
+    z = on_gpu(_logits(r, n, v).astype(np.float32), TYPES[dtype])
+    targets = r.integers(-1, v, n)
+    for top in (0, 7, 64):
+        want = O.token_logprobs(f64(z), targets, top, 0.9)
+        got = gpu.token_logprobs(z, on_gpu(targets, torch.int64), top, 0.9)
+        near_abs(got[0], want[0], SUM)
+        near_abs(got[1], want[1], 20 * SUM)
+        if top:
+            assert np.array_equal(got[2].cpu().numpy(), want[2])
+            near_abs(got[3], want[3], SUM)
 
 
 @pytest.mark.parametrize("teacher_dtype", ["f32", "bf16", "f16"])

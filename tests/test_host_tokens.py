@@ -38,6 +38,7 @@ def test_entry_points_refuse(oracle):
                 dict(stats=A + 4), dict(work=None), dict(size=need // 2)):
         assert logp(**bad) == inval, bad
     assert logp(v=4, stride=4) == inval                       # five alternatives of four
+    assert all(logp(**bad) == inval for bad in (dict(lp=A + 2), dict(h=A + 1), dict(ids=A + 2), dict(lps=A + 3)))
     back = lambda z=A, n=4, v=9, stride=9, t=A, stats=A, grad=1 << 24, gs=9: lib.dcih_token_logprobs_grad(   # noqa: E731
         z, 0, n, v, stride, t, 8, 1.0, stats, None, None, grad, gs, None)
     for bad in (dict(z=None), dict(t=None), dict(stats=None), dict(stats=A + 4), dict(grad=None), dict(gs=8), dict(grad=A + 4), dict(grad=A, gs=12)):
@@ -45,7 +46,7 @@ def test_entry_points_refuse(oracle):
     distill = lambda z=A, n=4, v=9, ids=A, width=8, t=A, kind=0, k=3, temp=1.0, loss=A, stats=None, grad=None, gs=9, work=A, size=1 << 20: (   # noqa: E731
         lib.dcih_distill(z, 0, n, v, 9, ids, width, t, kind, k, temp, loss, stats, None, grad, gs, work, size, None))
     for bad in (dict(z=None), dict(v=10), dict(ids=None), dict(width=0), dict(t=None), dict(kind=5), dict(k=0), dict(k=1025), dict(temp=0.0), dict(loss=None),
-                dict(stats=A + 8), dict(grad=A + 4), dict(grad=1 << 24, gs=8), dict(grad=1 << 24, size=63), dict(grad=1 << 24, work=None)):
+                dict(loss=A + 2), dict(stats=A + 8), dict(grad=A + 4), dict(grad=1 << 24, gs=8), dict(grad=1 << 24, size=63), dict(grad=1 << 24, work=None)):
         assert distill(**bad) == inval, bad
     assert lib.dcih_distill_grad(A, 0, 4, 9, 9, A, 8, A, 0, 3, 1.0, None, None, 1 << 24, 9, None) == inval
     assert lib.dcih_distill_grad(A, 0, 4, 9, 9, A, 8, A, 0, 0, 1.0, A, None, 1 << 24, 9, None) == inval
