@@ -475,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(EmbedArgs a, Work w, int
 }
 
 // ---- few tokens --------------------------------------------------------------------------
-constexpr int kFew = 2048, kFewLanes = kFew / kGroupThreads;
+constexpr int kFew = 4096, kFewLanes = kFew / kGroupThreads;
 constexpr int kFewRows = 256;        // rows of a workgroup at most
 
 // Up to kFew tokens by one launch: a workgroup reads all ids, puts the tokens of its `rows` rows in
@@ -499,6 +499,11 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
         const int64_t id = i < n ? id_at(a.ids, a.wide_ids, i) : -1;
         bin[j] = id >= row0 && id < min(a.num_rows, row0 + rows) ? (int)(id - row0) : -1;
     }
+    // all of its rows are zeros first, few are written again: nothing is waited for before these bytes leave
+    const int group = tid / lanes, groups = kGroupThreads / lanes, c = ((int)blockIdx.y * lanes + tid % lanes) * P::kLen;
+    const bool in = c < a.dim, whole = c + P::kLen <= a.dim;
+    if (in && !a.accumulate)
+        for (int r = group; r < rows && row0 + r < a.num_rows; r += groups) put_zeros<O, P::kLen>(a, row0 + r, c);
     for (int i = tid; i < kGroupWaves * kFewRows; i += kGroupThreads) s_count[i] = 0;
     __syncthreads();
     uint32_t* mine = s_count + wave * kFewRows;
@@ -532,12 +537,6 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     for (int j = 0; j < kFewLanes; j++)
         if (bin[j] >= 0) s_token[mine[bin[j]] + rank[j]] = (uint32_t)bin[j] << 16 | (uint32_t)((wave * kFewLanes + j) * kWave + lane);
     __syncthreads();
-    const int group = tid / lanes, groups = kGroupThreads / lanes, c = ((int)blockIdx.y * lanes + tid % lanes) * P::kLen;
-    const bool in = c < a.dim, whole = c + P::kLen <= a.dim;
-    // rows without tokens
-    if (in && !a.accumulate)
-        for (int r = group; r < rows && row0 + r < a.num_rows; r += groups)
-            if (s_start[r] == s_start[r + 1]) put_zeros<O, P::kLen>(a, row0 + r, c);
     const int share = ((int)all + groups - 1) / groups;
     const int from = min((int)all, group * share), to = min((int)all, from + share);
     float sum[P::kLen];

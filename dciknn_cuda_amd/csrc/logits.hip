@@ -585,14 +585,19 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         const float w = none || empty ? 0.f : weight * a.inv_t;
         char* dz = (char*)a.grad + row * a.grad_stride * (int64_t)sizeof(raw_t);
         const float share = w * exp2_fast(-log2s);           // the row's factor / the sum of the powers
-        auto gradient = [&](float x) { return w == 0.f ? 0.f : share * exp2_fast((x - m) * a.c2); };
+        // (a row without weight has gradient 0 whatever it holds: by the bits)
+        const uint32_t kept = w == 0.f ? 0u : ~0u;
+        auto gradient = [&](float x) { return share * exp2_fast((x - m) * a.c2); };
         auto put = [&](int u) {
             asm volatile("" : "+v"(raw[u]));             // (keeps the pieces packed: not the 32-bit values of the sums)
             float x[P::kLen];
             P::unpack(raw[u], x);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) x[k] = gradient(x[k]);
-            P::store_once((raw_t*)(dz + at_piece(u, pieces - 1)), P::pack(x));
+            u32x4 out = P::pack(x);
+#pragma unroll
+            for (int k = 0; k < 4; k++) out[k] &= kept;
+            P::store_once((raw_t*)(dz + at_piece(u, pieces - 1)), out);
         };
         // (without a next row one piece of this one is read instead, by all)
         const bool more = row + gridDim.x < a.n;
@@ -610,7 +615,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             if (u == (NV - 1) / 4) load_there(z);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)gradient((float)was_end);
+        if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)(kept ? gradient((float)was_end) : 0.f);
         // the teacher's part: the loss, and its tokens, each by the first of the slots that name it
         const int token = s_id[tid];
         const float q2 = (s_y[tid] - t.x) * a.c2 - t.y, q = token < 0 ? 0.f : exp2_fast(q2);
