@@ -497,12 +497,12 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     const int64_t block = first + blockIdx.x;
     const uint32_t run = (1u << run_bits) - 1;
     auto row_of_bin = [&](int bin) { return (((int64_t)(bin >> run_bits) * blocks + block) << run_bits) + (bin & run); };
-    const int n = (int)a.n;
+    const int n = (int)a.n, per = (n + kGroupThreads - 1) / kGroupThreads;      // rounds of 64 tokens for each wavefront
     int bin[kFewLanes], rank[kFewLanes];
 #pragma unroll
     for (int j = 0; j < kFewLanes; j++) {
-        const int i = (wave * kFewLanes + j) * kWave + lane;
-        const int64_t id = i < n ? id_at(a.ids, a.wide_ids, i) : -1;
+        const int i = (wave * per + j) * kWave + lane;
+        const int64_t id = j < per && i < n ? id_at(a.ids, a.wide_ids, i) : -1;
         bin[j] = -1;
         if (id >= 0 && id < a.num_rows) {
             const uint32_t r = (uint32_t)id >> run_bits, turn = r / (uint32_t)blocks;
@@ -520,6 +520,7 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     uint32_t* mine = s_count + wave * kFewRows;
 #pragma unroll
     for (int j = 0; j < kFewLanes; j++) {
+        if (j >= per) break;
         const unsigned long long here = __ballot(bin[j] >= 0);
         if (!here) continue;
         const unsigned long long same = same_key(here, (uint32_t)bin[j], 8);         // 2^8 = kFewRows
@@ -546,7 +547,7 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kFewLanes; j++)
-        if (bin[j] >= 0) s_token[mine[bin[j]] + rank[j]] = (uint32_t)bin[j] << 16 | (uint32_t)((wave * kFewLanes + j) * kWave + lane);
+        if (bin[j] >= 0) s_token[mine[bin[j]] + rank[j]] = (uint32_t)bin[j] << 16 | (uint32_t)((wave * per + j) * kWave + lane);
     __syncthreads();
     const int share = ((int)all + groups - 1) / groups;
     const int from = min((int)all, group * share), to = min((int)all, from + share);
