@@ -205,11 +205,20 @@ __device__ inline void for_tokens(const Work& w, int64_t chunk, uint32_t o0, uin
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const uint32_t at = t + j * kWave + lane_id();
-            int lane = 0;                            // the last one that starts at or before `at`: the one that holds it
+            // the lane that holds it is the last one that starts at or before it: often the same one for all 64
+            int lane = __popcll(__ballot(mine <= t + j * kWave)) - 1;
+            uint32_t first, before;
+            if (lane == __popcll(__ballot(mine <= t + j * kWave + kWave - 1)) - 1) {
+                first = (uint32_t)__builtin_amdgcn_readlane((int)o0, lane);
+                before = (uint32_t)__builtin_amdgcn_readlane((int)mine, lane);
+            } else {
+                lane = 0;
 #pragma unroll
-            for (int step = kWave / 2; step; step /= 2)
-                if ((uint32_t)__shfl((int)mine, lane + step) <= at) lane += step;
-            const uint32_t first = (uint32_t)__shfl((int)o0, lane), before = (uint32_t)__shfl((int)mine, lane);
+                for (int step = kWave / 2; step; step /= 2)
+                    if ((uint32_t)__shfl((int)mine, lane + step) <= at) lane += step;
+                first = (uint32_t)__shfl((int)o0, lane);
+                before = (uint32_t)__shfl((int)mine, lane);
+            }
             p[j] = Placed{0, 0};
             if (at < total) p[j] = w.placed[(chunk + lane) * kChunk + first + (at - before)];
         }
@@ -315,7 +324,11 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
         __syncthreads();
         each_token([&](Placed p, bool real) {
             const uint32_t bin = bin_of(w, p.row) - (uint32_t)bin0;
-            if (real && bin < kBins) atomicAdd(&s_count[wave][bin], 1u);
+            const bool mine = real && bin < kBins;
+            // the first lane's row by one addition for all its tokens: a bucket of many has mostly one row
+            const uint32_t lead = (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+            const unsigned long long same = __ballot(mine && bin == lead);
+            if (mine && (bin != lead || lanes_below(same) == 0)) atomicAdd(&s_count[wave][bin], bin == lead ? (uint32_t)__popcll(same) : 1u);
         });
         __syncthreads();
         uint32_t len = 0, all;
@@ -337,7 +350,8 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
             each_token([&](Placed p, bool real) {
                 const uint32_t bin = bin_of(w, p.row) - (uint32_t)bin0;
                 const bool mine = real && bin < kBins;
-                const unsigned long long same = same_key(__ballot(mine), bin, 10);       // 2^10 = kBins
+                const unsigned long long here = __ballot(mine), led = __ballot(mine && bin == (uint32_t)__builtin_amdgcn_readfirstlane((int)bin));
+                const unsigned long long same = here == led ? here : same_key(here, bin, 10);       // 2^10 = kBins
                 if (mine) {
                     const uint32_t rank = s_count[wave][bin] + lanes_below(same);
                     if (lanes_below(same) == 0) s_count[wave][bin] = rank + __popcll(same);
@@ -437,8 +451,9 @@ __device__ void join_row(const EmbedArgs& a, const Work& w, uint32_t at, int sli
             }
 #pragma unroll
             for (int j = 0; j < kAhead; j++) {
-                if (p0 + j * kGroups >= pieces) break;
-                sum.x += x[j].x; sum.y += x[j].y; sum.z += x[j].z; sum.w += x[j].w;
+                // (no branch: the compiler would move the loads behind it, to wait for one at a time)
+                const bool in = p0 + j * kGroups < pieces;
+                sum.x += in ? x[j].x : 0.f; sum.y += in ? x[j].y : 0.f; sum.z += in ? x[j].z : 0.f; sum.w += in ? x[j].w : 0.f;
             }
         }
     }
@@ -665,7 +680,7 @@ int grad(const EmbedArgs& a, hipStream_t s) {
         DCIH_HIP(hipGetLastError());
     }
     // groups of workgroups that fill the device, no more than there can be such rows
-    const int wide = (int)std::min<int64_t>(a.n / (w.piece * kWide + 1), 64), groups = (int)std::min<int64_t>(a.n / (w.piece + 1), 1024);
+    const int wide = (int)std::min<int64_t>(a.n / (w.piece * kWide + 1), 16), groups = (int)std::min<int64_t>(a.n / (w.piece + 1), 1024);
     const int64_t blocks = (int64_t)wide * ((a.dim + 63) / 64) + (int64_t)groups * ((a.dim + kThreads * 4 - 1) / (kThreads * 4));
     join_kernel<O><<<(uint32_t)blocks, kThreads, 0, s>>>(a, w, wide, groups);
     DCIH_HIP(hipGetLastError());
