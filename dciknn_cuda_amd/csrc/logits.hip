@@ -225,6 +225,8 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
 // every kRowThreads-th piece; a wavefront keeps its best pieces, too, and what one of them
 // finds to be the least that can still be among the best bounds the others' as well.  (Keeping
 // elements instead of pieces doubled the arithmetic, which is what bounds this kernel with alternatives.)
+// Without alternatives bound by memory: 8192 x 32000 f32 160 us (6.5 TB/s read), 4096 x 50000 bf16 70 us (5.9); with five of
+// them by its instructions: 78 us there, 84 for 4096 x 50001 f16, whose rows start within words.
 template <class T, int kMode, int kRowThreads, int U>
 __global__ __launch_bounds__(kRowThreads, 8) void logit_stats_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -313,7 +315,8 @@ __global__ __launch_bounds__(kRowThreads, 8) void logit_stats_kernel(LogitArgs a
     else finish_logprobs<T>(a, at_row, f, top, t, (float)z_t);
 }
 
-// Joins the splits (up to 64) of a row: one wavefront each.
+// Joins the splits (up to 64) of a row: one wavefront each.  Bound by waits: 6.8 us for 4 rows of 64 splits with 20
+// alternatives, as long as logit_stats_kernel takes for their 131072 bf16 each.
 template <class T, int kMode>
 __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
     __shared__ u64 s_top[kMode == kLogprobsTop ? kTopRoom : 1];
@@ -374,7 +377,9 @@ __device__ inline float slots_of_token(const int* s_id, const float* s_q, int fo
     return again ? -1.f : sum;
 }
 
-// Gradients by the logits from a row's statistics, one tile of a row per workgroup.
+// Gradients by the logits from a row's statistics, one tile of a row per workgroup: nothing is to be joined, so the
+// tiles are small and many.  Bound by memory: 8192 x 32000 f32 335 us (6.3 TB/s: part of what logit_stats_kernel read last
+// is in the last-level cache still).
 template <class T, int kMode, int U>
 __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -471,6 +476,8 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
 // pieces leave: the next row's loads take their registers and travel beside the stores.  Memory
 // operations are waited for in their order and counted where their number is known, so there are no branches about
 // them: beyond the row's end a thread reads (and writes, the same values again) the last piece once more.
+// Bound by memory: 8192 x 131072 bf16 868 us (4.9 TB/s read and written; a copy reaches 4.8); 1001 x 100003 f16, rows
+// that start at odd addresses, 120 us (3.3 TB/s, with four rows a workgroup at most hardly past its start).
 template <class T, int kRowThreads, int NV>
 __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -656,12 +663,16 @@ int stats_by(LogitArgs a, hipStream_t s) {
     return 0;
 }
 
-// With rows enough that one wavefront each fills the device, or too short for more, one takes a row:
-// nothing is to be joined.
+// With alternatives one wavefront takes a row where there are rows enough to fill the device, or rows too short for more:
+// each wavefront of a row has best pieces of its own to find (8192 x 32000 bf16 with 5 of them 94 us, 115 by four
+// wavefronts a row; 1024 x 1000 7.1 and 8.8; but 1024 x 50000 43 and 32).  Without, four take 81 us and one 85.
 template <class T, int kMode>
 int stats_of(const LogitArgs& a, hipStream_t s) {
-    const bool few = a.vocab <= 4 * kWave * Piece<T>::kLen;
-    return a.splits == 1 && (a.n >= 4096 || few) ? stats_by<T, kMode, kWave>(a, s) : stats_by<T, kMode, kThreads>(a, s);
+    if constexpr (kMode == kLogprobsTop) {
+        const bool few = a.vocab <= 4 * kWave * Piece<T>::kLen;
+        if (a.splits == 1 && (a.n >= 4096 || few)) return stats_by<T, kMode, kWave>(a, s);
+    }
+    return stats_by<T, kMode, kThreads>(a, s);
 }
 
 template <class T, int kRowThreads, int NV>
