@@ -358,23 +358,20 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
     }
 }
 
-// What the slots that name `token` add up to, in their order, where `slot` is the first of them; -1 where it is not.
-// (A NaN stays one.)  `fours`: slots by fours, those beyond the last named by no token.
-__device__ inline float slots_of_token(const int* s_id, const float* s_q, int fours, int token, int slot) {
+// What the slots that name `token` add up to, in their order.  Slots that name the same one get the same bits, and may all
+// write what they make of them.  `fours`: slots by fours, those beyond the last named by no token.
+__device__ inline float slots_of_token(const int* s_id, const float* s_q, int fours, int token) {
     float sum = 0.f;
-    bool again = false;
 #pragma unroll 4
     for (int i = 0; i < fours; i++) {
         const int4 id = reinterpret_cast<const int4*>(s_id)[i];
         const float4 q = reinterpret_cast<const float4*>(s_q)[i];
-        again |= (id.x == token && i * 4 < slot) || (id.y == token && i * 4 + 1 < slot) || (id.z == token && i * 4 + 2 < slot) ||
-                 (id.w == token && i * 4 + 3 < slot);
         sum += id.x == token ? q.x : 0.f;
         sum += id.y == token ? q.y : 0.f;
         sum += id.z == token ? q.z : 0.f;
         sum += id.w == token ? q.w : 0.f;
     }
-    return again ? -1.f : sum;
+    return sum;
 }
 
 // Gradients by the logits from a row's statistics, one tile of a row per workgroup: nothing is to be joined, so the
@@ -457,15 +454,14 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     if constexpr (kMode == kDistill) {
         if (!here) return;
         __syncthreads();
-        // the teacher's tokens, each by the first of the slots that name it
+        // the teacher's tokens
 #pragma unroll
         for (int o = 0; o < kOwn; o++) {
             const int j = o * kThreads + tid;
             if (j >= a.slots) break;
             const int id = s_id[j];
             if (id < 0) continue;
-            const float q = slots_of_token(s_id, s_q, (a.slots + 3) / 4, id, j);
-            if (q < 0.f) continue;
+            const float q = slots_of_token(s_id, s_q, (a.slots + 3) / 4, id);
             dz[id] = (typename T::raw)(c0 * (exp2_fast((own_z[o] - st.x) * a.c2 - st.y) - q));
         }
     }
@@ -623,7 +619,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             __builtin_amdgcn_sched_barrier(0);
         }
         if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)(kept ? gradient((float)was_end) : 0.f);
-        // the teacher's part: the loss, and its tokens, each by the first of the slots that name it
+        // the teacher's part: the loss, and its tokens
         const int token = s_id[tid];
         const float q2 = (s_y[tid] - t.x) * a.c2 - t.y, q = token < 0 ? 0.f : exp2_fast(q2);
         const float logp = none ? kNoLogit : (zy - m) * a.c2 - log2s;
@@ -639,8 +635,8 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
         }
         if (w != 0.f && token >= 0 && token < a.vocab) {
-            const float sum = slots_of_token(s_id, s_q, (a.slots + 3) / 4, token, tid);
-            if (!(sum < 0.f)) ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy - m) * a.c2) - w * sum);
+            const float sum = slots_of_token(s_id, s_q, (a.slots + 3) / 4, token);
+            ((raw_t*)dz)[token] = (raw_t)(share * exp2_fast((zy - m) * a.c2) - w * sum);
         }
         __syncthreads();
         if (!more) return;
