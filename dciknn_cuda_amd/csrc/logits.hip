@@ -721,12 +721,14 @@ int grad_of(LogitArgs a, hipStream_t s) {
 
 }  // namespace
 
-// Workgroups a row is split over: enough of them in all to fill the device, each with one
-// round of loads at least.
+// Workgroups a row is split over: enough of them in all to fill the device, each with a round of loads of all its threads
+// at least, and none of rows that are done before splits could be joined (4 rows of 16000 bf16: 4.2 us by a workgroup each,
+// 4.9 by 8 and the join, with 10 alternatives 11.9 and 12.5; 800: 8.4 and 10.2; but 4 of 50000 8.3 and 4.8, 500 16.3 and 15.1).
 int logit_splits(int64_t n, int vocab, int dtype) {
     const int64_t pieces = ((int64_t)vocab * type_bytes(dtype) + 15) / 16;
+    if (pieces <= 8 * kThreads) return 1;
     const int64_t most = (pieces + kThreads - 1) / kThreads, want = (1024 + n - 1) / n;
-    return (int)(want < 1 ? 1 : want > most ? (most > kMaxSplits ? kMaxSplits : most) : want > kMaxSplits ? kMaxSplits : want);
+    return (int)std::min<int64_t>(std::min(most, std::max<int64_t>(want, 1)), kMaxSplits);
 }
 
 int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
