@@ -50,7 +50,7 @@ __device__ inline void wave_fence() {
 // One step of a bitonic sort over the lanes, larger ones first: towards runs of SIZE.
 template <int SIZE, int STRIDE, class V>
 __device__ inline void sort_step(V& v) {
-    const V o = lane_xor<STRIDE>(v);
+    const V o = other_lane<STRIDE>(v);
     const bool larger = ((lane_id() & STRIDE) == 0) == (SIZE == kWave || (lane_id() & SIZE) == 0);
     v = (o > v) == larger ? o : v;
 }
@@ -212,7 +212,7 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
         const float logp = none ? kNoLogit : ((float)z[id] - f.m) * a.c2 - log2s;
         if (!(q == 0.f)) sum += q * (logq - logp);
     }
-    sum = wave_sum(sum) * kLn2;
+    sum = sum_of_lanes(sum) * kLn2;
     if (wrong || t.s != t.s) sum = log2s = __builtin_nanf("");
     if (empty) sum = 0.f;
     if (lane_id() == 0) {
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         const float logp = none ? kNoLogit : (zy - m) * a.c2 - log2s;
         float loss = q == 0.f ? 0.f : q * (q2 - logp);
         s_q[tid] = q;
-        loss = wave_sum(loss);
+        loss = sum_of_lanes(loss);
         if (lane_id() == 0) s_sum[wave] = loss;
         __syncthreads();
         if (tid == 0) {

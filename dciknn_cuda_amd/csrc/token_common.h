@@ -195,9 +195,34 @@ constexpr float kLog2e = 1.44269504088896341f;
 // factor themselves, so that a ruled-out entry adds 0 * -256 and not 0 * -inf.
 constexpr float kFloor2 = -256.f;
 
-__device__ inline float wave_max(float v) {
-    v = fmaxf(v, lane_xor<32>(v)); v = fmaxf(v, lane_xor<16>(v)); v = fmaxf(v, lane_xor<8>(v));
-    v = fmaxf(v, lane_xor<4>(v)); v = fmaxf(v, lane_xor<2>(v)); v = fmaxf(v, lane_xor<1>(v));
+// What lane (this one ^ O) holds, without the wait for LDS that lane_xor's swizzles by 4, 8 and 16 are.
+template <int O> __device__ inline uint32_t other_lane(uint32_t v) {
+    if constexpr (O == 4) {           // of 8 lanes in reverse, each four in reverse
+        return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);
+    } else if constexpr (O == 8) {    // of 16 lanes by a rotation
+        return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true);
+    } else if constexpr (O == 16) {   // [0] holds the even rows of 16 lanes twice each, [1] the odd ones
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return lane_id() & 16 ? r[0] : r[1];
+    } else {
+        return lane_xor_u32<O>(v);
+    }
+}
+template <int O> __device__ inline float other_lane(float v) {
+    return __builtin_bit_cast(float, other_lane<O>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int O> __device__ inline unsigned long long other_lane(unsigned long long v) {
+    return (unsigned long long)other_lane<O>((uint32_t)(v >> 32)) << 32 | other_lane<O>((uint32_t)v);
+}
+
+__device__ inline float max_of_lanes(float v) {
+    v = fmaxf(v, other_lane<32>(v)); v = fmaxf(v, other_lane<16>(v)); v = fmaxf(v, other_lane<8>(v));
+    v = fmaxf(v, other_lane<4>(v)); v = fmaxf(v, other_lane<2>(v)); v = fmaxf(v, other_lane<1>(v));
+    return v;
+}
+__device__ inline float sum_of_lanes(float v) {
+    v += other_lane<32>(v); v += other_lane<16>(v); v += other_lane<8>(v);
+    v += other_lane<4>(v); v += other_lane<2>(v); v += other_lane<1>(v);
     return v;
 }
 
@@ -246,9 +271,9 @@ struct Softmax {
     // Over a wavefront; every lane gets the result.
     template <bool kEntropy>
     __device__ void join_wave(float c2) {
-        const float top = wave_max(m), d = fmaxf((m - top) * c2, kFloor2), f = exp2_fast(d);
-        if (kEntropy) a = wave_sum(f * (a + d * s));
-        s = wave_sum(s * f);
+        const float top = max_of_lanes(m), d = fmaxf((m - top) * c2, kFloor2), f = exp2_fast(d);
+        if (kEntropy) a = sum_of_lanes(f * (a + d * s));
+        s = sum_of_lanes(s * f);
         m = top;
     }
 };
