@@ -96,10 +96,12 @@ struct WaveTop {
         for (int first = 0; first < count; first += kWave) {
             u64 e = first + lane_id() < count ? wait[first + lane_id()] : 0;
             sort_steps<2, 1>(e); sort_steps<4, 2>(e); sort_steps<8, 4>(e);
-            if (count - first > 8) {               // (the other lanes hold nothing)
-                sort_steps<16, 8>(e); sort_steps<32, 16>(e); sort_steps<64, 32>(e);
+            if (count - first > 8) sort_steps<16, 8>(e);               // (the other lanes hold nothing)
+            if (count - first > 16) {
+                sort_steps<32, 16>(e); sort_steps<64, 32>(e);
             }
-            merge_reversed(__shfl(e, kWave - 1 - lane_id()));
+            if (of_lane(best, 0)) merge_reversed(__shfl(e, kWave - 1 - lane_id()));
+            else best = e;
         }
         wave_fence();
         count = 0;
@@ -226,7 +228,7 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
 // finds to be the least that can still be among the best bounds the others' as well.  (Keeping
 // elements instead of pieces doubled the arithmetic, which is what bounds this kernel with alternatives.)
 // Without alternatives bound by memory: 8192 x 32000 f32 160 us (6.5 TB/s read), 4096 x 50000 bf16 70 us (5.9); with five of
-// them by its instructions: 78 us there, 84 for 4096 x 50001 f16, whose rows start within words.
+// them by its instructions: 78 us there, 84 for 4096 x 50001 f16, of which every second row starts within a word.
 template <class T, int kMode, int kRowThreads, int U>
 __global__ __launch_bounds__(kRowThreads, 8) void logit_stats_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(kRowThreads, 8) void logit_stats_kernel(LogitArgs a
     else finish_logprobs<T>(a, at_row, f, top, t, (float)z_t);
 }
 
-// Joins the splits (up to 64) of a row: one wavefront each.  Bound by waits: 6.8 us for 4 rows of 64 splits with 20
+// Joins the splits (up to 64) of a row: one wavefront each.  Bound by waits: 6.2 us for 4 rows of 64 splits with 20
 // alternatives, as long as logit_stats_kernel takes for their 131072 bf16 each.
 template <class T, int kMode>
 __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
@@ -472,8 +474,8 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
 // pieces leave: the next row's loads take their registers and travel beside the stores.  Memory
 // operations are waited for in their order and counted where their number is known, so there are no branches about
 // them: beyond the row's end a thread reads (and writes, the same values again) the last piece once more.
-// Bound by memory: 8192 x 131072 bf16 868 us (4.9 TB/s read and written; a copy reaches 4.8); 1001 x 100003 f16, rows
-// that start at odd addresses, 120 us (3.3 TB/s, with four rows a workgroup at most hardly past its start).
+// Bound by memory: 8192 x 131072 bf16 842 us (5.1 TB/s read and written; a copy reaches 4.8); 1001 x 100003 f16
+// 112 us (3.6 TB/s: with four rows a workgroup the first one's loads and the last one's stores are alone).
 template <class T, int kRowThreads, int NV>
 __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) {
     using P = Piece<T>;
@@ -672,7 +674,7 @@ int stats_of(const LogitArgs& a, hipStream_t s) {
 }
 
 template <class T, int kRowThreads, int NV>
-int distill_rows_by(const LogitArgs& a, int per_unit, hipStream_t s) {
+int distill_rows_by(const LogitArgs& a, int per_unit, hipStream_t s) {      // per_unit: workgroups that a compute unit holds
     const uint32_t groups = (uint32_t)std::min<int64_t>(a.n, 256 * per_unit);
     distill_rows_kernel<T, kRowThreads, NV><<<groups, kRowThreads, 0, s>>>(a);
     DCIH_HIP(hipGetLastError());
@@ -682,7 +684,9 @@ int distill_rows_by(const LogitArgs& a, int per_unit, hipStream_t s) {
 constexpr int kMostPieces = 16 * 1024;       // of a row in registers
 
 // The fewest threads that hold a row in 16 pieces each and a slot each: several rows are on a compute unit then,
-// and one's sums run while others' bytes travel.  Fewer pieces where they do.
+// and one's sums run while others' bytes travel.  (1024 threads for all: 16384 x 2000 bf16 379 us instead of 33, 8192 x 16000
+// 251 instead of 120, 4096 x 50000 233 instead of 187.)  Fewer pieces where they do: what a thread does not need it reads
+// again (16 for all: 73, 169 and 236 us).
 template <class T>
 int distill_rows_of(const LogitArgs& a, hipStream_t s) {
     const int pieces = a.vocab / Piece<T>::kLen;
@@ -752,8 +756,8 @@ int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
 }
 
 // Rows that fit a workgroup's registers, by one workgroup each; where they are long, only if there are enough of
-// them: one of 131072 bf16 takes 22 us by one workgroup and 13 by three launches over the device, 64 25 and 24, 128 27
-// and 33; one of 32000 takes 11 and 13.
+// them to give a compute unit in three one: one of 131072 bf16 takes 19 us by one workgroup and 9.5 by three launches over
+// the device, 64 22 and 20, 128 23 and 28; one of 32000 takes 8.4 and 9.6.
 bool distill_by_rows(const LogitArgs& a, int dtype) {
     const int len = 16 / type_bytes(dtype), pieces = a.vocab / len;
     return pieces >= 1 && pieces <= kMostPieces && (pieces <= 4096 || a.n >= 96);
