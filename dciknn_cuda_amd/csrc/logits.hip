@@ -693,7 +693,8 @@ int distill_rows_of(const LogitArgs& a, hipStream_t s) {
     if (a.slots <= 64) {
         if (pieces <= 4 * 64) return distill_rows_by<T, 64, 4>(a, 24, s);
         if (pieces <= 8 * 64) return distill_rows_by<T, 64, 8>(a, 20, s);
-        if (pieces <= 16 * 64) return distill_rows_by<T, 64, 16>(a, 16, s);
+        // (few rows wait for one wavefront's 16 pieces: 64 x 8000 bf16 7.7 us, 5.0 by four; 1000 x 8000 9.7 and 9.4, 4000 26 and 27)
+        if (pieces <= 16 * 64 && a.n >= 1024) return distill_rows_by<T, 64, 16>(a, 16, s);
     }
     if (a.slots <= 256) {
         if (pieces <= 4 * 256) return distill_rows_by<T, 256, 4>(a, 6, s);

@@ -526,3 +526,34 @@ def test_refusals(gpu):
                  lambda: gpu.distill_step(z[:2], ids[:2], teacher[:2], out=z[1:3])):
         with pytest.raises(ValueError):
             call()
+
+
+# ---- where one way of computing ends and the next begins ---------------------------------
+@pytest.mark.parametrize("n,v,k,dtype", [(1023, 5000, 10, "f16"), (1024, 5001, 64, "bf16"), (1100, 8191, 33, "f16"), (1024, 4095, 7, "f32")])
+def test_distillation_by_wavefronts(gpu, n, v, k, dtype):
+    test_distillation_by_rows(gpu, n, v, k, dtype)
+
+
+@pytest.mark.parametrize("dtype,n,v", [("bf16", 3, 16_376), ("f16", 3, 16_385), ("bf16", 2, 16_392), ("f32", 2, 8192), ("f32", 2, 8193), ("f16", 600, 17_001)])
+def test_token_logprobs_about_the_longest_row_of_one_workgroup(gpu, dtype, n, v):
+    test_token_logprobs(gpu, dtype, n, v)
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(30_000, 300_000, 20, "f32"), (30_000, 900, 72, "bf16"), (5000, 40, 9, "f16")])
+def test_lookup_gradient_of_half_the_tokens_one_row(gpu, n, v, d, dtype):
+    r = gen(n + d)
+    ids = np.where(r.random(n) < 0.5, 7, r.integers(0, v, n))
+    _grad_case(gpu, dtype, r.normal(size=(n, d)), ids, v, 1.0)
+    ids[:] = 7
+    ids[n // 2:n // 2 + 100] = r.integers(0, v, 100)
+    _grad_case(gpu, dtype, r.normal(size=(n, d)), ids, v, 1.0)
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 3, 1), (300, 40, 33), (6000, 500, 16)])
+def test_lookup_gradient_against_differences(gpu, n, v, d):
+    """The lookup is linear: with small whole numbers sum G (embed(W + E) - embed(W)) = sum E embed_grad(G), bit by bit."""
+    r = gen(n)
+    table, step, grad = (on_gpu(r.integers(-4, 5, shape), torch.float32) for shape in ((v, d), (v, d), (n, d)))
+    ids = on_gpu(r.integers(-1, v, n), torch.int64)
+    rise = (grad.double() * (gpu.embed(table + step, ids, 0.5) - gpu.embed(table, ids, 0.5)).double()).sum()
+    assert rise == (step.double() * gpu.embed_grad(grad, ids, v, 0.5).double()).sum()
