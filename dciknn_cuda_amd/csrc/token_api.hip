@@ -1,5 +1,6 @@
 // The entry points of include/dci_hip.h that work on tokens: checks of the arguments, the caller's
 // workspace laid out, launches.  No handle, no state; nothing here allocates, waits or throws.
+#include <algorithm>
 #include <initializer_list>
 #include <string>
 
@@ -26,6 +27,9 @@ const char* check_ids(const void* p, int id_bytes) {
     return aligned(p, id_bytes) ? nullptr : "ids not aligned to their size";
 }
 
+// Rows whose last byte has an address in 63 bits.
+bool near_enough(int64_t n, int64_t stride) { return stride <= (INT64_MAX >> 4) / std::max<int64_t>(n, 1); }
+
 bool all_aligned(std::initializer_list<const void*> arrays) {
     for (const void* p : arrays)
         if (!aligned(p, 4)) return false;
@@ -38,7 +42,7 @@ const char* check_logits(const void* z, int dtype, int64_t n, int vocab, int64_t
     if (const char* why = check_array(z, dtype)) return why;
     if (n < 0 || n > kMaxCount) return "bad number of rows";
     if (vocab <= 0 || vocab > DCIH_MAX_VOCAB) return "bad length of rows";
-    if (stride < vocab) return "rows overlap";
+    if (stride < vocab || !near_enough(n, stride)) return "rows overlap or are too far apart";
     if (!(temperature > 1e-30f) || !(temperature < 1e30f)) return "temperature must be a positive number";
     return nullptr;
 }
@@ -80,7 +84,7 @@ bool overlap(const void* a, int64_t bytes_a, const void* b, int64_t bytes_b) {
 // A gradient in the logits' place is of the same rows; anything between is refused.
 const char* check_grad(const void* z, const void* grad, int dtype, int64_t n, int vocab, int64_t stride, int64_t grad_stride) {
     if (const char* why = check_array(grad, dtype)) return why;
-    if (grad_stride < vocab) return "rows of the gradient overlap";
+    if (grad_stride < vocab || !near_enough(n, grad_stride)) return "rows of the gradient overlap or are too far apart";
     const int64_t b = type_bytes(dtype);
     if (n && !(z == grad && stride == grad_stride) &&
         overlap(z, ((n - 1) * stride + vocab) * b, grad, ((n - 1) * grad_stride + vocab) * b))
@@ -104,7 +108,8 @@ extern "C" {
 int dcih_embed(const void* d_table, int dtype, int64_t num_rows, int dim, int64_t row_stride, const void* d_ids,
                int id_bytes, int64_t num_ids, float scale, void* d_out, void* stream) {
     const char* who = "dcih_embed";
-    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
+    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount ||
+        !near_enough(num_rows, row_stride))
         return refuse(who, "bad size");
     if (const char* why = check_array(d_table, dtype)) return refuse(who, why);
     if (!num_ids) return DCIH_OK;
@@ -132,7 +137,8 @@ int dcih_embed_grad(const void* d_grad, int dtype, int64_t num_ids, int dim, int
                     int id_bytes, int64_t num_rows, float scale, int accumulate, void* d_out, int out_dtype,
                     void* d_work, int64_t work_bytes, void* stream) {
     const char* who = "dcih_embed_grad";
-    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount)
+    if (num_rows <= 0 || num_rows > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || row_stride < dim || num_ids < 0 || num_ids > kMaxCount ||
+        !near_enough(num_ids, row_stride))
         return refuse(who, "bad size");
     if (const char* why = check_array(d_out, out_dtype)) return refuse(who, why);
     if (out_dtype != dtype && out_dtype != DCIH_F32) return refuse(who, "sums are of the gradient's type or of 32 bits");

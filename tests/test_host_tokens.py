@@ -72,3 +72,13 @@ def test_workspace_grows_with_what_is_split():
     one = lib.dcih_logits_work(1, 131072, 2, 20)
     assert one > 16 and lib.dcih_logits_work(1, 131072, 2, 0) < one
     assert ctypes.sizeof(ctypes.c_int64) == 8 and lib.dcih_logits_work(0, 9, 0, 0) == 0
+
+
+def test_rows_too_far_apart(oracle):
+    """Distances whose product with the number of rows leaves 63 bits."""
+    from dciknn_cuda_amd import _capi
+    lib, far = _capi.lib(), 1 << 61
+    assert lib.dcih_embed(A, 0, 5, 8, far, A, 8, 3, 1.0, A, None) == -1
+    assert lib.dcih_embed_grad(A, 0, 3, 8, far, A, 8, 5, 1.0, 0, A, 0, A, 1 << 20, None) == -1
+    assert lib.dcih_token_logprobs(A, 0, 4, 9, far, A, 8, 1.0, 0, A, A, None, None, None, A, 1 << 20, None) == -1
+    assert lib.dcih_distill(A, 0, 4, 9, 9, A, 8, A, 0, 3, 1.0, A, None, None, 1 << 24, far, A, 1 << 20, None) == -1
