@@ -18,14 +18,14 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---- lookup ------------------------------------------------------------------------------
-// `lanes` (a power of two up to 256) neighbouring threads take one row: as many as it has pieces, so that short
-// rows leave no lane idle.  Bound by memory: 32768 tokens of text by 131072 x 4096 bf16 78 us (268 MB written, 98 MB
+// `lanes` (up to 256) neighbouring threads take one row: as many as it has pieces, so that few are idle.  Bound by memory: 32768 tokens of text by 131072 x 4096 bf16 78 us (268 MB written, 98 MB
 // of different rows read: 4.7 TB/s), 100000 x 128 f32 20 us (5.1 TB/s), 32 x 4096 bf16 4.2 us (a launch).
 template <class T>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(EmbedArgs a, int lanes, int64_t first) {
     using P = Piece<T>;
-    const int64_t i = first + (int64_t)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
-    if (i >= a.n) return;
+    const int per = kThreads / lanes, group = threadIdx.x / lanes;
+    const int64_t i = first + (int64_t)blockIdx.x * per + group;
+    if (group >= per || i >= a.n) return;
     const int64_t id = id_at(a.ids, a.wide_ids, i);
     typename T::raw* out = (typename T::raw*)a.out + i * a.dim;
     // an empty slot is a row of zeros; a row that does not exist is not passed over in silence
@@ -369,8 +369,8 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
             });
         } else if (!a.accumulate) {
             const int64_t many = min((int64_t)kBins, rows - bin0);
-            const int id = tid - kGroupThreads;
-            for (int64_t r = id / lanes; r < many; r += kGroupThreads / lanes) {
+            const int id = tid - kGroupThreads, groups = kGroupThreads / lanes;
+            for (int64_t r = id / lanes < groups ? id / lanes : many; r < many; r += groups) {
                 if (s_len[r]) continue;
                 for (int c = id % lanes * Piece<O>::kLen; c < a.dim; c += lanes * Piece<O>::kLen)
                     put_zeros<O, Piece<O>::kLen>(a, row_of(w, bucket, bin0 + r), c);
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
     }
 }
 
-// `lanes` (a power of two up to 64) neighbouring lanes take one window of w.piece tokens in one slice of
+// `lanes` (up to 64) neighbouring threads take one window of w.piece tokens in one slice of
 // the columns: they sum the pieces that START in the window, up to as many tokens of one row each.
 // Rows of up to w.piece tokens are one piece and final; the first piece of a longer one goes to
 // place 2 w + 1 of `part`, a later one to 2 w (a window w has at most one of each).  Windows, not rows, are
@@ -390,7 +390,9 @@ template <class T, class O>
 __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int lanes, int slices, int64_t first) {
     using P = Piece<T>;
     constexpr int kAhead = 8;
-    const int64_t unit = first + (int64_t)blockIdx.x * (kThreads / lanes) + threadIdx.x / lanes;
+    const int per = kThreads / lanes, group = threadIdx.x / lanes;
+    if (group >= per) return;
+    const int64_t unit = first + (int64_t)blockIdx.x * per + group;
     const int64_t window = unit / slices, total = *w.total;
     const int piece = w.piece;
     const int64_t begin = window * piece, end = min(total, begin + piece);
@@ -514,7 +516,7 @@ constexpr int kFewRows = 256;        // rows of a workgroup at most
 // 2^run_bits neighbouring rows in turn: the commonest tokens are often neighbours (4096 tokens of text by 50000 x 512
 // f16, 98 neighbouring rows each: 54 us instead of 18), while a run is to be worth a write.  `lanes` lanes are a group; each takes
 // the same share of the tokens, and the sum of a row that reaches over several shares is put together
-// by the group it starts in.  Bound by the waits of its steps (1000 tokens by 3000 x 100 f32: 6.9 us; four launches took 18),
+// by the group it starts in.  Bound by the waits of its steps (1000 tokens by 3000 x 100 f32: 6.4 us; four launches took 18),
 // by its zeros where the table is large (100 by 1M x 256 f32: 190 us, 5.4 TB/s).
 template <class T, class O>
 __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int rows, int run_bits, int64_t blocks, int lanes, int64_t first) {
@@ -541,7 +543,7 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     }
     // all of its rows are zeros first, few are written again: nothing is waited for before these bytes leave
     const int group = tid / lanes, groups = kGroupThreads / lanes, c = ((int)blockIdx.y * lanes + tid % lanes) * P::kLen;
-    const bool in = c < a.dim, whole = c + P::kLen <= a.dim;
+    const bool in = c < a.dim && group < groups, whole = c + P::kLen <= a.dim;
     if (in && !a.accumulate)
         for (int r = group; r < rows; r += groups)
             if (row_of_bin(r) < a.num_rows) put_zeros<O, P::kLen>(a, row_of_bin(r), c);
@@ -630,11 +632,12 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
 
 constexpr int64_t kMaxGrid = 1 << 22;     // workgroups of one launch (their threads are counted in 32 bits)
 
-// The smallest power of two that is no less than n, at most `most`.
+// Lanes for a row of n pieces, or for a share of it in whole lines of 128 bytes each of the fewest times: up to `most`
+// (a multiple of 8).  A line that two workgroups write in part costs both a line: 1 token by 250000 x 960 f32 262 us with
+// shares of 60 pieces, 180 with 64.
 int lanes_for(int n, int most) {
-    int l = 1;
-    while (l < n && l < most) l *= 2;
-    return l;
+    const int times = (n + most - 1) / most;
+    return times == 1 ? n : ((n + times - 1) / times + 7) / 8 * 8;
 }
 
 template <class T>
@@ -660,10 +663,14 @@ int room_for_counts() {
 
 template <class T, class O>
 int grad_of_few(const EmbedArgs& a, hipStream_t s) {
-    const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, kWave);
-    // runs of 512 bytes or more, 512 workgroups to fill the device
+    // a row of up to 128 pieces is not shared by workgroups (4000 tokens by 50000 x 520 f16 22 us, 26 in two slices), longer
+    // ones are by 64 (by 50000 x 2048 39 us, 42 with 128)
+    const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, pieces <= 2 * kWave ? 2 * kWave : kWave);
+    // runs of 512 bytes or more, 512 workgroups to fill the device; where rows share lines and few tokens can be one workgroup's,
+    // of 4096 (32 tokens by 410256 x 624 f16: 107 us, 142 with runs of a row)
+    const int64_t row_bytes = (int64_t)a.dim * (int)sizeof(typename O::raw), run_bytes = a.n <= 256 && row_bytes % 128 ? 4096 : 512;
     int run_bits = 0;
-    while (run_bits < 3 && (int64_t)a.dim * (int)sizeof(typename O::raw) << run_bits < 512) run_bits++;
+    while (run_bits < 3 && row_bytes << run_bits < run_bytes) run_bits++;
     const int64_t runs = ((a.num_rows - 1) >> run_bits) + 1;
     const int64_t turns = std::min<int64_t>(kFewRows >> run_bits, std::max<int64_t>(std::max(1, 8 >> run_bits), (runs + 511) / 512));
     const int64_t blocks = (runs + turns - 1) / turns, slices = (pieces + lanes - 1) / lanes;

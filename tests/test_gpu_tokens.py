@@ -557,3 +557,14 @@ def test_lookup_gradient_against_differences(gpu, n, v, d):
     ids = on_gpu(r.integers(-1, v, n), torch.int64)
     rise = (grad.double() * (gpu.embed(table + step, ids, 0.5) - gpu.embed(table, ids, 0.5)).double()).sum()
     assert rise == (step.double() * gpu.embed_grad(grad, ids, v, 0.5).double()).sum()
+
+
+# Rows of one group of threads that is no power of two, of two that share them in whole lines, of parts of runs.
+@pytest.mark.parametrize("n,v,d,dtype", [(40, 700, 624, "f16"), (300, 700, 625, "bf16"), (257, 9, 520, "f32"), (5000, 300, 168, "bf16"), (6000, 100, 1000, "f16"),
+                                         (4100, 90, 1333, "f32"), (256, 5000, 21, "f16"), (3000, 2000, 1030, "bf16")])
+def test_lookup_and_its_gradient_of_uneven_rows(gpu, n, v, d, dtype):
+    r = gen(n + v + d)
+    _grad_case(gpu, dtype, r.normal(size=(n, d)), r.integers(-1, v, n), v, 1.0)
+    table = on_gpu(r.normal(size=(v, d)), TYPES[dtype])
+    ids = on_gpu(r.integers(0, v, n), torch.int64)
+    assert torch.equal(gpu.embed(table, ids), table[ids])
