@@ -341,17 +341,24 @@ __global__ __launch_bounds__(kWave) void logit_join_kernel(LogitArgs a) {
             // The lists are in order: with k lists or more, the k-th largest of their first entries bounds
             // from below, and where no list has an entry above the bound at a place none has one behind it.
             constexpr int kAhead = 8;
-            u64 e[kAhead];
+            u64 e[kAhead], next[kAhead];
+            auto load = [&](u64 (&x)[kAhead], int p) {
+#pragma unroll
+                for (int j = 0; j < kAhead; j++) x[j] = lane < a.splits && p + j < a.top ? lists[p + j] : 0;
+            };
+            load(next, 0);
             for (int p = 0; p < a.top; p += kAhead) {
 #pragma unroll
-                for (int j = 0; j < kAhead; j++) e[j] = lane < a.splits && p + j < a.top ? lists[p + j] : 0;
+                for (int j = 0; j < kAhead; j++) e[j] = next[j];
+                load(next, p + kAhead);
                 if (p == 0) {
                     const uint32_t kth = kth_of_lanes((uint32_t)(e[0] >> 32), a.top);
                     if (a.top <= a.splits) top.least = (u64)kth << 32;
                 }
                 if (!__any(e[0] > top.least)) break;
 #pragma unroll
-                for (int j = 0; j < kAhead; j++) top.push(e[j] != 0, e[j]);
+                for (int j = 0; j < kAhead; j++)
+                    if (__any(e[j] > top.least)) top.push(e[j] != 0, e[j]);
                 top.settle();
             }
             top.settle();
