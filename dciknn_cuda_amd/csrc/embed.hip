@@ -74,6 +74,7 @@ struct Work {
     uint32_t* common;       // [2][n / piece]: where the rows with more tokens than a piece, and than kWide pieces, begin
     float* part;            // [2 * windows][width]: see sum_kernel
     int64_t chunks, windows;
+    int64_t cleared;        // rows that chunk_kernel writes zeros to: all or none
     int piece;              // tokens of a row that are summed by one group of lanes
     int bucket_bits, width;
 };
@@ -141,9 +142,20 @@ __device__ inline uint32_t group_scan(uint32_t v, uint32_t before, uint32_t* s_w
 // them by buckets as it goes, and the counts of the wavefronts before it give its places.  Bound by the
 // waits of its few steps: 5.6 us for 65536 tokens, 8.2 for 100000 by 1024 buckets (With one launch in
 // which every workgroup read all ids, 65536 tokens by 50001 x 2048 bf16 took 80 us more.)
-__global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, bool wide, int64_t n, int64_t num_rows, Work w) {
+// More workgroups write zeros to the table's first w.cleared rows, 16 bytes a thread in the order of the launch: the one
+// order that reaches 6.9 TB/s (rows in turn, or more bytes a thread: 4.4 to 6.1).
+template <class O>
+__global__ __launch_bounds__(kGroupThreads) void chunk_kernel(EmbedArgs a, Work w) {
     extern __shared__ uint32_t s_count[];                // [kGroupWaves][buckets]
     __shared__ uint32_t s_wave[kGroupWaves];
+    if (blockIdx.x >= w.chunks) {
+        const int64_t at = ((blockIdx.x - w.chunks) * kGroupThreads + threadIdx.x) * Piece<O>::kLen, end = w.cleared * a.dim;
+        if (at + Piece<O>::kLen <= end) Piece<O>::store((typename O::raw*)a.out + at, u32x4{0, 0, 0, 0});
+        else
+            for (int64_t i = at; i < end; i++) ((typename O::raw*)a.out)[i] = (typename O::raw)0.f;
+        return;
+    }
+    const int64_t n = a.n, num_rows = a.num_rows;
     const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), buckets = 1 << w.bucket_bits;
     const int64_t base = (int64_t)blockIdx.x * kChunk;
     int64_t id[kPerLane];
@@ -151,7 +163,7 @@ __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(const void* ids, b
 #pragma unroll
     for (int j = 0; j < kPerLane; j++) {
         const int64_t i = base + (wave * kPerLane + j) * kWave + lane;
-        id[j] = i < n ? id_at(ids, wide, i) : -1;
+        id[j] = i < n ? id_at(a.ids, a.wide_ids, i) : -1;
     }
     for (int i = tid; i < kGroupWaves * buckets; i += kGroupThreads) s_count[i] = 0;
     __syncthreads();
@@ -267,7 +279,7 @@ __device__ inline void put_sums(const EmbedArgs& a, uint32_t row, int c, const f
 }
 
 // (Plain stores: rows that start off a line's boundary are written in parts of lines, which the caches put together.
-// 10241 tokens by 49752 x 1593 f32: 91 us, 125 with non-temporal ones; 100000 by 1M x 128 f32: 132, and 129.)
+// 10241 tokens by 49752 x 1593 f32: 91 us, 125 with non-temporal ones.)
 template <class O, int N>
 __device__ inline void put_zeros(const EmbedArgs& a, int64_t row, int c) {
     using P = Piece<O>;
@@ -282,20 +294,21 @@ __device__ inline void put_zeros(const EmbedArgs& a, int64_t row, int c) {
 }
 
 // Second half of the grouping: a workgroup takes a bucket.  What the chunks hold of the buckets before it
-// is where its part of the order starts.  Bound by the zeros it writes, if there are many (1M x 128 f32, 460 MB: 94 us,
-// 4.9 TB/s), otherwise by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 100 MB of
-// zeros, 101 where 65536 of 131072 tokens have one row.  Half of its wavefronts read the bucket's tokens, in runs of the chunks, once to
-// count them by rows (up to kBins at a time) and once to put them into their places; the other half
-// meanwhile writes the rows without tokens, whose bytes hide the waits of the first.
-template <class O>
-__global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, Work w, int lanes) {
-    constexpr int kAllWaves = 2 * kGroupWaves;
+// is where its part of the order starts.  Eight wavefronts read the bucket's tokens, in runs of the chunks, once to
+// count them by rows (up to kBins at a time) and once to put them into their places.  Eight more
+// meanwhile write the rows without tokens, whose bytes hide the waits of the first, unless there is nothing to be written
+// or chunk_kernel has done it.  Bound by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 100 MB of
+// zeros, 101 where 65536 of 131072 tokens have one row; or by the waits of its steps, where buckets are many: without zeros
+// four workgroups are on a compute unit at once (100000 tokens added to 1M x 128 f32: 52 us in all, 63 with one at a time).
+template <class O, bool kZeros>
+__global__ __launch_bounds__((kZeros ? 2 : 1) * kGroupThreads, kZeros ? 4 : 8) void bucket_kernel(EmbedArgs a, Work w, int lanes) {
+    constexpr int kAllThreads = (kZeros ? 2 : 1) * kGroupThreads, kAllWaves = kAllThreads / kWave;
     __shared__ uint32_t s_count[kGroupWaves][kBins];
-    __shared__ uint32_t s_start[kBins], s_len[kBins];
+    __shared__ uint32_t s_start[kBins + 1];
     __shared__ uint32_t s_wave[kAllWaves], s_before[kGroupWaves], s_total[kGroupWaves];
-    static_assert(kBins == 2 * kGroupThreads, "a thread per row");
+    static_assert(kBins % kAllThreads == 0, "as many rows for each thread");
     const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id(), bucket = blockIdx.x, buckets = 1 << w.bucket_bits;
-    const bool reads = wave < kGroupWaves;
+    const bool reads = !kZeros || wave < kGroupWaves;
     const int64_t run = (w.chunks + kGroupWaves - 1) / kGroupWaves;
     const int64_t from = reads ? min(w.chunks, wave * run) : 0, to = reads ? min(w.chunks, from + run) : 0;
     uint32_t before = 0, total = 0, o0 = 0, o1 = 0;
@@ -329,7 +342,7 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
     if (bucket == 0 && tid == 0) w.total[0] = total;
     const int64_t rows = (a.num_rows - bucket + buckets - 1) >> w.bucket_bits;       // of this bucket
     for (int64_t bin0 = 0; bin0 < rows; bin0 += kBins) {
-        for (int i = tid; i < kGroupWaves * kBins; i += 2 * kGroupThreads) (&s_count[0][0])[i] = 0;
+        for (int i = tid; i < kGroupWaves * kBins; i += kAllThreads) (&s_count[0][0])[i] = 0;
         __syncthreads();
         each_token([&](Placed p, bool real) {
             const uint32_t bin = bin_of(w, p.row) - (uint32_t)bin0;
@@ -340,19 +353,21 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
             if (mine && (bin != lead || lanes_below(same) == 0)) atomicAdd(&s_count[wave][bin], bin == lead ? (uint32_t)__popcll(same) : 1u);
         });
         __syncthreads();
-        uint32_t len = 0, all;
-        for (int v = 0; v < kGroupWaves; v++) {
-            const uint32_t c = s_count[v][tid];
-            s_count[v][tid] = len;
-            len += c;
-        }
-        const uint32_t start = group_scan<kAllWaves>(len, before, s_wave, &all);
-        before += all;
-        s_start[tid] = start;
-        s_len[tid] = len;
-        if (len > (uint32_t)w.piece) {      // (in any order)
-            const int wide = len > (uint32_t)(w.piece * kWide);
-            w.common[wide * (a.n / w.piece) + atomicAdd(&w.total[1 + wide], 1u)] = start;
+        for (int bin = tid; bin < kBins; bin += kAllThreads) {
+            uint32_t len = 0, all;
+            for (int v = 0; v < kGroupWaves; v++) {
+                const uint32_t c = s_count[v][bin];
+                s_count[v][bin] = len;
+                len += c;
+            }
+            const uint32_t start = group_scan<kAllWaves>(len, before, s_wave, &all);
+            before += all;
+            s_start[bin] = start;
+            if (bin == kBins - 1) s_start[kBins] = start + len;
+            if (len > (uint32_t)w.piece) {      // (in any order)
+                const int wide = len > (uint32_t)(w.piece * kWide);
+                w.common[wide * (a.n / w.piece) + atomicAdd(&w.total[1 + wide], 1u)] = start;
+            }
         }
         __syncthreads();
         if (reads) {
@@ -364,14 +379,14 @@ __global__ __launch_bounds__(2 * kGroupThreads) void bucket_kernel(EmbedArgs a, 
                 if (mine) {
                     const uint32_t rank = s_count[wave][bin] + lanes_below(same);
                     if (lanes_below(same) == 0) s_count[wave][bin] = rank + __popcll(same);
-                    w.tokens[s_start[bin] + rank] = Token{p.row, p.at, rank, s_len[bin]};
+                    w.tokens[s_start[bin] + rank] = Token{p.row, p.at, rank, s_start[bin + 1] - s_start[bin]};
                 }
             });
-        } else if (!a.accumulate) {
+        } else if (kZeros) {
             const int64_t many = min((int64_t)kBins, rows - bin0);
             const int id = tid - kGroupThreads, groups = kGroupThreads / lanes;
             for (int64_t r = id / lanes < groups ? id / lanes : many; r < many; r += groups) {
-                if (s_len[r]) continue;
+                if (s_start[r + 1] != s_start[r]) continue;
                 for (int c = id % lanes * Piece<O>::kLen; c < a.dim; c += lanes * Piece<O>::kLen)
                     put_zeros<O, Piece<O>::kLen>(a, row_of(w, bucket, bin0 + r), c);
             }
@@ -652,10 +667,11 @@ int lookup(const EmbedArgs& a, hipStream_t s) {
 }
 
 // Room on the chip for chunk_kernel's counts, once for each device.
+template <class O>
 int room_for_counts() {
     static DeviceOnce once;
     return once.run([] {
-        DCIH_HIP(hipFuncSetAttribute((const void*)chunk_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+        DCIH_HIP(hipFuncSetAttribute((const void*)chunk_kernel<O>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                      kGroupWaves * (int)sizeof(uint32_t) << kMaxBucketBits));
         return 0;
     });
@@ -688,10 +704,17 @@ int grad(const EmbedArgs& a, hipStream_t s) {
     if (a.n <= kFew) return grad_of_few<T, O>(a, s);
     Work w;
     lay_out(w, a.work, a.n, a.dim, a.num_rows);
-    if (int rc = room_for_counts()) return rc;
-    chunk_kernel<<<(uint32_t)w.chunks, kGroupThreads, kGroupWaves * sizeof(uint32_t) << w.bucket_bits, s>>>(a.ids, a.wide_ids, a.n, a.num_rows, w);
+    if (int rc = room_for_counts<O>()) return rc;
+    constexpr int kCleared = kGroupThreads * Piece<O>::kLen;       // elements, by a workgroup
+    // Tables that stay empty for the most part are cleared first: 100000 tokens by 1M x 128 f32 126 us instead of 129, 20000 110
+    // instead of 120; but 65536 by 262144 x 512 f16 73 instead of 71.
+    w.cleared = a.accumulate || a.num_rows < 8 * a.n || a.num_rows > kMaxGrid * kCleared / a.dim ? 0 : a.num_rows;
+    const int64_t clearing = (w.cleared * a.dim + kCleared - 1) / kCleared;
+    chunk_kernel<O><<<(uint32_t)(w.chunks + clearing), kGroupThreads, kGroupWaves * sizeof(uint32_t) << w.bucket_bits, s>>>(a, w);
     DCIH_HIP(hipGetLastError());
-    bucket_kernel<O><<<1u << w.bucket_bits, 2 * kGroupThreads, 0, s>>>(a, w, lanes_for((a.dim + Piece<O>::kLen - 1) / Piece<O>::kLen, kWave));
+    const int out_lanes = lanes_for((a.dim + Piece<O>::kLen - 1) / Piece<O>::kLen, kWave);
+    if (a.accumulate || w.cleared) bucket_kernel<O, false><<<1u << w.bucket_bits, kGroupThreads, 0, s>>>(a, w, out_lanes);
+    else bucket_kernel<O, true><<<1u << w.bucket_bits, 2 * kGroupThreads, 0, s>>>(a, w, out_lanes);
     DCIH_HIP(hipGetLastError());
     const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, kWave);
     const int slices = (pieces + lanes - 1) / lanes, per = kThreads / lanes;

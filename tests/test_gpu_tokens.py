@@ -568,3 +568,11 @@ def test_lookup_and_its_gradient_of_uneven_rows(gpu, n, v, d, dtype):
     table = on_gpu(r.normal(size=(v, d)), TYPES[dtype])
     ids = on_gpu(r.integers(0, v, n), torch.int64)
     assert torch.equal(gpu.embed(table, ids), table[ids])
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(4097, 40_000, 5, "f16"), (4200, 33_700, 7, "f32"), (9000, 72_000, 3, "bf16"), (9000, 71_999, 3, "bf16")])
+def test_lookup_gradient_by_a_table_that_stays_empty(gpu, n, v, d, dtype):
+    r = gen(v)
+    _grad_case(gpu, dtype, r.normal(size=(n, d)), r.integers(-1, v + 1, n), v, 2.0)
+    got = gpu.embed_grad(torch.zeros(n, d, device="cuda", dtype=TYPES[dtype]), torch.full((n,), -1, device="cuda"), v)
+    assert not got.any()
