@@ -532,9 +532,9 @@ constexpr int kFewRows = 256;        // rows of a workgroup at most
 // f16, 98 neighbouring rows each: 54 us instead of 18), while a run is to be worth a write.  `lanes` lanes are a group; each takes
 // the same share of the tokens, and the sum of a row that reaches over several shares is put together
 // by the group it starts in.  Bound by the waits of its steps (1000 tokens by 3000 x 100 f32: 6.4 us; four launches took 18),
-// by its zeros where the table is large (100 by 1M x 256 f32: 190 us, 5.4 TB/s).
+// by its zeros where the table is large (100 by 1M x 256 f16: 96 us, 5.3 TB/s).
 template <class T, class O>
-__global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int rows, int run_bits, int64_t blocks, int lanes, int64_t first) {
+__global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, bool clears, int rows, int run_bits, int64_t blocks, int lanes, int64_t first) {
     using P = Piece<T>;
     constexpr int kAhead = 8;
     __shared__ uint32_t s_count[kGroupWaves * kFewRows], s_wave[kGroupWaves], s_start[kFewRows + 1];
@@ -559,11 +559,14 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, int row
     // all of its rows are zeros first, few are written again: nothing is waited for before these bytes leave
     const int group = tid / lanes, groups = kGroupThreads / lanes, c = ((int)blockIdx.y * lanes + tid % lanes) * P::kLen;
     const bool in = c < a.dim && group < groups, whole = c + P::kLen <= a.dim;
-    if (in && !a.accumulate)
+    if (in && clears)
         for (int r = group; r < rows; r += groups)
             if (row_of_bin(r) < a.num_rows) put_zeros<O, P::kLen>(a, row_of_bin(r), c);
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < kFewLanes; j++) any |= bin[j] >= 0;
     for (int i = tid; i < kGroupWaves * kFewRows; i += kGroupThreads) s_count[i] = 0;
-    __syncthreads();
+    if (!__syncthreads_or(any)) return;
     uint32_t* mine = s_count + wave * kFewRows;
 #pragma unroll
     for (int j = 0; j < kFewLanes; j++) {
@@ -677,6 +680,19 @@ int room_for_counts() {
     });
 }
 
+// The launch of chunk_kernel, which groups (w.chunks) and clears (w.cleared).
+template <class O>
+int group_and_clear(const EmbedArgs& a, const Work& w, hipStream_t s) {
+    constexpr int kCleared = kGroupThreads * Piece<O>::kLen;       // elements, by a workgroup
+    const int64_t clearing = (w.cleared * a.dim + kCleared - 1) / kCleared;
+    const size_t room = w.chunks ? kGroupWaves * sizeof(uint32_t) << w.bucket_bits : 0;
+    chunk_kernel<O><<<(uint32_t)(w.chunks + clearing), kGroupThreads, room, s>>>(a, w);
+    DCIH_HIP(hipGetLastError());
+    return 0;
+}
+template <class O>
+bool one_launch_clears(const EmbedArgs& a) { return a.num_rows <= kMaxGrid * kGroupThreads * Piece<O>::kLen / a.dim; }
+
 template <class T, class O>
 int grad_of_few(const EmbedArgs& a, hipStream_t s) {
     // a row of up to 128 pieces is not shared by workgroups (4000 tokens by 50000 x 520 f16 22 us, 26 in two slices), longer
@@ -691,9 +707,18 @@ int grad_of_few(const EmbedArgs& a, hipStream_t s) {
     const int64_t turns = std::min<int64_t>(kFewRows >> run_bits, std::max<int64_t>(std::max(1, 8 >> run_bits), (runs + 511) / 512));
     const int64_t blocks = (runs + turns - 1) / turns, slices = (pieces + lanes - 1) / lanes;
     const int rows = (int)(turns << run_bits);
+    // tables of 768 MB and more are cleared by a launch of their own (100 tokens by 1M x 256 f32 175 us, 190 by few_kernel alone;
+    // by half of that table 102 and 98)
+    bool clears = !a.accumulate;
+    if (clears && a.num_rows * row_bytes >= (int64_t)768 << 20 && one_launch_clears<O>(a)) {
+        Work w{};
+        w.cleared = a.num_rows;
+        if (int rc = group_and_clear<O>(a, w, s)) return rc;
+        clears = false;
+    }
     const int64_t most = std::max<int64_t>(1, kMaxGrid / slices);
     for (int64_t first = 0; first < blocks; first += most) {
-        few_kernel<T, O><<<dim3((uint32_t)std::min(most, blocks - first), (uint32_t)slices), kGroupThreads, 0, s>>>(a, rows, run_bits, blocks, lanes, first);
+        few_kernel<T, O><<<dim3((uint32_t)std::min(most, blocks - first), (uint32_t)slices), kGroupThreads, 0, s>>>(a, clears, rows, run_bits, blocks, lanes, first);
         DCIH_HIP(hipGetLastError());
     }
     return 0;
@@ -705,13 +730,10 @@ int grad(const EmbedArgs& a, hipStream_t s) {
     Work w;
     lay_out(w, a.work, a.n, a.dim, a.num_rows);
     if (int rc = room_for_counts<O>()) return rc;
-    constexpr int kCleared = kGroupThreads * Piece<O>::kLen;       // elements, by a workgroup
-    // Tables that stay empty for the most part are cleared first: 100000 tokens by 1M x 128 f32 126 us instead of 129, 20000 110
+    // Tables that stay empty for the most part are cleared first: 100000 tokens by 1M x 128 f32 125 us instead of 129, 20000 110
     // instead of 120; but 65536 by 262144 x 512 f16 73 instead of 71.
-    w.cleared = a.accumulate || a.num_rows < 8 * a.n || a.num_rows > kMaxGrid * kCleared / a.dim ? 0 : a.num_rows;
-    const int64_t clearing = (w.cleared * a.dim + kCleared - 1) / kCleared;
-    chunk_kernel<O><<<(uint32_t)(w.chunks + clearing), kGroupThreads, kGroupWaves * sizeof(uint32_t) << w.bucket_bits, s>>>(a, w);
-    DCIH_HIP(hipGetLastError());
+    w.cleared = !a.accumulate && a.num_rows >= 8 * a.n && one_launch_clears<O>(a) ? a.num_rows : 0;
+    if (int rc = group_and_clear<O>(a, w, s)) return rc;
     const int out_lanes = lanes_for((a.dim + Piece<O>::kLen - 1) / Piece<O>::kLen, kWave);
     if (a.accumulate || w.cleared) bucket_kernel<O, false><<<1u << w.bucket_bits, kGroupThreads, 0, s>>>(a, w, out_lanes);
     else bucket_kernel<O, true><<<1u << w.bucket_bits, 2 * kGroupThreads, 0, s>>>(a, w, out_lanes);

@@ -576,3 +576,18 @@ def test_lookup_gradient_by_a_table_that_stays_empty(gpu, n, v, d, dtype):
     _grad_case(gpu, dtype, r.normal(size=(n, d)), r.integers(-1, v + 1, n), v, 2.0)
     got = gpu.embed_grad(torch.zeros(n, d, device="cuda", dtype=TYPES[dtype]), torch.full((n,), -1, device="cuda"), v)
     assert not got.any()
+
+
+def test_lookup_gradient_of_few_tokens_by_a_large_table(gpu):
+    """One that a launch of its own clears: zeros everywhere but in the tokens' rows, to the last element."""
+    v, d = 800_001, 253                    # 810 MB
+    r = gen(9)
+    ids = np.concatenate([r.integers(0, v, 40), [0, v - 1, v - 1, -1, v]])
+    grad = on_gpu(r.normal(size=(45, d)), torch.float32)
+    got = gpu.embed_grad(grad, on_gpu(ids, torch.int64), v)
+    want = torch.zeros(v, d, device="cuda", dtype=torch.float64)
+    real = on_gpu((ids >= 0) & (ids < v), torch.bool)
+    want.index_add_(0, on_gpu(ids, torch.int64)[real], grad[real].double())
+    assert ((got.double() - want).abs() <= 2 * 2.0 ** -23 * want.abs().clamp(max=8)).all()
+    del want
+    assert torch.equal(gpu.embed_grad(grad, on_gpu(ids, torch.int64), v, out=torch.zeros_like(got)), got)
