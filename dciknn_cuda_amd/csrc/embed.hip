@@ -400,13 +400,21 @@ __global__ __launch_bounds__((kZeros ? 2 : 1) * kGroupThreads, kZeros ? 4 : 8) v
 // Rows of up to w.piece tokens are one piece and final; the first piece of a longer one goes to
 // place 2 w + 1 of `part`, a later one to 2 w (a window w has at most one of each).  Windows, not rows, are
 // what a group takes: a tenth of a text's tokens are one row's.  Bound by memory: 65536 tokens by 50001 x 2048
-// bf16 73 us (268 MB read, 105 MB written: 5.1 TB/s).
-template <class T, class O>
+// bf16 70 us (268 MB read, 105 MB written: 5.3 TB/s).
+template <class T, class O, bool kByWaves>
 __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int lanes, int slices, int64_t first) {
     using P = Piece<T>;
     constexpr int kAhead = 8;
-    const int per = kThreads / lanes, group = threadIdx.x / lanes;
+    if (kByWaves) lanes = kWave;
+    const int per = kThreads / lanes, group = kByWaves ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : threadIdx.x / lanes;
     if (group >= per) return;
+    // (With a wavefront for a window its tokens are read through the scalar cache, and half the registers do: 70 us for what
+    // takes 73 otherwise.)
+    auto token = [&](int64_t i) {
+        if (!kByWaves) return w.tokens[i];
+        const u32x4 x = ((const __attribute__((address_space(4))) u32x4*)w.tokens)[i];
+        return Token{x[0], x[1], x[2], x[3]};
+    };
     const int64_t unit = first + (int64_t)blockIdx.x * per + group;
     const int64_t window = unit / slices, total = *w.total;
     const int piece = w.piece;
@@ -417,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
     const bool whole = c + P::kLen <= a.dim;
     // the pieces that start here are tokens [t, stop): behind the rest of an earlier one, and up to
     // the end of the piece of the window's last token
-    const Token e0 = w.tokens[begin], e1 = w.tokens[end - 1];
+    const Token e0 = token(begin), e1 = token(end - 1);
     int64_t t = begin;
     if (e0.rank & (piece - 1)) t += min(piece - (e0.rank & (piece - 1)), e0.count - e0.rank);
     if (t >= end) return;
@@ -429,11 +437,11 @@ __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int 
         Token e[kAhead];
         u32x4 x[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; j++) e[j] = w.tokens[min(t + j, stop - 1)];
+        for (int j = 0; j < kAhead; j++) e[j] = token(min(t + j, stop - 1));
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
             const typename T::raw* row = (const typename T::raw*)a.rows + (int64_t)e[j].at * a.stride;
-            x[j] = whole ? P::load_once(row + c) : P::load_part(row, c, a.dim, 0.f);
+            x[j] = whole ? P::load_once((const typename T::raw*)((const char*)row + (uint32_t)c * (uint32_t)sizeof(typename T::raw))) : P::load_part(row, c, a.dim, 0.f);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; j++) {
@@ -743,7 +751,8 @@ int grad(const EmbedArgs& a, hipStream_t s) {
     const int64_t units = w.windows * slices;
     for (int64_t first = 0; first < units; first += kMaxGrid * per) {
         const int64_t groups = std::min(kMaxGrid, (units - first + per - 1) / per);
-        sum_kernel<T, O><<<(uint32_t)groups, kThreads, 0, s>>>(a, w, lanes, slices, first);
+        if (lanes == kWave) sum_kernel<T, O, true><<<(uint32_t)groups, kThreads, 0, s>>>(a, w, lanes, slices, first);
+        else sum_kernel<T, O, false><<<(uint32_t)groups, kThreads, 0, s>>>(a, w, lanes, slices, first);
         DCIH_HIP(hipGetLastError());
     }
     // groups of workgroups that fill the device, no more than there can be such rows

@@ -384,8 +384,8 @@ __device__ inline float slots_of_token(const int* s_id, const float* s_q, int fo
 }
 
 // Gradients by the logits from a row's statistics, one tile of a row per workgroup: nothing is to be joined, so the
-// tiles are small and many.  Bound by memory: 8192 x 32000 f32 335 us (6.3 TB/s: part of what logit_stats_kernel read last
-// is in the last-level cache still).
+// tiles are small and many.  Bound by memory: 8192 x 32000 f32 340 us (6.2 TB/s read and written; 362 with one or four pieces
+// a thread instead of two).
 template <class T, int kMode, int U>
 __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     using P = Piece<T>;
