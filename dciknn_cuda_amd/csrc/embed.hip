@@ -706,14 +706,16 @@ int grad_of_few(const EmbedArgs& a, hipStream_t s) {
     // a row of up to 128 pieces is not shared by workgroups (4000 tokens by 50000 x 520 f16 22 us, 26 in two slices), longer
     // ones are by 64 (by 50000 x 2048 39 us, 42 with 128)
     const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, pieces <= 2 * kWave ? 2 * kWave : kWave);
-    // runs of 512 bytes or more, 512 workgroups to fill the device; where rows share lines and few tokens can be one workgroup's,
+    // runs of 512 bytes or more; 512 workgroups to fill the device, each of which reads all ids (83 tokens by 5130 x 1872 f32 11 us,
+    // 19 with as many for each of the 8 slices, 4000 by 32000 x 4096 f16 65 and 91); where rows share lines and few tokens can be one workgroup's,
     // of 4096 (32 tokens by 410256 x 624 f16: 107 us, 142 with runs of a row)
     const int64_t row_bytes = (int64_t)a.dim * (int)sizeof(typename O::raw), run_bytes = a.n <= 256 && row_bytes % 128 ? 4096 : 512;
     int run_bits = 0;
     while (run_bits < 3 && row_bytes << run_bits < run_bytes) run_bits++;
     const int64_t runs = ((a.num_rows - 1) >> run_bits) + 1;
-    const int64_t turns = std::min<int64_t>(kFewRows >> run_bits, std::max<int64_t>(std::max(1, 8 >> run_bits), (runs + 511) / 512));
-    const int64_t blocks = (runs + turns - 1) / turns, slices = (pieces + lanes - 1) / lanes;
+    const int64_t slices = (pieces + lanes - 1) / lanes;
+    const int64_t turns = std::min<int64_t>(kFewRows >> run_bits, std::max<int64_t>(std::max(1, 8 >> run_bits), (runs * slices + 511) / 512));
+    const int64_t blocks = (runs + turns - 1) / turns;
     const int rows = (int)(turns << run_bits);
     // tables of 768 MB and more are cleared by a launch of their own (100 tokens by 1M x 256 f32 175 us, 190 by few_kernel alone;
     // by half of that table 102 and 98)
