@@ -23,7 +23,7 @@ def embed(table, ids, scale=1.0):
 
 def embed_grad(grad, ids, num_rows, scale=1.0, *, out=None):
     """The gradient of `embed` by its table: [num_rows, dim], row r the sum of `scale * grad[i]`
-    over the i with ids[i] = r.
+    over the i with ids[i] = r; empty slots and ids beyond the table add nothing.
 
     The sum's order depends on the ids alone: the same input gives the same bits.  With `out`
     ([num_rows, dim], contiguous, of grad's type or float32) the sums are added to it and it is returned; its
