@@ -2,10 +2,10 @@
 //
 //   out[i, :] = scale * W[id_i, :]            dW[v, :] = scale * sum over i with id_i = v of G[i, :]
 //
-// Both are bound by memory (figures are of one MI355X, whose copies reach 4.8 TB/s).  The gradient's sums are formed without atomics on values, in the
-// order of the tokens whatever the schedule: the tokens are first grouped by their row (chunk_kernel,
-// bucket_kernel), then summed in pieces of up to 16 tokens of one row (sum_kernel); the pieces of rows with more
-// tokens than that are joined by a third launch (join_kernel).  Sums are in 32 bits, rounded once.
+// Both are bound by memory (figures are of one MI355X, whose copies reach 4.8 TB/s).  The gradient's sums are formed
+// without atomics on values, in the order of the tokens whatever the schedule: the tokens are first grouped by their
+// row (chunk_kernel, bucket_kernel), then summed in pieces of up to 16 tokens of one row (sum_kernel); the pieces of
+// rows with more tokens than that are joined by a third launch (join_kernel).  Sums are in 32 bits, rounded once.
 #include "../../include/dci_hip.h"
 #include "token_common.h"
 
@@ -18,8 +18,9 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---- lookup ------------------------------------------------------------------------------
-// `lanes` (up to 256) neighbouring threads take one row: as many as it has pieces, so that few are idle.  Bound by memory: 32768 tokens of text by 131072 x 4096 bf16 78 us (268 MB written, 98 MB
-// of different rows read: 4.7 TB/s), 100000 x 128 f32 20 us (5.1 TB/s), 32 x 4096 bf16 4.2 us (a launch).
+// `lanes` (up to 256) neighbouring threads take one row: as many as it has pieces, so that few are idle.  Bound by
+// memory: 32768 tokens of text by 131072 x 4096 bf16 78 us (268 MB written, 98 MB of different rows read: 4.7 TB/s),
+// 100000 x 128 f32 20 us (5.1 TB/s), 32 x 4096 bf16 4.2 us (a launch).
 template <class T>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(EmbedArgs a, int lanes, int64_t first) {
     using P = Piece<T>;
@@ -105,10 +106,6 @@ __host__ inline size_t lay_out(Work& w, void* mem, int64_t n, int dim, int64_t n
     take(w.common, 2 * (n / w.piece));
     take(w.part, w.windows * 2 * w.width);
     return at;
-}
-
-__device__ inline int lanes_below(unsigned long long mask) {
-    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
 // The lanes of `in` whose keys (of `bits` bits) are the same as this one's.
@@ -293,13 +290,14 @@ __device__ inline void put_zeros(const EmbedArgs& a, int64_t row, int c) {
     }
 }
 
-// Second half of the grouping: a workgroup takes a bucket.  What the chunks hold of the buckets before it
-// is where its part of the order starts.  Eight wavefronts read the bucket's tokens, in runs of the chunks, once to
-// count them by rows (up to kBins at a time) and once to put them into their places.  Eight more
-// meanwhile write the rows without tokens, whose bytes hide the waits of the first, unless there is nothing to be written
-// or chunk_kernel has done it.  Bound by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 100 MB of
-// zeros, 101 where 65536 of 131072 tokens have one row; or by the waits of its steps, where buckets are many: without zeros
-// four workgroups are on a compute unit at once (100000 tokens added to 1M x 128 f32: 52 us in all, 63 with one at a time).
+// Second half of the grouping: a workgroup takes a bucket.  What the chunks hold of the buckets before it is where
+// its part of the order starts.  Eight wavefronts read the bucket's tokens, in runs of the chunks, once to count them
+// by rows (up to kBins at a time) and once to put them into their places.  Eight more meanwhile write the rows
+// without tokens, whose bytes hide the waits of the first, unless there is nothing to be written or chunk_kernel has
+// done it.  Bound by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 100
+// MB of zeros, 101 where 65536 of 131072 tokens have one row; or by the waits of its steps, where buckets are many:
+// without zeros four workgroups are on a compute unit at once (100000 tokens added to 1M x 128 f32: 52 us in all, 63
+// with one at a time).
 template <class O, bool kZeros>
 __global__ __launch_bounds__((kZeros ? 2 : 1) * kGroupThreads, kZeros ? 4 : 8) void bucket_kernel(EmbedArgs a, Work w, int lanes) {
     constexpr int kAllThreads = (kZeros ? 2 : 1) * kGroupThreads, kAllWaves = kAllThreads / kWave;
@@ -539,7 +537,7 @@ constexpr int kFewRows = 256;        // rows of a workgroup at most
 // 2^run_bits neighbouring rows in turn: the commonest tokens are often neighbours (4096 tokens of text by 50000 x 512
 // f16, 98 neighbouring rows each: 54 us instead of 18), while a run is to be worth a write.  `lanes` lanes are a group; each takes
 // the same share of the tokens, and the sum of a row that reaches over several shares is put together
-// by the group it starts in.  Bound by the waits of its steps (1000 tokens by 3000 x 100 f32: 6.4 us; four launches took 18),
+// by the group it starts in.  Bound by the waits of its steps (1000 tokens by 3000 x 100 f32: 6.6 us; four launches took 18),
 // by its zeros where the table is large (100 by 1M x 256 f16: 96 us, 5.3 TB/s).
 template <class T, class O>
 __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, bool clears, int rows, int run_bits, int64_t blocks, int lanes, int64_t first) {
@@ -706,9 +704,10 @@ int grad_of_few(const EmbedArgs& a, hipStream_t s) {
     // a row of up to 128 pieces is not shared by workgroups (4000 tokens by 50000 x 520 f16 22 us, 26 in two slices), longer
     // ones are by 64 (by 50000 x 2048 39 us, 42 with 128)
     const int pieces = (a.dim + Piece<T>::kLen - 1) / Piece<T>::kLen, lanes = lanes_for(pieces, pieces <= 2 * kWave ? 2 * kWave : kWave);
-    // runs of 512 bytes or more; 512 workgroups to fill the device, each of which reads all ids (83 tokens by 5130 x 1872 f32 11 us,
-    // 19 with as many for each of the 8 slices, 4000 by 32000 x 4096 f16 65 and 91); where rows share lines and few tokens can be one workgroup's,
-    // of 4096 (32 tokens by 410256 x 624 f16: 107 us, 142 with runs of a row)
+    // runs of 512 bytes or more; 512 workgroups to fill the device, each of which reads all ids (83 tokens by 5130 x
+    // 1872 f32 11 us, 19 with as many for each of the 8 slices, 4000 by 32000 x 4096 f16 65 and 91); where rows share
+    // lines and few tokens can be one workgroup's, of 4096 (32 tokens by 410256 x 624 f16: 107 us, 142 with runs of a
+    // row)
     const int64_t row_bytes = (int64_t)a.dim * (int)sizeof(typename O::raw), run_bytes = a.n <= 256 && row_bytes % 128 ? 4096 : 512;
     int run_bits = 0;
     while (run_bits < 3 && row_bytes << run_bits < run_bytes) run_bits++;

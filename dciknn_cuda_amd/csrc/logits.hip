@@ -36,10 +36,6 @@ __device__ inline u64 entry_of(float z, int index) {
 __device__ inline float entry_logit(u64 e) { return ord2f((uint32_t)(e >> 32)); }
 __device__ inline int entry_index(u64 e) { return (int)(0xffffffffu - (uint32_t)e); }
 
-__device__ inline int lanes_below(u64 mask) {
-    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-}
-
 // What one lane wrote to the wavefront's own part of LDS the others may read after this.
 __device__ inline void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

@@ -195,6 +195,11 @@ constexpr float kLog2e = 1.44269504088896341f;
 // factor themselves, so that a ruled-out entry adds 0 * -256 and not 0 * -inf.
 constexpr float kFloor2 = -256.f;
 
+// Set bits of `mask` below this lane's.
+__device__ inline int lanes_below(unsigned long long mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 // What lane (this one ^ O) holds, without the wait for LDS that lane_xor's swizzles by 4, 8 and 16 are.
 template <int O> __device__ inline uint32_t other_lane(uint32_t v) {
     if constexpr (O == 4) {           // of 8 lanes in reverse, each four in reverse
