@@ -488,6 +488,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
     __shared__ alignas(16) float s_q[kRowThreads];
     __shared__ float s_y[kRowThreads];
     __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
+    __shared__ float s_loss[kRowWaves];                  // (not s_sum: a wavefront behind may still read that one)
     __shared__ float4 s_teacher;                         // max, log2 sum, whether there is one, whether its ids and logits are sound
     const int tid = threadIdx.x, wave = tid / kWave;
     // whole pieces, and behind them less than one whose elements a thread each takes
@@ -631,11 +632,11 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         float loss = q == 0.f ? 0.f : q * (q2 - logp);
         s_q[tid] = q;
         loss = sum_of_lanes(loss);
-        if (lane_id() == 0) s_sum[wave] = loss;
+        if (lane_id() == 0) s_loss[wave] = loss;
         __syncthreads();
         if (tid == 0) {
             loss = 0.f;
-            for (int v = 0; v < kRowWaves; v++) loss += s_sum[v];
+            for (int v = 0; v < kRowWaves; v++) loss += s_loss[v];
             a.losses[row] = empty ? 0.f : t.w != 0.f ? __builtin_nanf("") : loss * kLn2;
             if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
         }

@@ -591,3 +591,16 @@ def test_lookup_gradient_of_few_tokens_by_a_large_table(gpu):
     assert ((got.double() - want).abs() <= 2 * 2.0 ** -23 * want.abs().clamp(max=8)).all()
     del want
     assert torch.equal(gpu.embed_grad(grad, on_gpu(ids, torch.int64), v, out=torch.zeros_like(got)), got)
+
+
+# Every number of threads, more rows than workgroups: wavefronts hand over sums, losses and slots of one row after the other.
+@pytest.mark.parametrize("n,v,k,dtype", [(7000, 1500, 64, "f16"), (3000, 4001, 200, "bf16"), (2000, 30_001, 130, "f16"), (1200, 60_000, 300, "bf16"), (700, 30_000, 900, "f32")])
+def test_distillation_of_many_rows_is_the_same_again(gpu, n, v, k, dtype):
+    """Losses far from the rows' sums, rows alike but for their place: a sum taken for another's would show."""
+    z = (40 * torch.rand(3, v, device="cuda")).to(TYPES[dtype]).repeat(-(-n // 3), 1)[:n]
+    ids, teacher = (t.repeat(-(-n // 3), 1)[:n] for t in (torch.randint(0, v, (3, k), device="cuda"), torch.randn(3, k, device="cuda")))
+    first = gpu.distill_step(z, ids, teacher)
+    for i in range(3):
+        losses, grad = gpu.distill_step(z, ids, teacher)
+        assert torch.equal(losses, first[0]) and torch.equal(grad, first[1])
+        assert torch.equal(losses, losses[:3].repeat(-(-n // 3))[:n]) and torch.equal(grad, grad[:3].repeat(-(-n // 3), 1)[:n])
