@@ -117,6 +117,23 @@ __device__ inline float teacher_at(const LogitArgs& a, int64_t i) {
     }
 }
 
+// (z - m) / T - log Z in 32 bits, what is returned of a logit: infinite only where the value itself is beyond them.  (The
+// difference of halves holds any two logits; a factor log2(e) / T, as the exponents have, is beyond 1 and would take
+// the lowest value to -inf.)
+__device__ inline float log_share(float z, float m, float half_t, float log_sum) { return (0.5f * z - 0.5f * m) / half_t - log_sum; }
+
+// Half of q (log q - log p), with the teacher's logit y, its maximum ym, the student's z and zm, `log_ratio` the logarithm of the
+// teacher's sum over the student's.  (The weight comes ahead of the quotient: log p may be beyond 32 bits where their product is not.)
+__device__ inline float half_loss(float q, float y, float ym, float z, float zm, float half_t, float log_ratio) {
+    const float h = 0.5f * q, d = (0.5f * y - 0.5f * ym) - (0.5f * z - 0.5f * zm);
+    return h * d / half_t - h * log_ratio;
+}
+// A loss from its half.  One that is beyond 32 bits by no more than a sum's rounding is the largest number: q_j that are 1 together
+// but for their rounding, all of them of tokens at the type's lowest value, are not to give infinity.
+__device__ inline float loss_of_half(float half) {
+    return half > 0.5f * __FLT_MAX__ && half <= 0.5f * __FLT_MAX__ * (1.f + 0x1p-18f) ? __FLT_MAX__ : half + half;
+}
+
 // Whether a row of logits holds nothing but -inf.
 __device__ inline bool nothing_left(const Softmax& f) { return f.m == kNoLogit && f.s == 0.f; }
 
@@ -146,12 +163,12 @@ template <class T>
 __device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& f, WaveTop& top, int64_t t, float z_t) {
     const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
     const bool none = nothing_left(f);
-    const float log2s = log2_fast(f.s);
-    const float entropy = none ? 0.f : (log2s - f.a / f.s) * kLn2;
+    const float log2s = log2_fast(f.s), log_s = logf(f.s);
+    const float entropy = none ? 0.f : log_s - f.a / f.s * kLn2;
     if (lane_id() == 0) {
         float lp = 0.f;
         if (t >= a.vocab) lp = __builtin_nanf("");
-        else if (t >= 0) lp = none ? kNoLogit : ((z_t - f.m) * a.c2 - log2s) * kLn2;
+        else if (t >= 0) lp = none ? kNoLogit : log_share(z_t, f.m, a.half_t, log_s);
         a.logprobs[row] = lp;
         a.entropy[row] = entropy;
         if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, entropy * kLog2e, 0.f);
@@ -165,7 +182,7 @@ __device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& 
     if (lane_id() < count) {
         const u64 e = top.best;
         ids[lane_id()] = entry_index(e);
-        lps[lane_id()] = ((entry_logit(e) - f.m) * a.c2 - log2s) * kLn2;
+        lps[lane_id()] = log_share(entry_logit(e), f.m, a.half_t, log_s);
     }
     // what is ruled out (or no number) follows in order of its index
     const float rest = f.s != f.s ? f.s : kNoLogit;
@@ -198,19 +215,17 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
     t.join_wave<false>(a.c2);
     wrong = __ballot(wrong) != 0;
     const bool empty = nothing_left(t), none = nothing_left(f);
-    const float log2t = log2_fast(t.s);
+    const float log2t = log2_fast(t.s), log_ratio = logf(t.s) - (none ? 0.f : logf(f.s));
     float log2s = log2_fast(f.s);
-    float sum = 0.f;
+    float sum = 0.f;      // of halves
     for (int j = lane_id(); j < a.slots; j += kWave) {
         const int64_t id = id_at(a.ids, a.wide_ids, at + j);
         const float y = id < 0 ? kNoLogit : teacher_at(a, at + j);
         if (y == kNoLogit || id >= a.vocab) continue;
-        const float logq = (y - t.m) * a.c2 - log2t;
-        const float q = exp2_fast(logq);
-        const float logp = none ? kNoLogit : ((float)z[id] - f.m) * a.c2 - log2s;
-        if (!(q == 0.f)) sum += q * (logq - logp);
+        const float q = exp2_fast((y - t.m) * a.c2 - log2t);
+        if (!(q == 0.f)) sum += half_loss(q, y, t.m, (float)z[id], none ? 0.f : f.m, a.half_t, log_ratio);
     }
-    sum = sum_of_lanes(sum) * kLn2;
+    sum = loss_of_half(sum_of_lanes(sum));
     if (wrong || t.s != t.s) sum = log2s = __builtin_nanf("");
     if (empty) sum = 0.f;
     if (lane_id() == 0) {
@@ -489,7 +504,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
     __shared__ float s_y[kRowThreads];
     __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
     __shared__ float s_loss[kRowWaves];                  // (not s_sum: a wavefront behind may still read that one)
-    __shared__ float4 s_teacher;                         // max, log2 sum, whether there is one, whether its ids and logits are sound
+    __shared__ float4 s_teacher;                         // max, log2 and log of the sum, 0 without one, NaN if its ids or logits are unsound
     const int tid = threadIdx.x, wave = tid / kWave;
     // whole pieces, and behind them less than one whose elements a thread each takes
     const int pieces = a.vocab / P::kLen, end = pieces * P::kLen + tid;
@@ -555,7 +570,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             }
             t.join_wave<false>(a.c2);
             wrong = __ballot(wrong) != 0 || t.s != t.s;
-            if (lane_id() == 0) s_teacher = make_float4(kept_max(t), log2_fast(t.s), nothing_left(t) ? 0.f : 1.f, wrong ? 1.f : 0.f);
+            if (lane_id() == 0) s_teacher = make_float4(kept_max(t), log2_fast(t.s), logf(t.s), nothing_left(t) ? 0.f : wrong ? __builtin_nanf("") : 1.f);
         }
         Softmax f = Softmax::none();
 #pragma unroll
@@ -587,8 +602,8 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         }
         f.join_wave<false>(a.c2);
         const float4 t = s_teacher;
-        const bool none = nothing_left(f), empty = t.z == 0.f;
-        const float m = kept_max(f), log2s = !empty && t.w != 0.f ? __builtin_nanf("") : log2_fast(f.s);
+        const bool none = nothing_left(f), empty = t.w == 0.f, wrong = t.w != t.w;
+        const float m = kept_max(f), log2s = wrong ? __builtin_nanf("") : log2_fast(f.s);
         // (read through the scalar cache: no vector load to wait for)
         const float weight = a.weights ? ((const __attribute__((address_space(4))) float*)a.weights)[row] : 1.f;
         const float w = none || empty ? 0.f : weight * a.inv_t;
@@ -627,9 +642,8 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)(kept ? gradient((float)was_end) : 0.f);
         // the teacher's part: the loss, and its tokens
         const int token = s_id[tid];
-        const float q2 = (s_y[tid] - t.x) * a.c2 - t.y, q = token < 0 ? 0.f : exp2_fast(q2);
-        const float logp = none ? kNoLogit : (zy - m) * a.c2 - log2s;
-        float loss = q == 0.f ? 0.f : q * (q2 - logp);
+        const float y = s_y[tid], q = token < 0 ? 0.f : exp2_fast((y - t.x) * a.c2 - t.y);
+        float loss = q == 0.f ? 0.f : half_loss(q, y, t.x, zy, none ? 0.f : m, a.half_t, t.z - (none ? 0.f : logf(f.s)));       // (half of it)
         s_q[tid] = q;
         loss = sum_of_lanes(loss);
         if (lane_id() == 0) s_loss[wave] = loss;
@@ -637,7 +651,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         if (tid == 0) {
             loss = 0.f;
             for (int v = 0; v < kRowWaves; v++) loss += s_loss[v];
-            a.losses[row] = empty ? 0.f : t.w != 0.f ? __builtin_nanf("") : loss * kLn2;
+            a.losses[row] = empty ? 0.f : wrong ? __builtin_nanf("") : loss_of_half(loss);
             if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
         }
         if (w != 0.f && token >= 0 && token < a.vocab) {

@@ -54,6 +54,7 @@ LogitArgs logit_args(const void* z, int dtype, int64_t n, int vocab, int64_t str
     a.stride = stride;
     a.vocab = vocab;
     a.inv_t = 1.f / temperature;
+    a.half_t = 0.5f * temperature;
     a.c2 = (float)(1.44269504088896340736 / (double)temperature);
     a.ids = ids;
     a.wide_ids = id_bytes == 8;

@@ -26,7 +26,7 @@ struct LogitArgs {
     const void* z;                // logits: row r at z + r * stride (elements)
     int64_t n, stride, first;     // `first`: the first row of a launch
     int vocab;
-    float c2, inv_t;              // log2(e) / temperature, 1 / temperature
+    float c2, inv_t, half_t;      // log2(e) / temperature, 1 / temperature, temperature / 2
     const void* ids;              // targets [n], or the teacher's ids [n][slots]
     bool wide_ids;
     int splits, per_split;        // workgroups of a row, 16-byte pieces of each
@@ -233,8 +233,8 @@ __device__ inline float sum_of_lanes(float v) {
 
 // Running statistics of a softmax over entries z at temperature T, exponents to the base 2
 // (c2 = log2(e) / T):  m = max z,  s = sum 2^((z - m) c2),  a = sum (z - m) c2 2^((z - m) c2).
-// The difference z - m is formed before the factor, so that the type's lowest value cannot
-// overflow.  With m = -inf nothing but -inf was seen and s = a = 0; a NaN or +inf leaves s = NaN.
+// The difference z - m is formed before the factor: a product that is beyond 32 bits, as the type's
+// lowest value gives, is -inf and 2 to it 0, as it should be.  With m = -inf nothing but -inf was seen and s = a = 0; a NaN or +inf leaves s = NaN.
 struct Softmax {
     float m, s, a;
 

@@ -604,3 +604,63 @@ def test_distillation_of_many_rows_is_the_same_again(gpu, n, v, k, dtype):
         losses, grad = gpu.distill_step(z, ids, teacher)
         assert torch.equal(losses, first[0]) and torch.equal(grad, first[1])
         assert torch.equal(losses, losses[:3].repeat(-(-n // 3))[:n]) and torch.equal(grad, grad[:3].repeat(-(-n // 3), 1)[:n])
+
+
+# Logits at the lowest value of their type: what the definition gives is a number wherever float32 holds it, and is returned.
+# (Off by the rounding of the difference, of the quotient and of the stored value: 2^-22 of it, beside what a sum is off.)
+def _all_near(got, want):
+    got = f64(got)
+    with np.errstate(over="ignore"):
+        beyond = np.isinf(want.astype(np.float32))
+    assert np.array_equal(np.isinf(got), beyond) and np.array_equal(got[beyond] > 0, want[beyond] > 0), (got, want)
+    far = np.abs(got - want)[~beyond] - 2 * SUM - 2.0 ** -22 * np.abs(want[~beyond])
+    assert (far <= 0).all(), far.max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("temperature", [0.9, 1.0, 1.2, 3.0])
+@pytest.mark.parametrize("n,v", [(3, 200), (2, 33_000), (4100, 320)])
+def test_log_probabilities_of_the_lowest_logits(gpu, dtype, temperature, n, v):
+    r = gen(v)
+    z = on_gpu(r.normal(size=(n, v)), TYPES[dtype])
+    z[:, 5:] = torch.finfo(TYPES[dtype]).min
+    if dtype != "f16":
+        z[1, :3] = 1e38                          # a difference beyond float32; its quotient by 3 is not
+    targets = r.integers(0, v, n)
+    want = O.token_logprobs(f64(z), targets, 8, temperature)
+    got = gpu.token_logprobs(z, on_gpu(targets, torch.int64), 8, temperature)
+    assert np.array_equal(got[2].cpu().numpy(), want[2])
+    for i in (0, 1, 3):
+        _all_near(got[i], want[i])
+    if dtype != "f16" and temperature == 1.0:
+        finite = torch.isfinite(torch.log_softmax(z.float(), 1).gather(1, on_gpu(targets, torch.int64)[:, None])[:, 0])
+        assert torch.isfinite(got[0][finite]).all() and finite[0]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("temperature", [0.9, 1.0, 3.0])
+@pytest.mark.parametrize("n,v", [(5, 300), (5, 9000), (5, 140_000), (100, 70_000)])
+def test_distillation_to_the_lowest_logits(gpu, dtype, temperature, n, v):
+    """The teacher names tokens that the student's mask has at the type's lowest value: one of them, some, all."""
+    r = gen(v + n)
+    z = on_gpu(r.normal(size=(n, v)), TYPES[dtype])
+    z[:, 50:] = torch.finfo(TYPES[dtype]).min
+    ids, teacher = r.integers(0, 50, (n, 7)), r.normal(size=(n, 7))
+    ids[0, 2] = 60
+    ids[1, 3:] = [50, 70, 80, 299]
+    ids[2] = r.integers(50, v, 7)                # the weights' sum is rounded, the loss is not to be beyond it
+    ids[3], teacher[3] = 77, -200.0 * np.arange(7)        # all of the weight on one
+    ids[4, :3], teacher[4, 3:] = 90, -np.inf
+    weights = np.full(n, 0.5)
+    d_teacher = on_gpu(teacher, torch.float32)
+    want, ref, size = O.distill(f64(z), ids, f64(d_teacher), temperature, weights)
+    losses, grad = gpu.distill_step(z, on_gpu(ids, torch.int64), d_teacher, on_gpu(weights, torch.float32), temperature)
+    _all_near(losses, want)
+    near(grad, ref, size, dtype)
+    z.requires_grad_()
+    loss = gpu.distill_loss(z, on_gpu(ids, torch.int32), d_teacher, temperature)
+    _all_near(loss, want)
+    if temperature > 0.95:
+        assert torch.isfinite(losses).all() and torch.isfinite(loss).all()
+    dz, = torch.autograd.grad(loss, z, on_gpu(weights, torch.float32))
+    near(dz, ref, size, dtype)
