@@ -122,11 +122,20 @@ __device__ inline float teacher_at(const LogitArgs& a, int64_t i) {
 // the lowest value to -inf.)
 __device__ inline float log_share(float z, float m, float half_t, float log_sum) { return (0.5f * z - 0.5f * m) / half_t - log_sum; }
 
+// 2^((z - m) c2) with what the difference and the product are rounded by made good: a teacher's weight is a factor of all that
+// its token adds to a loss and a gradient, and the two roundings of an exponent of 10 would take it 1e-6 from its value.
+__device__ inline float power_of(float z, float m, float c2, float c2_rest) {
+    const float d = z - m, x = d * c2, e = exp2_fast(x);
+    const float b = d - z, lost = (z - (d - b)) - (m + b);             // z - m = d + lost
+    const float rest = __builtin_fmaf(d, c2, -x) + __builtin_fmaf(d, c2_rest, lost * c2);
+    return e == 0.f ? 0.f : __builtin_fmaf(e, rest * kLn2, e);
+}
+
 // Half of q (log q - log p), with the teacher's logit y, its maximum ym, the student's z and zm, `log_ratio` the logarithm of the
-// teacher's sum over the student's.  (The weight comes ahead of the quotient: log p may be beyond 32 bits where their product is not.)
-__device__ inline float half_loss(float q, float y, float ym, float z, float zm, float half_t, float log_ratio) {
-    const float h = 0.5f * q, d = (0.5f * y - 0.5f * ym) - (0.5f * z - 0.5f * zm);
-    return h * d / half_t - h * log_ratio;
+// teacher's sum over the student's.  (The weight comes ahead of the logits: log p may be beyond 32 bits where their product is not.)
+__device__ inline float half_loss(float q, float y, float ym, float z, float zm, float inv_t, float log_ratio) {
+    const float d = (0.5f * y - 0.5f * ym) - (0.5f * z - 0.5f * zm);
+    return q * inv_t * d - 0.5f * q * log_ratio;
 }
 // A loss from its half.  One that is beyond 32 bits by no more than a sum's rounding is the largest number: q_j that are 1 together
 // but for their rounding, all of them of tokens at the type's lowest value, are not to give infinity.
@@ -163,7 +172,7 @@ template <class T>
 __device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& f, WaveTop& top, int64_t t, float z_t) {
     const typename T::raw* z = (const typename T::raw*)a.z + row * a.stride;
     const bool none = nothing_left(f);
-    const float log2s = log2_fast(f.s), log_s = logf(f.s);
+    const float log_s = logf(f.s);
     const float entropy = none ? 0.f : log_s - f.a / f.s * kLn2;
     if (lane_id() == 0) {
         float lp = 0.f;
@@ -171,7 +180,7 @@ __device__ void finish_logprobs(const LogitArgs& a, int64_t row, const Softmax& 
         else if (t >= 0) lp = none ? kNoLogit : log_share(z_t, f.m, a.half_t, log_s);
         a.logprobs[row] = lp;
         a.entropy[row] = entropy;
-        if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, entropy * kLog2e, 0.f);
+        if (a.stats) a.stats[row] = make_float4(kept_max(f), f.s, entropy * kLog2e, 0.f);
     }
     const int k = a.top;
     if (!k) return;
@@ -215,22 +224,22 @@ __device__ void finish_distill(const LogitArgs& a, int64_t row, const Softmax& f
     t.join_wave<false>(a.c2);
     wrong = __ballot(wrong) != 0;
     const bool empty = nothing_left(t), none = nothing_left(f);
-    const float log2t = log2_fast(t.s), log_ratio = logf(t.s) - (none ? 0.f : logf(f.s));
-    float log2s = log2_fast(f.s);
+    const float share = 1.f / t.s, log_ratio = logf(t.s) - (none ? 0.f : logf(f.s));
     float sum = 0.f;      // of halves
     for (int j = lane_id(); j < a.slots; j += kWave) {
         const int64_t id = id_at(a.ids, a.wide_ids, at + j);
         const float y = id < 0 ? kNoLogit : teacher_at(a, at + j);
         if (y == kNoLogit || id >= a.vocab) continue;
-        const float q = exp2_fast((y - t.m) * a.c2 - log2t);
-        if (!(q == 0.f)) sum += half_loss(q, y, t.m, (float)z[id], none ? 0.f : f.m, a.half_t, log_ratio);
+        const float q = power_of(y, t.m, a.c2, a.c2_rest) * share;
+        if (!(q == 0.f)) sum += half_loss(q, y, t.m, (float)z[id], none ? 0.f : f.m, a.inv_t, log_ratio);
     }
     sum = loss_of_half(sum_of_lanes(sum));
-    if (wrong || t.s != t.s) sum = log2s = __builtin_nanf("");
+    wrong |= t.s != t.s;
+    if (wrong) sum = __builtin_nanf("");
     if (empty) sum = 0.f;
     if (lane_id() == 0) {
         a.losses[row] = sum;
-        if (a.stats) a.stats[row] = make_float4(kept_max(f), log2s, kept_max(t), log2t);
+        if (a.stats) a.stats[row] = make_float4(kept_max(f), wrong ? __builtin_nanf("") : f.s, kept_max(t), share);
     }
 }
 
@@ -409,8 +418,10 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
     const Row<T> row(a.z, at_row, a.stride, a.vocab);
     typename T::raw* dz = (typename T::raw*)a.grad + at_row * a.grad_stride;
     const float4 st = a.stats[at_row];
-    // What a gradient is made of: dz = p (c0 + c1 log2 p) + at the target c2.
+    // What a gradient is made of: dz = p (c0 + c1 log2 p) + at_target, with p = 2^x / sum.  (The sum as a factor: its logarithm
+    // in the exponent, a number of 10 to 20, would bring a rounding of 1e-6 into every p.)
     float c0, c1 = 0.f, at_target = 0.f;
+    const float log2s = log2_fast(st.y);
     int64_t target = -1;
     bool zero = st.x == kNoLogit;
     if constexpr (kMode == kDistill) {
@@ -426,6 +437,7 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
         at_target = g;
         if (target >= a.vocab && g != 0.f) c0 = __builtin_nanf("");
     }
+    const float share0 = c0 / st.y, share1 = c1 / st.y;
     float own_z[kMode == kDistill ? kOwn : 1];
     bool here = false;
     if constexpr (kMode == kDistill) {
@@ -440,7 +452,7 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
                 const float y = teacher_at(a, at_row * a.slots + j);
                 const bool in = id >= 0 && id < a.vocab && id / P::kLen >= tile && id / P::kLen < tile + kTile && y != kNoLogit;
                 s_id[j] = in ? (int)id : -1;
-                s_q[j] = exp2_fast((y - st.z) * a.c2 - st.w);
+                s_q[j] = power_of(y, st.z, a.c2, a.c2_rest) * st.w;
                 if (in) own_z[o] = (float)row.z[id];       // before it is written over
                 here |= in;
             }
@@ -459,10 +471,9 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
             P::unpack(row.load(i), y);
 #pragma unroll
             for (int k = 0; k < P::kLen; k++) {
-                const float x = (y[k] - st.x) * a.c2 - st.y;      // log2 p
-                const float p = exp2_fast(x);
-                if constexpr (kMode == kDistill) y[k] = p * c0;
-                else y[k] = p * __builtin_fmaf(c1, fmaxf(x, kFloor2), c0);
+                const float x = (y[k] - st.x) * a.c2, e = exp2_fast(x);
+                if constexpr (kMode == kDistill) y[k] = e * share0;
+                else y[k] = e * __builtin_fmaf(share1, fmaxf(x - log2s, kFloor2), share0);
             }
             if (kMode != kDistill && target / P::kLen == i) {
 #pragma unroll
@@ -482,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void logit_grad_kernel(LogitArgs a) {
             const int id = s_id[j];
             if (id < 0) continue;
             const float q = slots_of_token(s_id, s_q, (a.slots + 3) / 4, id);
-            dz[id] = (typename T::raw)(c0 * (exp2_fast((own_z[o] - st.x) * a.c2 - st.y) - q));
+            dz[id] = (typename T::raw)(share0 * exp2_fast((own_z[o] - st.x) * a.c2) - c0 * q);
         }
     }
 }
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
     __shared__ float s_y[kRowThreads];
     __shared__ float s_max[kRowWaves], s_sum[kRowWaves];
     __shared__ float s_loss[kRowWaves];                  // (not s_sum: a wavefront behind may still read that one)
-    __shared__ float4 s_teacher;                         // max, log2 and log of the sum, 0 without one, NaN if its ids or logits are unsound
+    __shared__ float4 s_teacher;                         // max, 1 / sum, log sum, 0 without one and NaN if its ids or logits are unsound
     const int tid = threadIdx.x, wave = tid / kWave;
     // whole pieces, and behind them less than one whose elements a thread each takes
     const int pieces = a.vocab / P::kLen, end = pieces * P::kLen + tid;
@@ -570,7 +581,7 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
             }
             t.join_wave<false>(a.c2);
             wrong = __ballot(wrong) != 0 || t.s != t.s;
-            if (lane_id() == 0) s_teacher = make_float4(kept_max(t), log2_fast(t.s), logf(t.s), nothing_left(t) ? 0.f : wrong ? __builtin_nanf("") : 1.f);
+            if (lane_id() == 0) s_teacher = make_float4(kept_max(t), 1.f / t.s, log2_fast(t.s) * kLn2, nothing_left(t) ? 0.f : wrong ? __builtin_nanf("") : 1.f);
         }
         Softmax f = Softmax::none();
 #pragma unroll
@@ -603,12 +614,12 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         f.join_wave<false>(a.c2);
         const float4 t = s_teacher;
         const bool none = nothing_left(f), empty = t.w == 0.f, wrong = t.w != t.w;
-        const float m = kept_max(f), log2s = wrong ? __builtin_nanf("") : log2_fast(f.s);
+        const float m = kept_max(f), sum_z = wrong ? __builtin_nanf("") : f.s;
         // (read through the scalar cache: no vector load to wait for)
         const float weight = a.weights ? ((const __attribute__((address_space(4))) float*)a.weights)[row] : 1.f;
         const float w = none || empty ? 0.f : weight * a.inv_t;
         char* dz = (char*)a.grad + row * a.grad_stride * (int64_t)sizeof(raw_t);
-        const float share = w * exp2_fast(-log2s);           // the row's factor / the sum of the powers
+        const float share = w / sum_z;                       // the row's factor / the sum of the powers
         // (a row without weight has gradient 0 whatever it holds: by the bits)
         const uint32_t kept = w == 0.f ? 0u : ~0u;
         auto gradient = [&](float x) { return share * exp2_fast((x - m) * a.c2); };
@@ -642,17 +653,21 @@ __global__ __launch_bounds__(kRowThreads) void distill_rows_kernel(LogitArgs a) 
         if (end < a.vocab) ((raw_t*)dz)[end] = (raw_t)(kept ? gradient((float)was_end) : 0.f);
         // the teacher's part: the loss, and its tokens
         const int token = s_id[tid];
-        const float y = s_y[tid], q = token < 0 ? 0.f : exp2_fast((y - t.x) * a.c2 - t.y);
-        float loss = q == 0.f ? 0.f : half_loss(q, y, t.x, zy, none ? 0.f : m, a.half_t, t.z - (none ? 0.f : logf(f.s)));       // (half of it)
+        float q = 0.f, loss = 0.f;                           // (half of it)
+        if (__any(token >= 0)) {          // (logf, half as far off, in the place of the logarithms here and above: 113 instead of 111 us for 1001 x 100003)
+            const float y = s_y[tid];
+            q = token < 0 ? 0.f : power_of(y, t.x, a.c2, a.c2_rest) * t.y;
+            loss = q == 0.f ? 0.f : half_loss(q, y, t.x, zy, none ? 0.f : m, a.inv_t, t.z - (none ? 0.f : log2_fast(f.s) * kLn2));
+            loss = sum_of_lanes(loss);
+        }
         s_q[tid] = q;
-        loss = sum_of_lanes(loss);
         if (lane_id() == 0) s_loss[wave] = loss;
         __syncthreads();
         if (tid == 0) {
             loss = 0.f;
             for (int v = 0; v < kRowWaves; v++) loss += s_loss[v];
             a.losses[row] = empty ? 0.f : wrong ? __builtin_nanf("") : loss_of_half(loss);
-            if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, log2s, empty ? kNoLogit : t.x, t.y);
+            if (a.stats) a.stats[row] = make_float4(none ? kNoLogit : m, sum_z, empty ? kNoLogit : t.x, t.y);
         }
         if (w != 0.f && token >= 0 && token < a.vocab) {
             const float sum = slots_of_token(s_id, s_q, (a.slots + 3) / 4, token);

@@ -55,7 +55,9 @@ LogitArgs logit_args(const void* z, int dtype, int64_t n, int vocab, int64_t str
     a.vocab = vocab;
     a.inv_t = 1.f / temperature;
     a.half_t = 0.5f * temperature;
-    a.c2 = (float)(1.44269504088896340736 / (double)temperature);
+    const double c2 = 1.44269504088896340736 / (double)temperature;
+    a.c2 = (float)c2;
+    a.c2_rest = (float)(c2 - (double)a.c2);
     a.ids = ids;
     a.wide_ids = id_bytes == 8;
     a.splits = n ? logit_splits(n, vocab, dtype) : 1;

@@ -26,11 +26,12 @@ struct LogitArgs {
     const void* z;                // logits: row r at z + r * stride (elements)
     int64_t n, stride, first;     // `first`: the first row of a launch
     int vocab;
-    float c2, inv_t, half_t;      // log2(e) / temperature, 1 / temperature, temperature / 2
+    float c2, c2_rest;            // log2(e) / temperature and what it is rounded by
+    float inv_t, half_t;          // 1 / temperature, temperature / 2
     const void* ids;              // targets [n], or the teacher's ids [n][slots]
     bool wide_ids;
     int splits, per_split;        // workgroups of a row, 16-byte pieces of each
-    float4* stats;                // [n] (max, log2 sum, entropy / ln 2, -) or (max, log2 sum, teacher's max, teacher's log2 sum)
+    float4* stats;                // [n] (max, sum, entropy / ln 2, -) or (max, sum, teacher's max, 1 / teacher's sum)
     float4* part;                 // [n][splits] statistics of splits
     unsigned long long* part_top; // [n][splits][top] their best pieces
     // log probabilities
@@ -257,14 +258,17 @@ struct Softmax {
         for (int k = 1; k < N; k++) top = fmaxf(top, z[k]);
         add<N, kEntropy>(z, top, c2);
     }
-    // `top` is the largest of them.
+    // `top` is the largest of them.  Many are added up by themselves first: a thread has a thousand terms of a long row, and their
+    // sum one after the other was twice as far off as one in parts.
     template <int N, bool kEntropy>
     __device__ void add(const float (&z)[N], float top, float c2) {
+        constexpr bool kInParts = N > 8;
         top = fmaxf(top, m);
         const float ref = top == kNoLogit ? 0.f : top;
         const float d = fmaxf((m - ref) * c2, kFloor2), f = exp2_fast(d);
-        if (kEntropy) a = f * (a + d * s);
-        s *= f;
+        const float a0 = f * (a + d * s), s0 = s * f;
+        if (kEntropy) a = kInParts ? 0.f : a0;
+        s = kInParts ? 0.f : s0;
         m = top;
 #pragma unroll
         for (int k = 0; k < N; k++) {
@@ -272,6 +276,8 @@ struct Softmax {
             s += e;
             if (kEntropy) a = __builtin_fmaf(fmaxf(x, kFloor2), e, a);
         }
+        if (kInParts) s += s0;
+        if (kInParts && kEntropy) a += a0;
     }
     // Over a wavefront; every lane gets the result.
     template <bool kEntropy>

@@ -664,3 +664,49 @@ def test_distillation_to_the_lowest_logits(gpu, dtype, temperature, n, v):
         assert torch.isfinite(losses).all() and torch.isfinite(loss).all()
     dz, = torch.autograd.grad(loss, z, on_gpu(weights, torch.float32))
     near(dz, ref, size, dtype)
+
+
+# How far rounding goes on the whole.  A row's sum: a thread's terms are added up 4 to 32 at a time and these sums, some 25 here, one
+# after the other; log Z has a value of up to 16, of which half a unit is 4.8e-7, as the difference to it has, and the terms' own
+# exponents, up to 24 to the base 2, are rounded by up to 9.5e-7, independently for the hundreds of terms that a sum comes from.
+# Uniform errors of half a unit have a root mean square of half a unit / sqrt(3): 2.8e-7 twice, and the rest below that: 4.8e-7.
+@pytest.mark.parametrize("dtype,temperature", [("f16", 1.0), ("f32", 0.7), ("bf16", 1.0)])
+@pytest.mark.parametrize("top", [0, 5])
+def test_rounding_of_long_rows(gpu, dtype, temperature, top):
+    n, v = 4096, 50_001
+    z = (2.5 * torch.randn(n, v, device="cuda")).to(TYPES[dtype])
+    targets = torch.randint(0, v, (n,), device="cuda")
+    z[torch.arange(n, device="cuda"), targets] += (12 * torch.rand(n, device="cuda")).to(z.dtype)
+    z.requires_grad_()
+    got = gpu.token_logprobs(z, targets, top, temperature)
+    g = torch.randn(n, device="cuda")
+    dz, = torch.autograd.grad(got[0], z, g)
+    lp_off = h_off = off = size = 0.0
+    for a in range(0, n, 512):
+        logp = torch.log_softmax(z[a:a + 512].detach().double() / temperature, 1)
+        t = targets[a:a + 512, None]
+        lp_off += (got[0][a:a + 512].double() - logp.gather(1, t)[:, 0]).square().sum().item()
+        p = torch.exp(logp)
+        h_off += (got[1][a:a + 512].double() + (p * logp).sum(1)).square().sum().item()
+        want = -p.scatter_add(1, t, -torch.ones_like(t, dtype=torch.float64)) * (g[a:a + 512, None].double() / temperature)
+        off += (dz[a:a + 512].double() - want).square().sum().item()
+        size += want.square().sum().item()
+    assert (lp_off / n) ** 0.5 < 4.8e-7 and (h_off / n) ** 0.5 < 4.8e-7
+    # a gradient's largest terms, which its size comes from, have exponents below 4, of which half a unit is 1.2e-7 or less, twice
+    # (the product, the factor's own rounding); an exponential's, a sum's, a factor's and the result's roundings are 6e-8 each
+    if dtype == "f32":
+        assert (off / size) ** 0.5 < 2.0e-7
+
+
+# In a gradient from statistics the sum itself is a factor: the rounding of its logarithm (half a unit of 16 to 32 is 9.5e-7) has no part in it.
+@pytest.mark.parametrize("n,v", [(3, 262_145), (2000, 100_000), (200, 50_001)])
+def test_gradients_of_flat_rows(gpu, n, v):
+    """Logits alike: every term is 1 and every gradient is 1 / v, to four roundings and those of the sum (of whole numbers: none)."""
+    z = torch.full((n, v), 2.5, device="cuda", requires_grad=True)
+    ids, teacher = torch.zeros(n, 1, dtype=torch.int64, device="cuda"), torch.zeros(n, 1, device="cuda")
+    lp, _ = gpu.token_logprobs(z, ids[:, 0])
+    by_logp, = torch.autograd.grad(lp.sum(), z)
+    by_loss, = torch.autograd.grad(gpu.distill_loss(z, ids, teacher).sum(), z)
+    _, by_step = gpu.distill_step(z.detach(), ids, teacher)
+    for dz in (-by_logp, by_loss, by_step):
+        assert ((dz[:, 1:].double() * v - 1).abs() <= 4 * 2.0 ** -24).all()
