@@ -132,10 +132,11 @@ __device__ inline float power_of(float z, float m, float c2, float c2_rest) {
 }
 
 // Half of q (log q - log p), with the teacher's logit y, its maximum ym, the student's z and zm, `log_ratio` the logarithm of the
-// teacher's sum over the student's.  (The weight comes ahead of the logits: log p may be beyond 32 bits where their product is not.)
+// teacher's sum over the student's.  (The weight comes ahead of the temperature: log p may be beyond 32 bits where their product is
+// not, and a small weight by a large temperature is not to be 0 times a difference that is infinite.)
 __device__ inline float half_loss(float q, float y, float ym, float z, float zm, float inv_t, float log_ratio) {
     const float d = (0.5f * y - 0.5f * ym) - (0.5f * z - 0.5f * zm);
-    return q * inv_t * d - 0.5f * q * log_ratio;
+    return q * d * inv_t - 0.5f * q * log_ratio;
 }
 // A loss from its half.  One that is beyond 32 bits by no more than a sum's rounding is the largest number: q_j that are 1 together
 // but for their rounding, all of them of tokens at the type's lowest value, are not to give infinity.

@@ -710,3 +710,15 @@ def test_gradients_of_flat_rows(gpu, n, v):
     _, by_step = gpu.distill_step(z.detach(), ids, teacher)
     for dz in (-by_logp, by_loss, by_step):
         assert ((dz[:, 1:].double() * v - 1).abs() <= 4 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("v", [50, 20_000, 140_000])
+def test_distillation_of_a_small_weight_at_a_high_temperature(gpu, v):
+    """A weight of 4e-31 over a temperature of 1e20 is 0 in 32 bits; times a token that is ruled out it is not to be NaN."""
+    z = torch.randn(2, v, device="cuda")
+    z[0, 7] = -float("inf")
+    ids, teacher = torch.tensor([[3, 7], [3, 7]], device="cuda"), torch.tensor([[0.0, -7e21], [0.0, -7e21]], device="cuda")
+    want = O.distill(f64(z), ids.cpu().numpy(), f64(teacher), float(np.float32(1e20)), np.ones(2))[0]
+    assert want[0] == np.inf
+    near_abs(gpu.distill_loss(z, ids, teacher, 1e20), want, 2 * SUM)
+    near_abs(gpu.distill_step(z, ids, teacher, temperature=1e20)[0], want, 2 * SUM)
