@@ -176,6 +176,7 @@ __global__ __launch_bounds__(kGroupThreads) void chunk_kernel(EmbedArgs a, Work 
             rank[j] = have + lanes_below(same);
             if (lanes_below(same) == 0) mine[bucket] = have + __popcll(same);
         }
+        wave_fence();
     }
     __syncthreads();
     uint32_t before = 0;
@@ -379,6 +380,7 @@ __global__ __launch_bounds__((kZeros ? 2 : 1) * kGroupThreads, kZeros ? 4 : 8) v
                     if (lanes_below(same) == 0) s_count[wave][bin] = rank + __popcll(same);
                     w.tokens[s_start[bin] + rank] = Token{p.row, p.at, rank, s_start[bin + 1] - s_start[bin]};
                 }
+                wave_fence();
             });
         } else if (kZeros) {
             const int64_t many = min((int64_t)kBins, rows - bin0);
@@ -585,6 +587,7 @@ __global__ __launch_bounds__(kGroupThreads) void few_kernel(EmbedArgs a, bool cl
             rank[j] = have + lanes_below(same);
             if (lanes_below(same) == 0) mine[bin[j]] = have + __popcll(same);
         }
+        wave_fence();
     }
     __syncthreads();
     uint32_t len = 0, all;

@@ -36,13 +36,6 @@ __device__ inline u64 entry_of(float z, int index) {
 __device__ inline float entry_logit(u64 e) { return ord2f((uint32_t)(e >> 32)); }
 __device__ inline int entry_index(u64 e) { return (int)(0xffffffffu - (uint32_t)e); }
 
-// What one lane wrote to the wavefront's own part of LDS the others may read after this.
-__device__ inline void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // One step of a bitonic sort over the lanes, larger ones first: towards runs of SIZE.
 template <int SIZE, int STRIDE, class V>
 __device__ inline void sort_step(V& v) {

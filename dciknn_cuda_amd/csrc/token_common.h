@@ -201,6 +201,14 @@ __device__ inline int lanes_below(unsigned long long mask) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
 }
 
+// What one lane wrote to the wavefront's own part of LDS the others may read after this.  (It orders the compiler:
+// the wavefront's accesses to LDS are in their order as they are.)
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // What lane (this one ^ O) holds, without the wait for LDS that lane_xor's swizzles by 4, 8 and 16 are.
 template <int O> __device__ inline uint32_t other_lane(uint32_t v) {
     if constexpr (O == 4) {           // of 8 lanes in reverse, each four in reverse

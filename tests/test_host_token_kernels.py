@@ -45,3 +45,14 @@ def test_between_two_barriers_a_shared_array_is_read_or_written():
             assert not (reads and writes), "%s is read and written in part %d of the loop" % (name, i)
     for name in shared:
         assert any(uses(part, name)[0] for part in parts) and any(uses(part, name)[1] for part in parts), name
+
+
+@pytest.mark.parametrize("kernel", ["chunk_kernel", "bucket_kernel", "few_kernel"])
+def test_counts_that_lanes_hand_on_are_ordered(kernel):
+    """One lane stores a count that other lanes of its wavefront read a round later: between the two stands a fence, which
+    keeps the compiler from moving or remembering one over the other."""
+    body = body_of("embed.hip", kernel)
+    stores = list(re.finditer(r"lanes_below\(same\) == 0\) (?:mine|s_count\[wave\])\[[^;]*\] = [^;]*;", body))
+    assert len(stores) == 1
+    rest = body[stores[0].end():]
+    assert re.match(r"[^;]*?(?:w\.tokens[^;]*;\s*)?\}\s*wave_fence\(\);", rest, re.S), rest[:200]
