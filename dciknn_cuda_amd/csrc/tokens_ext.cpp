@@ -103,7 +103,13 @@ Tensor floats(c10::IntArrayRef shape, const Tensor& like) {
 const float* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 int id_bytes(const Tensor& ids) { return ids.scalar_type() == torch::kInt64 ? 8 : 4; }
 
+// A tangent of forward mode would be dropped in silence: its derivative is not formed.
+void no_tangent(const Tensor& t) {
+    if (t.defined() && t._fw_grad(0).defined()) throw std::runtime_error("the token operators have no derivatives in forward mode");
+}
+
 void once_only(const variable_list& grads) {
+    for (const auto& g : grads) no_tangent(g);
     if (!torch::GradMode::is_enabled()) return;
     for (const auto& g : grads)
         if (g.defined() && g.requires_grad()) throw std::runtime_error("the token operators can be differentiated once only");
@@ -128,6 +134,7 @@ Tensor embed_forward(const Tensor& table, const Tensor& ids_in, double scale) {
 }
 
 Tensor embed_grad(const Tensor& grad, const Tensor& ids_in, int64_t num_rows, double scale, const c10::optional<Tensor>& into) {
+    no_tangent(grad);
     const Rows r = rows_of(grad, "grad");
     const Tensor ids = ids_of(ids_in, grad, "ids");
     if (leading(grad) != ids.sizes()) bad_value("grad must have one row for each id");
@@ -136,6 +143,7 @@ Tensor embed_grad(const Tensor& grad, const Tensor& ids_in, int64_t num_rows, do
     Tensor out;
     if (into) {
         out = *into;
+        no_tangent(out);
         const int code = type_code(out, "out");
         if (code != r.dtype && code != DCIH_F32) bad_type("out must be of grad's type or float32");
         if (out.device() != grad.device()) bad_value("out must be on the other tensors' device");
@@ -170,6 +178,7 @@ struct Embed : torch::autograd::Function<Embed> {
 };
 
 Tensor embed(const Tensor& table, const Tensor& ids, double scale) {
+    no_tangent(table);
     return wants_grad(table) ? Embed::apply(table, ids, scale) : embed_forward(table, ids, scale);
 }
 
@@ -231,6 +240,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 };
 
 py::tuple token_logprobs(const Tensor& logits, const Tensor& targets, int64_t top, double temperature) {
+    no_tangent(logits);
     if (wants_grad(logits)) {
         const auto got = Logprobs::apply(logits, targets, top, temperature);
         return top ? py::make_tuple(got[0], got[1], got[2], got[3]) : py::make_tuple(got[0], got[1]);
@@ -260,6 +270,7 @@ Teacher teacher_of(const Tensor& ids, const Tensor& teacher, const Tensor& logit
 // (losses, statistics, gradient)
 std::vector<Tensor> distill_forward(const Tensor& logits, const Tensor& ids, const Tensor& teacher, double temperature, bool keep,
                                     bool grad, const Tensor& weights, const Tensor& into) {
+    for (const Tensor& x : {logits, teacher, weights, into}) no_tangent(x);
     const Rows r = rows_of(logits, "logits");
     const Teacher q = teacher_of(ids, teacher, logits);
     const float t = temperature_of(temperature);

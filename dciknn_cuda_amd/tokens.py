@@ -7,7 +7,7 @@ results rounded once.  Rows may be at any distance from one another and start an
 are contiguous; ids are int32 or int64 (`DCI.query(..., return_int=True)` returns int32), ids and factors of any
 strides.  An id below 0 marks an empty slot, as `DCI.query` leaves them; an id beyond the table or the
 vocabulary is never accessed and gives NaN.  Work goes to torch's current stream, without a wait;
-gradients are taken through torch.autograd, once.  Wrong types raise TypeError, wrong
+gradients are taken through torch.autograd, once, and backward: a tangent of forward mode is refused.  Wrong types raise TypeError, wrong
 shapes and values ValueError.  The reference, a search engine alone, has no counterpart.
 """
 from . import _dci_cuda as _ext   # built by `python -m dciknn_cuda_amd.build`; no fallback

@@ -722,3 +722,32 @@ def test_distillation_of_a_small_weight_at_a_high_temperature(gpu, v):
     assert want[0] == np.inf
     near_abs(gpu.distill_loss(z, ids, teacher, 1e20), want, 2 * SUM)
     near_abs(gpu.distill_step(z, ids, teacher, temperature=1e20)[0], want, 2 * SUM)
+
+
+# ---- derivatives that are not formed -----------------------------------------------------
+def test_tangents_of_forward_mode_are_refused(gpu):
+    import torch.autograd.forward_ad as forward
+    z, t = torch.randn(4, 9, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    ids, teacher, ones = torch.zeros(4, 3, dtype=torch.int64, device="cuda"), torch.zeros(4, 3, device="cuda"), torch.ones(4, device="cuda")
+    with forward.dual_level():
+        def dual(x):
+            return forward.make_dual(x, torch.ones_like(x))
+        for call in (lambda: gpu.embed(dual(z), t), lambda: gpu.embed(dual(z.clone().requires_grad_()), t), lambda: gpu.embed_grad(dual(z), t, 5),
+                     lambda: gpu.embed_grad(z, t, 5, out=dual(torch.zeros(5, 9, device="cuda"))), lambda: gpu.token_logprobs(dual(z), t),
+                     lambda: gpu.token_logprobs(dual(z), t, 3), lambda: gpu.distill_loss(dual(z), ids, teacher), lambda: gpu.distill_loss(z, ids, dual(teacher)),
+                     lambda: gpu.distill_step(dual(z), ids, teacher), lambda: gpu.distill_step(z, ids, dual(teacher)),
+                     lambda: gpu.distill_step(z, ids, teacher, dual(ones)), lambda: gpu.distill_step(z, ids, teacher, out=dual(torch.zeros_like(z)))):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                call()
+        # without one they compute as ever
+        assert torch.equal(gpu.embed(z, t), z[t]) and gpu.token_logprobs(z, t)[0].shape == (4,)
+
+
+def test_tangents_of_a_gradient_are_refused(gpu):
+    import torch.autograd.forward_ad as forward
+    z, t = torch.randn(4, 9, device="cuda", requires_grad=True), torch.zeros(4, dtype=torch.int64, device="cuda")
+    ids, teacher = torch.zeros(4, 3, dtype=torch.int64, device="cuda"), torch.zeros(4, 3, device="cuda")
+    with forward.dual_level():
+        for out in (gpu.embed(z, t), gpu.token_logprobs(z, t)[0], gpu.distill_loss(z, ids, teacher)):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.autograd.grad(out, z, forward.make_dual(torch.ones_like(out), torch.ones_like(out)))
