@@ -135,6 +135,7 @@ Tensor embed_forward(const Tensor& table, const Tensor& ids_in, double scale) {
 
 Tensor embed_grad(const Tensor& grad, const Tensor& ids_in, int64_t num_rows, double scale, const c10::optional<Tensor>& into) {
     no_tangent(grad);
+    if (wants_grad(grad)) bad_value("no gradient is formed by grad: detach it");
     const Rows r = rows_of(grad, "grad");
     const Tensor ids = ids_of(ids_in, grad, "ids");
     if (leading(grad) != ids.sizes()) bad_value("grad must have one row for each id");

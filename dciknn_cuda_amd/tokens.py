@@ -27,7 +27,7 @@ def embed_grad(grad, ids, num_rows, scale=1.0, *, out=None):
 
     The sum's order depends on the ids alone: the same input gives the same bits.  With `out`
     ([num_rows, dim], contiguous, of grad's type or float32) the sums are added to it and it is returned; its
-    rows without ids are not touched."""
+    rows without ids are not touched.  No gradient is formed by `grad`: one that requires it is refused."""
     return _ext._embed_grad(grad, ids, num_rows, scale, out)
 
 

@@ -751,3 +751,14 @@ def test_tangents_of_a_gradient_are_refused(gpu):
         for out in (gpu.embed(z, t), gpu.token_logprobs(z, t)[0], gpu.distill_loss(z, ids, teacher)):
             with pytest.raises(RuntimeError, match="forward mode"):
                 torch.autograd.grad(out, z, forward.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_embed_grad_forms_no_graph(gpu):
+    grad, ids = torch.randn(4, 9, device="cuda", requires_grad=True), torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="detach"):
+        gpu.embed_grad(grad, ids, 5)
+    with pytest.raises(ValueError, match="detach"):
+        gpu.embed_grad(grad * 2, ids, 5, out=torch.zeros(5, 9, device="cuda"))
+    want = gpu.embed_grad(grad.detach(), ids, 5)
+    with torch.no_grad():
+        assert torch.equal(gpu.embed_grad(grad, ids, 5), want)
