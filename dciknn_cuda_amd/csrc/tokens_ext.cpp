@@ -282,7 +282,6 @@ std::vector<Tensor> distill_forward(const Tensor& logits, const Tensor& ids, con
     if (into.defined()) {
         if (into.sizes() != logits.sizes() || into.scalar_type() != logits.scalar_type() || into.device() != logits.device())
             bad_value("out must have the shape, type and device of logits");
-        if (wants_grad(into)) bad_value("out must not require a gradient");
         o = rows_of(into, "out");
         if (into.data_ptr() == logits.data_ptr() ? (o.stride != r.stride && r.n > 1) : into.is_alias_of(logits))
             bad_value("out must be logits itself or share no memory with it");
@@ -337,6 +336,9 @@ Tensor distill_loss(const Tensor& logits, const Tensor& ids, const Tensor& teach
 
 std::tuple<Tensor, Tensor> distill_step(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const c10::optional<Tensor>& weights,
                                         double temperature, const c10::optional<Tensor>& into) {
+    // (logits that a model computed require a gradient, and theirs may take their place; a parameter's may not)
+    if (into && wants_grad(*into) && (into->is_leaf() || !into->is_same(logits)))
+        bad_value("out must not require a gradient, but for logits that are no leaf");
     torch::NoGradGuard no_grad;
     const auto got = distill_forward(logits, ids, teacher, temperature, false, true, weights ? *weights : Tensor(), into ? *into : Tensor());
     return {got[0], got[2]};

@@ -58,5 +58,6 @@ def distill_step(logits, ids, teacher, weights=None, temperature=1.0, *, out=Non
     one call, which reads the logits once where rows fit the chip; no autograd graph.
 
     weights [...] float32, ones if not given; a row with weight 0 has gradient 0 whatever it
-    holds.  `out`: where the gradient goes, also `logits` itself."""
+    holds.  `out`: where the gradient goes, also `logits` itself; a leaf that requires a gradient, or anything
+    else that does, is refused."""
     return _ext._distill_step(logits, ids, teacher, weights, temperature, out)

@@ -762,3 +762,22 @@ def test_embed_grad_forms_no_graph(gpu):
     want = gpu.embed_grad(grad.detach(), ids, 5)
     with torch.no_grad():
         assert torch.equal(gpu.embed_grad(grad, ids, 5), want)
+
+
+def test_distillation_into_what_requires_a_gradient(gpu):
+    z, ids, teacher = torch.randn(4, 9, device="cuda"), torch.randint(0, 9, (4, 3), device="cuda"), torch.randn(4, 3, device="cuda")
+    want = gpu.distill_step(z, ids, teacher)[1]
+    leaf, weight = z.clone().requires_grad_(), torch.eye(9, device="cuda", requires_grad=True)
+    for logits, out in ((leaf, leaf), (z, leaf), (z, torch.zeros(4, 9, device="cuda", requires_grad=True)), (z, z @ weight), (z @ weight, z @ weight)):
+        before = out.detach().clone()
+        with pytest.raises(ValueError, match="out must not require a gradient"):
+            gpu.distill_step(logits, ids, teacher, out=out)
+        assert torch.equal(out, before)
+    # a model's own logits give way to their gradient, which goes on to its weights
+    logits = z @ weight
+    _, dz = gpu.distill_step(logits, ids, teacher, out=logits)
+    assert dz is logits and torch.equal(dz, want)
+    by_weight, = torch.autograd.grad(logits, weight, dz.detach())
+    assert torch.allclose(by_weight, z.t() @ want, atol=1e-5)
+    with torch.no_grad():
+        assert torch.equal(gpu.distill_step(leaf, ids, teacher, out=leaf)[1], want)
