@@ -73,7 +73,9 @@ Rows rows_of(const Tensor& t, const char* what) {
     for (int64_t d = t.dim() - 2; d >= 0; d--) {
         if (t.size(d) != 1 && t.numel()) {
             if (r.n == 1) r.stride = t.stride(d);
-            else if (t.stride(d) != r.stride * r.n) bad_value(std::string(what) + ": the rows must be at one distance from each other");
+            else if (t.stride(d) != r.stride * r.n)
+                bad_value(std::string(what) + ": the rows must be at one distance from each other; of a batch cut to fewer rows each take all rows, "
+                                              "those cut off with ids of -1, or make it contiguous");
         }
         r.n *= t.size(d);
     }

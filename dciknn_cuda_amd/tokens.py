@@ -2,13 +2,16 @@
 and finds: rows taken by ids and the gradient by their table, log probabilities of tokens, and
 the loss against a teacher that is known by its best tokens, as a query's neighbours are.
 
-The tensors are float32, float16 or bfloat16 cuda tensors; sums are formed in 32 bits and
-results rounded once.  Rows may be at any distance from one another and start anywhere, their own elements
-are contiguous; ids are int32 or int64 (`DCI.query(..., return_int=True)` returns int32), ids and factors of any
-strides.  An id below 0 marks an empty slot, as `DCI.query` leaves them; an id beyond the table or the
-vocabulary is never accessed and gives NaN.  Work goes to torch's current stream, without a wait;
-gradients are taken through torch.autograd, once, and backward: a tangent of forward mode is refused.  Wrong types raise TypeError, wrong
-shapes and values ValueError.  The reference, a search engine alone, has no counterpart.
+The tensors are float32, float16 or bfloat16 cuda tensors; sums are formed in 32 bits and results
+rounded once.  Rows may start anywhere and be at any one distance from each other, their own elements are
+contiguous.  (`logits[:, :-1]` of a batch is at two distances and refused: give all rows, with targets
+or teacher's ids of -1 in the last ones, whose log probabilities, losses and gradients by them are 0;
+entropies are of all rows.)  Ids are int32 or int64 (`DCI.query(..., return_int=True)` returns int32), ids and
+factors of any strides.  An id below 0 marks an empty slot, as `DCI.query` leaves them; an id beyond the
+table or the vocabulary is never accessed and gives NaN.  Work goes to torch's current stream, without a
+wait; gradients are taken through torch.autograd, once, and backward: a tangent of forward mode is
+refused.  Wrong types raise TypeError, wrong shapes and values ValueError.  The reference, a search engine
+alone, has no counterpart.
 """
 from . import _dci_cuda as _ext   # built by `python -m dciknn_cuda_amd.build`; no fallback
 

@@ -781,3 +781,27 @@ def test_distillation_into_what_requires_a_gradient(gpu):
     assert torch.allclose(by_weight, z.t() @ want, atol=1e-5)
     with torch.no_grad():
         assert torch.equal(gpu.distill_step(leaf, ids, teacher, out=leaf)[1], want)
+
+
+@pytest.mark.parametrize("shape", [(3, 5, 700), (2, 40, 9001)])
+def test_next_tokens_of_a_batch(gpu, shape):
+    """Logits without their last position are at two distances; all of them with ids of -1 there are the same."""
+    b, t, v = shape
+    z = torch.randn(shape, device="cuda")
+    tokens, g = torch.randint(0, v, (b, t), device="cuda"), torch.randn(b, t - 1, device="cuda")
+    ids, teacher = torch.randint(0, v, (b, t, 4), device="cuda"), torch.randn(b, t, 4, device="cuda")
+    for call in (lambda: gpu.token_logprobs(z[:, :-1], tokens[:, 1:]), lambda: gpu.distill_loss(z[:, :-1], ids[:, :-1], teacher[:, :-1]),
+                 lambda: gpu.distill_step(z[:, :-1], ids[:, :-1], teacher[:, :-1])):
+        with pytest.raises(ValueError, match="ids of -1"):
+            call()
+    targets = torch.cat([tokens[:, 1:], torch.full_like(tokens[:, :1], -1)], 1)
+    ids[:, -1] = -1
+    whole, cut = z.clone().requires_grad_(), z[:, :-1].contiguous().requires_grad_()
+    for a, c in ((gpu.token_logprobs(whole, targets)[0], gpu.token_logprobs(cut, tokens[:, 1:])[0]),
+                 (gpu.distill_loss(whole, ids, teacher), gpu.distill_loss(cut, ids[:, :-1], teacher[:, :-1]))):
+        assert (a[:, -1] == 0).all()
+        near_abs(a[:, :-1], f64(c), SUM)
+        by_whole, = torch.autograd.grad(a[:, :-1], whole, g)
+        by_cut, = torch.autograd.grad(c, cut, g)
+        assert (by_whole[:, -1] == 0).all()
+        near(by_whole[:, :-1], f64(by_cut), np.abs(f64(by_cut)) + np.abs(f64(g))[:, :, None] * 1e-3, "f32", 2 * SUM)
