@@ -805,3 +805,93 @@ def test_next_tokens_of_a_batch(gpu, shape):
         by_cut, = torch.autograd.grad(c, cut, g)
         assert (by_whole[:, -1] == 0).all()
         near(by_whole[:, :-1], f64(by_cut), np.abs(f64(by_cut)) + np.abs(f64(g))[:, :, None] * 1e-3, "f32", 2 * SUM)
+
+
+# ---- many tokens: pieces of rows, joined, added to what is there ---------------------------
+def _many(gpu, ids, d, v, dtype, scale=0.5):
+    """The gradient of more tokens than one launch takes, written and added to a float32 and to an own-type gradient."""
+    ids = on_gpu(ids, torch.int64)
+    assert ids.numel() > 4096
+    grad = torch.randn(ids.numel(), d, device="cuda").to(TYPES[dtype])
+    valid = (ids >= 0) & (ids < v)
+    want = torch.zeros(v, d, dtype=torch.float64, device="cuda").index_add_(0, ids[valid], grad[valid].double() * scale)
+    size = torch.zeros(v, d, dtype=torch.float64, device="cuda").index_add_(0, ids[valid], grad[valid].double().abs() * scale)
+    count = torch.bincount(ids[valid], minlength=v).double()[:, None]
+    got = gpu.embed_grad(grad, ids, v, scale)
+    # an addition for each token, the factor, the sum with what is there: 2^-24 each; and one rounding to the type
+    far = (got.double() - want).abs() - HALF_UNIT[dtype] * want.abs() * 1.01 - LEAST[dtype] - (count + 2) * 2.0 ** -24 * size
+    assert (far <= 0).all()
+    assert torch.equal(got, gpu.embed_grad(grad, ids.int(), v, scale))
+    none = count[:, 0] == 0
+    assert not got[none].any()
+    for kind in {dtype, "f32"}:
+        base = torch.randn(v, d, device="cuda").to(TYPES[kind])
+        into = gpu.embed_grad(grad, ids, v, scale, out=base.clone())
+        sum_ = want + base.double()
+        far = (into.double() - sum_).abs() - HALF_UNIT[kind] * sum_.abs() * 1.01 - LEAST[kind] - (count + 3) * 2.0 ** -24 * (size + base.double().abs())
+        assert (far <= 0).all() and torch.equal(into[none], base[none])
+    return got
+
+
+# Pieces have 8 tokens (below 2^21 elements in all) or 16; rows of more than 16 pieces are joined by groups.
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d", [20, 100, 513])
+@pytest.mark.parametrize("counts", [[7, 8, 9, 15, 16, 17], [1, 31, 32, 33, 2, 127, 128, 129], [128, 1, 255, 256, 257, 136, 137], [2000, 1, 4096, 3]])
+def test_lookup_gradient_by_pieces(gpu, dtype, d, counts):
+    r = gen(d + sum(counts))
+    rows = np.repeat(np.arange(len(counts)), counts)
+    ids = np.concatenate([rows, r.integers(len(counts), 4000, max(4100, 5000 - len(rows)))])      # others, a few tokens each
+    n = len(ids)
+    assert (n * 20 < 1 << 21) and (n * 513 >= 1 << 21)
+    _many(gpu, ids, d, 4003, dtype)                        # the counted rows' tokens next to one another, from the first on
+    _many(gpu, r.permutation(ids), d, 4003, dtype)
+    _many(gpu, 4002 - ids, d, 4003, dtype)                 # the last rows of the table
+
+
+def test_lookup_gradient_of_a_million_tokens(gpu):
+    """More chunks of tokens than a wavefront looks at at a time, by few rows and by many."""
+    r = gen(17)
+    n = 1_100_001
+    for v, d, dtype in ((300, 3, "f32"), (70_000, 4, "bf16"), (2_200_000, 2, "f16")):
+        ids = np.where(np.arange(n) % 11 == 3, v // 3, r.integers(-1, v + 1, n))
+        _many(gpu, ids, d, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,v,d", [(1, 1, 1), (33, 5, 100), (700, 2500, 1025), (4096, 300, 40)])
+def test_lookup_gradient_of_few_tokens_added_to_its_own_type(gpu, dtype, n, v, d):
+    r = gen(n + v)
+    ids = r.integers(-1, v + 1, n)
+    grad = on_gpu(r.normal(size=(n, d)), TYPES[dtype])
+    want, size, count = O.embed_grad(f64(grad), ids, v, 0.5)
+    base = torch.randn(v, d, device="cuda").to(TYPES[dtype])
+    into = gpu.embed_grad(grad, on_gpu(ids, torch.int64), v, 0.5, out=base.clone())
+    near(into, want + f64(base), size + np.abs(f64(base)), dtype, (count[:, None] + 3) * 2.0 ** -24)
+    assert torch.equal(into[on_gpu(count == 0, torch.bool)], base[on_gpu(count == 0, torch.bool)])
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(9000, 700, 96, "bf16"), (5000, 90_000, 12, "f32")])
+def test_graph_of_the_gradient_of_many_tokens(gpu, n, v, d, dtype):
+    """Recorded and replayed: the launches that group, clear, sum and join, on other tokens each time."""
+    grad, ids = torch.randn(n, d, device="cuda").to(TYPES[dtype]), torch.randint(0, v, (n,), device="cuda")
+    total = torch.zeros(v, d, device="cuda")
+
+    def work():
+        return gpu.embed_grad(grad, ids, v, 0.5), gpu.embed_grad(grad, ids, v, 2.0, out=total)
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for i in range(4):
+        ids.copy_(torch.randint(-1, v, (n,), device="cuda") if i % 2 else torch.randint(0, 20, (n,), device="cuda"))
+        grad.copy_(torch.randn(n, d, device="cuda"))
+        total.copy_(torch.randn(v, d, device="cuda"))
+        before = total.clone()
+        want = [x.clone() for x in work()]
+        total.copy_(before)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
