@@ -295,7 +295,7 @@ __device__ inline void put_zeros(const EmbedArgs& a, int64_t row, int c) {
 // its part of the order starts.  Eight wavefronts read the bucket's tokens, in runs of the chunks, once to count them
 // by rows (up to kBins at a time) and once to put them into their places.  Eight more meanwhile write the rows
 // without tokens, whose bytes hide the waits of the first, unless there is nothing to be written or chunk_kernel has
-// done it.  Bound by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 100
+// done it.  Bound by its own instructions in the bucket of the commonest row: 31 us for 65536 tokens of text with 142
 // MB of zeros, 101 where 65536 of 131072 tokens have one row; or by the waits of its steps, where buckets are many:
 // without zeros four workgroups are on a compute unit at once (100000 tokens added to 1M x 128 f32: 52 us in all, 63
 // with one at a time).
@@ -400,7 +400,7 @@ __global__ __launch_bounds__((kZeros ? 2 : 1) * kGroupThreads, kZeros ? 4 : 8) v
 // Rows of up to w.piece tokens are one piece and final; the first piece of a longer one goes to
 // place 2 w + 1 of `part`, a later one to 2 w (a window w has at most one of each).  Windows, not rows, are
 // what a group takes: a tenth of a text's tokens are one row's.  Bound by memory: 65536 tokens by 50001 x 2048
-// bf16 70 us (268 MB read, 105 MB written: 5.3 TB/s).
+// bf16 70 us (268 MB read, 82 MB written: 5.0 TB/s).
 template <class T, class O, bool kByWaves>
 __global__ __launch_bounds__(kThreads) void sum_kernel(EmbedArgs a, Work w, int lanes, int slices, int64_t first) {
     using P = Piece<T>;

@@ -689,8 +689,12 @@ int stats_by(LogitArgs a, hipStream_t s) {
 }
 
 // With alternatives one wavefront takes a row where there are rows enough to fill the device, or rows too short for more:
-// each wavefront of a row has best pieces of its own to find (8192 x 32000 bf16 with 5 of them 94 us, 115 by four
-// wavefronts a row; 1024 x 1000 7.1 and 8.8; but 1024 x 50000 43 and 32).  Without, four take 81 us and one 85.
+// each wavefront of a row has best pieces of its own to find.  One and four, us, with 5 alternatives in bf16:
+//   rows of   1024         2048          3000          4096          8192
+//     9000    13.7  12.9   16.6  18.9    19.8  25.1    23.0  31.4    38.1  56.1
+//    50001    42.7  33.2   54.0  52.1    66.7  72.8    82.0  91.3     151   173
+//   131072    88.6  61.5    108   101     140   147     180   193     344   372
+// (f32: 40.2 and 26.7 for 1024 x 32000, 83.8 and 86.8 for 4096; 1024 x 1000 7.1 and 8.8.)  Without, four take 81 us and one 85.
 template <class T, int kMode>
 int stats_of(const LogitArgs& a, hipStream_t s) {
     if constexpr (kMode == kLogprobsTop) {
@@ -713,7 +717,9 @@ constexpr int kMostPieces = 16 * 1024;       // of a row in registers
 // The fewest threads that hold a row in 16 pieces each and a slot each: several rows are on a compute unit then,
 // and one's sums run while others' bytes travel.  (1024 threads for all: 16384 x 2000 bf16 379 us instead of 33, 8192 x 16000
 // 251 instead of 120, 4096 x 50000 233 instead of 187.)  Fewer pieces where they do: what a thread does not need it reads
-// again (16 for all: 73, 169 and 236 us).
+// again, which costs most where rows start off a boundary.  16 pieces for all instead of these, f16: 4 pieces 8192 x 1900 40 us
+// instead of 20, 8 pieces 8192 x 9000 143 instead of 85, 10 pieces 1001 x 81001 119 instead of 87, 13 pieces 1001 x 53001 65
+// instead of 56 and x 100003 125 instead of 109.
 template <class T>
 int distill_rows_of(const LogitArgs& a, hipStream_t s) {
     const int pieces = a.vocab / Piece<T>::kLen;
@@ -784,8 +790,9 @@ int logit_stats(LogitArgs a, int dtype, bool distill, hipStream_t s) {
 }
 
 // Rows that fit a workgroup's registers, by one workgroup each; where they are long, only if there are enough of
-// them to give a compute unit in three one: one of 131072 bf16 takes 19 us by one workgroup and 9.5 by three launches over
-// the device, 64 22 and 20, 128 23 and 28; one of 32000 takes 8.4 and 9.6.
+// them to give a compute unit in three one: one of 131072 bf16 takes 21 us by one workgroup and 13 by three launches over
+// the device, 64 22 and 20, 80 22.4 and 22.1, 96 23 and 24, 128 24 and 28; one of 32000 takes 8.6 and 9.6.  (Shorter ones part
+// earlier: of 60000 f32 1 takes 14 and 10, 32 15.2 and 14.9, 64 16 and 18; of 65536 bf16 1 takes 12.3 and 12.1, 64 14 and 17.)
 bool distill_by_rows(const LogitArgs& a, int dtype) {
     const int len = 16 / type_bytes(dtype), pieces = a.vocab / len;
     return pieces >= 1 && pieces <= kMostPieces && (pieces <= 4096 || a.n >= 96);

@@ -1,6 +1,5 @@
 // What the token operators share: element types, 16-byte pieces of rows that may start at any
-// element, ids of 4 or 8 bytes, the running
-// statistics of a softmax, and the launch interface.
+// element, ids of 4 or 8 bytes, the running statistics of a softmax, and the launch interface.
 #pragma once
 
 #include "common.h"
