@@ -388,7 +388,7 @@ int dcih_token_logprobs_grad(const void* d_logits, int dtype, int64_t num_rows, 
  * 1024), the teacher's logits of any of the types; a slot with an id below 0 or a logit of -inf is empty, an
  * id may stand in several slots.  With q = softmax(teacher / temperature) over a row's filled slots
  * and p = softmax(logits / temperature): d_losses[i] = sum_j q_j (log q_j - log p[id_j]); 0 without filled slots;
- * +inf where p is 0 at a filled slot; NaN for an id beyond the vocabulary.
+ * +inf where a filled slot names a token of logit -inf; NaN for an id beyond the vocabulary.
  * d_grad: NULL, or the gradient by the logits of sum_i d_weights[i] * d_losses[i] (d_weights NULL: ones),
  * in the logits' type and in their place or apart as above; rows with weight 0, without filled slots or of
  * nothing but -inf have gradient 0.  d_stats: NULL, or [num_rows][4] floats for dcih_distill_grad,
