@@ -87,6 +87,15 @@ SIGNATURES = {
     "dcih_distill_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int64, _c.c_void_p,
                                      _c.c_int, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float, _c.c_void_p,
                                      _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_scan_states": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int, _c.c_int]),
+    "dcih_scan_work": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_int64]),
+    "dcih_scan": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int64, _c.c_int64,
+                             _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int,
+                             _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_scan_grad": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int64, _c.c_int64,
+                                  _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int,
+                                  _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+                                  _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,864 @@
+// A gated linear recurrence over the tokens of sequences, each channel by itself, and its gradient:
+//
+//   a_t = 1 / (1 + e^-g_t),  h_t = a_t h_(t-1) + (1 - a_t) x_t        (gates)
+//   a_t = g_t,               h_t = a_t h_(t-1) + x_t                  (decays)
+//
+//   l_t = dh_t + a_(t+1) l_(t+1)        the gradient that reaches h_t
+//   gates:  dx_t = (1 - a_t) l_t,  dg_t = a_t (1 - a_t) l_t (h_(t-1) - x_t)
+//   decays: dx_t = l_t,            dg_t = l_t h_(t-1);        both: by the first state a_1 l_1
+//
+// Both directions are compositions of maps s -> A s + B, which are associative: a tile of kTile tokens by kLanes pieces
+// of 16 bytes is one workgroup's, in registers; each group of lanes composes its few tokens, the groups are joined in
+// shared memory, and a tile's map is joined to that of the tiles before it while these still run (see carry_of).  So every
+// element is read and written once.  The gradient forms h_(t-1) again, from x, g and the state before each tile, which
+// the forward call keeps in 32 bits: less to read than h itself, and not rounded.
+#include "../../include/dci_hip.h"
+#include "scan.h"
+
+#include <algorithm>
+
+namespace dcih {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kLanes = 16;                         // pieces of 16 bytes that a tile is wide
+constexpr int kTile = 128;                         // tokens of a tile
+constexpr int kShort = 16;                         // tokens that one thread takes
+constexpr int64_t kMaxGrid = 1 << 23;
+constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
+constexpr uint32_t kMapSet = 1, kStateSet = 2;
+
+typedef uint32_t u32x4_float __attribute__((ext_vector_type(4), aligned(4)));
+
+// L elements of a row: a 16-byte piece, or (L = 1, rows shorter than that) one.
+template <class T, int L> struct Span {
+    using raw_t = typename T::raw;
+    using P = Piece<T>;
+    u32x4 bits;
+    __device__ void load(const raw_t* p) {
+        static_assert(L == P::kLen, "a piece");
+        bits = P::load_once(p);
+    }
+    __device__ void get(float (&z)[L]) const { P::unpack(bits, z); }
+    __device__ static void store(raw_t* p, const float (&z)[L]) { P::store_once(p, P::pack(z)); }
+};
+template <class T> struct Span<T, 1> {
+    using raw_t = typename T::raw;
+    raw_t bits;
+    __device__ void load(const raw_t* p) { bits = *p; }
+    __device__ void get(float (&z)[1]) const { z[0] = (float)bits; }
+    __device__ static void store(raw_t* p, const float (&z)[1]) { *p = (raw_t)z[0]; }
+};
+
+template <int L> __device__ inline void load_floats(const float* p, float (&z)[L]) {
+    if constexpr (L % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < L; k += 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4_float*>(p + k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[k + i] = __builtin_bit_cast(float, (uint32_t)v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < L; k++) z[k] = p[k];
+    }
+}
+template <int L> __device__ inline void store_floats(float* p, const float (&z)[L]) {
+    if constexpr (L % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < L; k += 4) {
+            u32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = __builtin_bit_cast(uint32_t, z[k + i]);
+            *reinterpret_cast<u32x4_float*>(p + k) = v;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < L; k++) p[k] = z[k];
+    }
+}
+
+// What a gate is kept as: 1 - a where a is 1/2 or more, else -a (told apart by the sign, of zeros too).  The smaller of the
+// two is the one to round: with a alone, a channel that forgets over 1000 tokens would be off by 6e-5.  Exponent with
+// its product's rounding made good.
+__device__ inline float gate_of(float g) {
+    float y = -__builtin_fabsf(g);
+    y = y < -150.f ? -150.f : y;                      // (nothing is left there; NaN stays)
+    const float t = y * kLog2e;
+    const float rest = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, kLog2e, -t));
+    float e = exp2_fast(t);
+    e = __builtin_fmaf(e * kLn2, rest, e);
+    return __builtin_copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
+}
+__device__ inline bool holds(float c) { return __builtin_bit_cast(int, c) >= 0; }
+
+template <bool kDecay> __device__ inline float factor(float c) {          // a
+    if (kDecay) return c;
+    return holds(c) ? 1.f - c : -c;
+}
+template <bool kDecay> __device__ inline float step(float h, float x, float c) {
+    if (kDecay) return __builtin_fmaf(c, h, x);
+    return __builtin_fmaf(c, x - h, holds(c) ? h : x);       // h + (1 - a) (x - h), or x + a (h - x)
+}
+template <class T, int L, bool kDecay> __device__ inline void coefs_of(const Span<T, L>& s, float (&c)[L]) {
+    s.get(c);
+    if (!kDecay) {
+#pragma unroll
+        for (int k = 0; k < L; k++) c[k] = gate_of(c[k]);
+    }
+}
+
+// ---- one thread a channel ----------------------------------------------------------------
+// A server's step, or its drafts: few tokens of many sequences.  The state may be written where it is read.
+template <class T, int L, bool kDecay>
+__global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces, int64_t first) {
+    constexpr int U = 4;
+    using raw_t = typename T::raw;
+    const int64_t i = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t b = i / pieces;
+    if (b >= a.rows) return;
+    const int piece = (int)(i - b * pieces), own = piece * L, c0 = min(own, a.dim - L), length = (int)a.length;
+    int64_t len = length;
+    if (a.bounds) len = min(max(id_at(a.bounds, a.wide_bounds, b), (int64_t)0), len);
+    const raw_t *x = (const raw_t*)a.x + b * a.x_row + c0, *g = (const raw_t*)a.gates + (a.shared ? 0 : b * a.g_row) + c0;
+    raw_t* out = (raw_t*)a.h + b * length * a.dim + c0;
+    float h[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) h[k] = 0.f;
+    if (a.state) load_floats<L>(a.state + b * a.dim + c0, h);
+    for (int t0 = 0; t0 < length; t0 += U) {
+        Span<T, L> xs[U], gs[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t t = min(t0 + u, length - 1);
+            xs[u].load(x + t * a.x_step);
+            gs[u].load(g + t * a.g_step);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (t0 + u >= length) break;
+            const bool in = t0 + u < len;
+            float xv[L], c[L], y[L];
+            xs[u].get(xv);
+            coefs_of<T, L, kDecay>(gs[u], c);
+#pragma unroll
+            for (int k = 0; k < L; k++) {
+                const float next = step<kDecay>(h[k], xv[k], c[k]);
+                h[k] = in ? next : h[k];
+                y[k] = in ? next : 0.f;
+            }
+            raw_t* to = out + (int64_t)(t0 + u) * a.dim;
+            if (c0 == own) {
+                Span<T, L>::store(to, y);
+            } else {           // the row's last piece: what it shares with the one before is that one's, whose state may be written already
+#pragma unroll
+                for (int k = 0; k < L; k++)
+                    if (c0 + k >= own) to[k] = (raw_t)y[k];
+            }
+        }
+    }
+    if (!a.last) return;
+    float* last = a.last + b * a.dim + c0;
+    if (c0 == own) {
+        store_floats<L>(last, h);
+    } else {
+#pragma unroll
+        for (int k = 0; k < L; k++)
+            if (c0 + k >= own) last[k] = h[k];
+    }
+}
+
+// ---- tiles -------------------------------------------------------------------------------
+// A chain is a strip of kLanes pieces of one row of tokens; its tiles follow one another.  Blocks take the tiles of a chain by its
+// counter, so that a tile waits for none that is not running.
+struct Chains {
+    int pieces, strips, slots;         // pieces of a row; strips of them; channels of a strip, those beyond the row included
+    int64_t tiles, count;              // tiles of a chain, chains
+    uint32_t *tickets, *flags;         // [count]; [count][tiles] what is set: a hint of what to wait for
+    uint64_t* maps;                    // [count][tiles][slots] (A, B)
+    uint32_t* states;                  // [count][tiles][slots] the state behind a tile
+    float* sums;                       // [count][tiles][slots] (gradient of shared gates)
+};
+
+int span_len(int dim, int dtype) {
+    const int len = dtype == DCIH_F32 ? 4 : 8;
+    return dim >= len ? len : 1;
+}
+
+__host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t length, int dim, int dtype, bool shared) {
+    const int len = span_len(dim, dtype);
+    c.pieces = (dim + len - 1) / len;
+    c.strips = (c.pieces + kLanes - 1) / kLanes;
+    c.slots = kLanes * len;
+    c.tiles = (length + kTile - 1) / kTile;
+    c.count = rows * c.strips;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        char* p = (char*)mem + at;
+        at += (bytes + 255) / 256 * 256;
+        return p;
+    };
+    const int64_t cells = c.count * c.tiles * c.slots, chained = c.tiles > 1 ? 1 : 0;
+    c.tickets = (uint32_t*)take(chained * c.count * 4);
+    c.flags = (uint32_t*)take(chained * c.count * c.tiles * 4);
+    c.maps = (uint64_t*)take(chained * cells * 8);
+    c.states = (uint32_t*)take(chained * cells * 4);
+    c.sums = (float*)take(shared ? cells * 4 : 0);
+    return at;
+}
+
+__global__ __launch_bounds__(kThreads) void fill_kernel(u32x4* p, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i < n) p[i] = u32x4{kUnset, kUnset, kUnset, kUnset};
+}
+__global__ __launch_bounds__(kThreads) void copy_kernel(const float* from, float* to, int64_t n) {
+    const int64_t step = (int64_t)gridDim.x * kThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) to[i] = from ? from[i] : 0.f;
+}
+
+// Sequences without tokens: what reaches their end is what they began with.
+__global__ __launch_bounds__(kThreads) void empty_kernel(ScanArgs a, const float* from, float* to, int64_t first) {
+    const int64_t s = first + blockIdx.x;
+    bool empty;
+    if (a.form == kPacked) {
+        const int64_t lo = min(max(id_of_all(a.bounds, a.wide_bounds, s), (int64_t)0), a.length);
+        const int64_t hi = min(max(id_of_all(a.bounds, a.wide_bounds, s + 1), (int64_t)0), a.length);
+        empty = hi <= lo;
+    } else {
+        empty = id_of_all(a.bounds, a.wide_bounds, s) <= 0;
+    }
+    if (!empty) return;
+    for (int c = threadIdx.x; c < a.dim; c += kThreads) to[s * a.dim + c] = from ? from[s * a.dim + c] : 0.f;
+}
+
+__device__ inline uint32_t peek(const uint32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline uint64_t peek(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class V> __device__ inline void post(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline uint32_t word_of(float v) {
+    const uint32_t w = __builtin_bit_cast(uint32_t, v);
+    return w == kUnset ? 0x7fc00000u : w;
+}
+
+// Which tile of its chain a workgroup takes, counted in the direction of the scan.
+__device__ inline int64_t take_tile(const Chains& c, int64_t chain, uint32_t& s_ticket) {
+    if (c.tiles == 1) return 0;
+    if (threadIdx.x == 0) s_ticket = atomicAdd(&c.tickets[chain], 1u) - kUnset;       // the counter begins at kUnset
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(s_ticket);
+}
+
+// The state that enters tile `at` of a chain in channel `slot`.  A tile posts its map as soon as it has it, and the state
+// behind it when it knows the one before; a wavefront looks for the nearest tile before its own whose state is there and goes on from it by the
+// maps in between, in their order: that is what those tiles do themselves, so the bits do not depend on who was how far.
+// Words are waited for themselves; the flags only say which are worth a look.
+__device__ float carry_of(const Chains& c, int64_t chain, int64_t at, int slot) {
+    const uint32_t* flags = c.flags + chain * c.tiles;
+    const int lane = lane_id();
+    int behind;                                     // tiles between the one whose state is there and this one
+    for (;;) {
+        const int64_t tile = at - 1 - lane;
+        const uint32_t f = tile >= 0 ? peek(flags + tile) : kUnset;
+        const unsigned long long full = __ballot(f == kStateSet), some = __ballot(f != kUnset);
+        behind = full ? __builtin_ctzll(full) : -1;
+        if (full && (~some & ((1ull << behind) - 1)) == 0) break;
+        __builtin_amdgcn_s_sleep(2);
+    }
+    const int64_t base = (chain * c.tiles + at - 1 - behind) * c.slots + slot;
+    uint32_t w;
+    while ((w = peek(c.states + base)) == kUnset) {}
+    float h = __builtin_bit_cast(float, w);
+    const uint64_t* maps = c.maps + base + c.slots;
+    constexpr int U = 8;
+    for (int i = 0; i < behind; i += U) {
+        uint64_t m[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) m[u] = peek(maps + (int64_t)min(i + u, behind - 1) * c.slots);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (i + u >= behind) break;
+            while ((uint32_t)m[u] == kUnset || (uint32_t)(m[u] >> 32) == kUnset) m[u] = peek(maps + (int64_t)(i + u) * c.slots);
+            h = __builtin_fmaf(__builtin_bit_cast(float, (uint32_t)m[u]), h, __builtin_bit_cast(float, (uint32_t)(m[u] >> 32)));
+        }
+    }
+    return h;
+}
+
+// A channel's groups joined, by one thread: map (A, B) of each in the direction of the scan, `resets` those whose result does not
+// depend on what enters.  Leaves in B what enters each group; returns what enters the tile.
+template <int kGroups, bool kBack>
+__device__ float join_groups(const Chains& c, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
+    auto place = [&](int g) { return (kBack ? kGroups - 1 - g : g) * c.slots + slot; };
+    float in = 0.f;
+    if (c.tiles > 1) {
+        float A = 1.f, B = 0.f;
+#pragma unroll 8
+        for (int g = 0; g < kGroups; g++) {
+            const float ga = s_a[place(g)], gb = s_b[place(g)];
+            const bool reset = resets >> (kBack ? kGroups - 1 - g : g) & 1;
+            B = reset ? gb : __builtin_fmaf(ga, B, gb);
+            A *= ga;
+        }
+        const int64_t cell = chain * c.tiles + at, word = cell * c.slots + slot;
+        const bool follows = at + 1 < c.tiles;
+        if (resets) {
+            if (follows) post(c.states + word, word_of(B));
+            if (follows && slot == 0) post(c.flags + cell, kStateSet);
+        } else if (follows) {
+            post(c.maps + word, (uint64_t)word_of(B) << 32 | word_of(A));
+            if (slot == 0) post(c.flags + cell, kMapSet);
+        }
+        if (at) in = carry_of(c, chain, at, slot);
+        if (!resets && follows) {
+            post(c.states + word, word_of(__builtin_fmaf(A, in, B)));
+            if (slot == 0) post(c.flags + cell, kStateSet);
+        }
+    }
+    float h = in;
+#pragma unroll 8
+    for (int g = 0; g < kGroups; g++) {
+        const float ga = s_a[place(g)], gb = s_b[place(g)];
+        const bool reset = resets >> (kBack ? kGroups - 1 - g : g) & 1;
+        s_b[place(g)] = h;
+        h = reset ? gb : __builtin_fmaf(ga, h, gb);
+    }
+    return in;
+}
+
+// Where sequences begin and end among the tokens of a tile.  In groups of tokens without either, and with all of them
+// in one sequence, nobody asks.
+struct Marks {
+    int64_t row, length;              // a row of tokens, and how many it has
+    int64_t t0;                       // the tile's first token
+    int64_t lo, hi;                   // tokens [lo, hi) of the row are of sequences
+    const int *first, *end;           // (kPacked) [kTile] the sequence that begins or ends there, -1: none
+
+    __device__ Marks(const ScanArgs& a, int64_t row_, int64_t t0_) : row(row_), length(a.length), t0(t0_) {
+        if (a.form == kFlat) length = min(length, a.total - row * a.length);
+    }
+    __device__ static int64_t length_of(const ScanArgs& a, int64_t s, int64_t most) {
+        return a.bounds ? min(max(id_at(a.bounds, a.wide_bounds, s), (int64_t)0), most) : most;
+    }
+    // (kFlat) the sequence of a token, and its place there
+    __device__ int64_t of(const ScanArgs& a, int64_t t, int& place) const {
+        const uint32_t each = (uint32_t)a.each, s = (uint32_t)t / each;
+        place = (int)((uint32_t)t - s * each);
+        return row * ((uint32_t)a.length / each) + s;
+    }
+    __device__ bool in(const ScanArgs& a, int64_t t) const {
+        if (t < lo || t >= hi) return false;
+        if (a.form != kFlat || !a.bounds) return true;
+        int place;
+        const int64_t s = of(a, t, place);
+        return place < length_of(a, s, a.each);
+    }
+    __device__ int64_t begins(const ScanArgs& a, int64_t t) const {
+        if (a.form == kPacked) return first[t - t0];
+        if (a.form == kRows) return t ? -1 : row;
+        int place;
+        const int64_t s = of(a, t, place);
+        return place ? -1 : s;
+    }
+    __device__ int64_t ends(const ScanArgs& a, int64_t t) const {
+        if (a.form == kPacked) return end[t - t0];
+        if (a.form == kRows) return t == hi - 1 ? row : -1;
+        int place;
+        const int64_t s = of(a, t, place);
+        return place == length_of(a, s, a.each) - 1 ? s : -1;
+    }
+};
+
+// By all threads; `s_first`, `s_end` [kTile] and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
+__device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int* s_first, int* s_end, uint32_t& s_marked) {
+    if (a.form == kRows) {
+        m.lo = 0;
+        m.hi = Marks::length_of(a, m.row, a.length);
+    } else if (a.form == kFlat) {
+        m.lo = 0;
+        m.hi = m.length;
+    } else {
+        auto bound = [&](int64_t i) { return min(max(id_at(a.bounds, a.wide_bounds, i), (int64_t)0), a.length); };
+        m.lo = bound(0);
+        m.hi = bound(a.sequences);
+        m.first = s_first;
+        m.end = s_end;
+        for (int i = threadIdx.x; i < kTile; i += blockDim.x) s_first[i] = s_end[i] = -1;
+        if (threadIdx.x == 0) s_marked = 0;
+        // the last sequence that begins before the tile, by 64 places of a shrinking range at a time
+        int64_t from = 0, to = a.sequences;
+        while (to - from > 1) {
+            const int64_t wide = (to - from + kWave - 1) / kWave, at = from + (lane_id() + 1) * wide;
+            const int n = __popcll(__ballot(at < to && bound(at) < m.t0));
+            from += n * wide;
+            to = min(to, from + wide);
+        }
+        __syncthreads();
+        for (int64_t s = from;; s += blockDim.x) {
+            const int64_t mine = s + threadIdx.x;
+            if (mine < a.sequences) {
+                const int64_t lo = bound(mine), hi = bound(mine + 1);
+                if (hi > lo) {
+                    if (lo >= m.t0 && lo < m.t0 + kTile) {
+                        s_first[lo - m.t0] = (int)mine;
+                        atomicOr(&s_marked, 1u << ((int)(lo - m.t0) / per));
+                    }
+                    if (hi - 1 >= m.t0 && hi - 1 < m.t0 + kTile) {
+                        s_end[hi - 1 - m.t0] = (int)mine;
+                        atomicOr(&s_marked, 1u << ((int)(hi - 1 - m.t0) / per));
+                    }
+                }
+            }
+            if (s + blockDim.x >= a.sequences || bound(s + blockDim.x) >= m.t0 + kTile) break;
+        }
+    }
+}
+__device__ inline bool is_marked(const ScanArgs& a, const Marks& m, int64_t t, int per, int group, uint32_t s_marked) {
+    if (a.form == kFlat || t < m.lo || t + per > m.hi) return true;
+    if (a.form == kRows) return t == 0 || t + per == m.hi;
+    return s_marked >> group & 1;
+}
+
+template <class T, int L, bool kDecay, bool kShared>
+__global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, int64_t first) {
+    constexpr int kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    using raw_t = typename T::raw;
+    __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
+    __shared__ int s_first[kTile], s_end[kTile];
+    __shared__ uint32_t s_ticket, s_marked, s_resets;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const int64_t chain = (first + blockIdx.x) % c.count, row = chain / c.strips;
+    const int strip = (int)(chain - row * c.strips);
+    if (threadIdx.x == 0) s_resets = 0;
+    const int64_t at = take_tile(c, chain, s_ticket), t0 = at * kTile, t = t0 + group * U;
+    Marks m(a, row, t0);
+    const int piece = strip * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
+    const bool live = piece < c.pieces;
+    const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
+    const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
+    Span<T, L> xs[U], gs[kShared ? 1 : U];
+    if (kShared) gs[0].load(g);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t from = min(t + u, m.length - 1);
+        xs[u].load(x + from * a.x_step);
+        if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
+    }
+    find_marks(a, m, U, s_first, s_end, s_marked);
+    __syncthreads();
+    const bool marked = is_marked(a, m, t, U, group, s_marked);
+    auto first_state = [&](int64_t s, float (&h)[L]) {
+#pragma unroll
+        for (int k = 0; k < L; k++) h[k] = 0.f;
+        if (a.state) load_floats<L>(a.state + s * a.dim + c0, h);
+    };
+    // the group's map
+    float cs[kShared ? 1 : U][L], A[L], B[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; }
+#pragma unroll
+    for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
+    bool reset = false;
+    if (!marked) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float xv[L];
+            xs[u].get(xv);
+#pragma unroll
+            for (int k = 0; k < L; k++) {
+                const float co = cs[kShared ? 0 : u][k];
+                A[k] *= factor<kDecay>(co);
+                B[k] = step<kDecay>(B[k], xv[k], co);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (!m.in(a, t + u)) {
+                reset = true;
+#pragma unroll
+                for (int k = 0; k < L; k++) B[k] = 0.f;
+                continue;
+            }
+            const int64_t s = m.begins(a, t + u);
+            if (s >= 0) {
+                reset = true;
+                first_state(s, B);
+            }
+            float xv[L];
+            xs[u].get(xv);
+#pragma unroll
+            for (int k = 0; k < L; k++) {
+                const float co = cs[kShared ? 0 : u][k];
+                A[k] *= factor<kDecay>(co);
+                B[k] = step<kDecay>(B[k], xv[k], co);
+            }
+        }
+        if (reset && lane == 0) atomicOr(&s_resets, 1u << group);
+    }
+    const int slot = lane * L, mine = group * kSlots + slot;
+#pragma unroll
+    for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; }
+    __syncthreads();
+    if (threadIdx.x < kSlots) {
+        const float in = join_groups<kGroups, false>(c, chain, at, threadIdx.x, s_resets, s_a, s_b);
+        if (a.states) a.states[(chain * c.tiles + at) * kSlots + threadIdx.x] = in;
+    }
+    __syncthreads();
+    if (!live) return;
+    float h[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) h[k] = s_b[mine + k];
+    raw_t* out = (raw_t*)a.h + (row * a.length + t) * a.dim + c0;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float xv[L];
+        xs[u].get(xv);
+        if (marked) {
+            if (t + u >= m.length) break;
+            if (!m.in(a, t + u)) {
+#pragma unroll
+                for (int k = 0; k < L; k++) h[k] = 0.f;
+                Span<T, L>::store(out + (int64_t)u * a.dim, h);
+                continue;
+            }
+            const int64_t s = m.begins(a, t + u);
+            if (s >= 0) first_state(s, h);
+        }
+#pragma unroll
+        for (int k = 0; k < L; k++) h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
+        Span<T, L>::store(out + (int64_t)u * a.dim, h);
+        if (marked && a.last) {
+            const int64_t s = m.ends(a, t + u);
+            if (s >= 0) store_floats<L>(a.last + s * a.dim + c0, h);
+        }
+    }
+}
+
+// The gradient of a tile.  The states go forward from the one kept, the gradient that reaches them goes back from the tile
+// behind: its maps are s -> A s + Q of the same A.
+constexpr int kBackThreads = 512;
+
+template <class T, int L, bool kDecay, bool kShared>
+__global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first) {
+    constexpr int kGroups = kBackThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    static_assert(kGroups <= 32, "a bit for each group");
+    using raw_t = typename T::raw;
+    __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
+    __shared__ int s_first[kTile], s_end[kTile];
+    __shared__ uint32_t s_ticket, s_marked, s_resets, s_back_resets;
+    const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    const int64_t chain = (first + blockIdx.x) % c.count, row = chain / c.strips;
+    const int strip = (int)(chain - row * c.strips);
+    if (threadIdx.x == 0) s_resets = s_back_resets = 0;
+    const int64_t at = take_tile(c, chain, s_ticket), tile = c.tiles - 1 - at, t0 = tile * kTile, t = t0 + group * U;
+    Marks m(a, row, t0);
+    const int piece = strip * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
+    const bool live = piece < c.pieces;
+    const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
+    const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
+    const raw_t* dh = a.dh ? (const raw_t*)a.dh + row * a.length * a.dim + c0 : x;
+    const int64_t dh_step = a.dh ? a.dim : a.x_step;
+    Span<T, L> xs[U], gs[kShared ? 1 : U], ds[U];
+    if (kShared) gs[0].load(g);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t from = min(t + u, m.length - 1);
+        xs[u].load(x + from * a.x_step);
+        if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
+        ds[u].load(dh + from * dh_step);
+    }
+    find_marks(a, m, U, s_first, s_end, s_marked);
+    __syncthreads();
+    const bool marked = is_marked(a, m, t, U, group, s_marked), some = a.dh != nullptr;
+    auto first_state = [&](const float* from, int64_t s, float (&h)[L]) {
+#pragma unroll
+        for (int k = 0; k < L; k++) h[k] = 0.f;
+        if (from) load_floats<L>(from + s * a.dim + c0, h);
+    };
+    auto incoming = [&](int u, float (&d)[L]) {
+        ds[u].get(d);
+#pragma unroll
+        for (int k = 0; k < L; k++) d[k] = some ? d[k] : 0.f;
+    };
+    float cs[kShared ? 1 : U][L], A[L], B[L], Q[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; Q[k] = 0.f; }
+#pragma unroll
+    for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
+    bool reset = false, back_reset = false;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (marked) {
+            if (!m.in(a, t + u)) {
+                reset = true;
+#pragma unroll
+                for (int k = 0; k < L; k++) B[k] = 0.f;
+                continue;
+            }
+            const int64_t s = m.begins(a, t + u);
+            if (s >= 0) {
+                reset = true;
+                first_state(a.state, s, B);
+            }
+        }
+        float xv[L];
+        xs[u].get(xv);
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            const float co = cs[kShared ? 0 : u][k];
+            A[k] *= factor<kDecay>(co);
+            B[k] = step<kDecay>(B[k], xv[k], co);
+        }
+    }
+#pragma unroll
+    for (int u = U - 1; u >= 0; u--) {
+        bool begins = false;
+        if (marked) {
+            if (!m.in(a, t + u)) {
+                back_reset = true;
+#pragma unroll
+                for (int k = 0; k < L; k++) Q[k] = 0.f;
+                continue;
+            }
+            const int64_t s = m.ends(a, t + u);
+            if (s >= 0) {
+                back_reset = true;
+                first_state(a.dlast, s, Q);
+            }
+            begins = m.begins(a, t + u) >= 0;
+            back_reset |= begins;
+        }
+        float d[L];
+        incoming(u, d);
+#pragma unroll
+        for (int k = 0; k < L; k++) Q[k] = begins ? 0.f : factor<kDecay>(cs[kShared ? 0 : u][k]) * (d[k] + Q[k]);
+    }
+    if (lane == 0 && reset) atomicOr(&s_resets, 1u << group);
+    if (lane == 0 && back_reset) atomicOr(&s_back_resets, 1u << group);
+    const int slot = lane * L, mine = group * kSlots + slot;
+#pragma unroll
+    for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; s_q[mine + k] = Q[k]; }
+    __syncthreads();
+    // the states by some wavefronts, the gradients by others
+    if (threadIdx.x < kSlots) {
+        join_groups<kGroups, true>(c, chain, at, threadIdx.x, s_back_resets, s_a, s_q);
+    } else if (threadIdx.x < 2 * kSlots) {
+        const int own = threadIdx.x - kSlots;
+        float h = a.states[(chain * c.tiles + tile) * kSlots + own];
+#pragma unroll 8
+        for (int i = 0; i < kGroups; i++) {
+            const float ga = s_a[i * kSlots + own], gb = s_b[i * kSlots + own];
+            s_b[i * kSlots + own] = h;
+            h = s_resets >> i & 1 ? gb : __builtin_fmaf(ga, h, gb);
+        }
+    }
+    __syncthreads();
+    float h[L], l[L], before[U][L], sum[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        h[k] = s_b[mine + k];
+        l[k] = s_q[mine + k];
+        sum[k] = 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (marked) {
+            const int64_t s = m.in(a, t + u) ? m.begins(a, t + u) : -1;
+            if (s >= 0) first_state(a.state, s, h);
+        }
+        float xv[L];
+        xs[u].get(xv);
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            before[u][k] = h[k];
+            h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
+        }
+    }
+    const int64_t place = (row * a.length + t) * a.dim + c0;
+    raw_t *dx = a.dx ? (raw_t*)a.dx + place : nullptr, *dg = a.dgates && !kShared ? (raw_t*)a.dgates + place : nullptr;
+#pragma unroll
+    for (int u = U - 1; u >= 0; u--) {
+        float d[L], xv[L], by_x[L], by_g[L];
+        bool in = true;
+        if (marked) {
+            if (t + u >= m.length) continue;
+            in = m.in(a, t + u);
+            const int64_t s = in ? m.ends(a, t + u) : -1;
+            if (s >= 0) first_state(a.dlast, s, l);
+        }
+        incoming(u, d);
+        xs[u].get(xv);
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            const float co = cs[kShared ? 0 : u][k], f = factor<kDecay>(co);
+            const float reaches = d[k] + l[k];
+            if (kDecay) {
+                by_x[k] = reaches;
+                by_g[k] = reaches * before[u][k];
+            } else {
+                by_x[k] = reaches * (holds(co) ? co : 1.f + co);
+                by_g[k] = by_x[k] * f * (before[u][k] - xv[k]);
+            }
+            l[k] = f * reaches;
+            if (!in) by_x[k] = by_g[k] = l[k] = 0.f;
+            sum[k] += by_g[k];
+        }
+        if (live && dx) Span<T, L>::store(dx + (int64_t)u * a.dim, by_x);
+        if (live && dg) Span<T, L>::store(dg + (int64_t)u * a.dim, by_g);
+        if (marked && in) {
+            const int64_t s = m.begins(a, t + u);
+            if (s >= 0) {
+                if (live && a.dstate) store_floats<L>(a.dstate + s * a.dim + c0, l);
+#pragma unroll
+                for (int k = 0; k < L; k++) l[k] = 0.f;
+            }
+        }
+    }
+    if (!kShared || !a.dgates) return;
+    // (s_a is read by nobody any more)
+#pragma unroll
+    for (int k = 0; k < L; k++) s_a[mine + k] = sum[k];
+    __syncthreads();
+    if (threadIdx.x < kSlots) {
+        float total = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < kGroups; i++) total += s_a[i * kSlots + threadIdx.x];
+        c.sums[(chain * c.tiles + tile) * kSlots + threadIdx.x] = total;
+    }
+}
+
+// The tiles' sums of a shared gate's gradient, in 64 bits and one order.
+constexpr int kSumChannels = 16;
+template <class T>
+__global__ __launch_bounds__(1024) void sum_kernel(ScanArgs a, Chains c, int len) {
+    __shared__ double s_sum[1024];
+    const int own = threadIdx.x % kSumChannels, part = threadIdx.x / kSumChannels, parts = 1024 / kSumChannels;
+    const int channel = blockIdx.x * kSumChannels + own;
+    double sum = 0.0;
+    if (channel < a.dim) {
+        const int piece = channel / len, strip = piece / kLanes;
+        // (of the last piece's channels the first are those of the one before)
+        const int slot = piece % kLanes * len + channel - min(piece * len, a.dim - len);
+        const int64_t cells = a.rows * c.tiles;
+        for (int64_t i = part; i < cells; i += parts)
+            sum += c.sums[((i / c.tiles * c.strips + strip) * c.tiles + i % c.tiles) * c.slots + slot];
+    }
+    s_sum[threadIdx.x] = sum;
+    for (int half = parts / 2; half; half /= 2) {
+        __syncthreads();
+        if (part < half) s_sum[threadIdx.x] += s_sum[threadIdx.x + half * kSumChannels];
+    }
+    __syncthreads();
+    if (part == 0 && channel < a.dim) ((typename T::raw*)a.dgates)[channel] = (typename T::raw)(float)s_sum[threadIdx.x];
+}
+
+// ---- launches ----------------------------------------------------------------------------
+int fill(Chains& c, hipStream_t s) {
+    if (c.tiles <= 1) return 0;
+    const int64_t words = ((char*)c.sums - (char*)c.tickets) / 16;      // what lies before the sums
+    fill_kernel<<<(uint32_t)((words + kThreads - 1) / kThreads), kThreads, 0, s>>>((u32x4*)c.tickets, words);
+    DCIH_HIP(hipGetLastError());
+    return 0;
+}
+
+int fill_empty(const ScanArgs& a, const float* from, float* to, hipStream_t s) {
+    if (!a.bounds || !to) return 0;
+    for (int64_t first = 0; first < a.sequences; first += kMaxGrid) {
+        empty_kernel<<<(uint32_t)std::min(kMaxGrid, a.sequences - first), kThreads, 0, s>>>(a, from, to, first);
+        DCIH_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+template <class T, int L, bool kDecay, bool kShared>
+int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
+    Chains c{};
+    lay_out(c, a.work, a.rows, a.length, a.dim, dtype, gradient && a.shared);
+    if (int rc = fill(c, s)) return rc;
+    const int64_t blocks = c.count * c.tiles;
+    for (int64_t first = 0; first < blocks; first += kMaxGrid) {
+        const uint32_t grid = (uint32_t)std::min(kMaxGrid, blocks - first);
+        if (gradient) scan_grad_kernel<T, L, kDecay, kShared><<<grid, kBackThreads, 0, s>>>(a, c, first);
+        else scan_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first);
+        DCIH_HIP(hipGetLastError());
+    }
+    if (!gradient) return fill_empty(a, a.state, a.last, s);
+    if (kShared && a.dgates) {
+        sum_kernel<T><<<(uint32_t)((a.dim + kSumChannels - 1) / kSumChannels), 1024, 0, s>>>(a, c, L);
+        DCIH_HIP(hipGetLastError());
+    }
+    return fill_empty(a, a.dlast, a.dstate, s);
+}
+
+template <class T, int L, bool kDecay>
+int run_short(const ScanArgs& a, hipStream_t s) {
+    const int pieces = (a.dim + L - 1) / L;
+    const int64_t threads = a.rows * pieces, most = kMaxGrid * kThreads;
+    for (int64_t first = 0; first < threads; first += most) {
+        short_kernel<T, L, kDecay><<<(uint32_t)((std::min(most, threads - first) + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, pieces, first);
+        DCIH_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+template <class T, int L>
+int by_gates(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
+    if (!gradient && scan_is_short(a)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
+    if (a.decay) return a.shared ? run<T, L, true, true>(a, dtype, gradient, s) : run<T, L, true, false>(a, dtype, gradient, s);
+    return a.shared ? run<T, L, false, true>(a, dtype, gradient, s) : run<T, L, false, false>(a, dtype, gradient, s);
+}
+
+template <class T>
+int by_length(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
+    if (span_len(a.dim, dtype) == 1) return by_gates<T, 1>(a, dtype, gradient, s);
+    return by_gates<T, Piece<T>::kLen>(a, dtype, gradient, s);
+}
+
+// Short sequences that stand one behind the other share tiles: as many as one holds.
+ScanArgs flattened(ScanArgs a) {
+    auto flat = [&](int64_t row, int64_t step) { return row == a.length * step; };
+    if (a.form != kRows || 2 * a.length > kTile || a.rows == 1 || !flat(a.x_row, a.x_step) || (!a.shared && !flat(a.g_row, a.g_step)))
+        return a;
+    const int64_t together = kTile / a.length;
+    a.form = kFlat;
+    a.each = a.length;
+    a.total = a.rows * a.length;
+    a.length *= together;
+    a.rows = (a.rows + together - 1) / together;
+    a.x_row *= together;
+    a.g_row *= together;
+    return a;
+}
+
+int dispatch(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
+    switch (dtype) {
+        case DCIH_F32: return by_length<F32>(a, dtype, gradient, s);
+        case DCIH_F16: return by_length<F16>(a, dtype, gradient, s);
+        default: return by_length<BF16>(a, dtype, gradient, s);
+    }
+}
+
+}  // namespace
+
+int64_t scan_state_floats(int64_t rows, int64_t length, int dim, int dtype) {
+    Chains c{};
+    lay_out(c, nullptr, rows, length, dim, dtype, false);
+    return c.count * c.tiles * c.slots;
+}
+
+int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype, bool gradient, bool shared) {
+    Chains c{};
+    return lay_out(c, nullptr, rows, length, dim, dtype, gradient && shared);
+}
+
+bool scan_is_short(const ScanArgs& a) { return a.form == kRows && a.length <= kShort && !a.states; }
+
+int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a), dtype, false, s); }
+int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a), dtype, true, s); }
+
+int scan_copy(const float* from, float* to, int64_t n, hipStream_t s) {
+    copy_kernel<<<(uint32_t)std::min<int64_t>((n + kThreads - 1) / kThreads, 2048), kThreads, 0, s>>>(from, to, n);
+    DCIH_HIP(hipGetLastError());
+    return 0;
+}
+
+}  // namespace dcih

@@ -5,6 +5,7 @@
 #include <string>
 
 #include "../../include/dci_hip.h"
+#include "scan.h"
 #include "token_common.h"
 
 namespace dcih {
@@ -100,6 +101,57 @@ const char* check_teacher(const void* teacher, int teacher_dtype, int slots, con
     if (const char* why = check_ids(ids, id_bytes)) return why;
     return check_array(teacher, teacher_dtype);
 }
+
+// Tokens of a scan: rows, length and dim that are in bounds, and addresses in 63 bits.
+const char* check_scan_size(int64_t rows, int64_t length, int dim, int dtype, int64_t packed) {
+    if (!type_bytes(dtype)) return "unknown element type";
+    if (rows < 0 || rows > kMaxCount || length < 0 || length > kMaxCount || dim <= 0 || dim > DCIH_MAX_DIM || packed < 0 || packed > kMaxCount)
+        return "bad size";
+    if (packed && rows != 1) return "packed sequences are one row of tokens";
+    if (!near_enough(rows * std::max<int64_t>(length, 1), dim)) return "too many tokens";
+    return nullptr;
+}
+
+// Elements from the first of [rows][length][dim] to behind the last.
+int64_t scan_extent(int64_t rows, int64_t length, int dim, int64_t row, int64_t step) { return (rows - 1) * row + (length - 1) * step + dim; }
+
+const char* scan_args(ScanArgs& a, const void* x, int dtype, int64_t rows, int64_t length, int dim, int64_t x_row, int64_t x_step,
+                      const void* gates, int64_t g_row, int64_t g_step, int flags, const float* state, const void* bounds, int id_bytes,
+                      int64_t packed) {
+    if (const char* why = check_scan_size(rows, length, dim, dtype, packed)) return why;
+    if (flags & ~(DCIH_SCAN_DECAYS | DCIH_SCAN_SHARED)) return "unknown flags";
+    if (packed && !bounds) return "packed sequences need offsets";
+    if (bounds)
+        if (const char* why = check_ids(bounds, id_bytes)) return why;
+    if (!all_aligned({state})) return "states not aligned to their elements";
+    a.shared = (flags & DCIH_SCAN_SHARED) != 0;
+    if (rows && length) {
+        if (const char* why = check_array(x, dtype)) return why;
+        if (const char* why = check_array(gates, dtype)) return why;
+        if (a.shared) g_row = g_step = 0;
+        if (x_row < 0 || x_step < 0 || g_row < 0 || g_step < 0) return "distances are not negative";
+        if (!near_enough(rows, std::max(x_row, g_row)) || !near_enough(length, std::max(x_step, g_step))) return "tokens are too far apart";
+    }
+    a.x = x;
+    a.gates = gates;
+    a.x_row = x_row;
+    a.x_step = x_step;
+    a.g_row = g_row;
+    a.g_step = g_step;
+    a.rows = rows;
+    a.length = length;
+    a.sequences = packed ? packed : rows;
+    a.dim = dim;
+    a.form = packed ? kPacked : kRows;
+    a.decay = (flags & DCIH_SCAN_DECAYS) != 0;
+    a.state = state;
+    a.bounds = bounds;
+    a.wide_bounds = id_bytes == 8;
+    return nullptr;
+}
+
+// States in their own place: where one thread does not have a channel from first to last, the new ones wait in the workspace.
+int64_t last_bytes(int64_t sequences, int dim) { return (sequences * dim * 4 + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace dcih
@@ -265,6 +317,81 @@ int dcih_distill_grad(const void* d_logits, int dtype, int64_t num_rows, int voc
     a.grad = d_grad;
     a.grad_stride = grad_stride;
     return logit_grad(a, dtype, true, (hipStream_t)stream);
+}
+
+int64_t dcih_scan_states(int64_t rows, int64_t length, int dim, int dtype) {
+    if (const char* why = check_scan_size(rows, length, dim, dtype, 0)) return refuse("dcih_scan_states", why);
+    return scan_state_floats(rows, length, dim, dtype);
+}
+
+int64_t dcih_scan_work(int64_t rows, int64_t length, int dim, int dtype, int64_t packed_sequences) {
+    if (const char* why = check_scan_size(rows, length, dim, dtype, packed_sequences)) return refuse("dcih_scan_work", why);
+    return scan_work_bytes(rows, length, dim, dtype, true, true) + last_bytes(packed_sequences ? packed_sequences : rows, dim);
+}
+
+int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim, int64_t x_row, int64_t x_step, const void* d_gates,
+              int64_t g_row, int64_t g_step, int flags, const float* d_state, const void* d_bounds, int id_bytes,
+              int64_t packed_sequences, void* d_h, float* d_last, float* d_states, void* d_work, int64_t work_bytes, void* stream) {
+    const char* who = "dcih_scan";
+    hipStream_t s = (hipStream_t)stream;
+    ScanArgs a{};
+    if (const char* why = scan_args(a, d_x, dtype, rows, length, dim, x_row, x_step, d_gates, g_row, g_step, flags, d_state, d_bounds, id_bytes, packed_sequences))
+        return refuse(who, why);
+    if (!all_aligned({d_last, d_states})) return refuse(who, "states not aligned to their elements");
+    const int64_t states = a.sequences * dim;
+    if (d_last && d_state && d_last != d_state && overlap(d_last, states * 4, d_state, states * 4))
+        return refuse(who, "the last states overlap the first without being in their place");
+    if (!rows || !length) return d_last && d_last != d_state && states ? scan_copy(d_state, d_last, states, s) : DCIH_OK;
+    if (const char* why = check_array(d_h, dtype)) return refuse(who, why);
+    const int64_t b = type_bytes(dtype), h_bytes = rows * length * dim * b;
+    if (overlap(d_h, h_bytes, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
+        overlap(d_h, h_bytes, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b))
+        return refuse(who, "h overlaps x or the gates");
+    const int64_t own = scan_work_bytes(rows, length, dim, dtype, true, true);
+    if (work_bytes < own + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
+    if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
+    a.h = d_h;
+    a.last = d_last;
+    a.states = d_states;
+    a.work = d_work;
+    const bool waits = d_last && d_last == d_state && !scan_is_short(a);
+    if (waits) a.last = (float*)((char*)d_work + own);
+    if (int rc = scan(a, dtype, s)) return rc;
+    return waits ? scan_copy(a.last, d_last, states, s) : DCIH_OK;
+}
+
+int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int dim, int64_t x_row, int64_t x_step, const void* d_gates,
+                   int64_t g_row, int64_t g_step, int flags, const float* d_state, const void* d_bounds, int id_bytes,
+                   int64_t packed_sequences, const float* d_states, const void* d_dh, const float* d_dlast, void* d_dx, void* d_dgates,
+                   float* d_dstate, void* d_work, int64_t work_bytes, void* stream) {
+    const char* who = "dcih_scan_grad";
+    hipStream_t s = (hipStream_t)stream;
+    ScanArgs a{};
+    if (const char* why = scan_args(a, d_x, dtype, rows, length, dim, x_row, x_step, d_gates, g_row, g_step, flags, d_state, d_bounds, id_bytes, packed_sequences))
+        return refuse(who, why);
+    if (!all_aligned({d_states, d_dlast, d_dstate})) return refuse(who, "states not aligned to their elements");
+    if (!aligned(d_dh, type_bytes(dtype)) || !aligned(d_dx, type_bytes(dtype)) || !aligned(d_dgates, type_bytes(dtype)))
+        return refuse(who, "gradients not aligned to their elements");
+    const int64_t b = type_bytes(dtype), states = a.sequences * dim, cells = rows * length * dim * b;
+    if (!rows || !length) {
+        if (a.shared && d_dgates) return refuse(who, "no tokens to sum a shared gate's gradient over");
+        return d_dstate && states ? scan_copy(d_dlast, d_dstate, states, s) : DCIH_OK;
+    }
+    if (!d_states) return refuse(who, "null array");
+    for (const void* out : {(const void*)d_dx, a.shared ? nullptr : (const void*)d_dgates})
+        if (out && (overlap(out, cells, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
+                    overlap(out, cells, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b) || (d_dh && overlap(out, cells, d_dh, cells))))
+            return refuse(who, "a gradient overlaps what it is formed from");
+    if (work_bytes < scan_work_bytes(rows, length, dim, dtype, true, true) || !d_work) return refuse(who, "workspace too small");
+    if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
+    a.states = const_cast<float*>(d_states);
+    a.dh = d_dh;
+    a.dlast = d_dlast;
+    a.dx = d_dx;
+    a.dgates = d_dgates;
+    a.dstate = d_dstate;
+    a.work = d_work;
+    return scan_grad(a, dtype, s);
 }
 
 }  // extern "C"

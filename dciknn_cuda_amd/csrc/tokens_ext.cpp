@@ -346,6 +346,151 @@ std::tuple<Tensor, Tensor> distill_step(const Tensor& logits, const Tensor& ids,
     return {got[0], got[2]};
 }
 
+// ---- gated recurrence --------------------------------------------------------------------
+// What a scan is over: x [rows, length, dim], or [tokens, dim] with sequences between offsets.
+struct Scan {
+    int dtype = 0, flags = 0, dim = 0;
+    int64_t rows = 1, length = 0, sequences = 0, packed = 0;
+    int64_t x_row = 0, x_step = 0, g_row = 0, g_step = 0;
+    Tensor bounds;
+
+    int bound_bytes() const { return bounds.defined() ? id_bytes(bounds) : 4; }
+    const void* bound_data() const { return bounds.defined() ? bounds.data_ptr() : nullptr; }
+};
+
+// The states of all sequences, float32 and contiguous; undefined where none are given.
+Tensor states_of(const c10::optional<Tensor>& t, const Scan& s, const Tensor& x, const char* what) {
+    if (!t || !t->defined()) return Tensor();
+    if (!t->is_cuda()) bad_type(std::string(what) + " must be a cuda tensor");
+    if (t->scalar_type() != torch::kFloat32) bad_type(std::string(what) + " must be float32");
+    if (t->device() != x.device()) bad_value(std::string(what) + " must be on the other tensors' device");
+    if (t->sizes() != c10::IntArrayRef({s.sequences, s.dim})) bad_value(std::string(what) + " must be [sequences, dim]");
+    return t->contiguous();
+}
+
+Scan scan_of(const Tensor& x, const Tensor& gates, bool decay, const Tensor& lengths, const Tensor& offsets) {
+    Scan s;
+    s.dtype = type_code(x, "x");
+    if (type_code(gates, "gates") != s.dtype) bad_type("gates must be of x's type");
+    if (gates.device() != x.device()) bad_value("gates must be on the other tensors' device");
+    if (x.dim() != 2 && x.dim() != 3) bad_value("x must be [batch, length, dim] or [tokens, dim]");
+    const bool batch = x.dim() == 3;
+    if (x.size(-1) < 1 || x.size(-1) > DCIH_MAX_DIM) bad_value("x must have from 1 to 2**20 channels");
+    s.dim = (int)x.size(-1);
+    if (s.dim > 1 && (x.stride(-1) != 1 || gates.stride(-1) != 1)) bad_value("the channels of a token must be next to one another");
+    const bool shared = gates.dim() == 1;
+    if (shared ? gates.size(0) != s.dim : gates.sizes() != x.sizes()) bad_value("gates must be of x's shape, or one for each channel");
+    s.flags = (decay ? DCIH_SCAN_DECAYS : 0) | (shared ? DCIH_SCAN_SHARED : 0);
+    s.rows = batch ? x.size(0) : 1;
+    s.length = x.size(-2);
+    if (s.rows > 0x7fffffff || s.length > 0x7fffffff) bad_value("x has too many tokens");
+    s.x_row = batch ? x.stride(0) : 0;
+    s.x_step = x.stride(-2);
+    if (!shared) {
+        s.g_row = batch ? gates.stride(0) : 0;
+        s.g_step = gates.stride(-2);
+    }
+    s.sequences = s.rows;
+    if (lengths.defined()) {
+        if (!batch) bad_value("lengths are for x of [batch, length, dim]; sequences of [tokens, dim] are between offsets");
+        s.bounds = ids_of(lengths, x, "lengths");
+        if (s.bounds.dim() != 1 || s.bounds.size(0) != s.rows) bad_value("lengths must be [batch]");
+    }
+    if (offsets.defined()) {
+        if (batch) bad_value("offsets are for x of [tokens, dim]; a batch may have lengths");
+        s.bounds = ids_of(offsets, x, "offsets");
+        if (s.bounds.dim() != 1 || s.bounds.size(0) < 2) bad_value("offsets must be [sequences + 1]");
+        if (s.bounds.size(0) - 1 > 0x7fffffff) bad_value("too many sequences");
+        s.packed = s.sequences = s.bounds.size(0) - 1;
+    }
+    return s;
+}
+
+Tensor or_none(const c10::optional<Tensor>& t) { return t ? *t : Tensor(); }
+c10::optional<Tensor> if_given(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+
+// (h, last states, states for the gradient)
+variable_list scan_forward(const Scan& s, const Tensor& x, const Tensor& gates, const Tensor& state, const Tensor& into, bool keep) {
+    c10::DeviceGuard guard(x.device());
+    const Tensor h = torch::empty(x.sizes(), x.options().requires_grad(false).memory_format(torch::MemoryFormat::Contiguous));
+    const Tensor last = into.defined() ? into : floats({s.sequences, s.dim}, x);
+    Tensor states;
+    if (keep) states = floats({dcih_scan_states(s.rows, s.length, s.dim, s.dtype)}, x);
+    const int64_t need = dcih_scan_work(s.rows, s.length, s.dim, s.dtype, s.packed);
+    check(need);
+    const Tensor work = bytes(need, x);
+    if (s.sequences)
+        check(dcih_scan(x.data_ptr(), s.dtype, s.rows, s.length, s.dim, s.x_row, s.x_step, gates.data_ptr(), s.g_row, s.g_step, s.flags,
+                        data_or_null(state), s.bound_data(), s.bound_bytes(), s.packed, h.data_ptr(), last.data_ptr<float>(),
+                        keep ? states.data_ptr<float>() : nullptr, work.data_ptr(), need, stream_of(x)));
+    return {h, last, states};
+}
+
+struct GatedScan : torch::autograd::Function<GatedScan> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gates, const c10::optional<Tensor>& state_in, bool decay,
+                                 const c10::optional<Tensor>& lengths_in, const c10::optional<Tensor>& offsets_in) {
+        const Tensor state = or_none(state_in), lengths = or_none(lengths_in), offsets = or_none(offsets_in);
+        const Scan s = scan_of(x, gates, decay, lengths, offsets);
+        const auto got = scan_forward(s, x, gates, state, Tensor(), true);
+        ctx->save_for_backward({x, gates, state, lengths, offsets, got[2]});
+        ctx->saved_data["decay"] = decay;
+        ctx->set_materialize_grads(false);
+        return {got[0], got[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once_only(grads);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &gates = saved[1], &state = saved[2];
+        const Scan s = scan_of(x, gates, ctx->saved_data["decay"].toBool(), saved[3], saved[4]);
+        Tensor dx, dgates, dstate;
+        if (grads[0].defined() || grads[1].defined()) {
+            const Tensor dh = grads[0].defined() ? grads[0].contiguous() : Tensor(), dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+            c10::DeviceGuard guard(x.device());
+            const auto plain = x.options().requires_grad(false).memory_format(torch::MemoryFormat::Contiguous);
+            if (ctx->needs_input_grad(0)) dx = torch::empty(x.sizes(), plain);
+            if (ctx->needs_input_grad(1)) dgates = s.rows && s.length ? torch::empty(gates.sizes(), plain) : torch::zeros(gates.sizes(), plain);
+            if (state.defined() && ctx->needs_input_grad(2)) dstate = floats(state.sizes(), x);
+            const int64_t need = dcih_scan_work(s.rows, s.length, s.dim, s.dtype, s.packed);
+            check(need);
+            const Tensor work = bytes(need, x);
+            if (s.sequences)
+                check(dcih_scan_grad(x.data_ptr(), s.dtype, s.rows, s.length, s.dim, s.x_row, s.x_step, gates.data_ptr(), s.g_row, s.g_step, s.flags,
+                                     data_or_null(state), s.bound_data(), s.bound_bytes(), s.packed, saved[5].data_ptr<float>(),
+                                     dh.defined() ? dh.data_ptr() : nullptr, data_or_null(dlast), dx.defined() && dx.numel() ? dx.data_ptr() : nullptr,
+                                     dgates.defined() && s.rows && s.length ? dgates.data_ptr() : nullptr, dstate.defined() ? dstate.data_ptr<float>() : nullptr,
+                                     work.data_ptr(), need, stream_of(x)));
+        }
+        return {dx, dgates, dstate, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gates, const c10::optional<Tensor>& state_in, bool decay,
+                                      const c10::optional<Tensor>& lengths_in, const c10::optional<Tensor>& offsets_in,
+                                      const c10::optional<Tensor>& into) {
+    const Tensor lengths = or_none(lengths_in), offsets = or_none(offsets_in);
+    const Scan s = scan_of(x, gates, decay, lengths, offsets);
+    const Tensor state = states_of(state_in, s, x, "state");
+    for (const Tensor& t : {x, gates, state}) no_tangent(t);
+    const bool wanted = wants_grad(x) || wants_grad(gates) || (state.defined() && wants_grad(state));
+    if (!into) {
+        if (!wanted) {
+            const auto got = scan_forward(s, x, gates, state, Tensor(), false);
+            return {got[0], got[1]};
+        }
+        const auto got = GatedScan::apply(x, gates, if_given(state), decay, lengths_in, offsets_in);
+        return {got[0], got[1]};
+    }
+    if (wanted) bad_value("last is for calls without gradients");
+    no_tangent(*into);
+    if (into->is_cuda() && !into->is_contiguous()) bad_value("last must be contiguous");
+    states_of(into, s, x, "last");
+    if (wants_grad(*into)) bad_value("last must not require a gradient");
+    if (into->is_alias_of(x) || into->is_alias_of(gates)) bad_value("last must not share the memory of x or gates");
+    into->unsafeGetTensorImpl()->bump_version();
+    const auto got = scan_forward(s, x, gates, state, *into, false);
+    return {got[0], *into};
+}
+
 }  // namespace
 
 void bind_tokens(py::module_& m) {
@@ -353,5 +498,6 @@ void bind_tokens(py::module_& m) {
     m.def("_embed_grad", &embed_grad, "Gradient of _embed by the table. (HIP)");
     m.def("_token_logprobs", &token_logprobs, "Log probabilities, entropies, best alternatives. (HIP)");
     m.def("_distill_loss", &distill_loss, "Loss against a teacher's top logits. (HIP)");
+    m.def("_gated_scan", &gated_scan, "Gated linear recurrence over the tokens of sequences. (HIP)");
     m.def("_distill_step", &distill_step, "Loss against a teacher's top logits and its gradient. (HIP)");
 }

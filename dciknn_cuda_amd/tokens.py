@@ -64,3 +64,16 @@ def distill_step(logits, ids, teacher, weights=None, temperature=1.0, *, out=Non
     holds.  `out`: where the gradient goes, also `logits` itself; a leaf that requires a gradient, or anything
     else that does, is refused."""
     return _ext._distill_step(logits, ids, teacher, weights, temperature, out)
+
+
+def gated_scan(x, gates, state=None, *, decay=False, lengths=None, offsets=None, last=None):
+    """(h, last) of a linear recurrence over the tokens of sequences, each channel by itself: with a = sigmoid(gates)
+    h_t = a_t * h_(t-1) + (1 - a_t) * x_t, with `decay` a = gates and h_t = a_t * h_(t-1) + x_t.
+
+    x [batch, length, dim], with `lengths` [batch] the tokens of each (h is 0 behind them, and nothing there is looked
+    at), or x [tokens, dim], one sequence or, with `offsets` [sequences + 1], those between them one behind the other.  gates are of
+    x's shape, or [dim] for all tokens; state [sequences, dim] float32 is what stands before the first tokens, zeros if not given.  h is of x's
+    shape and type, last [sequences, dim] float32 the state behind the last tokens.  The channels of a token are next to one another, tokens and
+    rows at any distances.  A server's step is a length of 1, with `last=state` in place.  States are in 32 bits; one that is not finite
+    leaves none finite behind it in its sequence.  Differentiable by x, gates and state, not with `last`."""
+    return _ext._gated_scan(x, gates, state, decay, lengths, offsets, last)
