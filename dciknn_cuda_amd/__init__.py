@@ -6,7 +6,7 @@ training or serving a model on its rows and neighbours takes (see `tokens.py`).
 """
 __version__ = "0.1.0"
 
-_TOKENS = ["embed", "embed_grad", "token_logprobs", "distill_loss", "distill_step", "gated_scan"]
+_TOKENS = ["embed", "embed_grad", "token_logprobs", "distill_loss", "distill_step", "gated_scan", "grad_norm", "clip_grads", "verify_drafts"]
 __all__ = ["DCI", "MDCI"] + _TOKENS
 
 

@@ -96,7 +96,20 @@ SIGNATURES = {
                                   _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p, _c.c_int,
                                   _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
                                   _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_clip_work": (_c.c_int64, [_c.c_void_p, _c.c_int64]),
+    "dcih_grad_norm": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_double, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
+    "dcih_clip": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_double, _c.c_double, _c.c_void_p, _c.c_void_p, _c.c_int64,
+                             _c.c_void_p]),
+    "dcih_verify_work": (_c.c_int64, [_c.c_int64, _c.c_int, _c.c_int, _c.c_int]),
+    "dcih_verify": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int64, _c.c_int, _c.c_int, _c.c_int64, _c.c_void_p, _c.c_int,
+                               _c.c_void_p, _c.c_void_p, _c.c_int, _c.c_void_p, _c.c_int, _c.c_int, _c.c_float,
+                               _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p]),
 }
+
+
+class Span(_c.Structure):
+    """dcih_span: elements that dcih_grad_norm and dcih_clip take."""
+    _fields_ = [("data", _c.c_void_p), ("out", _c.c_void_p), ("count", _c.c_int64), ("dtype", _c.c_int), ("out_dtype", _c.c_int)]
 
 _lib = None
 

@@ -1,12 +1,15 @@
 // The entry points of include/dci_hip.h that work on tokens: checks of the arguments, the caller's
 // workspace laid out, launches.  No handle, no state; nothing here allocates, waits or throws.
 #include <algorithm>
+#include <cmath>
 #include <initializer_list>
 #include <string>
 
 #include "../../include/dci_hip.h"
+#include "clip.h"
 #include "scan.h"
 #include "token_common.h"
+#include "verify.h"
 
 namespace dcih {
 namespace {
@@ -148,6 +151,30 @@ const char* scan_args(ScanArgs& a, const void* x, int dtype, int64_t rows, int64
     a.bounds = bounds;
     a.wide_bounds = id_bytes == 8;
     return nullptr;
+}
+
+const char* check_spans(const dcih_span* spans, int64_t n, bool written) {
+    if (n < 0 || n > kMaxCount || (n && !spans)) return "bad number of spans";
+    for (int64_t i = 0; i < n; i++) {
+        const dcih_span& p = spans[i];
+        if (p.count < 0 || p.count > INT64_MAX >> 8) return "bad length of a span";
+        if (!p.count) continue;
+        if (const char* why = check_array(p.data, p.dtype)) return why;
+        if (!written) continue;
+        if (const char* why = check_array(p.out, p.out_dtype)) return why;
+        if (p.out_dtype != p.dtype && p.out_dtype != DCIH_F32) return "what is written is of the span's type or of 32 bits";
+        if (!(p.out == p.data && p.out_dtype == p.dtype) && overlap(p.data, p.count * type_bytes(p.dtype), p.out, p.count * type_bytes(p.out_dtype)))
+            return "what is written overlaps the span without being in its place";
+    }
+    return clip_fits(spans, n) ? nullptr : "too many elements";
+}
+
+const char* check_clip(const dcih_span* spans, int64_t n, bool written, double scale, const float* norm, const void* work, int64_t bytes) {
+    if (const char* why = check_spans(spans, n, written)) return why;
+    if (!std::isfinite(scale)) return "scale must be a finite number";
+    if (!norm || !aligned(norm, 4)) return "no place for the norm";
+    if (!work || bytes < clip_work_bytes(spans, n)) return "workspace too small";
+    return aligned(work, 16) ? nullptr : "workspace not aligned to 16 bytes";
 }
 
 // States in their own place: where one thread does not have a channel from first to last, the new ones wait in the workspace.
@@ -392,6 +419,69 @@ int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int
     a.dstate = d_dstate;
     a.work = d_work;
     return scan_grad(a, dtype, s);
+}
+
+int64_t dcih_clip_work(const dcih_span* spans, int64_t num_spans) {
+    if (const char* why = check_spans(spans, num_spans, false)) return refuse("dcih_clip_work", why);
+    return clip_work_bytes(spans, num_spans);
+}
+
+int dcih_grad_norm(const dcih_span* spans, int64_t num_spans, double scale, float* d_norm, void* d_work, int64_t work_bytes, void* stream) {
+    if (const char* why = check_clip(spans, num_spans, false, scale, d_norm, d_work, work_bytes)) return refuse("dcih_grad_norm", why);
+    return grad_norm(spans, num_spans, scale, d_norm, d_work, (hipStream_t)stream);
+}
+
+int dcih_clip(const dcih_span* spans, int64_t num_spans, double max_norm, double scale, float* d_norm, void* d_work, int64_t work_bytes,
+              void* stream) {
+    if (const char* why = check_clip(spans, num_spans, true, scale, d_norm, d_work, work_bytes)) return refuse("dcih_clip", why);
+    if (!(max_norm >= 0.0)) return refuse("dcih_clip", "max_norm must not be negative");
+    return clip_grads(spans, num_spans, max_norm, scale, d_norm, d_work, (hipStream_t)stream);
+}
+
+int64_t dcih_verify_work(int64_t num_sequences, int drafts, int vocab, int dtype) {
+    if (num_sequences < 0 || drafts < 0 || drafts > kMaxDrafts || num_sequences > kMaxCount / (drafts + 1) || vocab <= 0 || vocab > DCIH_MAX_VOCAB ||
+        !type_bytes(dtype))
+        return refuse("dcih_verify_work", "bad argument");
+    return verify_work_bytes(num_sequences * (drafts + 1), vocab, dtype);
+}
+
+int dcih_verify(const void* d_logits, int dtype, int64_t num_sequences, int drafts, int vocab, int64_t row_stride, const void* d_drafts,
+                int id_bytes, const float* d_uniforms, const void* d_slot_ids, int slot_id_bytes, const void* d_teacher, int teacher_dtype,
+                int slots, float temperature, int32_t* d_tokens, int32_t* d_accepted, float* d_logprobs, void* d_work, int64_t work_bytes,
+                void* stream) {
+    const char* who = "dcih_verify";
+    if (drafts < 0 || drafts > kMaxDrafts) return refuse(who, "bad number of drafts");
+    if (num_sequences < 0 || num_sequences > kMaxCount / (drafts + 1)) return refuse(who, "bad number of sequences");
+    if (const char* why = check_logits(d_logits, dtype, num_sequences * (drafts + 1), vocab, row_stride, temperature)) return refuse(who, why);
+    if (!num_sequences) return DCIH_OK;
+    if (drafts)
+        if (const char* why = check_ids(d_drafts, id_bytes)) return refuse(who, why);
+    if (drafts && d_slot_ids)
+        if (const char* why = check_teacher(d_teacher, teacher_dtype, slots, d_slot_ids, slot_id_bytes)) return refuse(who, why);
+    if (!d_uniforms || !d_tokens || !d_accepted || !d_logprobs) return refuse(who, "null array");
+    if (!all_aligned({d_uniforms, d_tokens, d_accepted, d_logprobs})) return refuse(who, "arrays not aligned to their elements");
+    if (!d_work || work_bytes < verify_work_bytes(num_sequences * (drafts + 1), vocab, dtype)) return refuse(who, "workspace too small");
+    if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
+    VerifyArgs a{};
+    a.z = d_logits;
+    a.n = num_sequences;
+    a.stride = row_stride;
+    a.drafts = drafts;
+    a.vocab = vocab;
+    a.c2 = 1.44269504088896340736 / (double)temperature;
+    a.ids = d_drafts;
+    a.wide_ids = id_bytes == 8;
+    a.uniforms = d_uniforms;
+    a.slot_ids = drafts ? d_slot_ids : nullptr;
+    a.wide_slots = slot_id_bytes == 8;
+    a.teacher = d_teacher;
+    a.teacher_dtype = teacher_dtype;
+    a.slots = slots;
+    a.tokens = d_tokens;
+    a.accepted = d_accepted;
+    a.logprobs = d_logprobs;
+    a.work = d_work;
+    return verify(a, dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

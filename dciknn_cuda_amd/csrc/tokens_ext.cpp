@@ -5,6 +5,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -491,6 +492,139 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gates, cons
     return {got[0], *into};
 }
 
+// ---- norm of gradients, clipping ---------------------------------------------------------
+using Tensors = std::vector<Tensor>;
+
+std::vector<dcih_span> spans_of(const Tensors& grads, const c10::optional<Tensors>& into) {
+    if (into && into->size() != grads.size()) bad_value("out must have one tensor for each gradient");
+    std::vector<dcih_span> spans;
+    spans.reserve(grads.size());
+    for (size_t i = 0; i < grads.size(); i++) {
+        const Tensor &g = grads[i], &o = into ? (*into)[i] : g;
+        dcih_span p{};
+        p.dtype = type_code(g, "a gradient");
+        if (g.device() != grads[0].device()) bad_value("the gradients must be on one device");
+        if (!g.is_non_overlapping_and_dense()) bad_value("a gradient's elements must be one behind the other in some order of its dimensions");
+        no_tangent(g);
+        p.out_dtype = into ? type_code(o, "out") : p.dtype;
+        if (into) {
+            if (p.out_dtype != p.dtype && p.out_dtype != DCIH_F32) bad_type("out must be of the gradient's type or float32");
+            if (o.device() != g.device()) bad_value("out must be on the gradients' device");
+            bool alike = o.sizes() == g.sizes();
+            for (int64_t d = 0; alike && d < g.dim(); d++) alike = g.size(d) == 1 || o.stride(d) == g.stride(d);
+            if (!alike) bad_value("out must have the gradient's shape and strides");
+            no_tangent(o);
+        }
+        p.data = g.data_ptr();
+        p.out = o.data_ptr();
+        p.count = g.numel();
+        if (p.count) spans.push_back(p);
+    }
+    return spans;
+}
+
+// No two of what is written may overlap, nor any of it another gradient.
+void check_apart(const std::vector<dcih_span>& spans) {
+    struct Range { uintptr_t from, to; bool written; };
+    std::vector<Range> ranges;
+    ranges.reserve(2 * spans.size());
+    auto size = [](int dtype) { return dtype == DCIH_F32 ? 4 : 2; };
+    for (const auto& p : spans) {
+        ranges.push_back({(uintptr_t)p.out, (uintptr_t)p.out + p.count * size(p.out_dtype), true});
+        if (p.data != p.out || p.dtype != p.out_dtype) ranges.push_back({(uintptr_t)p.data, (uintptr_t)p.data + p.count * size(p.dtype), false});
+    }
+    auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
+    if (!std::is_sorted(ranges.begin(), ranges.end(), before)) std::sort(ranges.begin(), ranges.end(), before);
+    uintptr_t read = 0, written = 0;          // how far what lies before reaches
+    for (const auto& r : ranges) {
+        if (r.from < written || (r.written && r.from < read)) bad_value("a tensor that is written must not share memory with another one of the call");
+        (r.written ? written : read) = std::max(r.written ? written : read, r.to);
+    }
+}
+
+double scale_of(double scale) {
+    if (!std::isfinite(scale)) bad_value("scale must be a finite number");
+    return scale;
+}
+
+Tensor norm_of_none() { return torch::zeros({}, torch::kFloat32); }
+
+Tensor grad_norm(const Tensors& grads, double scale) {
+    scale_of(scale);
+    if (grads.empty()) return norm_of_none();
+    const auto spans = spans_of(grads, c10::nullopt);
+    for (const Tensor& g : grads)
+        if (wants_grad(g)) bad_value("no gradient is formed by the gradients: detach them");
+    c10::DeviceGuard guard(grads[0].device());
+    const Tensor norm = floats({}, grads[0]);
+    const int64_t need = dcih_clip_work(spans.data(), spans.size());
+    check(need);
+    const Tensor work = bytes(need, grads[0]);
+    check(dcih_grad_norm(spans.data(), spans.size(), scale, norm.data_ptr<float>(), work.data_ptr(), need, stream_of(grads[0])));
+    return norm;
+}
+
+Tensor clip_grads(const Tensors& grads, double max_norm, double scale, const c10::optional<Tensors>& into) {
+    scale_of(scale);
+    if (!(max_norm >= 0.0)) bad_value("max_norm must not be negative");
+    if (grads.empty() && (!into || into->empty())) return norm_of_none();
+    const auto spans = spans_of(grads, into);
+    check_apart(spans);
+    for (const Tensors* list : {&grads, into ? &*into : nullptr})
+        for (size_t i = 0; list && i < list->size(); i++)
+            if (wants_grad((*list)[i])) bad_value("no gradient is formed by or of the gradients: detach them");
+    for (const Tensor& t : into ? *into : grads) t.unsafeGetTensorImpl()->bump_version();
+    c10::DeviceGuard guard(grads[0].device());
+    const Tensor norm = floats({}, grads[0]);
+    const int64_t need = dcih_clip_work(spans.data(), spans.size());
+    check(need);
+    const Tensor work = bytes(need, grads[0]);
+    check(dcih_clip(spans.data(), spans.size(), max_norm, scale, norm.data_ptr<float>(), work.data_ptr(), need, stream_of(grads[0])));
+    return norm;
+}
+
+// ---- verification of drafts --------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Tensor& drafts_in, const Tensor& uniforms, const c10::optional<Tensor>& ids_in,
+                                                 const c10::optional<Tensor>& teacher_in, double temperature) {
+    const Rows r = rows_of(logits, "logits");
+    if (logits.dim() != 3 || logits.size(1) < 1) bad_value("logits must be [batch, drafts + 1, vocab]");
+    const int64_t n = logits.size(0), k = logits.size(1) - 1;
+    if (k > DCIH_MAX_DRAFTS) bad_value("a sequence has up to 256 drafts");
+    const Tensor drafts = ids_of(drafts_in, logits, "drafts");
+    if (drafts.sizes() != c10::IntArrayRef({n, k})) bad_value("drafts must be [batch, drafts], one fewer than rows of logits");
+    const Tensor u = factors_of(uniforms, leading(logits), logits, "uniforms");
+    if (ids_in.has_value() != teacher_in.has_value()) bad_value("ids and teacher are given together");
+    const float t = temperature_of(temperature);
+    Teacher q;
+    if (ids_in) {
+        const Tensor ids = ids_of(*ids_in, logits, "ids");
+        q.dtype = type_code(*teacher_in, "teacher");
+        if (teacher_in->device() != logits.device()) bad_value("teacher must be on the other tensors' device");
+        if (ids.dim() != 3 || ids.size(0) != n || ids.size(1) != k || teacher_in->sizes() != ids.sizes()) bad_value("ids and teacher must be [batch, drafts, slots]");
+        if (ids.size(2) < 1 || ids.size(2) > 1024) bad_value("a draft's distribution has from 1 to 1024 slots");
+        q.ids = ids;
+        q.logits = teacher_in->contiguous();
+        q.slots = (int)ids.size(2);
+    }
+    for (const Tensor& x : {logits, uniforms, q.logits}) {
+        no_tangent(x);
+        if (x.defined() && wants_grad(x)) bad_value("no gradient is formed through tokens: detach the inputs");
+    }
+    c10::DeviceGuard guard(logits.device());
+    const auto whole = logits.options().dtype(torch::kInt32).requires_grad(false);
+    const Tensor tokens = torch::empty({n, k + 1}, whole), accepted = torch::empty({n}, whole), logprobs = floats({n, k + 1}, logits);
+    if (n) {
+        const int64_t need = dcih_verify_work(n, (int)k, (int)r.len, r.dtype);
+        check(need);
+        const Tensor work = bytes(need, logits);
+        check(dcih_verify(logits.data_ptr(), r.dtype, n, (int)k, (int)r.len, r.stride, k ? drafts.data_ptr() : nullptr, id_bytes(drafts), u.data_ptr<float>(),
+                          q.ids.defined() && k ? q.ids.data_ptr() : nullptr, q.ids.defined() ? id_bytes(q.ids) : 4,
+                          q.logits.defined() && k ? q.logits.data_ptr() : nullptr, q.dtype, q.slots, t, tokens.data_ptr<int32_t>(),
+                          accepted.data_ptr<int32_t>(), logprobs.data_ptr<float>(), work.data_ptr(), need, stream_of(logits)));
+    }
+    return {tokens, accepted, logprobs};
+}
+
 }  // namespace
 
 void bind_tokens(py::module_& m) {
@@ -499,5 +633,8 @@ void bind_tokens(py::module_& m) {
     m.def("_token_logprobs", &token_logprobs, "Log probabilities, entropies, best alternatives. (HIP)");
     m.def("_distill_loss", &distill_loss, "Loss against a teacher's top logits. (HIP)");
     m.def("_gated_scan", &gated_scan, "Gated linear recurrence over the tokens of sequences. (HIP)");
+    m.def("_grad_norm", &grad_norm, "Norm of a model's gradients. (HIP)");
+    m.def("_clip_grads", &clip_grads, "Gradients clipped by their norm. (HIP)");
+    m.def("_verify_drafts", &verify_drafts, "Drafted tokens against the model's probabilities. (HIP)");
     m.def("_distill_step", &distill_step, "Loss against a teacher's top logits and its gradient. (HIP)");
 }

@@ -1,0 +1,381 @@
+// Drafted tokens t_i of a sequence against the model's probabilities p_i = softmax(z_i / temperature), from given random
+// numbers u: t_i stands while u_i q_i(t_i) < p_i(t_i), with q_i what it was drawn from (1 for a draft that was named for
+// certain).  Where the first does not, a token is drawn from max(p_i - q_i, 0), behind the last one from p_i: the first with
+// u_k (sum of all weights) < (sum of the weights up to it).
+//
+// A token is right or wrong: everything that decides on one is in 64 bits, exponentials included, so that a random number has to
+// be within 1e-13 of a border to be taken to its wrong side (in 32 bits the borders of 131072 tokens cover some hundredths of [0, 1)).
+#include "../../include/dci_hip.h"
+#include "verify.h"
+
+#include <algorithm>
+
+namespace dcih {
+namespace {
+
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kChunk = 2048;                   // entries of a row that one wavefront adds up
+constexpr int64_t kMaxGrid = 1 << 23;
+
+struct alignas(16) Sum { double s; float m; float pad; };        // sum of 2^((z - m) c2), m = max z
+
+// 2^x to 2e-13 of it: n whole, 2^f by its series.  0 for x = -inf, NaN for NaN.
+__device__ inline double exp2_wide(double x) {
+    const double n = __builtin_rint(x), f = x - n;
+    double p = 7.054911620801121e-09;           // ln(2)^10 / 10!
+    p = __builtin_fma(p, f, 1.0178086009239696e-07);
+    p = __builtin_fma(p, f, 1.3215486790144305e-06);
+    p = __builtin_fma(p, f, 1.5252733804059838e-05);
+    p = __builtin_fma(p, f, 0.00015403530393381606);
+    p = __builtin_fma(p, f, 0.0013333558146428441);
+    p = __builtin_fma(p, f, 0.009618129107628477);
+    p = __builtin_fma(p, f, 0.055504108664821576);
+    p = __builtin_fma(p, f, 0.2402265069591007);
+    p = __builtin_fma(p, f, 0.6931471805599453);
+    p = __builtin_fma(p, f, 1.0);
+    const double y = __builtin_ldexp(p, (int)__builtin_fmax(n, -2000.0));
+    return x < -1100.0 ? 0.0 : y;
+}
+// The weight of an entry beside the largest (m2 = m c2, of a finite m).
+__device__ inline double weight_of(float z, double c2, double m2) { return exp2_wide(__builtin_fma((double)z, c2, -m2)); }
+
+__device__ inline double lanes_sum(double v) {
+#pragma unroll
+    for (int o = kWave / 2; o; o /= 2) v += __builtin_bit_cast(double, lane_xor_any(__builtin_bit_cast(unsigned long long, v), o));
+    return v;
+}
+
+// A wavefront adds up `per` chunks of a row, one after the other.  Rows behind a sequence's last draft are asked for by nobody.
+template <class T>
+__global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums, int chunks, int per, int64_t first) {
+    using P = Piece<T>;
+    constexpr int U = kChunk / kWave / P::kLen;
+    const int splits = (chunks + per - 1) / per, lane = lane_id();
+    const int64_t item = first + (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t row = item / splits, b = row / (a.drafts + 1);
+    if (b >= a.n) return;
+    const int i = (int)(row - b * (a.drafts + 1)), from = (int)(item - row * splits) * per, to = min(chunks, from + per);
+    for (int j = lane; __any(j < i); j += kWave)
+        if (__any(j < i && id_at(a.ids, a.wide_ids, b * a.drafts + j) < 0)) return;
+    const Row<T> r(a.z, row, a.stride, a.vocab);
+    for (int c = from; c < to; c++) {
+        u32x4 raw[U];
+        const int piece = c * (kChunk / P::kLen) + lane;
+        if ((c + 1) * (kChunk / P::kLen) <= r.pieces) {
+            r.load_runs(piece, kWave, raw);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) raw[u] = r.load(piece + u * kWave);
+        }
+        float m = kNoLogit;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float z[P::kLen];
+            P::unpack(raw[u], z);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) m = fmaxf(m, z[k]);
+        }
+        m = max_of_lanes(m);
+        const double m2 = (double)(m == kNoLogit ? 0.f : m) * a.c2;
+        double s = 0.0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float z[P::kLen];
+            P::unpack(raw[u], z);
+#pragma unroll
+            for (int k = 0; k < P::kLen; k++) s += weight_of(z[k], a.c2, m2);
+        }
+        s = lanes_sum(s);
+        if (lane == 0) sums[row * chunks + c] = Sum{s, m, 0.f};
+    }
+}
+
+// Sums up to and including each thread's, in the order of the threads.
+__device__ inline double scan_threads(double v, double* s_part) {
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int o = 1; o < kWave; o *= 2) {
+        const double other = __shfl_up(v, o);
+        if (lane >= o) v += other;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s_part[wave] = v;
+    __syncthreads();
+    double before = 0.0;
+    for (int w = 0; w < wave; w++) before += s_part[w];
+    return before + v;
+}
+
+__device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
+    switch (a.teacher_dtype) {
+        case DCIH_F32: return ((const float*)a.teacher)[i];
+        case DCIH_F16: return (float)((const _Float16*)a.teacher)[i];
+        default: return (float)((const __bf16*)a.teacher)[i];
+    }
+}
+
+constexpr int kSlots = 1024;
+constexpr double kLog2eWide = 1.44269504088896340736;
+
+// One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
+// from the row that it comes from, by chunks, then among the entries of one.
+template <class T>
+__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Sum* sums, int chunks, int64_t first) {
+    constexpr int kPer = kChunk / kThreads;
+    __shared__ double s_total[kMaxDrafts + 1], s_part[kWaves], s_weight[kChunk], s_gone[kSlots], s_target;
+    __shared__ float s_max[kMaxDrafts + 1];
+    __shared__ int s_kept[kMaxDrafts], s_id[kSlots], s_chunk, s_token, s_last, s_slots;
+    const int64_t b = first + blockIdx.x;
+    const int k = a.drafts, lane = lane_id(), wave = threadIdx.x / kWave, tid = threadIdx.x;
+    const double c2 = a.c2;
+    const typename T::raw* logits = (const typename T::raw*)a.z + b * (k + 1) * a.stride;
+    auto draft_at = [&](int i) { return id_at(a.ids, a.wide_ids, b * k + i); };
+    // how many drafts there are
+    if (tid == 0) {
+        s_slots = k;                                  // (for the moment)
+        s_chunk = s_token = s_last = -1;
+    }
+    __syncthreads();
+    for (int i = tid; i < k; i += kThreads)
+        if (draft_at(i) < 0) atomicMin(&s_slots, i);
+    __syncthreads();
+    const int given = s_slots;
+    for (int i = wave; i <= given; i += kWaves) {
+        const Sum* part = sums + (b * (k + 1) + i) * chunks;
+        float m = kNoLogit;
+        for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, part[c].m);
+        m = max_of_lanes(m);
+        const double m2 = (double)(m == kNoLogit ? 0.f : m) * c2;
+        double s = 0.0;
+        for (int c = lane; c < chunks; c += kWave) {
+            const Sum p = part[c];
+            s += p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, m2);
+        }
+        s = lanes_sum(s);
+        if (lane == 0) {
+            s_total[i] = s;
+            s_max[i] = m;
+        }
+        if (i == given) continue;
+        const int64_t t = draft_at(i);
+        // the probability that it was drawn with
+        double q = 1.0;
+        if (a.slot_ids) {
+            const int64_t at = (b * k + i) * a.slots;
+            float top = kNoLogit;
+            for (int j = lane; j < a.slots; j += kWave)
+                if (id_at(a.slot_ids, a.wide_slots, at + j) >= 0) top = fmaxf(top, teacher_at(a, at + j));
+            top = max_of_lanes(top);
+            const double top2 = (double)(top == kNoLogit ? 0.f : top) * kLog2eWide;
+            double all = 0.0, its = 0.0;
+            for (int j = lane; j < a.slots; j += kWave) {
+                const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
+                const double w = id < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top2);
+                all += w;
+                its += id == t ? w : 0.0;
+            }
+            all = lanes_sum(all);
+            its = lanes_sum(its);
+            q = all == 0.0 ? 0.0 : its / all;
+        }
+        if (lane == 0) {
+            const double p = t < a.vocab ? weight_of((float)logits[i * a.stride + t], c2, m2) : 0.0;
+            s_kept[i] = p > 0.0 && (double)a.uniforms[b * (k + 1) + i] * q * s < p;
+        }
+    }
+    __syncthreads();
+    int kept = 0;
+    while (kept < given && s_kept[kept]) kept++;
+    // row `kept` names the next token
+    const double total = s_total[kept], m2 = (double)(s_max[kept] == kNoLogit ? 0.f : s_max[kept]) * c2;
+    const typename T::raw* row = logits + kept * a.stride;
+    const Sum* part = sums + (b * (k + 1) + kept) * chunks;
+    bool fine = total > 0.0 && total < __builtin_huge_val();
+    // what is taken off its weights: ids and amounts, each id once
+    int slots = 0;
+    if (kept < given && fine) {
+        if (!a.slot_ids) {
+            slots = 1;
+            if (tid == 0) {
+                const int64_t t = draft_at(kept);
+                s_id[0] = t < a.vocab ? (int)t : -1;
+                s_gone[0] = total;
+            }
+        } else {
+            slots = a.slots;
+            const int64_t at = (b * k + kept) * a.slots;
+            float top = kNoLogit;
+            for (int j = tid; j < slots; j += kThreads) {
+                const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
+                s_id[j] = id < 0 ? -1 : id < a.vocab ? (int)id : a.vocab;
+                if (id >= 0) top = fmaxf(top, teacher_at(a, at + j));
+            }
+            top = max_of_lanes(top);
+            if (lane == 0) s_part[wave] = top;
+            __syncthreads();
+            for (int w = 0; w < kWaves; w++) top = fmaxf(top, (float)s_part[w]);
+            const double top2 = (double)(top == kNoLogit ? 0.f : top) * kLog2eWide;
+            double all = 0.0;
+            for (int j = tid; j < slots; j += kThreads) {
+                const double w = s_id[j] < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top2);
+                s_gone[j] = w;
+                all += w;
+            }
+            all = lanes_sum(all);
+            __syncthreads();
+            if (lane == 0) s_part[wave] = all;
+            __syncthreads();
+            all = 0.0;
+            for (int w = 0; w < kWaves; w++) all += s_part[w];
+            fine = all < __builtin_huge_val();
+            // a token of several slots stands in the first of them
+            double mine[kSlots / kThreads];
+#pragma unroll
+            for (int e = 0; e < kSlots / kThreads; e++) {
+                const int j = tid + e * kThreads;
+                mine[e] = 0.0;
+                if (j >= slots) continue;
+                bool leads = s_id[j] >= 0 && s_id[j] < a.vocab;
+                for (int o = 0; o < slots; o++) {
+                    const bool same = s_id[o] == s_id[j];
+                    if (same) mine[e] += s_gone[o];
+                    leads &= !(same && o < j);
+                }
+                if (!leads) mine[e] = -1.0;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kSlots / kThreads; e++) {
+                const int j = tid + e * kThreads;
+                if (j >= slots) continue;
+                if (mine[e] < 0.0) s_id[j] = -1;
+                else s_gone[j] = all == 0.0 ? 0.0 : mine[e] / all * total;
+            }
+        }
+    }
+    __syncthreads();
+    auto less = [&](int j) {           // what entry s_id[j] weighs less than in p
+        const double w = weight_of((float)row[s_id[j]], c2, m2);
+        return w - max(w - s_gone[j], 0.0);
+    };
+    const float u = a.uniforms[b * (k + 1) + k];
+    fine = fine && u == u;
+    // the chunk: a run of chunks for each thread
+    const int each = (chunks + kThreads - 1) / kThreads, begin = min(chunks, tid * each), end = min(chunks, begin + each);
+    auto chunk_sum = [&](int c) {
+        const Sum p = part[c];
+        double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, m2);
+        for (int j = 0; j < slots; j++)
+            if (s_id[j] >= 0 && s_id[j] / kChunk == c) s -= less(j);
+        return max(s, 0.0);
+    };
+    double all = 0.0, before = 0.0, own = 0.0;
+    for (int turn = 0; fine && turn < 2; turn++) {
+        own = 0.0;
+        for (int c = begin; c < end; c++) own += chunk_sum(c);
+        before = scan_threads(own, s_part);
+        all = 0.0;
+        for (int w = 0; w < kWaves; w++) all += s_part[w];
+        if (all > 0.0) break;
+        slots = 0;                       // nothing is left of p but roundings: drawn from p itself
+    }
+    if (fine) {
+        const double target = min(max((double)u, 0.0), 1.0) * all;
+        if (own > 0.0 && before - own <= target) atomicMax(&s_last, tid);      // (the last thread with weights below the target)
+        __syncthreads();
+        if (tid == s_last) {
+            double sum = before - own;
+            int at = -1;
+            double rest = 0.0;
+            for (int c = begin; c < end; c++) {
+                const double s = chunk_sum(c);
+                if (s > 0.0 && sum <= target) {
+                    at = c;
+                    rest = target - sum;
+                }
+                sum += s;
+            }
+            s_chunk = at;
+            s_target = rest;
+        }
+        __syncthreads();
+        // the entry
+        const int chunk = s_chunk, from = chunk * kChunk;
+        if (chunk >= 0) {
+#pragma unroll
+            for (int e = 0; e < kPer; e++) {
+                const int i = e * kThreads + tid;
+                s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, m2) : 0.0;
+            }
+            __syncthreads();
+            for (int j = tid; j < slots; j += kThreads)
+                if (s_id[j] >= from && s_id[j] < from + kChunk) s_weight[s_id[j] - from] = max(s_weight[s_id[j] - from] - s_gone[j], 0.0);
+            if (tid == 0) s_last = -1;
+            __syncthreads();
+            double w[kPer];
+            own = 0.0;
+#pragma unroll
+            for (int e = 0; e < kPer; e++) {
+                w[e] = s_weight[tid * kPer + e];
+                own += w[e];
+            }
+            double sum = scan_threads(own, s_part) - own;
+            int found = -1;
+#pragma unroll
+            for (int e = 0; e < kPer; e++) {
+                if (w[e] > 0.0 && sum <= s_target) found = tid * kPer + e;
+                sum += w[e];
+            }
+            if (found >= 0) atomicMax(&s_last, found);
+            __syncthreads();
+            if (tid == 0 && s_last >= 0) s_token = from + s_last;
+        }
+    }
+    __syncthreads();
+    const int token = s_token;
+    for (int i = tid; i <= k; i += kThreads) {
+        const int64_t t = i < kept ? draft_at(i) : i == kept ? token : -1;
+        float logp = 0.f;
+        if (i <= kept) {
+            if (t >= 0) logp = (float)(((double)(float)logits[i * a.stride + t] * c2 - (double)s_max[i] * c2) * 0.693147180559945309417 - log(s_total[i]));
+            else logp = __builtin_nanf("");
+        }
+        a.tokens[b * (k + 1) + i] = (int32_t)t;
+        a.logprobs[b * (k + 1) + i] = logp;
+    }
+    if (tid == 0) a.accepted[b] = kept;
+}
+
+int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
+
+template <class T>
+int run(const VerifyArgs& a, hipStream_t s) {
+    const int chunks = chunks_of(a.vocab);
+    const int64_t rows = a.n * (a.drafts + 1);
+    // wavefronts that fill the device
+    const int per = (int)std::min<int64_t>(chunks, std::max<int64_t>(1, rows * chunks / 16384));
+    const int64_t items = rows * ((chunks + per - 1) / per), most = kMaxGrid * kWaves;
+    for (int64_t first = 0; first < items; first += most) {
+        sums_kernel<T><<<(uint32_t)((std::min(most, items - first) + kWaves - 1) / kWaves), kThreads, 0, s>>>(a, (Sum*)a.work, chunks, per, first);
+        DCIH_HIP(hipGetLastError());
+    }
+    for (int64_t first = 0; first < a.n; first += kMaxGrid) {
+        verify_kernel<T><<<(uint32_t)std::min(kMaxGrid, a.n - first), kThreads, 0, s>>>(a, (const Sum*)a.work, chunks, first);
+        DCIH_HIP(hipGetLastError());
+    }
+    return 0;
+}
+
+}  // namespace
+
+int64_t verify_work_bytes(int64_t rows, int vocab, int) { return rows * chunks_of(vocab) * (int64_t)sizeof(Sum); }
+
+int verify(const VerifyArgs& a, int dtype, hipStream_t s) {
+    switch (dtype) {
+        case DCIH_F32: return run<F32>(a, s);
+        case DCIH_F16: return run<F16>(a, s);
+        default: return run<BF16>(a, s);
+    }
+}
+
+}  // namespace dcih

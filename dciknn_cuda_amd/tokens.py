@@ -77,3 +77,36 @@ def gated_scan(x, gates, state=None, *, decay=False, lengths=None, offsets=None,
     rows at any distances.  A server's step is a length of 1, with `last=state` in place.  States are in 32 bits; one that is not finite
     leaves none finite behind it in its sequence.  Differentiable by x, gates and state, not with `last`."""
     return _ext._gated_scan(x, gates, state, decay, lengths, offsets, last)
+
+
+def grad_norm(grads, scale=1.0):
+    """The norm of a model's gradients times `scale`, all of them as one vector: a float32 tensor of no dimensions.
+
+    grads: tensors of any of the types and shapes, mixed, each dense (in any order of its dimensions).  Squares are summed in 64 bits in an
+    order that depends on the shapes alone."""
+    return _ext._grad_norm(list(grads), scale)
+
+
+def clip_grads(grads, max_norm, scale=1.0, *, out=None):
+    """Multiplies the gradients, in their place or into `out`, by `scale * min(1, max_norm / norm)`; returns the norm before
+    clipping, `grad_norm(grads, scale)`, without waiting for it.
+
+    `scale` undoes a loss's factor.  out: for each gradient a tensor of its shape and strides, of its type or float32; no two
+    tensors of a call may share memory.  A norm that is infinite or NaN clips nothing (out = grads * scale)."""
+    return _ext._clip_grads(list(grads), max_norm, scale, None if out is None else list(out))
+
+
+def verify_drafts(logits, drafts, uniforms, ids=None, teacher=None, temperature=1.0):
+    """(tokens, accepted, logprobs): which drafted tokens stand before the model's probabilities, and the token behind them.
+
+    drafts [batch, k] (0 to 256, the first below 0 ends a sequence's), logits [batch, k + 1, vocab] with row i what the model says
+    behind i of them: p = softmax(logits / temperature).  ids and teacher [batch, k, slots]: the tokens a draft was drawn from and their
+    logits, q = softmax(teacher) over the filled slots, as in `distill_loss` (for tokens drawn from a model's best, what `token_logprobs`
+    returns for them); without them a draft was named for certain, as by the nearest neighbour.  uniforms [batch, k + 1] float32 in [0, 1):
+    draft i stands while uniforms[i] * q(draft) < p(draft); the next token is drawn by uniforms[k] from max(p - q, 0) of the first that does not,
+    else from the last p, as the first at which the running sum of the weights is above that share of all.
+    The tokens are distributed as if drawn from the model one by one.
+
+    tokens [batch, k + 1] int32: the accepted [batch] drafts, the next token, -1 behind it; logprobs float32: their log p,
+    0 behind them.  A row without probabilities (NaN, +inf, nothing but -inf) gives -1 with NaN.  Decided in 64 bits."""
+    return _ext._verify_drafts(logits, drafts, uniforms, ids, teacher, temperature)

@@ -434,6 +434,44 @@ int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int
                    int64_t packed_sequences, const float* d_states, const void* d_dh, const float* d_dlast, void* d_dx, void* d_dgates,
                    float* d_dstate, void* d_work, int64_t work_bytes, void* stream);
 
+/*
+ * The norm of all gradients of a model, and gradients times a factor that bounds it.  A span is `count` elements one behind the
+ * other at `data`; `out` is where they go times the factor: `data` itself with out_dtype = dtype, or an array of the same type or DCIH_F32 that
+ * overlaps no span.  The array of spans is the host's and read during the call only.
+ *   norm = |scale| sqrt(sum of squares),  out = data * scale * min(1, max_norm / norm)
+ * d_norm gets the norm (before clipping).  Where it is no number or infinite nothing is clipped (out = data * scale).
+ * Squares are summed in 64 bits in an order that depends on the spans alone.
+ */
+typedef struct {
+    const void* data;
+    void* out;
+    int64_t count;
+    int dtype, out_dtype;
+} dcih_span;
+int64_t dcih_clip_work(const dcih_span* spans, int64_t num_spans);
+int dcih_grad_norm(const dcih_span* spans, int64_t num_spans, double scale, float* d_norm, void* d_work, int64_t work_bytes, void* stream);
+int dcih_clip(const dcih_span* spans, int64_t num_spans, double max_norm, double scale, float* d_norm, void* d_work, int64_t work_bytes,
+              void* stream);
+
+/*
+ * Drafted tokens against the model's probabilities.  Sequence b has `drafts` tokens d_drafts[b][drafts] (0 to 256; the first
+ * below 0 ends them) and drafts + 1 rows of logits; row i of it, at d_logits + (b * (drafts + 1) + i) * row_stride, follows i of them: p_i =
+ * softmax(logits / temperature).  What draft i was drawn from: q_i = softmax over the filled slots (id not below 0, logit above -inf) of
+ * d_slot_ids and d_teacher, both [num_sequences][drafts][slots] (1 to 1024 slots, an id may stand in several), or with d_slot_ids NULL the draft for
+ * certain.  With the random numbers u = d_uniforms[b] ([drafts + 1], in [0, 1)) draft i stands if all before it do and
+ * u_i q_i(draft) < p_i(draft).  The next token is drawn from max(p_i - q_i, 0) of the first that does not (from p_i where that leaves
+ * nothing), behind the last one from p: the first with u_drafts * (sum of all weights) < (sum of the weights up to it).
+ * d_accepted [num_sequences]: how many stand; d_tokens, d_logprobs [num_sequences][drafts + 1]: these, the next token and
+ * -1, and their log p_i (0 for -1).  A draft beyond the vocabulary does not stand.  A row that holds NaN or +inf or nothing but
+ * -inf, or whose slots do or whose random number is NaN, gives no token: -1 with a log probability of NaN.  What decides is formed in 64 bits.
+ */
+#define DCIH_MAX_DRAFTS 256
+int64_t dcih_verify_work(int64_t num_sequences, int drafts, int vocab, int dtype);
+int dcih_verify(const void* d_logits, int dtype, int64_t num_sequences, int drafts, int vocab, int64_t row_stride, const void* d_drafts,
+                int id_bytes, const float* d_uniforms, const void* d_slot_ids, int slot_id_bytes, const void* d_teacher, int teacher_dtype,
+                int slots, float temperature, int32_t* d_tokens, int32_t* d_accepted, float* d_logprobs, void* d_work, int64_t work_bytes,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
