@@ -150,8 +150,8 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(Table t, const double* s
     __shared__ double s_part[kThreads / kWave];
     const double total = (joined ? sums[n] : sum_of(sums, n, s_part)), length = sqrt(total) * fabs(scale);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)length;
-    // (a norm that is no number or infinite clips nothing)
-    const float factor = (float)(length > max_norm && length < __builtin_huge_val() ? max_norm / length * scale : scale);
+    // (a norm that is no number, or infinite as it is returned, clips nothing)
+    const float factor = (float)(length > max_norm && (float)length < __builtin_huge_valf() ? max_norm / length * scale : scale);
     const uint32_t unit = t.units - 1 - blockIdx.x;
     const int i = span_of(t, unit);
     if (factor == 1.f && t.in[i] == t.out[i]) return;

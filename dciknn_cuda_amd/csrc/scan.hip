@@ -16,6 +16,7 @@
 #include "scan.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace dcih {
 namespace {
@@ -411,10 +412,33 @@ __device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int* s_f
         }
     }
 }
-__device__ inline bool is_marked(const ScanArgs& a, const Marks& m, int64_t t, int per, int group, uint32_t s_marked) {
-    if (a.form == kFlat || t < m.lo || t + per > m.hi) return true;
-    if (a.form == kRows) return t == 0 || t + per == m.hi;
-    return s_marked >> group & 1;
+// What a group of `per` tokens from `t` on has to know of them: a bit for each.  (Bits and selects, and one branch for a whole wavefront:
+// hipcc 7.2 lost a factor of A where lanes left the loop over the tokens by `continue`.)
+struct Bits {
+    uint32_t in, first, end;
+    bool any;                         // of the wavefront's groups one has a beginning, an end, or tokens of no sequence
+
+    __device__ Bits(const ScanArgs& a, const Marks& m, int64_t t, int per, int group, uint32_t s_marked) : in(~0u), first(0), end(0) {
+        bool marked = a.form == kFlat || t < m.lo || t + per > m.hi;
+        if (a.form == kRows) marked |= t == 0 || t + per == m.hi;
+        if (a.form == kPacked) marked |= s_marked >> group & 1;
+        any = __any(marked);
+        if (!any) return;
+        in = 0;
+        for (int u = 0; u < per; u++) {
+            const bool inside = m.in(a, t + u);
+            in |= (uint32_t)inside << u;
+            first |= (uint32_t)(inside && m.begins(a, t + u) >= 0) << u;
+            end |= (uint32_t)(inside && m.ends(a, t + u) >= 0) << u;
+        }
+    }
+    __device__ bool resets(int per) const { return first || (~in & ((1u << per) - 1)); }
+};
+
+// Runs `body` as the wavefront has marks or not: without them nothing is asked for each token.
+template <class Body> __device__ __forceinline__ void by_marks(bool any, Body body) {
+    if (any) body(std::true_type{});
+    else body(std::false_type{});
 }
 
 template <class T, int L, bool kDecay, bool kShared>
@@ -444,8 +468,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, in
     }
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
-    const bool marked = is_marked(a, m, t, U, group, s_marked);
-    auto first_state = [&](int64_t s, float (&h)[L]) {
+    const Bits bits(a, m, t, U, group, s_marked);
+    auto first_state = [&](int u, float (&h)[L]) {
+        const int64_t s = m.begins(a, t + u);
 #pragma unroll
         for (int k = 0; k < L; k++) h[k] = 0.f;
         if (a.state) load_floats<L>(a.state + s * a.dim + c0, h);
@@ -456,44 +481,22 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, in
     for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; }
 #pragma unroll
     for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
-    bool reset = false;
-    if (!marked) {
+    by_marks(bits.any, [&](auto asks) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            const bool in = !asks || (bits.in >> u & 1);
+            if (asks && (bits.first >> u & 1)) first_state(u, B);
             float xv[L];
             xs[u].get(xv);
 #pragma unroll
             for (int k = 0; k < L; k++) {
                 const float co = cs[kShared ? 0 : u][k];
                 A[k] *= factor<kDecay>(co);
-                B[k] = step<kDecay>(B[k], xv[k], co);
+                B[k] = in ? step<kDecay>(B[k], xv[k], co) : 0.f;
             }
         }
-    } else {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (!m.in(a, t + u)) {
-                reset = true;
-#pragma unroll
-                for (int k = 0; k < L; k++) B[k] = 0.f;
-                continue;
-            }
-            const int64_t s = m.begins(a, t + u);
-            if (s >= 0) {
-                reset = true;
-                first_state(s, B);
-            }
-            float xv[L];
-            xs[u].get(xv);
-#pragma unroll
-            for (int k = 0; k < L; k++) {
-                const float co = cs[kShared ? 0 : u][k];
-                A[k] *= factor<kDecay>(co);
-                B[k] = step<kDecay>(B[k], xv[k], co);
-            }
-        }
-        if (reset && lane == 0) atomicOr(&s_resets, 1u << group);
-    }
+    });
+    if (lane == 0 && bits.resets(U)) atomicOr(&s_resets, 1u << group);
     const int slot = lane * L, mine = group * kSlots + slot;
 #pragma unroll
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; }
@@ -508,29 +511,19 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, in
 #pragma unroll
     for (int k = 0; k < L; k++) h[k] = s_b[mine + k];
     raw_t* out = (raw_t*)a.h + (row * a.length + t) * a.dim + c0;
+    by_marks(bits.any, [&](auto asks) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        float xv[L];
-        xs[u].get(xv);
-        if (marked) {
-            if (t + u >= m.length) break;
-            if (!m.in(a, t + u)) {
+        for (int u = 0; u < U; u++) {
+            const bool in = !asks || (bits.in >> u & 1);
+            if (asks && (bits.first >> u & 1)) first_state(u, h);
+            float xv[L];
+            xs[u].get(xv);
 #pragma unroll
-                for (int k = 0; k < L; k++) h[k] = 0.f;
-                Span<T, L>::store(out + (int64_t)u * a.dim, h);
-                continue;
-            }
-            const int64_t s = m.begins(a, t + u);
-            if (s >= 0) first_state(s, h);
+            for (int k = 0; k < L; k++) h[k] = in ? step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]) : 0.f;
+            if (!asks || t + u < m.length) Span<T, L>::store(out + (int64_t)u * a.dim, h);
+            if (asks && (bits.end >> u & 1) && a.last) store_floats<L>(a.last + m.ends(a, t + u) * a.dim + c0, h);
         }
-#pragma unroll
-        for (int k = 0; k < L; k++) h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
-        Span<T, L>::store(out + (int64_t)u * a.dim, h);
-        if (marked && a.last) {
-            const int64_t s = m.ends(a, t + u);
-            if (s >= 0) store_floats<L>(a.last + s * a.dim + c0, h);
-        }
-    }
+    });
 }
 
 // The gradient of a tile.  The states go forward from the one kept, the gradient that reaches them goes back from the tile
@@ -568,8 +561,9 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
     }
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
-    const bool marked = is_marked(a, m, t, U, group, s_marked), some = a.dh != nullptr;
-    auto first_state = [&](const float* from, int64_t s, float (&h)[L]) {
+    const Bits bits(a, m, t, U, group, s_marked);
+    const bool some = a.dh != nullptr;
+    auto state_of = [&](const float* from, int64_t s, float (&h)[L]) {
 #pragma unroll
         for (int k = 0; k < L; k++) h[k] = 0.f;
         if (from) load_floats<L>(from + s * a.dim + c0, h);
@@ -584,56 +578,32 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
     for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; Q[k] = 0.f; }
 #pragma unroll
     for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
-    bool reset = false, back_reset = false;
+    by_marks(bits.any, [&](auto asks) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (marked) {
-            if (!m.in(a, t + u)) {
-                reset = true;
+        for (int u = 0; u < U; u++) {
+            const bool in = !asks || (bits.in >> u & 1);
+            if (asks && (bits.first >> u & 1)) state_of(a.state, m.begins(a, t + u), B);
+            float xv[L];
+            xs[u].get(xv);
 #pragma unroll
-                for (int k = 0; k < L; k++) B[k] = 0.f;
-                continue;
-            }
-            const int64_t s = m.begins(a, t + u);
-            if (s >= 0) {
-                reset = true;
-                first_state(a.state, s, B);
+            for (int k = 0; k < L; k++) {
+                const float co = cs[kShared ? 0 : u][k];
+                A[k] *= factor<kDecay>(co);
+                B[k] = in ? step<kDecay>(B[k], xv[k], co) : 0.f;
             }
         }
-        float xv[L];
-        xs[u].get(xv);
 #pragma unroll
-        for (int k = 0; k < L; k++) {
-            const float co = cs[kShared ? 0 : u][k];
-            A[k] *= factor<kDecay>(co);
-            B[k] = step<kDecay>(B[k], xv[k], co);
+        for (int u = U - 1; u >= 0; u--) {
+            const bool on = !asks || (bits.in & ~bits.first) >> u & 1;       // what reaches the token goes on to the one before
+            if (asks && (bits.end >> u & 1)) state_of(a.dlast, m.ends(a, t + u), Q);
+            float d[L];
+            incoming(u, d);
+#pragma unroll
+            for (int k = 0; k < L; k++) Q[k] = on ? factor<kDecay>(cs[kShared ? 0 : u][k]) * (d[k] + Q[k]) : 0.f;
         }
-    }
-#pragma unroll
-    for (int u = U - 1; u >= 0; u--) {
-        bool begins = false;
-        if (marked) {
-            if (!m.in(a, t + u)) {
-                back_reset = true;
-#pragma unroll
-                for (int k = 0; k < L; k++) Q[k] = 0.f;
-                continue;
-            }
-            const int64_t s = m.ends(a, t + u);
-            if (s >= 0) {
-                back_reset = true;
-                first_state(a.dlast, s, Q);
-            }
-            begins = m.begins(a, t + u) >= 0;
-            back_reset |= begins;
-        }
-        float d[L];
-        incoming(u, d);
-#pragma unroll
-        for (int k = 0; k < L; k++) Q[k] = begins ? 0.f : factor<kDecay>(cs[kShared ? 0 : u][k]) * (d[k] + Q[k]);
-    }
-    if (lane == 0 && reset) atomicOr(&s_resets, 1u << group);
-    if (lane == 0 && back_reset) atomicOr(&s_back_resets, 1u << group);
+    });
+    if (lane == 0 && bits.resets(U)) atomicOr(&s_resets, 1u << group);
+    if (lane == 0 && (bits.resets(U) || bits.end)) atomicOr(&s_back_resets, 1u << group);
     const int slot = lane * L, mine = group * kSlots + slot;
 #pragma unroll
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; s_q[mine + k] = Q[k]; }
@@ -659,60 +629,52 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
         l[k] = s_q[mine + k];
         sum[k] = 0.f;
     }
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        if (marked) {
-            const int64_t s = m.in(a, t + u) ? m.begins(a, t + u) : -1;
-            if (s >= 0) first_state(a.state, s, h);
-        }
-        float xv[L];
-        xs[u].get(xv);
-#pragma unroll
-        for (int k = 0; k < L; k++) {
-            before[u][k] = h[k];
-            h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
-        }
-    }
     const int64_t place = (row * a.length + t) * a.dim + c0;
     raw_t *dx = a.dx ? (raw_t*)a.dx + place : nullptr, *dg = a.dgates && !kShared ? (raw_t*)a.dgates + place : nullptr;
+    by_marks(bits.any, [&](auto asks) {
 #pragma unroll
-    for (int u = U - 1; u >= 0; u--) {
-        float d[L], xv[L], by_x[L], by_g[L];
-        bool in = true;
-        if (marked) {
-            if (t + u >= m.length) continue;
-            in = m.in(a, t + u);
-            const int64_t s = in ? m.ends(a, t + u) : -1;
-            if (s >= 0) first_state(a.dlast, s, l);
-        }
-        incoming(u, d);
-        xs[u].get(xv);
+        for (int u = 0; u < U; u++) {
+            if (asks && (bits.first >> u & 1)) state_of(a.state, m.begins(a, t + u), h);
+            float xv[L];
+            xs[u].get(xv);
 #pragma unroll
-        for (int k = 0; k < L; k++) {
-            const float co = cs[kShared ? 0 : u][k], f = factor<kDecay>(co);
-            const float reaches = d[k] + l[k];
-            if (kDecay) {
-                by_x[k] = reaches;
-                by_g[k] = reaches * before[u][k];
-            } else {
-                by_x[k] = reaches * (holds(co) ? co : 1.f + co);
-                by_g[k] = by_x[k] * f * (before[u][k] - xv[k]);
+            for (int k = 0; k < L; k++) {
+                before[u][k] = h[k];
+                h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
             }
-            l[k] = f * reaches;
-            if (!in) by_x[k] = by_g[k] = l[k] = 0.f;
-            sum[k] += by_g[k];
         }
-        if (live && dx) Span<T, L>::store(dx + (int64_t)u * a.dim, by_x);
-        if (live && dg) Span<T, L>::store(dg + (int64_t)u * a.dim, by_g);
-        if (marked && in) {
-            const int64_t s = m.begins(a, t + u);
-            if (s >= 0) {
-                if (live && a.dstate) store_floats<L>(a.dstate + s * a.dim + c0, l);
+#pragma unroll
+        for (int u = U - 1; u >= 0; u--) {
+            const bool in = !asks || (bits.in >> u & 1);
+            if (asks && (bits.end >> u & 1)) state_of(a.dlast, m.ends(a, t + u), l);
+            float d[L], xv[L], by_x[L], by_g[L];
+            incoming(u, d);
+            xs[u].get(xv);
+#pragma unroll
+            for (int k = 0; k < L; k++) {
+                const float co = cs[kShared ? 0 : u][k], f = factor<kDecay>(co);
+                const float reaches = d[k] + l[k];
+                if (kDecay) {
+                    by_x[k] = in ? reaches : 0.f;
+                    by_g[k] = in ? reaches * before[u][k] : 0.f;
+                } else {
+                    by_x[k] = in ? reaches * (holds(co) ? co : 1.f + co) : 0.f;
+                    by_g[k] = in ? by_x[k] * f * (before[u][k] - xv[k]) : 0.f;
+                }
+                l[k] = in ? f * reaches : 0.f;
+                sum[k] += by_g[k];
+            }
+            if (live && (!asks || t + u < m.length)) {
+                if (dx) Span<T, L>::store(dx + (int64_t)u * a.dim, by_x);
+                if (dg) Span<T, L>::store(dg + (int64_t)u * a.dim, by_g);
+            }
+            if (asks && (bits.first >> u & 1)) {
+                if (live && a.dstate) store_floats<L>(a.dstate + m.begins(a, t + u) * a.dim + c0, l);
 #pragma unroll
                 for (int k = 0; k < L; k++) l[k] = 0.f;
             }
         }
-    }
+    });
     if (!kShared || !a.dgates) return;
     // (s_a is read by nobody any more)
 #pragma unroll

@@ -409,7 +409,7 @@ int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int
         if (out && (overlap(out, cells, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
                     overlap(out, cells, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b) || (d_dh && overlap(out, cells, d_dh, cells))))
             return refuse(who, "a gradient overlaps what it is formed from");
-    if (work_bytes < scan_work_bytes(rows, length, dim, dtype, true, true) || !d_work) return refuse(who, "workspace too small");
+    if (work_bytes < scan_work_bytes(rows, length, dim, dtype, true, true) + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     a.states = const_cast<float*>(d_states);
     a.dh = d_dh;

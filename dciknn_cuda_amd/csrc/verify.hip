@@ -36,8 +36,10 @@ __device__ inline double exp2_wide(double x) {
     const double y = __builtin_ldexp(p, (int)__builtin_fmax(n, -2000.0));
     return x < -1100.0 ? 0.0 : y;
 }
-// The weight of an entry beside the largest (m2 = m c2, of a finite m).
-__device__ inline double weight_of(float z, double c2, double m2) { return exp2_wide(__builtin_fma((double)z, c2, -m2)); }
+// The weight of an entry beside the largest.  The difference is formed before the factor: of the type's lowest values it is exact.
+__device__ inline double weight_of(float z, double c2, double m) { return exp2_wide(((double)z - m) * c2); }
+// What weights are relative to, for a row of nothing but -inf too.
+__device__ inline double base_of(float m) { return (double)(m == kNoLogit ? 0.f : m); }
 
 __device__ inline double lanes_sum(double v) {
 #pragma unroll
@@ -76,14 +78,14 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
             for (int k = 0; k < P::kLen; k++) m = fmaxf(m, z[k]);
         }
         m = max_of_lanes(m);
-        const double m2 = (double)(m == kNoLogit ? 0.f : m) * a.c2;
+        const double base = base_of(m);
         double s = 0.0;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float z[P::kLen];
             P::unpack(raw[u], z);
 #pragma unroll
-            for (int k = 0; k < P::kLen; k++) s += weight_of(z[k], a.c2, m2);
+            for (int k = 0; k < P::kLen; k++) s += weight_of(z[k], a.c2, base);
         }
         s = lanes_sum(s);
         if (lane == 0) sums[row * chunks + c] = Sum{s, m, 0.f};
@@ -145,11 +147,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         float m = kNoLogit;
         for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, part[c].m);
         m = max_of_lanes(m);
-        const double m2 = (double)(m == kNoLogit ? 0.f : m) * c2;
+        const double base = base_of(m);
         double s = 0.0;
         for (int c = lane; c < chunks; c += kWave) {
             const Sum p = part[c];
-            s += p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, m2);
+            s += p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
         }
         s = lanes_sum(s);
         if (lane == 0) {
@@ -166,11 +168,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             for (int j = lane; j < a.slots; j += kWave)
                 if (id_at(a.slot_ids, a.wide_slots, at + j) >= 0) top = fmaxf(top, teacher_at(a, at + j));
             top = max_of_lanes(top);
-            const double top2 = (double)(top == kNoLogit ? 0.f : top) * kLog2eWide;
+            const double top_base = base_of(top);
             double all = 0.0, its = 0.0;
             for (int j = lane; j < a.slots; j += kWave) {
                 const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
-                const double w = id < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top2);
+                const double w = id < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top_base);
                 all += w;
                 its += id == t ? w : 0.0;
             }
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             q = all == 0.0 ? 0.0 : its / all;
         }
         if (lane == 0) {
-            const double p = t < a.vocab ? weight_of((float)logits[i * a.stride + t], c2, m2) : 0.0;
+            const double p = t < a.vocab ? weight_of((float)logits[i * a.stride + t], c2, base) : 0.0;
             s_kept[i] = p > 0.0 && (double)a.uniforms[b * (k + 1) + i] * q * s < p;
         }
     }
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
     int kept = 0;
     while (kept < given && s_kept[kept]) kept++;
     // row `kept` names the next token
-    const double total = s_total[kept], m2 = (double)(s_max[kept] == kNoLogit ? 0.f : s_max[kept]) * c2;
+    const double total = s_total[kept], base = base_of(s_max[kept]);
     const typename T::raw* row = logits + kept * a.stride;
     const Sum* part = sums + (b * (k + 1) + kept) * chunks;
     bool fine = total > 0.0 && total < __builtin_huge_val();
@@ -214,10 +216,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             if (lane == 0) s_part[wave] = top;
             __syncthreads();
             for (int w = 0; w < kWaves; w++) top = fmaxf(top, (float)s_part[w]);
-            const double top2 = (double)(top == kNoLogit ? 0.f : top) * kLog2eWide;
+            const double top_base = base_of(top);
             double all = 0.0;
             for (int j = tid; j < slots; j += kThreads) {
-                const double w = s_id[j] < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top2);
+                const double w = s_id[j] < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top_base);
                 s_gone[j] = w;
                 all += w;
             }
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
     }
     __syncthreads();
     auto less = [&](int j) {           // what entry s_id[j] weighs less than in p
-        const double w = weight_of((float)row[s_id[j]], c2, m2);
+        const double w = weight_of((float)row[s_id[j]], c2, base);
         return w - max(w - s_gone[j], 0.0);
     };
     const float u = a.uniforms[b * (k + 1) + k];
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
     const int each = (chunks + kThreads - 1) / kThreads, begin = min(chunks, tid * each), end = min(chunks, begin + each);
     auto chunk_sum = [&](int c) {
         const Sum p = part[c];
-        double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, m2);
+        double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
         for (int j = 0; j < slots; j++)
             if (s_id[j] >= 0 && s_id[j] / kChunk == c) s -= less(j);
         return max(s, 0.0);
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
 #pragma unroll
             for (int e = 0; e < kPer; e++) {
                 const int i = e * kThreads + tid;
-                s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, m2) : 0.0;
+                s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, base) : 0.0;
             }
             __syncthreads();
             for (int j = tid; j < slots; j += kThreads)
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         const int64_t t = i < kept ? draft_at(i) : i == kept ? token : -1;
         float logp = 0.f;
         if (i <= kept) {
-            if (t >= 0) logp = (float)(((double)(float)logits[i * a.stride + t] * c2 - (double)s_max[i] * c2) * 0.693147180559945309417 - log(s_total[i]));
+            if (t >= 0) logp = (float)(((double)(float)logits[i * a.stride + t] - (double)s_max[i]) * c2 * 0.693147180559945309417 - log(s_total[i]));
             else logp = __builtin_nanf("");
         }
         a.tokens[b * (k + 1) + i] = (int32_t)t;
