@@ -15,29 +15,49 @@ namespace dcih {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSpans = 120;                     // of a launch: 3.8 KB of arguments
-constexpr int64_t kMinUnit = 2048, kMaxUnit = 65536;     // elements that a workgroup takes
-constexpr int64_t kUnits = 4096;                // in all, where units are not the largest yet
+constexpr int kRead = 240, kWritten = 160;      // spans of a launch: 3.9 KB of arguments
+constexpr int64_t kMinUnit = 2048, kMaxUnit = 65536;     // elements that a workgroup takes at a time
+constexpr int64_t kUnits = 8192;                // in all, where units are not the largest yet
 constexpr int64_t kFewSums = kThreads;          // up to here every workgroup joins the sums itself
+constexpr int64_t kMaxSpan = (int64_t)1 << 31;  // elements of an entry: longer spans are several
 constexpr int64_t kMaxGrid = 1 << 23;
+constexpr uint32_t kBlocks = 2048;              // workgroups of a launch that writes
 
-struct Table {
-    const void* in[kSpans];
-    void* out[kSpans];
-    int64_t count[kSpans];
-    uint32_t first[kSpans];                     // a span's first unit of the launch
-    uint8_t types[kSpans];                      // 3 * type + type of what is written
+// Where spans lie. A type is kept beside the address, which has 57 bits.
+struct Place {
+    uint64_t bits;
+    __host__ void set(const void* p, int dtype) { bits = (uint64_t)(uintptr_t)p | (uint64_t)dtype << 60; }
+    __device__ int dtype() const { return (int)(bits >> 60); }
+    template <class T> __device__ typename T::raw* at(int64_t i) const { return (typename T::raw*)(uintptr_t)(bits & ((1ull << 60) - 1)) + i; }
+};
+struct Entry { Place in; uint32_t count, first; };          // `first`: the first unit of the launch
+struct ReadTable {
     int spans;
-    uint32_t units;
-    int64_t unit;                               // elements
+    uint32_t units, unit;
+    Entry e[kRead];
+    __host__ void set(int i, const void* data, int dtype, const void*, int) { e[i].in.set(data, dtype); }
+    static constexpr int kRoom = kRead;
+};
+struct WriteTable {
+    int spans;
+    uint32_t units, unit;
+    bool moves;                 // something is written to another place
+    Entry e[kWritten];
+    Place out[kWritten];
+    __host__ void set(int i, const void* data, int dtype, void* to, int out_dtype) {
+        e[i].in.set(data, dtype);
+        out[i].set(to, out_dtype);
+        moves = (i && moves) || e[i].in.bits != out[i].bits;
+    }
+    static constexpr int kRoom = kWritten;
 };
 
 // The span of a unit: the last that begins at it or before.
-__device__ inline int span_of(const Table& t, uint32_t unit) {
+template <class Table> __device__ inline int span_of(const Table& t, uint32_t unit) {
     int lo = 0, hi = t.spans;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (t.first[mid] <= unit) lo = mid;
+        if (t.e[mid].first <= unit) lo = mid;
         else hi = mid;
     }
     return lo;
@@ -84,16 +104,16 @@ template <class T> __device__ double squares(const typename T::raw* p, int64_t n
 }
 
 // One pass over all gradients, bound by memory.
-__global__ __launch_bounds__(kThreads) void squares_kernel(Table t, double* sums) {
+__global__ __launch_bounds__(kThreads) void squares_kernel(ReadTable t, double* sums) {
     __shared__ double s_part[kThreads / kWave];
     const uint32_t unit = blockIdx.x;
-    const int i = span_of(t, unit);
-    const int64_t from = (int64_t)(unit - t.first[i]) * t.unit, n = min(t.unit, t.count[i] - from);
+    const Entry e = t.e[span_of(t, unit)];
+    const int64_t from = (int64_t)(unit - e.first) * t.unit, n = min((int64_t)t.unit, (int64_t)e.count - from);
     double sum;
-    switch (t.types[i] / 3) {
-        case DCIH_F32: sum = squares<F32>((const float*)t.in[i] + from, n); break;
-        case DCIH_F16: sum = squares<F16>((const _Float16*)t.in[i] + from, n); break;
-        default: sum = squares<BF16>((const __bf16*)t.in[i] + from, n);
+    switch (e.in.dtype()) {
+        case DCIH_F32: sum = squares<F32>(e.in.at<F32>(from), n); break;
+        case DCIH_F16: sum = squares<F16>(e.in.at<F16>(from), n); break;
+        default: sum = squares<BF16>(e.in.at<BF16>(from), n);
     }
     sum = sum_of_threads(sum, s_part);
     if (threadIdx.x == 0) sums[unit] = sum;
@@ -114,54 +134,56 @@ __global__ __launch_bounds__(1024) void norm_kernel(double* sums, int64_t n, dou
     *norm = (float)(sqrt(sum) * scale);
 }
 
+// L elements in the place of L others: 16 bytes of what is written, so that a wavefront's stores are whole lines.
 template <class T, class O> __device__ void scaled(const typename T::raw* p, typename O::raw* out, int64_t n, float factor) {
-    using P = Piece<T>;
-    constexpr int U = 8, L = P::kLen, K = Piece<O>::kLen;
+    constexpr int U = 8, L = Piece<O>::kLen;
+    typedef typename T::raw in_vec __attribute__((ext_vector_type(L)));
+    typedef in_vec in_vec_any __attribute__((aligned(sizeof(typename T::raw))));
+    typedef float float_vec __attribute__((ext_vector_type(L)));
     const int64_t pieces = n / L;
-    auto put = [&](int64_t i, u32x4 x) {
+    auto get = [&](int64_t i) -> in_vec { return *(const in_vec_any*)(p + i * L); };
+    auto put = [&](int64_t i, in_vec x) {
+        const float_vec y = __builtin_convertvector(x, float_vec) * factor;
         float z[L];
-        P::unpack(x, z);
 #pragma unroll
-        for (int k = 0; k < L; k++) z[k] *= factor;
-#pragma unroll
-        for (int k = 0; k < L; k += K) {
-            float y[K];
-#pragma unroll
-            for (int j = 0; j < K; j++) y[j] = z[k + j];
-            Piece<O>::store_once(out + i * L + k, Piece<O>::pack(y));
-        }
+        for (int k = 0; k < L; k++) z[k] = y[k];
+        Piece<O>::store_once(out + i * L, Piece<O>::pack(z));
     };
     int64_t i = threadIdx.x;
     for (; i + (U - 1) * kThreads < pieces; i += U * kThreads) {
-        u32x4 x[U];
+        in_vec x[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) x[u] = P::load(p + (i + u * kThreads) * L);
+        for (int u = 0; u < U; u++) x[u] = get(i + u * kThreads);
 #pragma unroll
         for (int u = 0; u < U; u++) put(i + u * kThreads, x[u]);
     }
-    for (; i < pieces; i += kThreads) put(i, P::load(p + i * L));
+    for (; i < pieces; i += kThreads) put(i, get(i));
     const int64_t rest = pieces * L + threadIdx.x;
     if (rest < n) out[rest] = (typename O::raw)((float)p[rest] * factor);
 }
 
-// The last units first: what the sums read last is in the caches still.  Where nothing is clipped or scaled and the
+// The tables come in reverse: what the sums read last is in the caches still.  Where nothing is clipped or scaled and the
 // gradients stay in their place there is nothing to do.
-__global__ __launch_bounds__(kThreads) void clip_kernel(Table t, const double* sums, int64_t n, bool joined, double scale, double max_norm, float* norm) {
+__global__ __launch_bounds__(kThreads) void clip_kernel(WriteTable t, const double* sums, int64_t n, bool joined, double scale, double max_norm, float* norm) {
     __shared__ double s_part[kThreads / kWave];
     const double total = (joined ? sums[n] : sum_of(sums, n, s_part)), length = sqrt(total) * fabs(scale);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)length;
     // (a norm that is no number, or infinite as it is returned, clips nothing)
     const float factor = (float)(length > max_norm && (float)length < __builtin_huge_valf() ? max_norm / length * scale : scale);
-    const uint32_t unit = t.units - 1 - blockIdx.x;
-    const int i = span_of(t, unit);
-    if (factor == 1.f && t.in[i] == t.out[i]) return;
-    const int64_t from = (int64_t)(unit - t.first[i]) * t.unit, left = min(t.unit, t.count[i] - from);
-    switch (t.types[i]) {
-        case 3 * DCIH_F32 + DCIH_F32: scaled<F32, F32>((const float*)t.in[i] + from, (float*)t.out[i] + from, left, factor); break;
-        case 3 * DCIH_F16 + DCIH_F16: scaled<F16, F16>((const _Float16*)t.in[i] + from, (_Float16*)t.out[i] + from, left, factor); break;
-        case 3 * DCIH_F16 + DCIH_F32: scaled<F16, F32>((const _Float16*)t.in[i] + from, (float*)t.out[i] + from, left, factor); break;
-        case 3 * DCIH_BF16 + DCIH_F32: scaled<BF16, F32>((const __bf16*)t.in[i] + from, (float*)t.out[i] + from, left, factor); break;
-        default: scaled<BF16, BF16>((const __bf16*)t.in[i] + from, (__bf16*)t.out[i] + from, left, factor);
+    if (factor == 1.f && !t.moves) return;
+    for (uint32_t unit = blockIdx.x; unit < t.units; unit += gridDim.x) {
+        const int i = span_of(t, unit);
+        const Entry e = t.e[i];
+        const Place out = t.out[i];
+        if (factor == 1.f && e.in.bits == out.bits) continue;
+        const int64_t from = (int64_t)(unit - e.first) * t.unit, left = min((int64_t)t.unit, (int64_t)e.count - from);
+        switch (3 * e.in.dtype() + out.dtype()) {
+            case 3 * DCIH_F32 + DCIH_F32: scaled<F32, F32>(e.in.at<F32>(from), out.at<F32>(from), left, factor); break;
+            case 3 * DCIH_F16 + DCIH_F16: scaled<F16, F16>(e.in.at<F16>(from), out.at<F16>(from), left, factor); break;
+            case 3 * DCIH_F16 + DCIH_F32: scaled<F16, F32>(e.in.at<F16>(from), out.at<F32>(from), left, factor); break;
+            case 3 * DCIH_BF16 + DCIH_F32: scaled<BF16, F32>(e.in.at<BF16>(from), out.at<F32>(from), left, factor); break;
+            default: scaled<BF16, BF16>(e.in.at<BF16>(from), out.at<BF16>(from), left, factor);
+        }
     }
 }
 
@@ -176,51 +198,44 @@ int64_t unit_for(const dcih_span* spans, int64_t n, int64_t& units) {
     }
 }
 
-// Calls `launch` with tables of the spans in order, or in reverse.
-template <class Launch>
+// Calls `launch` with tables of the spans in order, or with the same ones from the last to the first.
+template <class Table, class Launch>
 int by_tables(const dcih_span* spans, int64_t n, int64_t unit, bool reverse, Launch launch) {
-    int64_t before = 0, all = 0;
-    for (int64_t i = 0; i < n; i++) all += units_of(spans[i].count, unit);
+    // (parts of spans: of kMaxSpan elements each but the last)
+    auto parts_of = [&](int64_t i) { return (spans[i].count + kMaxSpan - 1) / kMaxSpan; };
+    int64_t i = reverse ? n - 1 : 0, part = reverse && n ? parts_of(i) - 1 : 0, before = 0;
+    auto more = [&] { return reverse ? i >= 0 : i < n; };
+    auto next = [&] {
+        if (reverse) {
+            if (--part < 0 && --i >= 0) part = parts_of(i) - 1;
+        } else if (++part >= parts_of(i)) {
+            i++;
+            part = 0;
+        }
+    };
     Table t;
-    t.unit = unit;
-    t.spans = 0;
-    t.units = 0;
-    auto flush = [&](int64_t at) {
-        const int rc = t.spans ? launch(t, at) : 0;
+    t.unit = (uint32_t)unit;
+    while (more()) {
         t.spans = 0;
         t.units = 0;
-        return rc;
-    };
-    // (a table holds spans [from, to) in ascending order in both directions)
-    int64_t from = 0, to = reverse ? n : 0;
-    while (reverse ? to > 0 : from < n) {
-        if (reverse) {
-            from = to;
-            for (int taken = 0; from > 0 && taken < kSpans; ) taken += spans[--from].count > 0;
-        } else {
-            to = from;
-            for (int taken = 0; to < n && taken < kSpans; ) taken += spans[to++].count > 0;
+        for (; more() && t.spans < Table::kRoom; next()) {
+            if (part < 0 || part >= parts_of(i)) continue;          // an empty span
+            const int64_t from = part * kMaxSpan, count = std::min(kMaxSpan, spans[i].count - from);
+            t.set(t.spans, (const char*)spans[i].data + from * type_bytes(spans[i].dtype), spans[i].dtype,
+                  (char*)spans[i].out + from * type_bytes(spans[i].out_dtype), spans[i].out_dtype);
+            t.e[t.spans].count = (uint32_t)count;
+            t.e[t.spans++].first = t.units;
+            t.units += (uint32_t)units_of(count, unit);
         }
-        for (int64_t i = from; i < to; i++) {
-            if (!spans[i].count) continue;
-            t.in[t.spans] = spans[i].data;
-            t.out[t.spans] = spans[i].out;
-            t.count[t.spans] = spans[i].count;
-            t.types[t.spans] = (uint8_t)(3 * spans[i].dtype + spans[i].out_dtype);
-            t.first[t.spans++] = t.units;
-            t.units += (uint32_t)units_of(spans[i].count, unit);
-        }
-        const int64_t taken = t.units;
-        if (int rc = flush(reverse ? all - before - taken : before)) return rc;
-        before += taken;
-        if (reverse) to = from;
-        else from = to;
+        if (t.spans)
+            if (int rc = launch(t, before)) return rc;
+        before += t.units;
     }
     return 0;
 }
 
 int sum_up(const dcih_span* spans, int64_t n, int64_t unit, double* sums, hipStream_t s) {
-    return by_tables(spans, n, unit, false, [&](const Table& t, int64_t at) {
+    return by_tables<ReadTable>(spans, n, unit, false, [&](const ReadTable& t, int64_t at) {
         squares_kernel<<<t.units, kThreads, 0, s>>>(t, sums + at);
         DCIH_HIP(hipGetLastError());
         return 0;
@@ -263,8 +278,8 @@ int clip_grads(const dcih_span* spans, int64_t n, double max_norm, double scale,
     if (joined)
         if (int rc = join(sums, units, scale, norm, s)) return rc;
     bool first = !joined;
-    return by_tables(spans, n, unit, true, [&](const Table& t, int64_t) {
-        clip_kernel<<<t.units, kThreads, 0, s>>>(t, sums, units, joined, scale, max_norm, first ? norm : nullptr);
+    return by_tables<WriteTable>(spans, n, unit, true, [&](const WriteTable& t, int64_t) {
+        clip_kernel<<<std::min(t.units, kBlocks), kThreads, 0, s>>>(t, sums, units, joined, scale, max_norm, first ? norm : nullptr);
         DCIH_HIP(hipGetLastError());
         first = false;
         return 0;
