@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kRead = 240, kWritten = 160;      // spans of a launch: 3.9 KB of arguments
-constexpr int64_t kMinUnit = 2048, kMaxUnit = 65536;     // elements that a workgroup takes at a time
+constexpr int64_t kMaxUnit = 65536;             // elements that a workgroup takes at a time, 2048 at least
 constexpr int64_t kUnits = 8192;                // in all, where units are not the largest yet
 constexpr int64_t kFewSums = kThreads;          // up to here every workgroup joins the sums itself
 constexpr int64_t kMaxSpan = (int64_t)1 << 31;  // elements of an entry: longer spans are several
@@ -189,13 +189,15 @@ __global__ __launch_bounds__(kThreads) void clip_kernel(WriteTable t, const doub
 
 int64_t units_of(int64_t count, int64_t unit) { return (count + unit - 1) / unit; }
 
-// Elements of a unit: as few as give no more than kUnits of them.
+// Elements of a unit, a power of two: as few as give no more than about kUnits of them.
 int64_t unit_for(const dcih_span* spans, int64_t n, int64_t& units) {
-    for (int64_t unit = kMinUnit;; unit *= 2) {
-        units = 0;
-        for (int64_t i = 0; i < n; i++) units += units_of(spans[i].count, unit);
-        if (units <= kUnits || unit == kMaxUnit) return unit;
-    }
+    int64_t all = 0;
+    for (int64_t i = 0; i < n; i++) all += spans[i].count;
+    int bits = 11;
+    while (((int64_t)1 << bits) < kMaxUnit && (all >> bits) + n > kUnits) bits++;
+    units = 0;
+    for (int64_t i = 0; i < n; i++) units += (spans[i].count + ((int64_t)1 << bits) - 1) >> bits;
+    return (int64_t)1 << bits;
 }
 
 // Calls `launch` with tables of the spans in order, or with the same ones from the last to the first.

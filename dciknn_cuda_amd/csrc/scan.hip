@@ -22,14 +22,19 @@ namespace dcih {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kLanes = 16;                         // pieces of 16 bytes that a tile is wide
+constexpr int kLanes = 8;                          // pieces of 16 bytes that a tile is wide: a line
 constexpr int kTile = 128;                         // tokens of a tile
+constexpr int kWaves = 4, kBackWaves = 3;          // of a SIMD: registers enough for a tile, tiles enough to hide one another's waits
 constexpr int kShort = 16;                         // tokens that one thread takes
 constexpr int64_t kMaxGrid = 1 << 23;
 constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
 constexpr uint32_t kMapSet = 1, kStateSet = 2;
 
 typedef uint32_t u32x4_float __attribute__((ext_vector_type(4), aligned(4)));
+
+// Makes the compiler take a register's contents for others: what was computed from it before is computed again, not kept in more
+// registers from one loop over a group's tokens to the next.
+template <class V> __device__ __forceinline__ void renew(V& v) { asm volatile("" : "+v"(v)); }
 
 // L elements of a row: a 16-byte piece, or (L = 1, rows shorter than that) one.
 template <class T, int L> struct Span {
@@ -41,6 +46,8 @@ template <class T, int L> struct Span {
         bits = P::load_once(p);
     }
     __device__ void get(float (&z)[L]) const { P::unpack(bits, z); }
+    __device__ void clear() { bits = u32x4{0, 0, 0, 0}; }
+    __device__ void renew() { dcih::renew(bits); }
     __device__ static void store(raw_t* p, const float (&z)[L]) { P::store_once(p, P::pack(z)); }
 };
 template <class T> struct Span<T, 1> {
@@ -48,6 +55,8 @@ template <class T> struct Span<T, 1> {
     raw_t bits;
     __device__ void load(const raw_t* p) { bits = *p; }
     __device__ void get(float (&z)[1]) const { z[0] = (float)bits; }
+    __device__ void clear() { bits = (raw_t)0.f; }
+    __device__ void renew() {}
     __device__ static void store(raw_t* p, const float (&z)[1]) { *p = (raw_t)z[0]; }
 };
 
@@ -79,35 +88,46 @@ template <int L> __device__ inline void store_floats(float* p, const float (&z)[
     }
 }
 
-// What a gate is kept as: 1 - a where a is 1/2 or more, else -a (told apart by the sign, of zeros too).  The smaller of the
-// two is the one to round: with a alone, a channel that forgets over 1000 tokens would be off by 6e-5.  Exponent with
-// its product's rounding made good.
-__device__ inline float gate_of(float g) {
-    float y = -__builtin_fabsf(g);
-    y = y < -150.f ? -150.f : y;                      // (nothing is left there; NaN stays)
-    const float t = y * kLog2e;
-    const float rest = __builtin_fmaf(y, 1.92596299e-8f, __builtin_fmaf(y, kLog2e, -t));
-    float e = exp2_fast(t);
-    e = __builtin_fmaf(e * kLn2, rest, e);
-    return __builtin_copysignf(e * __builtin_amdgcn_rcpf(1.f + e), g);
-}
-__device__ inline bool holds(float c) { return __builtin_bit_cast(int, c) >= 0; }
-
-template <bool kDecay> __device__ inline float factor(float c) {          // a
-    if (kDecay) return c;
-    return holds(c) ? 1.f - c : -c;
-}
-template <bool kDecay> __device__ inline float step(float h, float x, float c) {
-    if (kDecay) return __builtin_fmaf(c, h, x);
-    return __builtin_fmaf(c, x - h, holds(c) ? h : x);       // h + (1 - a) (x - h), or x + a (h - x)
-}
-template <class T, int L, bool kDecay> __device__ inline void coefs_of(const Span<T, L>& s, float (&c)[L]) {
-    s.get(c);
-    if (!kDecay) {
-#pragma unroll
-        for (int k = 0; k < L; k++) c[k] = gate_of(c[k]);
+// e^-|g|.  log2(e) in two parts, the first of so few bits that its product with 16-bit types is exact.
+template <class T> __device__ inline float exp_below(float g) {
+    const float y = -__builtin_fabsf(g);
+    if constexpr (sizeof(typename T::raw) == 2) {
+        constexpr float kHigh = std::is_same<T, BF16>::value ? 47274.f / 32768.f : 5909.f / 4096.f;
+        constexpr float kRest = (float)((1.44269504088896340736 - kHigh) * 0.693147180559945309417);
+        const float e = exp2_fast(y * kHigh);
+        return __builtin_fmaf(e, fmaxf(y * kRest, -1.f), e);        // (0 for y = -inf, NaN for NaN)
+    } else {
+        const float z = y < -150.f ? -150.f : y;                    // (nothing is left there; NaN stays)
+        const float t = z * kLog2e, rest = __builtin_fmaf(z, 1.92596299e-8f, __builtin_fmaf(z, kLog2e, -t));
+        const float e = exp2_fast(t);
+        return __builtin_fmaf(e * kLn2, rest, e);
     }
 }
+
+// a and 1 - a of a gate.  The smaller of the two is computed, the other is what is missing to 1: a channel that forgets over
+// thousands of tokens keeps the digits of 1 - a.
+struct Gate { float a, keep; };
+template <class T> __device__ inline float lesser_of(float g) {
+    const float e = exp_below<T>(g);
+    return e * __builtin_amdgcn_rcpf(1.f + e);
+}
+__device__ inline Gate gate_by(float small, float sign) {
+    const float big = 1.f - small;
+    const bool holds = __builtin_bit_cast(int, sign) >= 0;
+    return Gate{holds ? big : small, holds ? small : big};
+}
+// A token's factor of the state and what is added to it, of a gate and an input.
+template <class T, bool kDecay> __device__ inline Gate coefs_of(float g) {
+    if (kDecay) return Gate{g, 1.f};
+    return gate_by(lesser_of<T>(g), g);
+}
+// Where one register has to do: the smaller one with the gate's sign (decays as they are).
+template <class T, bool kDecay> __device__ inline float packed_of(float g) { return kDecay ? g : __builtin_copysignf(lesser_of<T>(g), g); }
+template <bool kDecay> __device__ inline Gate coefs_of(float packed) {
+    if (kDecay) return Gate{packed, 1.f};
+    return gate_by(__builtin_fabsf(packed), packed);
+}
+template <bool kDecay> __device__ inline float step(float h, float x, Gate c) { return __builtin_fmaf(c.a, h, kDecay ? x : c.keep * x); }
 
 // ---- one thread a channel ----------------------------------------------------------------
 // A server's step, or its drafts: few tokens of many sequences.  The state may be written where it is read.
@@ -141,10 +161,10 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
             const bool in = t0 + u < len;
             float xv[L], c[L], y[L];
             xs[u].get(xv);
-            coefs_of<T, L, kDecay>(gs[u], c);
+            gs[u].get(c);
 #pragma unroll
             for (int k = 0; k < L; k++) {
-                const float next = step<kDecay>(h[k], xv[k], c[k]);
+                const float next = step<kDecay>(h[k], xv[k], coefs_of<T, kDecay>(c[k]));
                 h[k] = in ? next : h[k];
                 y[k] = in ? next : 0.f;
             }
@@ -170,12 +190,12 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
 }
 
 // ---- tiles -------------------------------------------------------------------------------
-// A chain is a strip of kLanes pieces of one row of tokens; its tiles follow one another.  Blocks take the tiles of a chain by its
-// counter, so that a tile waits for none that is not running.
+// A chain is a strip of kLanes pieces of one row of tokens; its tiles follow one another.  Workgroups take tiles by counters, those of a
+// chain in order: what a tile waits for was taken before it, by a workgroup that waits for nothing taken later.
 struct Chains {
     int pieces, strips, slots;         // pieces of a row; strips of them; channels of a strip, those beyond the row included
     int64_t tiles, count;              // tiles of a chain, chains
-    uint32_t *tickets, *flags;         // [count]; [count][tiles] what is set: a hint of what to wait for
+    uint32_t *tickets, *flags;         // what was taken; [count][tiles] what is set: a hint of what to wait for
     uint64_t* maps;                    // [count][tiles][slots] (A, B)
     uint32_t* states;                  // [count][tiles][slots] the state behind a tile
     float* sums;                       // [count][tiles][slots] (gradient of shared gates)
@@ -186,7 +206,7 @@ int span_len(int dim, int dtype) {
     return dim >= len ? len : 1;
 }
 
-__host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t length, int dim, int dtype, bool shared) {
+__host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t length, int dim, int dtype, bool gradient, bool shared) {
     const int len = span_len(dim, dtype);
     c.pieces = (dim + len - 1) / len;
     c.strips = (c.pieces + kLanes - 1) / kLanes;
@@ -204,7 +224,7 @@ __host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t leng
     c.flags = (uint32_t*)take(chained * c.count * c.tiles * 4);
     c.maps = (uint64_t*)take(chained * cells * 8);
     c.states = (uint32_t*)take(chained * cells * 4);
-    c.sums = (float*)take(shared ? cells * 4 : 0);
+    c.sums = (float*)take(gradient && shared ? cells * 4 : 0);
     return at;
 }
 
@@ -217,35 +237,39 @@ __global__ __launch_bounds__(kThreads) void copy_kernel(const float* from, float
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) to[i] = from ? from[i] : 0.f;
 }
 
-// Sequences without tokens: what reaches their end is what they began with.
-__global__ __launch_bounds__(kThreads) void empty_kernel(ScanArgs a, const float* from, float* to, int64_t first) {
-    const int64_t s = first + blockIdx.x;
-    bool empty;
-    if (a.form == kPacked) {
-        const int64_t lo = min(max(id_of_all(a.bounds, a.wide_bounds, s), (int64_t)0), a.length);
-        const int64_t hi = min(max(id_of_all(a.bounds, a.wide_bounds, s + 1), (int64_t)0), a.length);
-        empty = hi <= lo;
-    } else {
-        empty = id_of_all(a.bounds, a.wide_bounds, s) <= 0;
+// Sequences without tokens: what reaches their end is what they began with.  By workgroups of their own behind those of the tiles.
+constexpr int kEmpty = 16;                          // sequences of a workgroup, up to kEmptyGrid workgroups
+constexpr int64_t kEmptyGrid = 4096;
+__device__ inline void pass_empty(const ScanArgs& a, int64_t block, int64_t blocks, const float* from, float* to) {
+    const int waves = kThreads / kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (int64_t s = block * waves + wave; s < a.sequences; s += blocks * waves) {
+        int64_t lo = 0, hi = id_of_all(a.bounds, a.wide_bounds, a.form == kPacked ? s + 1 : s);
+        if (a.form == kPacked) lo = max(id_of_all(a.bounds, a.wide_bounds, s), (int64_t)0);
+        if (a.form == kPacked) hi = min(hi, a.length);
+        if (hi > lo) continue;
+        for (int c = lane_id(); c < a.dim; c += kWave) to[s * a.dim + c] = from ? from[s * a.dim + c] : 0.f;
     }
-    if (!empty) return;
-    for (int c = threadIdx.x; c < a.dim; c += kThreads) to[s * a.dim + c] = from ? from[s * a.dim + c] : 0.f;
 }
 
 __device__ inline uint32_t peek(const uint32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ inline uint64_t peek(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class V> __device__ inline void post(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
 __device__ inline uint32_t word_of(float v) {
     const uint32_t w = __builtin_bit_cast(uint32_t, v);
     return w == kUnset ? 0x7fc00000u : w;
 }
 
-// Which tile of its chain a workgroup takes, counted in the direction of the scan.
-__device__ inline int64_t take_tile(const Chains& c, int64_t chain, uint32_t& s_ticket) {
-    if (c.tiles == 1) return 0;
-    if (threadIdx.x == 0) s_ticket = atomicAdd(&c.tickets[chain], 1u) - kUnset;       // the counter begins at kUnset
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(s_ticket);
+// Item i of all is the next tile of a chain, in the direction of the scan, and each chain has as many items as tiles.  Neighbouring
+// items, which run on different XCDs, are neighbouring strips, and from one round to the next the strips go on by one: an XCD that always
+// had the same ones would use a few of its cache's channels only.  By one thread; returns chain * tiles + place.
+__device__ inline int64_t take_tile(const Chains& c, int64_t i) {
+    if (c.tiles == 1) return i;
+    const int64_t round = i / c.count, at = i - round * c.count, row = at / c.strips;
+    const int64_t chain = row * c.strips + (at - row * c.strips + round) % c.strips;
+    return chain * c.tiles + (atomicAdd(&c.tickets[chain], 1u) - kUnset);        // the counter begins at kUnset
 }
 
 // The state that enters tile `at` of a chain in channel `slot`.  A tile posts its map as soon as it has it, and the state
@@ -254,40 +278,48 @@ __device__ inline int64_t take_tile(const Chains& c, int64_t chain, uint32_t& s_
 // Words are waited for themselves; the flags only say which are worth a look.
 __device__ float carry_of(const Chains& c, int64_t chain, int64_t at, int slot) {
     const uint32_t* flags = c.flags + chain * c.tiles;
+    const int64_t last = (chain * c.tiles + at - 1) * c.slots + slot;
     const int lane = lane_id();
+    const int64_t tile = at - 1 - lane;
     int behind;                                     // tiles between the one whose state is there and this one
+    uint32_t w;
     for (;;) {
-        const int64_t tile = at - 1 - lane;
+        w = peek(c.states + last);
         const uint32_t f = tile >= 0 ? peek(flags + tile) : kUnset;
+        if (__all(w != kUnset)) return __builtin_bit_cast(float, w);
         const unsigned long long full = __ballot(f == kStateSet), some = __ballot(f != kUnset);
         behind = full ? __builtin_ctzll(full) : -1;
         if (full && (~some & ((1ull << behind) - 1)) == 0) break;
-        __builtin_amdgcn_s_sleep(2);
+        __builtin_amdgcn_s_sleep(1);
     }
-    const int64_t base = (chain * c.tiles + at - 1 - behind) * c.slots + slot;
-    uint32_t w;
-    while ((w = peek(c.states + base)) == kUnset) {}
-    float h = __builtin_bit_cast(float, w);
+    const int64_t base = last - (int64_t)behind * c.slots;
     const uint64_t* maps = c.maps + base + c.slots;
     constexpr int U = 8;
-    for (int i = 0; i < behind; i += U) {
-        uint64_t m[U];
+    uint64_t m[U];
+    auto load_maps = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < U; u++) m[u] = peek(maps + (int64_t)min(i + u, behind - 1) * c.slots);
+        for (int u = 0; u < U; u++) m[u] = i + u < behind ? peek(maps + (int64_t)(i + u) * c.slots) : 0;
+    };
+    load_maps(0);
+    while ((w = peek(c.states + base)) == kUnset) {}
+    float h = __builtin_bit_cast(float, w);
+    for (int i = 0; i < behind; i += U) {
+        if (i) load_maps(i);
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (i + u >= behind) break;
-            while ((uint32_t)m[u] == kUnset || (uint32_t)(m[u] >> 32) == kUnset) m[u] = peek(maps + (int64_t)(i + u) * c.slots);
-            h = __builtin_fmaf(__builtin_bit_cast(float, (uint32_t)m[u]), h, __builtin_bit_cast(float, (uint32_t)(m[u] >> 32)));
+            if (i + u < behind) {
+                while ((uint32_t)m[u] == kUnset || (uint32_t)(m[u] >> 32) == kUnset) m[u] = peek(maps + (int64_t)(i + u) * c.slots);
+                h = __builtin_fmaf(__builtin_bit_cast(float, (uint32_t)m[u]), h, __builtin_bit_cast(float, (uint32_t)(m[u] >> 32)));
+            }
         }
     }
     return h;
 }
 
 // A channel's groups joined, by one thread: map (A, B) of each in the direction of the scan, `resets` those whose result does not
-// depend on what enters.  Leaves in B what enters each group; returns what enters the tile.
+// depend on what enters.  Leaves in B what enters each group.
 template <int kGroups, bool kBack>
-__device__ float join_groups(const Chains& c, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
+__device__ void join_groups(const Chains& c, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
     auto place = [&](int g) { return (kBack ? kGroups - 1 - g : g) * c.slots + slot; };
     float in = 0.f;
     if (c.tiles > 1) {
@@ -322,7 +354,6 @@ __device__ float join_groups(const Chains& c, int64_t chain, int64_t at, int slo
         s_b[place(g)] = h;
         h = reset ? gb : __builtin_fmaf(ga, h, gb);
     }
-    return in;
 }
 
 // Where sequences begin and end among the tokens of a tile.  In groups of tokens without either, and with all of them
@@ -331,7 +362,7 @@ struct Marks {
     int64_t row, length;              // a row of tokens, and how many it has
     int64_t t0;                       // the tile's first token
     int64_t lo, hi;                   // tokens [lo, hi) of the row are of sequences
-    const int *first, *end;           // (kPacked) [kTile] the sequence that begins or ends there, -1: none
+    const int *first, *end;           // (kPacked) for each token of the tile the sequence that begins or ends there, -1: none
 
     __device__ Marks(const ScanArgs& a, int64_t row_, int64_t t0_) : row(row_), length(a.length), t0(t0_) {
         if (a.form == kFlat) length = min(length, a.total - row * a.length);
@@ -368,8 +399,9 @@ struct Marks {
     }
 };
 
-// By all threads; `s_first`, `s_end` [kTile] and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
-__device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int* s_first, int* s_end, uint32_t& s_marked) {
+// By all threads; `s_first`, `s_end` and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
+template <int kTokens>
+__device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int (&s_first)[kTokens], int (&s_end)[kTokens], uint32_t& s_marked) {
     if (a.form == kRows) {
         m.lo = 0;
         m.hi = Marks::length_of(a, m.row, a.length);
@@ -377,20 +409,22 @@ __device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int* s_f
         m.lo = 0;
         m.hi = m.length;
     } else {
-        auto bound = [&](int64_t i) { return min(max(id_at(a.bounds, a.wide_bounds, i), (int64_t)0), a.length); };
-        m.lo = bound(0);
-        m.hi = bound(a.sequences);
+        auto cut = [&](int64_t o) { return min(max(o, (int64_t)0), a.length); };
+        auto bound = [&](int64_t i) { return cut(id_at(a.bounds, a.wide_bounds, i)); };
+        auto bound_of_all = [&](int64_t i) { return cut(id_of_all(a.bounds, a.wide_bounds, i)); };
+        m.lo = bound_of_all(0);
+        m.hi = bound_of_all(a.sequences);
         m.first = s_first;
         m.end = s_end;
-        for (int i = threadIdx.x; i < kTile; i += blockDim.x) s_first[i] = s_end[i] = -1;
+        for (int i = threadIdx.x; i < kTokens; i += blockDim.x) s_first[i] = s_end[i] = -1;
         if (threadIdx.x == 0) s_marked = 0;
-        // the last sequence that begins before the tile, by 64 places of a shrinking range at a time
+        // the last sequence that begins before the tile, through the scalar cache: loads of tokens are under way, and what the
+        // vector memory answers comes in order
         int64_t from = 0, to = a.sequences;
         while (to - from > 1) {
-            const int64_t wide = (to - from + kWave - 1) / kWave, at = from + (lane_id() + 1) * wide;
-            const int n = __popcll(__ballot(at < to && bound(at) < m.t0));
-            from += n * wide;
-            to = min(to, from + wide);
+            const int64_t mid = from + (to - from) / 2;
+            if (bound_of_all(mid) < m.t0) from = mid;
+            else to = mid;
         }
         __syncthreads();
         for (int64_t s = from;; s += blockDim.x) {
@@ -398,25 +432,26 @@ __device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int* s_f
             if (mine < a.sequences) {
                 const int64_t lo = bound(mine), hi = bound(mine + 1);
                 if (hi > lo) {
-                    if (lo >= m.t0 && lo < m.t0 + kTile) {
+                    if (lo >= m.t0 && lo < m.t0 + kTokens) {
                         s_first[lo - m.t0] = (int)mine;
                         atomicOr(&s_marked, 1u << ((int)(lo - m.t0) / per));
                     }
-                    if (hi - 1 >= m.t0 && hi - 1 < m.t0 + kTile) {
+                    if (hi - 1 >= m.t0 && hi - 1 < m.t0 + kTokens) {
                         s_end[hi - 1 - m.t0] = (int)mine;
                         atomicOr(&s_marked, 1u << ((int)(hi - 1 - m.t0) / per));
                     }
                 }
             }
-            if (s + blockDim.x >= a.sequences || bound(s + blockDim.x) >= m.t0 + kTile) break;
+            if (s + blockDim.x >= a.sequences || bound_of_all(s + blockDim.x) >= m.t0 + kTokens) break;
         }
     }
 }
-// What a group of `per` tokens from `t` on has to know of them: a bit for each.  (Bits and selects, and one branch for a whole wavefront:
-// hipcc 7.2 lost a factor of A where lanes left the loop over the tokens by `continue`.)
+// What a group of `per` tokens from `t` on has to know of them, a bit for each: which are of a sequence, its first, its last.  Tokens
+// of no sequence are zeros that begin and end at zero.  (No lane leaves the loops over the tokens early: hipcc 7.2 lost a
+// factor of A there.)
 struct Bits {
     uint32_t in, first, end;
-    bool any;                         // of the wavefront's groups one has a beginning, an end, or tokens of no sequence
+    bool any;                         // some group of the wavefront has other tokens than those in the middle of a sequence
 
     __device__ Bits(const ScanArgs& a, const Marks& m, int64_t t, int per, int group, uint32_t s_marked) : in(~0u), first(0), end(0) {
         bool marked = a.form == kFlat || t < m.lo || t + per > m.hi;
@@ -432,29 +467,41 @@ struct Bits {
             end |= (uint32_t)(inside && m.ends(a, t + u) >= 0) << u;
         }
     }
-    __device__ bool resets(int per) const { return first || (~in & ((1u << per) - 1)); }
+    __device__ bool is_in(int u) const { return in >> u & 1; }
+    __device__ bool is_end(int u) const { return end >> u & 1; }
+    __device__ bool is_first(int u) const { return first >> u & 1; }
+    __device__ bool starts(int u) const { return (first | ~in) >> u & 1; }      // what comes from the token before does not enter
+    __device__ bool stops(int u) const { return (end | ~in) >> u & 1; }         // nor what comes back from the one behind
+    __device__ bool starts_any(int per) const { return (first | ~in) & ((1u << per) - 1); }
+    __device__ bool stops_any(int per) const { return (end | ~in) & ((1u << per) - 1); }
 };
 
-// Runs `body` as the wavefront has marks or not: without them nothing is asked for each token.
+// Runs `body` as the wavefront has marks or not: without them there is no branch about a token.
 template <class Body> __device__ __forceinline__ void by_marks(bool any, Body body) {
     if (any) body(std::true_type{});
     else body(std::false_type{});
 }
 
 template <class T, int L, bool kDecay, bool kShared>
-__global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, int64_t first) {
+__global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
     constexpr int kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    static_assert(kGroups <= 32, "a bit for each group");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
-    __shared__ uint32_t s_ticket, s_marked, s_resets;
+    __shared__ uint32_t s_marked, s_resets;
+    __shared__ int64_t s_item;
+    if (first + blockIdx.x >= c.count * c.tiles) return pass_empty(a, first + blockIdx.x - c.count * c.tiles, empty, a.state, a.last);
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const int64_t chain = (first + blockIdx.x) % c.count, row = chain / c.strips;
-    const int strip = (int)(chain - row * c.strips);
-    if (threadIdx.x == 0) s_resets = 0;
-    const int64_t at = take_tile(c, chain, s_ticket), t0 = at * kTile, t = t0 + group * U;
+    if (threadIdx.x == 0) {
+        s_resets = 0;
+        s_item = take_tile(c, first + blockIdx.x);
+    }
+    __syncthreads();
+    const int64_t item = uniform(s_item), chain = item / c.tiles, at = item - chain * c.tiles, row = chain / c.strips;
+    const int64_t t0 = at * kTile, t = t0 + group * U;
     Marks m(a, row, t0);
-    const int piece = strip * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
+    const int piece = (int)(chain - row * c.strips) * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
     const bool live = piece < c.pieces;
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
@@ -469,41 +516,51 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, in
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
     const Bits bits(a, m, t, U, group, s_marked);
-    auto first_state = [&](int u, float (&h)[L]) {
-        const int64_t s = m.begins(a, t + u);
+    if (bits.any)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (!bits.is_in(u)) {
+                xs[u].clear();
+                if (!kShared) gs[kShared ? 0 : u].clear();
+            }
+    auto start = [&](int u, float (&h)[L]) {
 #pragma unroll
         for (int k = 0; k < L; k++) h[k] = 0.f;
-        if (a.state) load_floats<L>(a.state + s * a.dim + c0, h);
+        if (a.state && bits.is_in(u)) load_floats<L>(a.state + m.begins(a, t + u) * a.dim + c0, h);
     };
-    // the group's map
-    float cs[kShared ? 1 : U][L], A[L], B[L];
+    // the tokens' maps, and the group's
+    float as[kShared ? 1 : U][L], bs[U][L], A[L], B[L];
 #pragma unroll
     for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; }
 #pragma unroll
-    for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
+    for (int u = 0; u < U; u++) {          // (a shared gate's are the same for every u: formed once)
+        float g[L];
+        gs[kShared ? 0 : u].get(g);
+        xs[u].get(bs[u]);
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            const Gate co = coefs_of<T, kDecay>(g[k]);
+            as[kShared ? 0 : u][k] = co.a;
+            if (!kDecay) bs[u][k] *= co.keep;
+            A[k] *= co.a;
+        }
+    }
     by_marks(bits.any, [&](auto asks) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const bool in = !asks || (bits.in >> u & 1);
-            if (asks && (bits.first >> u & 1)) first_state(u, B);
-            float xv[L];
-            xs[u].get(xv);
+            if (asks && bits.starts(u)) start(u, B);
 #pragma unroll
-            for (int k = 0; k < L; k++) {
-                const float co = cs[kShared ? 0 : u][k];
-                A[k] *= factor<kDecay>(co);
-                B[k] = in ? step<kDecay>(B[k], xv[k], co) : 0.f;
-            }
+            for (int k = 0; k < L; k++) B[k] = __builtin_fmaf(as[kShared ? 0 : u][k], B[k], bs[u][k]);
         }
     });
-    if (lane == 0 && bits.resets(U)) atomicOr(&s_resets, 1u << group);
+    if (lane == 0 && bits.starts_any(U)) atomicOr(&s_resets, 1u << group);
     const int slot = lane * L, mine = group * kSlots + slot;
 #pragma unroll
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; }
     __syncthreads();
     if (threadIdx.x < kSlots) {
-        const float in = join_groups<kGroups, false>(c, chain, at, threadIdx.x, s_resets, s_a, s_b);
-        if (a.states) a.states[(chain * c.tiles + at) * kSlots + threadIdx.x] = in;
+        join_groups<kGroups, false>(c, chain, at, threadIdx.x, s_resets, s_a, s_b);
+        if (a.states) a.states[item * kSlots + threadIdx.x] = s_b[threadIdx.x];
     }
     __syncthreads();
     if (!live) return;
@@ -514,35 +571,39 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(ScanArgs a, Chains c, in
     by_marks(bits.any, [&](auto asks) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const bool in = !asks || (bits.in >> u & 1);
-            if (asks && (bits.first >> u & 1)) first_state(u, h);
-            float xv[L];
-            xs[u].get(xv);
+            if (asks && bits.starts(u)) start(u, h);
 #pragma unroll
-            for (int k = 0; k < L; k++) h[k] = in ? step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]) : 0.f;
+            for (int k = 0; k < L; k++) h[k] = __builtin_fmaf(as[kShared ? 0 : u][k], h[k], bs[u][k]);
+            if (asks && kShared && !bits.is_in(u))            // (whatever the gate holds)
+#pragma unroll
+                for (int k = 0; k < L; k++) h[k] = 0.f;
             if (!asks || t + u < m.length) Span<T, L>::store(out + (int64_t)u * a.dim, h);
-            if (asks && (bits.end >> u & 1) && a.last) store_floats<L>(a.last + m.ends(a, t + u) * a.dim + c0, h);
+            if (asks && bits.is_end(u) && a.last) store_floats<L>(a.last + m.ends(a, t + u) * a.dim + c0, h);
         }
     });
 }
 
 // The gradient of a tile.  The states go forward from the one kept, the gradient that reaches them goes back from the tile
 // behind: its maps are s -> A s + Q of the same A.
-constexpr int kBackThreads = 512;
-
 template <class T, int L, bool kDecay, bool kShared>
-__global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first) {
-    constexpr int kGroups = kBackThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
-    static_assert(kGroups <= 32, "a bit for each group");
+__global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
+    constexpr int kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    static_assert(kGroups <= 32 && 2 * kSlots <= kThreads, "a bit for each group, threads for both directions");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
-    __shared__ uint32_t s_ticket, s_marked, s_resets, s_back_resets;
+    __shared__ uint32_t s_marked, s_resets, s_back_resets;
+    __shared__ int64_t s_item;
+    if (first + blockIdx.x >= c.count * c.tiles) return pass_empty(a, first + blockIdx.x - c.count * c.tiles, empty, a.dlast, a.dstate);
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    const int64_t chain = (first + blockIdx.x) % c.count, row = chain / c.strips;
+    if (threadIdx.x == 0) {
+        s_resets = s_back_resets = 0;
+        s_item = take_tile(c, first + blockIdx.x);
+    }
+    __syncthreads();
+    const int64_t item = uniform(s_item), chain = item / c.tiles, at = item - chain * c.tiles, row = chain / c.strips;
     const int strip = (int)(chain - row * c.strips);
-    if (threadIdx.x == 0) s_resets = s_back_resets = 0;
-    const int64_t at = take_tile(c, chain, s_ticket), tile = c.tiles - 1 - at, t0 = tile * kTile, t = t0 + group * U;
+    const int64_t tile = c.tiles - 1 - at, t0 = tile * kTile, t = t0 + group * U;
     Marks m(a, row, t0);
     const int piece = strip * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
     const bool live = piece < c.pieces;
@@ -562,48 +623,71 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
     const Bits bits(a, m, t, U, group, s_marked);
-    const bool some = a.dh != nullptr;
-    auto state_of = [&](const float* from, int64_t s, float (&h)[L]) {
+    if (bits.any)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (!bits.is_in(u)) {
+                xs[u].clear();
+                ds[u].clear();
+                if (!kShared) gs[kShared ? 0 : u].clear();
+            }
+    if (!a.dh)
+#pragma unroll
+        for (int u = 0; u < U; u++) ds[u].clear();
+    auto start = [&](int u, float (&h)[L]) {
 #pragma unroll
         for (int k = 0; k < L; k++) h[k] = 0.f;
-        if (from) load_floats<L>(from + s * a.dim + c0, h);
+        if (a.state && bits.is_in(u)) load_floats<L>(a.state + m.begins(a, t + u) * a.dim + c0, h);
     };
-    auto incoming = [&](int u, float (&d)[L]) {
-        ds[u].get(d);
+    auto stop = [&](int u, float (&l)[L]) {
 #pragma unroll
-        for (int k = 0; k < L; k++) d[k] = some ? d[k] : 0.f;
+        for (int k = 0; k < L; k++) l[k] = 0.f;
+        if (a.dlast && bits.is_in(u)) load_floats<L>(a.dlast + m.ends(a, t + u) * a.dim + c0, l);
     };
     float cs[kShared ? 1 : U][L], A[L], B[L], Q[L];
+    auto again = [&] {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            xs[u].renew();
+            ds[u].renew();
+            if (!kShared || !u)
+#pragma unroll
+                for (int k = 0; k < L; k++) renew(cs[kShared ? 0 : u][k]);
+        }
+    };
 #pragma unroll
     for (int k = 0; k < L; k++) { A[k] = 1.f; B[k] = 0.f; Q[k] = 0.f; }
 #pragma unroll
-    for (int u = 0; u < (kShared ? 1 : U); u++) coefs_of<T, L, kDecay>(gs[u], cs[u]);
-    by_marks(bits.any, [&](auto asks) {
+    for (int u = 0; u < (kShared ? 1 : U); u++) {
+        gs[u].get(cs[u]);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const bool in = !asks || (bits.in >> u & 1);
-            if (asks && (bits.first >> u & 1)) state_of(a.state, m.begins(a, t + u), B);
-            float xv[L];
-            xs[u].get(xv);
+        for (int k = 0; k < L; k++) cs[u][k] = packed_of<T, kDecay>(cs[u][k]);
+    }
+    again();
 #pragma unroll
-            for (int k = 0; k < L; k++) {
-                const float co = cs[kShared ? 0 : u][k];
-                A[k] *= factor<kDecay>(co);
-                B[k] = in ? step<kDecay>(B[k], xv[k], co) : 0.f;
-            }
+    for (int u = 0; u < U; u++) {
+        if (bits.starts(u)) start(u, B);
+        float xv[L];
+        xs[u].get(xv);
+#pragma unroll
+        for (int k = 0; k < L; k++) {
+            const Gate c = coefs_of<kDecay>(cs[kShared ? 0 : u][k]);
+            A[k] *= c.a;
+            B[k] = step<kDecay>(B[k], xv[k], c);
         }
+    }
+    again();
 #pragma unroll
-        for (int u = U - 1; u >= 0; u--) {
-            const bool on = !asks || (bits.in & ~bits.first) >> u & 1;       // what reaches the token goes on to the one before
-            if (asks && (bits.end >> u & 1)) state_of(a.dlast, m.ends(a, t + u), Q);
-            float d[L];
-            incoming(u, d);
+    for (int u = U - 1; u >= 0; u--) {
+        if (bits.stops(u)) stop(u, Q);
+        float d[L];
+        ds[u].get(d);
 #pragma unroll
-            for (int k = 0; k < L; k++) Q[k] = on ? factor<kDecay>(cs[kShared ? 0 : u][k]) * (d[k] + Q[k]) : 0.f;
-        }
-    });
-    if (lane == 0 && bits.resets(U)) atomicOr(&s_resets, 1u << group);
-    if (lane == 0 && (bits.resets(U) || bits.end)) atomicOr(&s_back_resets, 1u << group);
+        for (int k = 0; k < L; k++) Q[k] = coefs_of<kDecay>(cs[kShared ? 0 : u][k]).a * (d[k] + Q[k]);
+    }
+    again();
+    if (lane == 0 && bits.starts_any(U)) atomicOr(&s_resets, 1u << group);
+    if (lane == 0 && bits.stops_any(U)) atomicOr(&s_back_resets, 1u << group);
     const int slot = lane * L, mine = group * kSlots + slot;
 #pragma unroll
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; s_q[mine + k] = Q[k]; }
@@ -613,7 +697,7 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
         join_groups<kGroups, true>(c, chain, at, threadIdx.x, s_back_resets, s_a, s_q);
     } else if (threadIdx.x < 2 * kSlots) {
         const int own = threadIdx.x - kSlots;
-        float h = a.states[(chain * c.tiles + tile) * kSlots + own];
+        float h = tile ? a.states[(chain * c.tiles + tile) * kSlots + own] : 0.f;      // (a row begins with a sequence, or with tokens of none)
 #pragma unroll 8
         for (int i = 0; i < kGroups; i++) {
             const float ga = s_a[i * kSlots + own], gb = s_b[i * kSlots + own];
@@ -631,50 +715,40 @@ __global__ __launch_bounds__(kBackThreads) void scan_grad_kernel(ScanArgs a, Cha
     }
     const int64_t place = (row * a.length + t) * a.dim + c0;
     raw_t *dx = a.dx ? (raw_t*)a.dx + place : nullptr, *dg = a.dgates && !kShared ? (raw_t*)a.dgates + place : nullptr;
-    by_marks(bits.any, [&](auto asks) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (asks && (bits.first >> u & 1)) state_of(a.state, m.begins(a, t + u), h);
-            float xv[L];
-            xs[u].get(xv);
+    for (int u = 0; u < U; u++) {
+        if (bits.starts(u)) start(u, h);
+        float xv[L];
+        xs[u].get(xv);
 #pragma unroll
-            for (int k = 0; k < L; k++) {
-                before[u][k] = h[k];
-                h[k] = step<kDecay>(h[k], xv[k], cs[kShared ? 0 : u][k]);
-            }
+        for (int k = 0; k < L; k++) {
+            before[u][k] = h[k];
+            h[k] = step<kDecay>(h[k], xv[k], coefs_of<kDecay>(cs[kShared ? 0 : u][k]));
         }
+    }
+    again();
 #pragma unroll
-        for (int u = U - 1; u >= 0; u--) {
-            const bool in = !asks || (bits.in >> u & 1);
-            if (asks && (bits.end >> u & 1)) state_of(a.dlast, m.ends(a, t + u), l);
-            float d[L], xv[L], by_x[L], by_g[L];
-            incoming(u, d);
-            xs[u].get(xv);
+    for (int u = U - 1; u >= 0; u--) {
+        if (bits.stops(u)) stop(u, l);
+        float d[L], xv[L], by_x[L], by_g[L];
+        ds[u].get(d);
+        xs[u].get(xv);
 #pragma unroll
-            for (int k = 0; k < L; k++) {
-                const float co = cs[kShared ? 0 : u][k], f = factor<kDecay>(co);
-                const float reaches = d[k] + l[k];
-                if (kDecay) {
-                    by_x[k] = in ? reaches : 0.f;
-                    by_g[k] = in ? reaches * before[u][k] : 0.f;
-                } else {
-                    by_x[k] = in ? reaches * (holds(co) ? co : 1.f + co) : 0.f;
-                    by_g[k] = in ? by_x[k] * f * (before[u][k] - xv[k]) : 0.f;
-                }
-                l[k] = in ? f * reaches : 0.f;
-                sum[k] += by_g[k];
-            }
-            if (live && (!asks || t + u < m.length)) {
-                if (dx) Span<T, L>::store(dx + (int64_t)u * a.dim, by_x);
-                if (dg) Span<T, L>::store(dg + (int64_t)u * a.dim, by_g);
-            }
-            if (asks && (bits.first >> u & 1)) {
-                if (live && a.dstate) store_floats<L>(a.dstate + m.begins(a, t + u) * a.dim + c0, l);
-#pragma unroll
-                for (int k = 0; k < L; k++) l[k] = 0.f;
-            }
+        for (int k = 0; k < L; k++) {
+            const Gate c = coefs_of<kDecay>(cs[kShared ? 0 : u][k]);
+            const float reaches = d[k] + l[k];
+            by_x[k] = kDecay ? reaches : reaches * c.keep;
+            l[k] = c.a * reaches;
+            by_g[k] = kDecay ? reaches * before[u][k] : l[k] * c.keep * (before[u][k] - xv[k]);
+            if (kShared && !bits.is_in(u)) by_x[k] = by_g[k] = 0.f;
+            if (kShared) sum[k] += by_g[k];
         }
-    });
+        if (live && t + u < m.length) {
+            if (dx) Span<T, L>::store(dx + (int64_t)u * a.dim, by_x);
+            if (dg) Span<T, L>::store(dg + (int64_t)u * a.dim, by_g);
+        }
+        if (bits.is_first(u) && live && a.dstate) store_floats<L>(a.dstate + m.begins(a, t + u) * a.dim + c0, l);
+    }
     if (!kShared || !a.dgates) return;
     // (s_a is read by nobody any more)
 #pragma unroll
@@ -722,33 +796,25 @@ int fill(Chains& c, hipStream_t s) {
     return 0;
 }
 
-int fill_empty(const ScanArgs& a, const float* from, float* to, hipStream_t s) {
-    if (!a.bounds || !to) return 0;
-    for (int64_t first = 0; first < a.sequences; first += kMaxGrid) {
-        empty_kernel<<<(uint32_t)std::min(kMaxGrid, a.sequences - first), kThreads, 0, s>>>(a, from, to, first);
-        DCIH_HIP(hipGetLastError());
-    }
-    return 0;
-}
-
 template <class T, int L, bool kDecay, bool kShared>
 int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     Chains c{};
-    lay_out(c, a.work, a.rows, a.length, a.dim, dtype, gradient && a.shared);
+    lay_out(c, a.work, a.rows, a.length, a.dim, dtype, gradient, a.shared);
     if (int rc = fill(c, s)) return rc;
-    const int64_t blocks = c.count * c.tiles;
-    for (int64_t first = 0; first < blocks; first += kMaxGrid) {
-        const uint32_t grid = (uint32_t)std::min(kMaxGrid, blocks - first);
-        if (gradient) scan_grad_kernel<T, L, kDecay, kShared><<<grid, kBackThreads, 0, s>>>(a, c, first);
-        else scan_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first);
+    // (workgroups that pass on the states of sequences without tokens)
+    const int64_t empty = a.bounds && (gradient ? a.dstate : a.last) ? std::min((a.sequences + kEmpty - 1) / kEmpty, kEmptyGrid) : 0;
+    const int64_t tiles = c.count * c.tiles;
+    for (int64_t first = 0; first < tiles + empty; first += kMaxGrid) {
+        const uint32_t grid = (uint32_t)std::min(kMaxGrid, tiles + empty - first);
+        if (gradient) scan_grad_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first, empty);
+        else scan_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first, empty);
         DCIH_HIP(hipGetLastError());
     }
-    if (!gradient) return fill_empty(a, a.state, a.last, s);
-    if (kShared && a.dgates) {
+    if (gradient && kShared && a.dgates) {
         sum_kernel<T><<<(uint32_t)((a.dim + kSumChannels - 1) / kSumChannels), 1024, 0, s>>>(a, c, L);
         DCIH_HIP(hipGetLastError());
     }
-    return fill_empty(a, a.dlast, a.dstate, s);
+    return 0;
 }
 
 template <class T, int L, bool kDecay>
@@ -776,11 +842,11 @@ int by_length(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
 }
 
 // Short sequences that stand one behind the other share tiles: as many as one holds.
-ScanArgs flattened(ScanArgs a) {
+ScanArgs flattened(ScanArgs a, int tile) {
     auto flat = [&](int64_t row, int64_t step) { return row == a.length * step; };
-    if (a.form != kRows || 2 * a.length > kTile || a.rows == 1 || !flat(a.x_row, a.x_step) || (!a.shared && !flat(a.g_row, a.g_step)))
+    if (a.form != kRows || 2 * a.length > tile || a.rows == 1 || !flat(a.x_row, a.x_step) || (!a.shared && !flat(a.g_row, a.g_step)))
         return a;
-    const int64_t together = kTile / a.length;
+    const int64_t together = tile / a.length;
     a.form = kFlat;
     a.each = a.length;
     a.total = a.rows * a.length;
@@ -788,6 +854,7 @@ ScanArgs flattened(ScanArgs a) {
     a.rows = (a.rows + together - 1) / together;
     a.x_row *= together;
     a.g_row *= together;
+    a.states = nullptr;               // (rows begin with sequences)
     return a;
 }
 
@@ -803,19 +870,19 @@ int dispatch(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
 
 int64_t scan_state_floats(int64_t rows, int64_t length, int dim, int dtype) {
     Chains c{};
-    lay_out(c, nullptr, rows, length, dim, dtype, false);
+    lay_out(c, nullptr, rows, length, dim, dtype, false, false);
     return c.count * c.tiles * c.slots;
 }
 
 int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype, bool gradient, bool shared) {
     Chains c{};
-    return lay_out(c, nullptr, rows, length, dim, dtype, gradient && shared);
+    return lay_out(c, nullptr, rows, length, dim, dtype, gradient, shared);
 }
 
 bool scan_is_short(const ScanArgs& a) { return a.form == kRows && a.length <= kShort && !a.states; }
 
-int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a), dtype, false, s); }
-int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a), dtype, true, s); }
+int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, kTile), dtype, false, s); }
+int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, kTile), dtype, true, s); }
 
 int scan_copy(const float* from, float* to, int64_t n, hipStream_t s) {
     copy_kernel<<<(uint32_t)std::min<int64_t>((n + kThreads - 1) / kThreads, 2048), kThreads, 0, s>>>(from, to, n);
