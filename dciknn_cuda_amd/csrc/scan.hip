@@ -41,10 +41,9 @@ template <class T, int L> struct Span {
     using raw_t = typename T::raw;
     using P = Piece<T>;
     u32x4 bits;
-    __device__ void load(const raw_t* p) {
-        static_assert(L == P::kLen, "a piece");
-        bits = P::load_once(p);
-    }
+    static_assert(L == P::kLen, "a piece");
+    __device__ void load(const raw_t* p) { bits = P::load(p); }
+    __device__ void load_once(const raw_t* p) { bits = P::load_once(p); }
     __device__ void get(float (&z)[L]) const { P::unpack(bits, z); }
     __device__ void clear() { bits = u32x4{0, 0, 0, 0}; }
     __device__ void renew() { dcih::renew(bits); }
@@ -54,6 +53,7 @@ template <class T> struct Span<T, 1> {
     using raw_t = typename T::raw;
     raw_t bits;
     __device__ void load(const raw_t* p) { bits = *p; }
+    __device__ void load_once(const raw_t* p) { bits = *p; }
     __device__ void get(float (&z)[1]) const { z[0] = (float)bits; }
     __device__ void clear() { bits = (raw_t)0.f; }
     __device__ void renew() {}
@@ -195,6 +195,8 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
 struct Chains {
     int pieces, strips, slots;         // pieces of a row; strips of them; channels of a strip, those beyond the row included
     int64_t tiles, count;              // tiles of a chain, chains
+    bool once;                         // tokens are read past the caches
+    bool apart;                        // rows are whole lines: strips share none
     uint32_t *tickets, *flags;         // what was taken; [count][tiles] what is set: a hint of what to wait for
     uint64_t* maps;                    // [count][tiles][slots] (A, B)
     uint32_t* states;                  // [count][tiles][slots] the state behind a tile
@@ -263,12 +265,19 @@ __device__ inline uint32_t word_of(float v) {
 }
 
 // Item i of all is the next tile of a chain, in the direction of the scan, and each chain has as many items as tiles.  Neighbouring
-// items, which run on different XCDs, are neighbouring strips, and from one round to the next the strips go on by one: an XCD that always
-// had the same ones would use a few of its cache's channels only.  By one thread; returns chain * tiles + place.
+// items run on different XCDs.  From one round to the next the strips go on by one: an XCD that always had the same ones would use a
+// few of its cache's channels only (65536 x 4096 bf16 packed 351 us, 403 so).  Strips that share lines with their neighbours stand 8
+// items from them, so that most of them are on one XCD and close in time (30011 x 1023 f16 with gradients 202 us, 239 apart; with
+// rows of whole lines 375 and 351 of the first case).  By one thread; returns chain * tiles + place.
 __device__ inline int64_t take_tile(const Chains& c, int64_t i) {
     if (c.tiles == 1) return i;
     const int64_t round = i / c.count, at = i - round * c.count, row = at / c.strips;
-    const int64_t chain = row * c.strips + (at - row * c.strips + round) % c.strips;
+    int strip = (int)(at - row * c.strips);
+    if (!c.apart) {
+        const int xcd = strip % 8, rest = c.strips % 8;
+        strip = xcd * (c.strips / 8) + min(xcd, rest) + strip / 8;
+    }
+    const int64_t chain = row * c.strips + (strip + round) % c.strips;
     return chain * c.tiles + (atomicAdd(&c.tickets[chain], 1u) - kUnset);        // the counter begins at kUnset
 }
 
@@ -507,11 +516,20 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
     Span<T, L> xs[U], gs[kShared ? 1 : U];
     if (kShared) gs[0].load(g);
+    if (c.once) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t from = min(t + u, m.length - 1);
-        xs[u].load(x + from * a.x_step);
-        if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
+        for (int u = 0; u < U; u++) {
+            const int64_t from = min(t + u, m.length - 1);
+            xs[u].load_once(x + from * a.x_step);
+            if (!kShared) gs[kShared ? 0 : u].load_once(g + from * a.g_step);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t from = min(t + u, m.length - 1);
+            xs[u].load(x + from * a.x_step);
+            if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
+        }
     }
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
@@ -613,12 +631,22 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     const int64_t dh_step = a.dh ? a.dim : a.x_step;
     Span<T, L> xs[U], gs[kShared ? 1 : U], ds[U];
     if (kShared) gs[0].load(g);
+    if (c.once) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int64_t from = min(t + u, m.length - 1);
-        xs[u].load(x + from * a.x_step);
-        if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
-        ds[u].load(dh + from * dh_step);
+        for (int u = 0; u < U; u++) {
+            const int64_t from = min(t + u, m.length - 1);
+            xs[u].load_once(x + from * a.x_step);
+            if (!kShared) gs[kShared ? 0 : u].load_once(g + from * a.g_step);
+            ds[u].load_once(dh + from * dh_step);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t from = min(t + u, m.length - 1);
+            xs[u].load(x + from * a.x_step);
+            if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
+            ds[u].load(dh + from * dh_step);
+        }
     }
     find_marks(a, m, U, s_first, s_end, s_marked);
     __syncthreads();
@@ -800,6 +828,11 @@ template <class T, int L, bool kDecay, bool kShared>
 int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     Chains c{};
     lay_out(c, a.work, a.rows, a.length, a.dim, dtype, gradient, a.shared);
+    constexpr int kSize = sizeof(typename T::raw), kLine = 128;
+    c.apart = a.x_step * kSize % kLine == 0 && (uintptr_t)a.x % kLine == 0 && a.dim * kSize % kLine == 0;
+    // what the caches hold is read through them: 30011 x 1024 f16 with gradients 164 us, 171 past them; what they do not, past them
+    // (65536 x 4096 bf16 packed 351 us, 366)
+    c.once = c.apart && a.rows * a.length * a.dim * kSize * (kShared ? 1 : 2) > (int64_t)256 << 20;
     if (int rc = fill(c, s)) return rc;
     // (workgroups that pass on the states of sequences without tokens)
     const int64_t empty = a.bounds && (gradient ? a.dstate : a.last) ? std::min((a.sequences + kEmpty - 1) / kEmpty, kEmptyGrid) : 0;
