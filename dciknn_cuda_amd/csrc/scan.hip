@@ -7,7 +7,7 @@
 //   gates:  dx_t = (1 - a_t) l_t,  dg_t = a_t (1 - a_t) l_t (h_(t-1) - x_t)
 //   decays: dx_t = l_t,            dg_t = l_t h_(t-1);        both: by the first state a_1 l_1
 //
-// Both directions are compositions of maps s -> A s + B, which are associative: a tile of kTile tokens by kLanes pieces
+// Both directions are compositions of maps s -> A s + B, which are associative: a tile of 128 or 256 tokens by kLanes pieces
 // of 16 bytes is one workgroup's, in registers; each group of lanes composes its few tokens, the groups are joined in
 // shared memory, and a tile's map is joined to that of the tiles before it while these still run (see carry_of).  So every
 // element is read and written once.  The gradient forms h_(t-1) again, from x, g and the state before each tile, which
@@ -23,7 +23,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLanes = 8;                          // pieces of 16 bytes that a tile is wide: a line
-constexpr int kTile = 128;                         // tokens of a tile
+// Tokens of a tile: as many as fill the registers with pieces of `len` elements.
+constexpr int tile_of(int len) { return len == 8 ? 128 : 256; }
 constexpr int kWaves = 4, kBackWaves = 3;          // of a SIMD: registers enough for a tile, tiles enough to hide one another's waits
 constexpr int kShort = 16;                         // tokens that one thread takes
 constexpr int64_t kMaxGrid = 1 << 23;
@@ -213,7 +214,7 @@ __host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t leng
     c.pieces = (dim + len - 1) / len;
     c.strips = (c.pieces + kLanes - 1) / kLanes;
     c.slots = kLanes * len;
-    c.tiles = (length + kTile - 1) / kTile;
+    c.tiles = (length + tile_of(len) - 1) / tile_of(len);
     c.count = rows * c.strips;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -493,7 +494,7 @@ template <class Body> __device__ __forceinline__ void by_marks(bool any, Body bo
 
 template <class T, int L, bool kDecay, bool kShared>
 __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
-    constexpr int kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    constexpr int kTile = tile_of(L), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32, "a bit for each group");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
@@ -605,7 +606,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
 // behind: its maps are s -> A s + Q of the same A.
 template <class T, int L, bool kDecay, bool kShared>
 __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
-    constexpr int kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    constexpr int kTile = tile_of(L), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32 && 2 * kSlots <= kThreads, "a bit for each group, threads for both directions");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
@@ -914,8 +915,8 @@ int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype, bool g
 
 bool scan_is_short(const ScanArgs& a) { return a.form == kRows && a.length <= kShort && !a.states; }
 
-int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, kTile), dtype, false, s); }
-int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, kTile), dtype, true, s); }
+int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, tile_of(span_len(a.dim, dtype))), dtype, false, s); }
+int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, tile_of(span_len(a.dim, dtype))), dtype, true, s); }
 
 int scan_copy(const float* from, float* to, int64_t n, hipStream_t s) {
     copy_kernel<<<(uint32_t)std::min<int64_t>((n + kThreads - 1) / kThreads, 2048), kThreads, 0, s>>>(from, to, n);

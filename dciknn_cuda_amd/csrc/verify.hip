@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kChunk = 2048;                   // entries of a row that one wavefront adds up
+constexpr int kChoosers = 512, kChooserWaves = kChoosers / kWave;
 constexpr int64_t kMaxGrid = 1 << 23;
 
 struct alignas(16) Sum { double s; float m; float pad; };        // sum of 2^((z - m) c2), m = max z
@@ -47,11 +48,22 @@ __device__ inline double lanes_sum(double v) {
     return v;
 }
 
+// 2^(i / 64), i below 64, as 2^x is put together for whole rows.
+constexpr int kParts = 64;
+constexpr double kC1 = 0.010830424696249145, kC2 = 5.864904955056169e-05, kC3 = 2.1173137155464774e-07, kC4 = 5.732851688640402e-10;      // (ln(2) / 64)^k / k!
+__device__ inline void fill_table(double* s_table) {
+    if (threadIdx.x < kParts) s_table[threadIdx.x] = exp2_wide((double)threadIdx.x / kParts);
+}
+
 // A wavefront adds up `per` chunks of a row, one after the other.  Rows behind a sequence's last draft are asked for by nobody.
+// Bound by its instructions: 10 of 64 bits and 9 others an entry, 512 x 131072 bf16 XXX us (the bytes alone take 25).
 template <class T>
 __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums, int chunks, int per, int64_t first) {
     using P = Piece<T>;
     constexpr int U = kChunk / kWave / P::kLen;
+    __shared__ double s_table[kParts];
+    fill_table(s_table);
+    __syncthreads();
     const int splits = (chunks + per - 1) / per, lane = lane_id();
     const int64_t item = first + (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = item / splits, b = row / (a.drafts + 1);
@@ -60,6 +72,8 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
     for (int j = lane; __any(j < i); j += kWave)
         if (__any(j < i && id_at(a.ids, a.wide_ids, b * a.drafts + j) < 0)) return;
     const Row<T> r(a.z, row, a.stride, a.vocab);
+    const double scale = a.c2 * kParts;
+    const double deepest = -1000.0 / a.c2;                 // weights of less than 2^-1000 are that
     for (int c = from; c < to; c++) {
         u32x4 raw[U];
         const int piece = c * (kChunk / P::kLen) + lane;
@@ -70,12 +84,16 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
             for (int u = 0; u < U; u++) raw[u] = r.load(piece + u * kWave);
         }
         float m = kNoLogit;
+        bool bad = false;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float z[P::kLen];
             P::unpack(raw[u], z);
 #pragma unroll
-            for (int k = 0; k < P::kLen; k++) m = fmaxf(m, z[k]);
+            for (int k = 0; k < P::kLen; k++) {
+                m = fmaxf(m, z[k]);
+                bad |= z[k] != z[k];
+            }
         }
         m = max_of_lanes(m);
         const double base = base_of(m);
@@ -85,9 +103,26 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
             float z[P::kLen];
             P::unpack(raw[u], z);
 #pragma unroll
-            for (int k = 0; k < P::kLen; k++) s += weight_of(z[k], a.c2, base);
+            for (int k = 0; k < P::kLen; k++) {
+                // 2^y = 2^(whole / 64) 2^(rest / 64), |rest| <= 1/2: the series ends 4e-14 short.  The sum with 1.5 2^52 holds `whole`
+                // in its low word.
+                constexpr double kMagic = 6755399441055744.0;
+                const double d = __builtin_fmax((double)z[k] - base, deepest);
+                const double t = __builtin_fma(d, scale, kMagic), f = __builtin_fma(d, scale, -(t - kMagic));
+                const int whole = (int)__builtin_bit_cast(unsigned long long, t);
+                double q = kC4;
+                q = __builtin_fma(q, f, kC3);
+                q = __builtin_fma(q, f, kC2);
+                q = __builtin_fma(q, f, kC1);
+                q = __builtin_fma(q, f, 1.0);
+                unsigned long long w = __builtin_bit_cast(unsigned long long, s_table[whole & (kParts - 1)]);
+                w += (unsigned long long)(uint32_t)((whole >> 6) << 20) << 32;
+                s = __builtin_fma(__builtin_bit_cast(double, w), q, s);
+            }
         }
         s = lanes_sum(s);
+        if (m == kNoLogit) s = 0.0;
+        if (__any(bad) || m == -kNoLogit) s = __builtin_nan("");
         if (lane == 0) sums[row * chunks + c] = Sum{s, m, 0.f};
     }
 }
@@ -117,15 +152,15 @@ __device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
 }
 
 constexpr int kSlots = 1024;
-constexpr double kLog2eWide = 1.44269504088896340736;
+constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.693147180559945309417;
 
 // One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
 // from the row that it comes from, by chunks, then among the entries of one.
 template <class T>
-__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Sum* sums, int chunks, int64_t first) {
-    constexpr int kPer = kChunk / kThreads;
-    __shared__ double s_total[kMaxDrafts + 1], s_part[kWaves], s_weight[kChunk], s_gone[kSlots], s_target;
-    __shared__ float s_max[kMaxDrafts + 1];
+__global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const Sum* sums, int chunks, int64_t first) {
+    constexpr int kPer = kChunk / kChoosers;
+    __shared__ double s_total[kMaxDrafts + 1], s_part[kChooserWaves], s_weight[kChunk], s_gone[kSlots], s_less[kSlots], s_target;
+    __shared__ float s_max[kMaxDrafts + 1], s_logp[kMaxDrafts];
     __shared__ int s_kept[kMaxDrafts], s_id[kSlots], s_chunk, s_token, s_last, s_slots;
     const int64_t b = first + blockIdx.x;
     const int k = a.drafts, lane = lane_id(), wave = threadIdx.x / kWave, tid = threadIdx.x;
@@ -138,11 +173,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         s_chunk = s_token = s_last = -1;
     }
     __syncthreads();
-    for (int i = tid; i < k; i += kThreads)
+    for (int i = tid; i < k; i += kChoosers)
         if (draft_at(i) < 0) atomicMin(&s_slots, i);
     __syncthreads();
     const int given = s_slots;
-    for (int i = wave; i <= given; i += kWaves) {
+    for (int i = wave; i <= given; i += kChooserWaves) {
         const Sum* part = sums + (b * (k + 1) + i) * chunks;
         float m = kNoLogit;
         for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, part[c].m);
@@ -181,8 +216,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             q = all == 0.0 ? 0.0 : its / all;
         }
         if (lane == 0) {
-            const double p = t < a.vocab ? weight_of((float)logits[i * a.stride + t], c2, base) : 0.0;
+            const float z = t < a.vocab ? (float)logits[i * a.stride + t] : kNoLogit;
+            const double p = weight_of(z, c2, base);
             s_kept[i] = p > 0.0 && (double)a.uniforms[b * (k + 1) + i] * q * s < p;
+            s_logp[i] = (float)(((double)z - base) * c2 * kLn2Wide - log(s));
         }
     }
     __syncthreads();
@@ -207,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             slots = a.slots;
             const int64_t at = (b * k + kept) * a.slots;
             float top = kNoLogit;
-            for (int j = tid; j < slots; j += kThreads) {
+            for (int j = tid; j < slots; j += kChoosers) {
                 const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
                 s_id[j] = id < 0 ? -1 : id < a.vocab ? (int)id : a.vocab;
                 if (id >= 0) top = fmaxf(top, teacher_at(a, at + j));
@@ -215,10 +252,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             top = max_of_lanes(top);
             if (lane == 0) s_part[wave] = top;
             __syncthreads();
-            for (int w = 0; w < kWaves; w++) top = fmaxf(top, (float)s_part[w]);
+            for (int w = 0; w < kChooserWaves; w++) top = fmaxf(top, (float)s_part[w]);
             const double top_base = base_of(top);
             double all = 0.0;
-            for (int j = tid; j < slots; j += kThreads) {
+            for (int j = tid; j < slots; j += kChoosers) {
                 const double w = s_id[j] < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top_base);
                 s_gone[j] = w;
                 all += w;
@@ -228,13 +265,13 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             if (lane == 0) s_part[wave] = all;
             __syncthreads();
             all = 0.0;
-            for (int w = 0; w < kWaves; w++) all += s_part[w];
+            for (int w = 0; w < kChooserWaves; w++) all += s_part[w];
             fine = all < __builtin_huge_val();
             // a token of several slots stands in the first of them
-            double mine[kSlots / kThreads];
+            double mine[kSlots / kChoosers];
 #pragma unroll
-            for (int e = 0; e < kSlots / kThreads; e++) {
-                const int j = tid + e * kThreads;
+            for (int e = 0; e < kSlots / kChoosers; e++) {
+                const int j = tid + e * kChoosers;
                 mine[e] = 0.0;
                 if (j >= slots) continue;
                 bool leads = s_id[j] >= 0 && s_id[j] < a.vocab;
@@ -247,8 +284,8 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
             }
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < kSlots / kThreads; e++) {
-                const int j = tid + e * kThreads;
+            for (int e = 0; e < kSlots / kChoosers; e++) {
+                const int j = tid + e * kChoosers;
                 if (j >= slots) continue;
                 if (mine[e] < 0.0) s_id[j] = -1;
                 else s_gone[j] = all == 0.0 ? 0.0 : mine[e] / all * total;
@@ -256,19 +293,21 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         }
     }
     __syncthreads();
-    auto less = [&](int j) {           // what entry s_id[j] weighs less than in p
-        const double w = weight_of((float)row[s_id[j]], c2, base);
-        return w - max(w - s_gone[j], 0.0);
-    };
+    for (int j = tid; j < slots; j += kChoosers)           // what entry s_id[j] weighs less than in p
+        if (s_id[j] >= 0) {
+            const double w = weight_of((float)row[s_id[j]], c2, base);
+            s_less[j] = w - max(w - s_gone[j], 0.0);
+        }
+    __syncthreads();
     const float u = a.uniforms[b * (k + 1) + k];
     fine = fine && u == u;
     // the chunk: a run of chunks for each thread
-    const int each = (chunks + kThreads - 1) / kThreads, begin = min(chunks, tid * each), end = min(chunks, begin + each);
+    const int each = (chunks + kChoosers - 1) / kChoosers, begin = min(chunks, tid * each), end = min(chunks, begin + each);
     auto chunk_sum = [&](int c) {
         const Sum p = part[c];
         double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
-        for (int j = 0; j < slots; j++)
-            if (s_id[j] >= 0 && s_id[j] / kChunk == c) s -= less(j);
+#pragma unroll 4
+        for (int j = 0; j < slots; j++) s -= s_id[j] >= 0 && s_id[j] / kChunk == c ? s_less[j] : 0.0;
         return max(s, 0.0);
     };
     double all = 0.0, before = 0.0, own = 0.0;
@@ -277,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         for (int c = begin; c < end; c++) own += chunk_sum(c);
         before = scan_threads(own, s_part);
         all = 0.0;
-        for (int w = 0; w < kWaves; w++) all += s_part[w];
+        for (int w = 0; w < kChooserWaves; w++) all += s_part[w];
         if (all > 0.0) break;
         slots = 0;                       // nothing is left of p but roundings: drawn from p itself
     }
@@ -306,11 +345,11 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
         if (chunk >= 0) {
 #pragma unroll
             for (int e = 0; e < kPer; e++) {
-                const int i = e * kThreads + tid;
+                const int i = e * kChoosers + tid;
                 s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, base) : 0.0;
             }
             __syncthreads();
-            for (int j = tid; j < slots; j += kThreads)
+            for (int j = tid; j < slots; j += kChoosers)
                 if (s_id[j] >= from && s_id[j] < from + kChunk) s_weight[s_id[j] - from] = max(s_weight[s_id[j] - from] - s_gone[j], 0.0);
             if (tid == 0) s_last = -1;
             __syncthreads();
@@ -335,13 +374,10 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a, const Su
     }
     __syncthreads();
     const int token = s_token;
-    for (int i = tid; i <= k; i += kThreads) {
+    for (int i = tid; i <= k; i += kChoosers) {
         const int64_t t = i < kept ? draft_at(i) : i == kept ? token : -1;
-        float logp = 0.f;
-        if (i <= kept) {
-            if (t >= 0) logp = (float)(((double)(float)logits[i * a.stride + t] - (double)s_max[i]) * c2 * 0.693147180559945309417 - log(s_total[i]));
-            else logp = __builtin_nanf("");
-        }
+        float logp = i < kept ? s_logp[i] : 0.f;
+        if (i == kept) logp = t >= 0 ? (float)(((double)(float)row[t] - base) * c2 * kLn2Wide - log(total)) : __builtin_nanf("");
         a.tokens[b * (k + 1) + i] = (int32_t)t;
         a.logprobs[b * (k + 1) + i] = logp;
     }
@@ -362,7 +398,7 @@ int run(const VerifyArgs& a, hipStream_t s) {
         DCIH_HIP(hipGetLastError());
     }
     for (int64_t first = 0; first < a.n; first += kMaxGrid) {
-        verify_kernel<T><<<(uint32_t)std::min(kMaxGrid, a.n - first), kThreads, 0, s>>>(a, (const Sum*)a.work, chunks, first);
+        choose_kernel<T><<<(uint32_t)std::min(kMaxGrid, a.n - first), kChoosers, 0, s>>>(a, (const Sum*)a.work, chunks, first);
         DCIH_HIP(hipGetLastError());
     }
     return 0;
