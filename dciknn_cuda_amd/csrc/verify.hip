@@ -42,10 +42,28 @@ __device__ inline double weight_of(float z, double c2, double m) { return exp2_w
 // What weights are relative to, for a row of nothing but -inf too.
 __device__ inline double base_of(float m) { return (double)(m == kNoLogit ? 0.f : m); }
 
+template <int O> __device__ inline double other_lane(double v) {
+    return __builtin_bit_cast(double, dcih::other_lane<O>(__builtin_bit_cast(unsigned long long, v)));
+}
 __device__ inline double lanes_sum(double v) {
-#pragma unroll
-    for (int o = kWave / 2; o; o /= 2) v += __builtin_bit_cast(double, lane_xor_any(__builtin_bit_cast(unsigned long long, v), o));
+    v += other_lane<32>(v); v += other_lane<16>(v); v += other_lane<8>(v);
+    v += other_lane<4>(v); v += other_lane<2>(v); v += other_lane<1>(v);
     return v;
+}
+// Sums over the lanes up to and including each one's.
+template <int kControl, int kRows> __device__ inline double add_shifted(double v) {
+    const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)w, kControl, kRows, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(w >> 32), kControl, kRows, 0xf, false);
+    return v + __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ inline double lanes_scan(double v) {
+    v = add_shifted<0x111, 0xf>(v);      // row_shr:1
+    v = add_shifted<0x112, 0xf>(v);
+    v = add_shifted<0x114, 0xf>(v);
+    v = add_shifted<0x118, 0xf>(v);
+    v = add_shifted<0x142, 0xa>(v);      // row_bcast:15 into rows 1 and 3
+    return add_shifted<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
 }
 
 // 2^(i / 64), i below 64, as 2^x is put together for whole rows.
@@ -130,11 +148,7 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
 // Sums up to and including each thread's, in the order of the threads.
 __device__ inline double scan_threads(double v, double* s_part) {
     const int lane = lane_id(), wave = threadIdx.x / kWave;
-#pragma unroll
-    for (int o = 1; o < kWave; o *= 2) {
-        const double other = __shfl_up(v, o);
-        if (lane >= o) v += other;
-    }
+    v = lanes_scan(v);
     __syncthreads();
     if (lane == kWave - 1) s_part[wave] = v;
     __syncthreads();
@@ -151,7 +165,7 @@ __device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
     }
 }
 
-constexpr int kSlots = 1024;
+constexpr int kSlots = 1024, kNearChunks = 256;      // chunks whose amounts are added up beside the slots
 constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.693147180559945309417;
 
 // One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
@@ -159,11 +173,13 @@ constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.6931471805599
 template <class T>
 __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const Sum* sums, int chunks, int64_t first) {
     constexpr int kPer = kChunk / kChoosers;
-    __shared__ double s_total[kMaxDrafts + 1], s_part[kChooserWaves], s_weight[kChunk], s_gone[kSlots], s_less[kSlots], s_target;
+    __shared__ double s_total[kMaxDrafts + 1], s_part[kChooserWaves], s_weight[kChunk], s_gone[kSlots], s_target;
+    __shared__ unsigned long long s_fixed[kSlots], s_taken[kNearChunks];
     __shared__ float s_max[kMaxDrafts + 1], s_logp[kMaxDrafts];
-    __shared__ int s_kept[kMaxDrafts], s_id[kSlots], s_chunk, s_token, s_last, s_slots;
+    __shared__ int s_kept[kMaxDrafts], s_id[kSlots], s_chunk_of[kSlots], s_chunk, s_token, s_last, s_slots;
     const int64_t b = first + blockIdx.x;
     const int k = a.drafts, lane = lane_id(), wave = threadIdx.x / kWave, tid = threadIdx.x;
+    const float u = a.uniforms[b * (k + 1) + k];
     const double c2 = a.c2;
     const typename T::raw* logits = (const typename T::raw*)a.z + b * (k + 1) * a.stride;
     auto draft_at = [&](int i) { return id_at(a.ids, a.wide_ids, b * k + i); };
@@ -230,9 +246,14 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     const typename T::raw* row = logits + kept * a.stride;
     const Sum* part = sums + (b * (k + 1) + kept) * chunks;
     bool fine = total > 0.0 && total < __builtin_huge_val();
-    // what is taken off its weights: ids and amounts, each id once
+    // what is taken off its weights: ids and amounts, each id once.  (Amounts that several threads add up are whole numbers of 2^-52 of
+    // the largest, or of 2^-60 of the total: their order does not matter.)
+    const int each = (chunks + kChoosers - 1) / kChoosers, begin = min(chunks, tid * each), end = min(chunks, begin + each);
+    Sum mine{};
+    if (begin < end) mine = part[begin];
     int slots = 0;
     if (kept < given && fine) {
+        for (int c = tid; c < kNearChunks; c += kChoosers) s_taken[c] = 0;
         if (!a.slot_ids) {
             slots = 1;
             if (tid == 0) {
@@ -243,72 +264,89 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
         } else {
             slots = a.slots;
             const int64_t at = (b * k + kept) * a.slots;
-            float top = kNoLogit;
-            for (int j = tid; j < slots; j += kChoosers) {
-                const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
-                s_id[j] = id < 0 ? -1 : id < a.vocab ? (int)id : a.vocab;
-                if (id >= 0) top = fmaxf(top, teacher_at(a, at + j));
+            constexpr int E = kSlots / kChoosers;
+            int id[E];
+            float z[E], top = kNoLogit;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = tid + e * kChoosers;
+                id[e] = -2;
+                z[e] = kNoLogit;
+                if (j >= slots) continue;
+                const int64_t wide = id_at(a.slot_ids, a.wide_slots, at + j);
+                z[e] = teacher_at(a, at + j);
+                id[e] = wide < 0 ? -1 : wide < a.vocab ? (int)wide : a.vocab;
+                z[e] = wide < 0 ? kNoLogit : z[e];
+                top = fmaxf(top, z[e]);
             }
             top = max_of_lanes(top);
             if (lane == 0) s_part[wave] = top;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = tid + e * kChoosers;
+                s_id[j] = id[e];
+                s_fixed[j] = 0;
+            }
             __syncthreads();
             for (int w = 0; w < kChooserWaves; w++) top = fmaxf(top, (float)s_part[w]);
             const double top_base = base_of(top);
-            double all = 0.0;
-            for (int j = tid; j < slots; j += kChoosers) {
-                const double w = s_id[j] < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top_base);
-                s_gone[j] = w;
-                all += w;
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int j = tid + e * kChoosers;
+                if (id[e] < 0) continue;
+                const double w = weight_of(z[e], kLog2eWide, top_base);
+                bad |= !(w <= 1.0);
+                // a token of several slots stands in the first of them
+                int lead = j;
+                for (int o = 0; o < j; o += 8) {
+                    int found = j;
+#pragma unroll
+                    for (int i = 7; i >= 0; i--) found = s_id[o + i] == id[e] && o + i < j ? o + i : found;
+                    lead = found < lead ? found : lead;
+                }
+                if (!bad) atomicAdd(&s_fixed[lead], (unsigned long long)(w * 0x1p52));
             }
-            all = lanes_sum(all);
+            fine = !__syncthreads_or(bad);
+            unsigned long long sum = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += s_fixed[tid + e * kChoosers];
+            double all = lanes_sum((double)sum);
             __syncthreads();
             if (lane == 0) s_part[wave] = all;
             __syncthreads();
             all = 0.0;
             for (int w = 0; w < kChooserWaves; w++) all += s_part[w];
-            fine = all < __builtin_huge_val();
-            // a token of several slots stands in the first of them
-            double mine[kSlots / kChoosers];
+            const double share = all == 0.0 ? 0.0 : total / all;
 #pragma unroll
-            for (int e = 0; e < kSlots / kChoosers; e++) {
+            for (int e = 0; e < E; e++) {
                 const int j = tid + e * kChoosers;
-                mine[e] = 0.0;
-                if (j >= slots) continue;
-                bool leads = s_id[j] >= 0 && s_id[j] < a.vocab;
-                for (int o = 0; o < slots; o++) {
-                    const bool same = s_id[o] == s_id[j];
-                    if (same) mine[e] += s_gone[o];
-                    leads &= !(same && o < j);
-                }
-                if (!leads) mine[e] = -1.0;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kSlots / kChoosers; e++) {
-                const int j = tid + e * kChoosers;
-                if (j >= slots) continue;
-                if (mine[e] < 0.0) s_id[j] = -1;
-                else s_gone[j] = all == 0.0 ? 0.0 : mine[e] / all * total;
+                s_gone[j] = (double)s_fixed[j] * share;
+                if (id[e] == a.vocab || s_fixed[j] == 0) s_id[j] = -1;
             }
         }
     }
     __syncthreads();
-    for (int j = tid; j < slots; j += kChoosers)           // what entry s_id[j] weighs less than in p
-        if (s_id[j] >= 0) {
-            const double w = weight_of((float)row[s_id[j]], c2, base);
-            s_less[j] = w - max(w - s_gone[j], 0.0);
-        }
+    const double to_fixed = 0x1p60 / total;
+    for (int j = tid; j < (slots + 7) / 8 * 8; j += kChoosers) {           // what entry s_id[j] weighs less than in p
+        const int id = j < slots ? s_id[j] : -1;
+        const double w = id >= 0 ? weight_of((float)row[id], c2, base) : 0.0, less = id >= 0 ? w - max(w - s_gone[j], 0.0) : 0.0;
+        s_fixed[j] = (unsigned long long)(less * to_fixed);
+        s_chunk_of[j] = id >= 0 ? id / kChunk : -1;
+        if (id >= 0 && id / kChunk < kNearChunks) atomicAdd(&s_taken[id / kChunk], s_fixed[j]);
+    }
     __syncthreads();
-    const float u = a.uniforms[b * (k + 1) + k];
     fine = fine && u == u;
     // the chunk: a run of chunks for each thread
-    const int each = (chunks + kChoosers - 1) / kChoosers, begin = min(chunks, tid * each), end = min(chunks, begin + each);
-    auto chunk_sum = [&](int c) {
-        const Sum p = part[c];
-        double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
-#pragma unroll 4
-        for (int j = 0; j < slots; j++) s -= s_id[j] >= 0 && s_id[j] / kChunk == c ? s_less[j] : 0.0;
-        return max(s, 0.0);
+    auto chunk_sum = [&](int c) -> double {
+        const Sum p = c == begin ? mine : part[c];
+        const double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
+        unsigned long long taken = 0;
+        if (!slots) return s;
+        if (c < kNearChunks) taken = s_taken[c];
+        else
+            for (int o = 0; o < slots; o++) taken += s_chunk_of[o] == c ? s_fixed[o] : 0;
+        return __builtin_fmax(s - (double)taken * (total * 0x1p-60), 0.0);
     };
     double all = 0.0, before = 0.0, own = 0.0;
     for (int turn = 0; fine && turn < 2; turn++) {
@@ -327,8 +365,9 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
         if (tid == s_last) {
             double sum = before - own;
             int at = -1;
-            double rest = 0.0;
-            for (int c = begin; c < end; c++) {
+            double rest = target - sum;
+            if (end - begin == 1) at = begin;
+            for (int c = begin; end - begin > 1 && c < end; c++) {
                 const double s = chunk_sum(c);
                 if (s > 0.0 && sum <= target) {
                     at = c;
