@@ -493,30 +493,48 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gates, cons
 }
 
 // ---- norm of gradients, clipping ---------------------------------------------------------
-using Tensors = std::vector<Tensor>;
+// A list of tensors, looked at in place: a model has thousands of gradients.
+struct Tensors {
+    py::list list;
+    size_t size() const { return list.size(); }
+    bool empty() const { return list.empty(); }
+    const Tensor& operator[](size_t i) const {
+        PyObject* p = PyList_GET_ITEM(list.ptr(), (Py_ssize_t)i);
+        if (!THPVariable_Check(p)) bad_type("a gradient must be a tensor");
+        return THPVariable_Unpack(p);
+    }
+};
 
-std::vector<dcih_span> spans_of(const Tensors& grads, const c10::optional<Tensors>& into) {
+void no_gradient(const Tensor& t) {
+    no_tangent(t);
+    if (t.requires_grad() && torch::GradMode::is_enabled()) bad_value("no gradient is formed by or of the gradients: detach them");
+}
+
+std::vector<dcih_span> spans_of(const Tensors& grads, const Tensors* into) {
     if (into && into->size() != grads.size()) bad_value("out must have one tensor for each gradient");
     std::vector<dcih_span> spans;
     spans.reserve(grads.size());
-    for (size_t i = 0; i < grads.size(); i++) {
+    const size_t n = grads.size();
+    c10::Device device(c10::kCPU);
+    for (size_t i = 0; i < n; i++) {
         const Tensor &g = grads[i], &o = into ? (*into)[i] : g;
         dcih_span p{};
         p.dtype = type_code(g, "a gradient");
-        if (g.device() != grads[0].device()) bad_value("the gradients must be on one device");
+        if (!i) device = g.device();
+        if (g.device() != device) bad_value("the gradients must be on one device");
         if (!g.is_non_overlapping_and_dense()) bad_value("a gradient's elements must be one behind the other in some order of its dimensions");
-        no_tangent(g);
+        no_gradient(g);
         p.out_dtype = into ? type_code(o, "out") : p.dtype;
         if (into) {
             if (p.out_dtype != p.dtype && p.out_dtype != DCIH_F32) bad_type("out must be of the gradient's type or float32");
-            if (o.device() != g.device()) bad_value("out must be on the gradients' device");
+            if (o.device() != device) bad_value("out must be on the gradients' device");
             bool alike = o.sizes() == g.sizes();
             for (int64_t d = 0; alike && d < g.dim(); d++) alike = g.size(d) == 1 || o.stride(d) == g.stride(d);
             if (!alike) bad_value("out must have the gradient's shape and strides");
-            no_tangent(o);
+            no_gradient(o);
         }
         p.data = g.data_ptr();
-        p.out = o.data_ptr();
+        p.out = into ? o.data_ptr() : const_cast<void*>(p.data);
         p.count = g.numel();
         if (p.count) spans.push_back(p);
     }
@@ -549,12 +567,11 @@ double scale_of(double scale) {
 
 Tensor norm_of_none() { return torch::zeros({}, torch::kFloat32); }
 
-Tensor grad_norm(const Tensors& grads, double scale) {
+Tensor grad_norm(const py::list& list, double scale) {
+    const Tensors grads{list};
     scale_of(scale);
     if (grads.empty()) return norm_of_none();
-    const auto spans = spans_of(grads, c10::nullopt);
-    for (const Tensor& g : grads)
-        if (wants_grad(g)) bad_value("no gradient is formed by the gradients: detach them");
+    const auto spans = spans_of(grads, nullptr);
     c10::DeviceGuard guard(grads[0].device());
     const Tensor norm = floats({}, grads[0]);
     const int64_t need = dcih_clip_work(spans.data(), spans.size());
@@ -564,16 +581,14 @@ Tensor grad_norm(const Tensors& grads, double scale) {
     return norm;
 }
 
-Tensor clip_grads(const Tensors& grads, double max_norm, double scale, const c10::optional<Tensors>& into) {
+Tensor clip_grads(const py::list& list, double max_norm, double scale, const c10::optional<py::list>& out) {
+    const Tensors grads{list}, into{out ? *out : py::list()};
     scale_of(scale);
     if (!(max_norm >= 0.0)) bad_value("max_norm must not be negative");
-    if (grads.empty() && (!into || into->empty())) return norm_of_none();
-    const auto spans = spans_of(grads, into);
+    if (grads.empty() && into.empty()) return norm_of_none();
+    const auto spans = spans_of(grads, out ? &into : nullptr);
     check_apart(spans);
-    for (const Tensors* list : {&grads, into ? &*into : nullptr})
-        for (size_t i = 0; list && i < list->size(); i++)
-            if (wants_grad((*list)[i])) bad_value("no gradient is formed by or of the gradients: detach them");
-    for (const Tensor& t : into ? *into : grads) t.unsafeGetTensorImpl()->bump_version();
+    for (size_t i = 0; i < grads.size(); i++) (out ? into : grads)[i].unsafeGetTensorImpl()->bump_version();
     c10::DeviceGuard guard(grads[0].device());
     const Tensor norm = floats({}, grads[0]);
     const int64_t need = dcih_clip_work(spans.data(), spans.size());
