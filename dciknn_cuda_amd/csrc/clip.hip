@@ -21,7 +21,7 @@ constexpr int64_t kUnits = 8192;                // in all, where units are not t
 constexpr int64_t kFewSums = kThreads;          // up to here every workgroup joins the sums itself
 constexpr int64_t kMaxSpan = (int64_t)1 << 31;  // elements of an entry: longer spans are several
 constexpr int64_t kMaxGrid = 1 << 23;
-constexpr uint32_t kBlocks = 2048;              // workgroups of a launch that writes
+constexpr uint32_t kBlocks = 1024;              // workgroups of a launch that writes
 
 // Where spans lie. A type is kept beside the address, which has 57 bits.
 struct Place {

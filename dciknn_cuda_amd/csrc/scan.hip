@@ -23,8 +23,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kLanes = 8;                          // pieces of 16 bytes that a tile is wide: a line
-// Tokens of a tile: as many as fill the registers with pieces of `len` elements.
-constexpr int tile_of(int len) { return len == 8 ? 128 : 256; }
+// Tokens of a tile, with pieces of `len` elements: as many as the gradient's registers hold.  (8 x 4096 x 1024 f32 with gradients 230 us, with 256
+// tokens 241 to 253; with shared gates 139 either way, and a chain of 20000 tokens by 64 has half the tiles: 18 and 21 us instead of 26 and 27.)
+constexpr int tile_of(int len, bool shared) { return len == 8 || (len == 4 && !shared) ? 128 : 256; }
 constexpr int kWaves = 4, kBackWaves = 3;          // of a SIMD: registers enough for a tile, tiles enough to hide one another's waits
 constexpr int kShort = 16;                         // tokens that one thread takes
 constexpr int64_t kMaxGrid = 1 << 23;
@@ -214,7 +215,8 @@ __host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t leng
     c.pieces = (dim + len - 1) / len;
     c.strips = (c.pieces + kLanes - 1) / kLanes;
     c.slots = kLanes * len;
-    c.tiles = (length + tile_of(len) - 1) / tile_of(len);
+    const int tile = tile_of(len, shared);
+    c.tiles = (length + tile - 1) / tile;
     c.count = rows * c.strips;
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -494,7 +496,7 @@ template <class Body> __device__ __forceinline__ void by_marks(bool any, Body bo
 
 template <class T, int L, bool kDecay, bool kShared>
 __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
-    constexpr int kTile = tile_of(L), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    constexpr int kTile = tile_of(L, kShared), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32, "a bit for each group");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
@@ -606,7 +608,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
 // behind: its maps are s -> A s + Q of the same A.
 template <class T, int L, bool kDecay, bool kShared>
 __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
-    constexpr int kTile = tile_of(L), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
+    constexpr int kTile = tile_of(L, kShared), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32 && 2 * kSlots <= kThreads, "a bit for each group, threads for both directions");
     using raw_t = typename T::raw;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
@@ -908,15 +910,15 @@ int64_t scan_state_floats(int64_t rows, int64_t length, int dim, int dtype) {
     return c.count * c.tiles * c.slots;
 }
 
-int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype, bool gradient, bool shared) {
+int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype) {
     Chains c{};
-    return lay_out(c, nullptr, rows, length, dim, dtype, gradient, shared);
+    return std::max(lay_out(c, nullptr, rows, length, dim, dtype, true, true), lay_out(c, nullptr, rows, length, dim, dtype, true, false));
 }
 
 bool scan_is_short(const ScanArgs& a) { return a.form == kRows && a.length <= kShort && !a.states; }
 
-int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, tile_of(span_len(a.dim, dtype))), dtype, false, s); }
-int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, tile_of(span_len(a.dim, dtype))), dtype, true, s); }
+int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, false, s); }
+int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, true, s); }
 
 int scan_copy(const float* from, float* to, int64_t n, hipStream_t s) {
     copy_kernel<<<(uint32_t)std::min<int64_t>((n + kThreads - 1) / kThreads, 2048), kThreads, 0, s>>>(from, to, n);

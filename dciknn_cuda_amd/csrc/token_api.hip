@@ -353,7 +353,7 @@ int64_t dcih_scan_states(int64_t rows, int64_t length, int dim, int dtype) {
 
 int64_t dcih_scan_work(int64_t rows, int64_t length, int dim, int dtype, int64_t packed_sequences) {
     if (const char* why = check_scan_size(rows, length, dim, dtype, packed_sequences)) return refuse("dcih_scan_work", why);
-    return scan_work_bytes(rows, length, dim, dtype, true, true) + last_bytes(packed_sequences ? packed_sequences : rows, dim);
+    return scan_work_bytes(rows, length, dim, dtype) + last_bytes(packed_sequences ? packed_sequences : rows, dim);
 }
 
 int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim, int64_t x_row, int64_t x_step, const void* d_gates,
@@ -374,7 +374,7 @@ int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim,
     if (overlap(d_h, h_bytes, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
         overlap(d_h, h_bytes, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b))
         return refuse(who, "h overlaps x or the gates");
-    const int64_t own = scan_work_bytes(rows, length, dim, dtype, true, true);
+    const int64_t own = scan_work_bytes(rows, length, dim, dtype);
     if (work_bytes < own + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     a.h = d_h;
@@ -409,7 +409,7 @@ int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int
         if (out && (overlap(out, cells, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
                     overlap(out, cells, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b) || (d_dh && overlap(out, cells, d_dh, cells))))
             return refuse(who, "a gradient overlaps what it is formed from");
-    if (work_bytes < scan_work_bytes(rows, length, dim, dtype, true, true) + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
+    if (work_bytes < scan_work_bytes(rows, length, dim, dtype) + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     a.states = const_cast<float*>(d_states);
     a.dh = d_dh;

@@ -134,7 +134,8 @@ def test_broadcast_gates_and_inputs(gpu):
     x, gate = torch.randn(4, 50, 16, generator=g).cuda(), torch.randn(16, generator=g).cuda().requires_grad_()
     h, _ = gpu.gated_scan(x, gate)
     wide, _ = gpu.gated_scan(x, gate.expand(4, 50, 16))
-    assert torch.equal(h, wide)
+    # the groups of tokens that are joined may be others: each is off by 16 half steps of the largest magnitude for each of up to 50 tokens
+    assert (h - wide).abs().max() <= 2 * 50 * 16 * O.STEP * x.abs().max()
     w = torch.randn(4, 50, 16, generator=g).cuda()
     a, = torch.autograd.grad((h * w).sum(), gate)
     b, = torch.autograd.grad((wide * w).sum(), gate)
