@@ -411,12 +411,31 @@ struct Marks {
     }
 };
 
+// (kRows) How many tokens of a row are its sequence's.
+__device__ inline int64_t row_end(const ScanArgs& a, int64_t row) {
+    return a.bounds ? min(max(id_of_all(a.bounds, a.wide_bounds, row), (int64_t)0), a.length) : a.length;
+}
+
+// A tile behind the end of a row's sequence: zeros, without a look at the tokens.  What enters the next tile is zero too.
+template <class T, int L>
+__device__ inline void write_zeros(const Chains& c, int64_t item, int64_t at, typename T::raw* out, int64_t step, int64_t tokens, bool live) {
+    float zeros[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) zeros[k] = 0.f;
+    if (out && live)
+        for (int64_t u = 0; u < tokens; u++) Span<T, L>::store(out + u * step, zeros);
+    if (at + 1 < c.tiles && threadIdx.x < c.slots) {
+        post(c.states + (item - item % c.tiles + at) * c.slots + threadIdx.x, 0u);
+        if (threadIdx.x == 0) post(c.flags + item - item % c.tiles + at, kStateSet);
+    }
+}
+
 // By all threads; `s_first`, `s_end` and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
 template <int kTokens>
 __device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int (&s_first)[kTokens], int (&s_end)[kTokens], uint32_t& s_marked) {
     if (a.form == kRows) {
         m.lo = 0;
-        m.hi = Marks::length_of(a, m.row, a.length);
+        m.hi = row_end(a, m.row);
     } else if (a.form == kFlat) {
         m.lo = 0;
         m.hi = m.length;
@@ -515,6 +534,8 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     Marks m(a, row, t0);
     const int piece = (int)(chain - row * c.strips) * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
     const bool live = piece < c.pieces;
+        if (a.form == kRows && a.bounds && t0 >= row_end(a, row))
+        return write_zeros<T, L>(c, item, at, (raw_t*)a.h + (row * a.length + t) * a.dim + c0, a.dim, min((int64_t)U, m.length - t), live);
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
     Span<T, L> xs[U], gs[kShared ? 1 : U];
@@ -630,6 +651,13 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     const bool live = piece < c.pieces;
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
+    if (a.form == kRows && a.bounds && t0 >= row_end(a, row)) {
+        const int64_t place = (row * a.length + t) * a.dim + c0, own = min((int64_t)U, m.length - t);
+        write_zeros<T, L>(c, item, at, a.dx ? (raw_t*)a.dx + place : nullptr, a.dim, own, live);
+        if (!kShared && a.dgates) write_zeros<T, L>(c, item, c.tiles, (raw_t*)a.dgates + place, a.dim, own, live);
+        if (kShared && a.dgates && threadIdx.x < kSlots) c.sums[(chain * c.tiles + tile) * kSlots + threadIdx.x] = 0.f;
+        return;
+    }
     const raw_t* dh = a.dh ? (const raw_t*)a.dh + row * a.length * a.dim + c0 : x;
     const int64_t dh_step = a.dh ? a.dim : a.x_step;
     Span<T, L> xs[U], gs[kShared ? 1 : U], ds[U];

@@ -374,6 +374,9 @@ int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim,
     if (overlap(d_h, h_bytes, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
         overlap(d_h, h_bytes, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b))
         return refuse(who, "h overlaps x or the gates");
+    if (d_last && (overlap(d_last, states * 4, d_h, h_bytes) || overlap(d_last, states * 4, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
+                   overlap(d_last, states * 4, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b)))
+        return refuse(who, "the last states overlap x, the gates or h");
     const int64_t own = scan_work_bytes(rows, length, dim, dtype);
     if (work_bytes < own + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");

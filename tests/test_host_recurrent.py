@@ -21,7 +21,7 @@ def test_scan_refuses(oracle):
         lib.dcih_scan(x, dtype, rows, length, dim, xr, xs, g, gr, gs, flags, state, bounds, width, packed, h, last, states, work, size, None))
     bad_scan = [dict(x=None), dict(x=A + 1), dict(dtype=5), dict(rows=-1), dict(length=1 << 31), dict(dim=0), dict(xr=-1), dict(xs=-16), dict(g=None), dict(gr=-1),
                 dict(xs=1 << 58), dict(gr=1 << 60), dict(flags=4), dict(state=A + 2), dict(bounds=A + 2), dict(bounds=A, width=3), dict(packed=2), dict(rows=1, packed=2),
-                dict(h=None), dict(h=A), dict(h=A + 100), dict(h=B + 1), dict(last=A + 1), dict(states=A + 3), dict(state=A, last=A + 4), dict(work=None), dict(work=A + 8), dict(size=need - 1)]
+                dict(h=None), dict(h=A), dict(h=A + 100), dict(h=B + 1), dict(last=A + 1), dict(states=A + 3), dict(state=A, last=A + 4), dict(last=B), dict(last=A + 64), dict(work=None), dict(work=A + 8), dict(size=need - 1)]
     for bad in bad_scan:
         assert scan(**bad) == -1, bad
         assert lib.dcih_last_error().startswith(b"dcih_scan: ")
