@@ -34,7 +34,7 @@ struct ScanArgs {
 
 int64_t scan_state_floats(int64_t rows, int64_t length, int dim, int dtype);
 int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype);       // of either direction, whatever the gates
-bool scan_is_short(const ScanArgs& a);      // one thread has a channel of a sequence from the first token to the last
+bool scan_is_short(const ScanArgs& a, int dtype);      // one thread has a channel of a sequence from the first token to the last
 int scan(const ScanArgs& a, int dtype, hipStream_t s);
 int scan_grad(const ScanArgs& a, int dtype, hipStream_t s);
 int scan_copy(const float* from, float* to, int64_t n, hipStream_t s);

@@ -29,7 +29,11 @@ constexpr int tile_of(int len, bool shared) { return len == 8 || (len == 4 && !s
 // Wavefronts of a SIMD: registers enough for a tile, tiles enough to hide one another's waits (one more each way spills: 8 x 4096 x 2048
 // with gradients 262 us instead of 238; one less is as fast).
 constexpr int kWaves = 4, kBackWaves = 3;
-constexpr int kShort = 16;                         // tokens that one thread takes: 32 x 1 x 4096 bf16 3.4 us, a launch
+// Tokens that one thread takes: 32 x 1 x 4096 bf16 3.4 us, a launch.  More where threads are many: 512 x 40 x 2048 bf16 42 us, 58 by tiles (512 x 64 x
+// 1024 38 and 43, 256 x 24 x 1024 13.2 and 13.8; but 256 x 32 x 1024 17.1 and 14.6).
+constexpr int kShort = 16, kShortOfMany = 64;
+constexpr int64_t kManyThreads = 1280;             // for each token
+constexpr int kApart = 32;                         // words from one chain's counter to the next: a line takes an atomic operation in 11 ns
 constexpr int64_t kMaxGrid = 1 << 23;
 constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
 constexpr uint32_t kMapSet = 1, kStateSet = 2;
@@ -204,6 +208,7 @@ struct Chains {
     uint32_t *tickets, *flags;         // what was taken; [count][tiles] what is set: a hint of what to wait for
     uint64_t* maps;                    // [count][tiles][slots] (A, B)
     uint32_t* states;                  // [count][tiles][slots] the state behind a tile
+    int32_t* from;                     // (kPacked) [tiles] the last sequence that begins before a tile
     float* sums;                       // [count][tiles][slots] (gradient of shared gates)
 };
 
@@ -227,17 +232,37 @@ __host__ inline int64_t lay_out(Chains& c, void* mem, int64_t rows, int64_t leng
         return p;
     };
     const int64_t cells = c.count * c.tiles * c.slots, chained = c.tiles > 1 ? 1 : 0;
-    c.tickets = (uint32_t*)take(chained * c.count * 4);
+    c.tickets = (uint32_t*)take(chained * c.count * kApart * 4);
     c.flags = (uint32_t*)take(chained * c.count * c.tiles * 4);
     c.maps = (uint64_t*)take(chained * cells * 8);
     c.states = (uint32_t*)take(chained * cells * 4);
+    c.from = (int32_t*)take(chained * c.tiles * 4);
     c.sums = (float*)take(gradient && shared ? cells * 4 : 0);
     return at;
 }
 
-__global__ __launch_bounds__(kThreads) void fill_kernel(u32x4* p, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i < n) p[i] = u32x4{kUnset, kUnset, kUnset, kUnset};
+// The last sequence that begins before a token, by `bound`, which cuts offsets to [0, length].
+template <class Bound> __device__ inline int64_t last_before(int64_t sequences, int64_t token, Bound bound) {
+    int64_t from = 0, to = sequences;
+    while (to - from > 1) {
+        const int64_t mid = from + (to - from) / 2;
+        if (bound(mid) < token) from = mid;
+        else to = mid;
+    }
+    return from;
+}
+__device__ inline int64_t cut(const ScanArgs& a, int64_t o) { return min(max(o, (int64_t)0), a.length); }
+
+// The mark of what is not posted yet, and by the workgroups behind the first `blocks` where each tile looks for its sequences: there
+// every workgroup would look for itself, ten steps that wait for one another.
+__global__ __launch_bounds__(kThreads) void fill_kernel(u32x4* p, int64_t n, int64_t blocks, ScanArgs a, int32_t* from, int64_t tiles, int tokens) {
+    if (blockIdx.x < blocks) {
+        const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+        if (i < n) p[i] = u32x4{kUnset, kUnset, kUnset, kUnset};
+        return;
+    }
+    const int64_t i = ((int64_t)blockIdx.x - blocks) * kThreads + threadIdx.x;
+    if (i < tiles) from[i] = (int32_t)last_before(a.sequences, i * tokens, [&](int64_t s) { return cut(a, id_at(a.bounds, a.wide_bounds, s)); });
 }
 __global__ __launch_bounds__(kThreads) void copy_kernel(const float* from, float* to, int64_t n) {
     const int64_t step = (int64_t)gridDim.x * kThreads;
@@ -283,7 +308,7 @@ __device__ inline int64_t take_tile(const Chains& c, int64_t i) {
         strip = xcd * (c.strips / 8) + min(xcd, rest) + strip / 8;
     }
     const int64_t chain = row * c.strips + (strip + round) % c.strips;
-    return chain * c.tiles + (atomicAdd(&c.tickets[chain], 1u) - kUnset);        // the counter begins at kUnset
+    return chain * c.tiles + (atomicAdd(&c.tickets[chain * kApart], 1u) - kUnset);        // the counter begins at kUnset
 }
 
 // The state that enters tile `at` of a chain in channel `slot`.  A tile posts its map as soon as it has it, and the state
@@ -308,7 +333,7 @@ __device__ float carry_of(const Chains& c, int64_t chain, int64_t at, int slot) 
     }
     const int64_t base = last - (int64_t)behind * c.slots;
     const uint64_t* maps = c.maps + base + c.slots;
-    constexpr int U = 8;
+    constexpr int U = 16;
     uint64_t m[U];
     auto load_maps = [&](int i) {
 #pragma unroll
@@ -433,52 +458,56 @@ __device__ inline void write_zeros(const Chains& c, int64_t item, int64_t at, ty
 }
 
 // By all threads; `s_first`, `s_end` and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
+// What finds the sequences of a tile (kPacked): the first of them that may begin or end there, and each thread's bounds, asked for ahead
+// of the tokens (what the vector memory answers comes in order).
+struct Found {
+    int64_t from = 0, lo = 0, hi = 0;
+    __device__ Found(const ScanArgs& a, const Chains& c, int64_t tile, int64_t t0) {
+        if (a.form != kPacked) return;
+        if (c.tiles > 1) from = ((const __attribute__((address_space(4))) int32_t*)c.from)[tile];
+        else from = last_before(a.sequences, t0, [&](int64_t s) { return cut(a, id_of_all(a.bounds, a.wide_bounds, s)); });
+        ask(a, from);
+    }
+    __device__ void ask(const ScanArgs& a, int64_t s) {
+        const int64_t mine = s + threadIdx.x;
+        lo = hi = 0;
+        if (mine >= a.sequences) return;
+        lo = cut(a, id_at(a.bounds, a.wide_bounds, mine));
+        hi = cut(a, id_at(a.bounds, a.wide_bounds, mine + 1));
+    }
+};
 template <int kTokens>
-__device__ inline void find_marks(const ScanArgs& a, Marks& m, int per, int (&s_first)[kTokens], int (&s_end)[kTokens], uint32_t& s_marked) {
-    if (a.form == kRows) {
-        m.lo = 0;
-        m.hi = row_end(a, m.row);
-    } else if (a.form == kFlat) {
-        m.lo = 0;
-        m.hi = m.length;
-    } else {
-        auto cut = [&](int64_t o) { return min(max(o, (int64_t)0), a.length); };
-        auto bound = [&](int64_t i) { return cut(id_at(a.bounds, a.wide_bounds, i)); };
-        auto bound_of_all = [&](int64_t i) { return cut(id_of_all(a.bounds, a.wide_bounds, i)); };
-        m.lo = bound_of_all(0);
-        m.hi = bound_of_all(a.sequences);
-        m.first = s_first;
-        m.end = s_end;
-        for (int i = threadIdx.x; i < kTokens; i += blockDim.x) s_first[i] = s_end[i] = -1;
-        if (threadIdx.x == 0) s_marked = 0;
-        // the last sequence that begins before the tile, through the scalar cache: loads of tokens are under way, and what the
-        // vector memory answers comes in order
-        int64_t from = 0, to = a.sequences;
-        while (to - from > 1) {
-            const int64_t mid = from + (to - from) / 2;
-            if (bound_of_all(mid) < m.t0) from = mid;
-            else to = mid;
-        }
-        __syncthreads();
-        for (int64_t s = from;; s += blockDim.x) {
-            const int64_t mine = s + threadIdx.x;
-            if (mine < a.sequences) {
-                const int64_t lo = bound(mine), hi = bound(mine + 1);
-                if (hi > lo) {
-                    if (lo >= m.t0 && lo < m.t0 + kTokens) {
-                        s_first[lo - m.t0] = (int)mine;
-                        atomicOr(&s_marked, 1u << ((int)(lo - m.t0) / per));
-                    }
-                    if (hi - 1 >= m.t0 && hi - 1 < m.t0 + kTokens) {
-                        s_end[hi - 1 - m.t0] = (int)mine;
-                        atomicOr(&s_marked, 1u << ((int)(hi - 1 - m.t0) / per));
-                    }
-                }
+__device__ inline void find_marks(const ScanArgs& a, Found f, Marks& m, int per, int (&s_first)[kTokens], int (&s_end)[kTokens], uint32_t& s_marked) {
+    m.lo = 0;
+    m.hi = m.length;
+    if (a.form == kRows) m.hi = row_end(a, m.row);
+    if (a.form != kPacked) return;
+    auto bound_of_all = [&](int64_t i) { return cut(a, id_of_all(a.bounds, a.wide_bounds, i)); };
+    m.lo = bound_of_all(0);
+    m.hi = bound_of_all(a.sequences);
+    m.first = s_first;
+    m.end = s_end;
+    for (int i = threadIdx.x; i < kTokens; i += blockDim.x) s_first[i] = s_end[i] = -1;
+    if (threadIdx.x == 0) s_marked = 0;
+    __syncthreads();
+    for (int64_t s = f.from;;) {
+        const int mine = (int)(s + threadIdx.x);
+        if (f.hi > f.lo) {
+            if (f.lo >= m.t0 && f.lo < m.t0 + kTokens) {
+                s_first[f.lo - m.t0] = mine;
+                atomicOr(&s_marked, 1u << ((int)(f.lo - m.t0) / per));
             }
-            if (s + blockDim.x >= a.sequences || bound_of_all(s + blockDim.x) >= m.t0 + kTokens) break;
+            if (f.hi - 1 >= m.t0 && f.hi - 1 < m.t0 + kTokens) {
+                s_end[f.hi - 1 - m.t0] = mine;
+                atomicOr(&s_marked, 1u << ((int)(f.hi - 1 - m.t0) / per));
+            }
         }
+        s += blockDim.x;
+        if (s >= a.sequences || bound_of_all(s) >= m.t0 + kTokens) break;
+        f.ask(a, s);
     }
 }
+
 // What a group of `per` tokens from `t` on has to know of them, a bit for each: which are of a sequence, its first, its last.  Tokens
 // of no sequence are zeros that begin and end at zero.  (No lane leaves the loops over the tokens early: hipcc 7.2 lost a
 // factor of A there.)
@@ -543,6 +572,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
         return write_zeros<T, L>(c, item, at, (raw_t*)a.h + (row * a.length + t) * a.dim + c0, a.dim, min((int64_t)U, m.length - t), live);
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
+    const Found found(a, c, at, t0);
     Span<T, L> xs[U], gs[kShared ? 1 : U];
     if (kShared) gs[0].load(g);
     if (c.once) {
@@ -560,7 +590,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
             if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
         }
     }
-    find_marks(a, m, U, s_first, s_end, s_marked);
+    find_marks(a, found, m, U, s_first, s_end, s_marked);
     __syncthreads();
     const Bits bits(a, m, t, U, group, s_marked);
     if (bits.any)
@@ -665,6 +695,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     }
     const raw_t* dh = a.dh ? (const raw_t*)a.dh + row * a.length * a.dim + c0 : x;
     const int64_t dh_step = a.dh ? a.dim : a.x_step;
+    const Found found(a, c, tile, t0);
     Span<T, L> xs[U], gs[kShared ? 1 : U], ds[U];
     if (kShared) gs[0].load(g);
     if (c.once) {
@@ -684,7 +715,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
             ds[u].load(dh + from * dh_step);
         }
     }
-    find_marks(a, m, U, s_first, s_end, s_marked);
+    find_marks(a, found, m, U, s_first, s_end, s_marked);
     __syncthreads();
     const Bits bits(a, m, t, U, group, s_marked);
     if (bits.any)
@@ -852,10 +883,11 @@ __global__ __launch_bounds__(1024) void sum_kernel(ScanArgs a, Chains c, int len
 }
 
 // ---- launches ----------------------------------------------------------------------------
-int fill(Chains& c, hipStream_t s) {
+int fill(const ScanArgs& a, const Chains& c, int tokens, hipStream_t s) {
     if (c.tiles <= 1) return 0;
-    const int64_t words = ((char*)c.sums - (char*)c.tickets) / 16;      // what lies before the sums
-    fill_kernel<<<(uint32_t)((words + kThreads - 1) / kThreads), kThreads, 0, s>>>((u32x4*)c.tickets, words);
+    const int64_t words = ((char*)c.from - (char*)c.tickets) / 16, blocks = (words + kThreads - 1) / kThreads;
+    const int64_t more = a.form == kPacked ? (c.tiles + kThreads - 1) / kThreads : 0;
+    fill_kernel<<<(uint32_t)(blocks + more), kThreads, 0, s>>>((u32x4*)c.tickets, words, blocks, a, c.from, c.tiles, tokens);
     DCIH_HIP(hipGetLastError());
     return 0;
 }
@@ -869,7 +901,7 @@ int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     // what the caches hold is read through them: 30011 x 1024 f16 with gradients 164 us, 171 past them; what they do not, past them
     // (65536 x 4096 bf16 packed 351 us, 366)
     c.once = c.apart && a.rows * a.length * a.dim * kSize * (kShared ? 1 : 2) > (int64_t)256 << 20;
-    if (int rc = fill(c, s)) return rc;
+    if (int rc = fill(a, c, tile_of(L, kShared), s)) return rc;
     // (workgroups that pass on the states of sequences without tokens)
     const int64_t empty = a.bounds && (gradient ? a.dstate : a.last) ? std::min((a.sequences + kEmpty - 1) / kEmpty, kEmptyGrid) : 0;
     const int64_t tiles = c.count * c.tiles;
@@ -899,7 +931,7 @@ int run_short(const ScanArgs& a, hipStream_t s) {
 
 template <class T, int L>
 int by_gates(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
-    if (!gradient && scan_is_short(a)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
+    if (!gradient && scan_is_short(a, dtype)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
     if (a.decay) return a.shared ? run<T, L, true, true>(a, dtype, gradient, s) : run<T, L, true, false>(a, dtype, gradient, s);
     return a.shared ? run<T, L, false, true>(a, dtype, gradient, s) : run<T, L, false, false>(a, dtype, gradient, s);
 }
@@ -948,9 +980,13 @@ int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype) {
     return std::max(lay_out(c, nullptr, rows, length, dim, dtype, true, true), lay_out(c, nullptr, rows, length, dim, dtype, true, false));
 }
 
-bool scan_is_short(const ScanArgs& a) { return a.form == kRows && a.length <= kShort && !a.states; }
+bool scan_is_short(const ScanArgs& a, int dtype) {
+    if (a.form != kRows || a.length > kShortOfMany) return false;
+    const int len = span_len(a.dim, dtype);
+    return a.length <= kShort || a.rows * ((a.dim + len - 1) / len) >= kManyThreads * a.length;
+}
 
-int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a) ? a : flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, false, s); }
+int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a, dtype) ? a : flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, false, s); }
 int scan_grad(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, true, s); }
 
 int scan_copy(const float* from, float* to, int64_t n, hipStream_t s) {

@@ -384,7 +384,7 @@ int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim,
     a.last = d_last;
     a.states = d_states;
     a.work = d_work;
-    const bool waits = d_last && d_last == d_state && !scan_is_short(a);
+    const bool waits = d_last && d_last == d_state && !scan_is_short(a, dtype);
     if (waits) a.last = (float*)((char*)d_work + own);
     if (int rc = scan(a, dtype, s)) return rc;
     return waits ? scan_copy(a.last, d_last, states, s) : DCIH_OK;
