@@ -568,7 +568,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     Marks m(a, row, t0);
     const int piece = (int)(chain - row * c.strips) * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
     const bool live = piece < c.pieces;
-        if (a.form == kRows && a.bounds && t0 >= row_end(a, row))
+    if (a.form == kRows && a.bounds && t0 >= row_end(a, row))
         return write_zeros<T, L>(c, item, at, (raw_t*)a.h + (row * a.length + t) * a.dim + c0, a.dim, min((int64_t)U, m.length - t), live);
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;

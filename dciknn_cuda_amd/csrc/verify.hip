@@ -15,10 +15,11 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kChunk = 2048;                   // entries of a row that one wavefront adds up
+constexpr int kSumWaves = 6;                   // of a SIMD (512 x 131072 bf16 with the choice 44.7 us; 4, as the registers would have it, 47.5; 8 50)
 constexpr int kChoosers = 512, kChooserWaves = kChoosers / kWave;
 constexpr int64_t kMaxGrid = 1 << 23;
 
-struct alignas(16) Sum { double s; float m; float pad; };        // sum of 2^((z - m) c2), m = max z
+struct alignas(16) Sum { double s; float m; float pad; };        // sum of 2^((z - m) c2), m = 0 or max z
 
 // 2^x to 1e-15 of it: n whole, 2^f by its series.  0 for x = -inf, NaN for NaN.
 __device__ inline double exp2_wide(double x) {
@@ -68,20 +69,43 @@ __device__ inline double lanes_scan(double v) {
     return add_shifted<0x143, 0xc>(v);   // row_bcast:31 into rows 2 and 3
 }
 
-// 2^(i / 64), i below 64, as 2^x is put together for whole rows.
-constexpr int kParts = 64;
-constexpr double kC1 = 0.010830424696249145, kC2 = 5.864904955056169e-05, kC3 = 2.1173137155464774e-07, kC4 = 5.732851688640402e-10;      // (ln(2) / 64)^k / k!
-__device__ inline void fill_table(double* s_table) {
-    if (threadIdx.x < kParts) s_table[threadIdx.x] = exp2_wide((double)threadIdx.x / kParts);
+// 2^(i / 256), i below 256, as 2^x is put together for whole rows: less i / 256 in its exponent's place, so that adding all of n / 256 there
+// leaves 2^(n / 256), n = i mod 256.
+constexpr int kParts = 256;
+// 2^(f / 256), |f| <= 1/2, by its series to f^3, with 0.207 f^2 for f^4: 2.5e-14 off at most, and 1 at 0, so that a certain token's share is 1
+constexpr double kC1 = 0.0027076061740622863, kC2 = 3.665566060704036e-06, kC3 = 3.3083026805413713e-09;
+constexpr int kPart = 20 - 8;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ inline void fill_table(u32x2* s_table) {
+    static_assert(kParts == kThreads, "a part for each thread");
+    u32x2 part = __builtin_bit_cast(u32x2, exp2_wide((double)threadIdx.x / kParts));
+    part.y -= threadIdx.x << kPart;
+    s_table[threadIdx.x] = part;
+}
+// s + 2^(d scale / 256): 2^(whole / 256) 2^(rest / 256).  The sum with 1.5 2^52 holds `whole` in its low word.
+__device__ inline double add_power(double d, double scale, double s, const u32x2* s_table) {
+    constexpr double kMagic = 6755399441055744.0;
+    const double t = __builtin_fma(d, scale, kMagic), f = __builtin_fma(d, scale, -(t - kMagic));
+    const uint32_t whole = (uint32_t)__builtin_bit_cast(unsigned long long, t);
+    double q = kC3;
+    q = __builtin_fma(q, f, kC2);
+    q = __builtin_fma(q, f, kC1);
+    q = __builtin_fma(q, f, 1.0);
+    u32x2 part = s_table[whole & (kParts - 1)];
+    part.y += whole << kPart;
+    return __builtin_fma(__builtin_bit_cast(double, part), q, s);
 }
 
 // A wavefront adds up `per` chunks of a row, one after the other.  Rows behind a sequence's last draft are asked for by nobody.
-// Bound by its instructions: 10 of 64 bits and 9 others an entry, 512 x 131072 bf16 43 us (the bytes alone take 25).
+// Weights are relative to 1 where 64 bits have room for that, as logits have it: no look for the largest first.  A sum that says otherwise
+// is formed again, relative to the chunk's largest.
+// Bound by its instructions: 9 of 64 bits and 6 others an entry, 512 x 131072 bf16 35 us (the bytes alone take 25).  By a table of 64 and
+// one more term, relative to each chunk's largest: 43.
 template <class T>
-__global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums, int chunks, int per, int64_t first) {
+__global__ __launch_bounds__(kThreads, kSumWaves) void sums_kernel(VerifyArgs a, Sum* sums, int chunks, int per, int64_t first) {
     using P = Piece<T>;
     constexpr int U = kChunk / kWave / P::kLen;
-    __shared__ double s_table[kParts];
+    __shared__ u32x2 s_table[kParts];
     fill_table(s_table);
     __syncthreads();
     const int splits = (chunks + per - 1) / per, lane = lane_id();
@@ -94,6 +118,8 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
     const Row<T> r(a.z, row, a.stride, a.vocab);
     const double scale = a.c2 * kParts;
     const double deepest = -1000.0 / a.c2;                 // weights of less than 2^-1000 are that
+    const bool plain = a.c2 > 1e-27 && a.c2 < 1e30;        // `most` is far from the ends of its type
+    const float most = (float)(900.0 / a.c2);
     for (int c = from; c < to; c++) {
         u32x4 raw[U];
         const int piece = c * (kChunk / P::kLen) + lane;
@@ -103,45 +129,47 @@ __global__ __launch_bounds__(kThreads) void sums_kernel(VerifyArgs a, Sum* sums,
 #pragma unroll
             for (int u = 0; u < U; u++) raw[u] = r.load(piece + u * kWave);
         }
-        float m = kNoLogit;
+        float m = 0.f;
         bool bad = false;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            float z[P::kLen];
-            P::unpack(raw[u], z);
-#pragma unroll
-            for (int k = 0; k < P::kLen; k++) {
-                m = fmaxf(m, z[k]);
-                bad |= z[k] != z[k];
-            }
-        }
-        m = max_of_lanes(m);
-        const double base = base_of(m);
         double s = 0.0;
+        if (plain) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float z[P::kLen];
-            P::unpack(raw[u], z);
+            for (int u = 0; u < U; u++) {
+                float z[P::kLen];
+                P::unpack(raw[u], z);
 #pragma unroll
-            for (int k = 0; k < P::kLen; k++) {
-                // 2^y = 2^(whole / 64) 2^(rest / 64), |rest| <= 1/2: the series ends 4e-14 short.  The sum with 1.5 2^52 holds `whole`
-                // in its low word.
-                constexpr double kMagic = 6755399441055744.0;
-                const double d = __builtin_fmax((double)z[k] - base, deepest);
-                const double t = __builtin_fma(d, scale, kMagic), f = __builtin_fma(d, scale, -(t - kMagic));
-                const int whole = (int)__builtin_bit_cast(unsigned long long, t);
-                double q = kC4;
-                q = __builtin_fma(q, f, kC3);
-                q = __builtin_fma(q, f, kC2);
-                q = __builtin_fma(q, f, kC1);
-                q = __builtin_fma(q, f, 1.0);
-                unsigned long long w = __builtin_bit_cast(unsigned long long, s_table[whole & (kParts - 1)]);
-                w += (unsigned long long)(uint32_t)((whole >> 6) << 20) << 32;
-                s = __builtin_fma(__builtin_bit_cast(double, w), q, s);
+                for (int k = 0; k < P::kLen; k++) {
+                    bad |= z[k] != z[k];
+                    s = add_power((double)__builtin_amdgcn_fmed3f(z[k], -most, most), scale, s, s_table);
+                }
             }
+            s = lanes_sum(s);
         }
-        s = lanes_sum(s);
-        if (m == kNoLogit) s = 0.0;
+        if (!(s > 0x1p-800 && s < 0x1p890)) {              // nothing of -inf counts, nothing was cut
+            m = kNoLogit;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float z[P::kLen];
+                P::unpack(raw[u], z);
+#pragma unroll
+                for (int k = 0; k < P::kLen; k++) {
+                    m = fmaxf(m, z[k]);
+                    bad |= z[k] != z[k];
+                }
+            }
+            m = max_of_lanes(m);
+            const double base = base_of(m);
+            s = 0.0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float z[P::kLen];
+                P::unpack(raw[u], z);
+#pragma unroll
+                for (int k = 0; k < P::kLen; k++) s = add_power(__builtin_fmax((double)z[k] - base, deepest), scale, s, s_table);
+            }
+            s = lanes_sum(s);
+            if (m == kNoLogit) s = 0.0;
+        }
         if (__any(bad) || m == -kNoLogit) s = __builtin_nan("");
         if (lane == 0) sums[row * chunks + c] = Sum{s, m, 0.f};
     }

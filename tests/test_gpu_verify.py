@@ -63,6 +63,25 @@ def test_temperatures(gpu, temperature):
     check(gpu, z, drafts, u, temperature=temperature)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("temperature", [1e-29, 1e-3, 1.0, 1e3, 1e29])
+def test_rows_of_all_magnitudes(gpu, temperature, dtype):
+    """Some stretches of a row beyond what powers of 2 in 64 bits reach, up or down, others not; all of it shifted; nothing but that."""
+    z, drafts, u, ids, teacher = inputs(8, 2, 9000, 6, "f32", seed=21)
+    z[0, :, :2048] += 2000.0
+    z[1, :, 2048:5000] -= 2000.0
+    z[2, :, :] -= 700.0
+    z[3, :, 4096:] += 600.0
+    z[4, :, :4096] = -math.inf
+    z[5] += 3000.0
+    z[6] -= 3000.0
+    z[7, :, 3000:] = -math.inf
+    z[7, :, :2048] -= 630.0
+    z = (z * temperature).clamp(-3e38, 3e38).to(TYPES[dtype])
+    check(gpu, z, drafts, u, ids, teacher, temperature, on_border=True)
+    check(gpu, z, drafts, u, temperature=temperature, on_border=True)
+
+
 @pytest.mark.parametrize("slots", [200, 1023, 1024])
 @pytest.mark.parametrize("teacher_type", ["f32", "f16", "bf16"])
 def test_many_slots(gpu, slots, teacher_type):
