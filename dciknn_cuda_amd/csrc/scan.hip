@@ -29,10 +29,14 @@ constexpr int tile_of(int len, bool shared) { return len == 8 || (len == 4 && !s
 // Wavefronts of a SIMD: registers enough for a tile, tiles enough to hide one another's waits (one more each way spills: 8 x 4096 x 2048
 // with gradients 262 us instead of 238; one less is as fast).
 constexpr int kWaves = 4, kBackWaves = 3;
-// Tokens that one thread takes: 32 x 1 x 4096 bf16 3.4 us, a launch.  More where threads are many: 512 x 40 x 2048 bf16 42 us, 58 by tiles (512 x 64 x
-// 1024 38 and 43, 256 x 24 x 1024 13.2 and 13.8; but 256 x 32 x 1024 17.1 and 14.6).
-constexpr int kShort = 16, kShortOfMany = 64;
-constexpr int64_t kManyThreads = 1280;             // for each token
+// Tokens that one thread takes.  More where channels are many, for each token (512 x 40 x 2048 bf16 42 us, 58 by tiles; 512 x 48 x 1024 28 and 43,
+// 128 x 48 x 1024 23 and 13).
+constexpr int kShort = 32, kShortOfMany = 64;
+constexpr int64_t kManyPieces = 1280;
+// Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 5.2 us,
+// 8.7 by pieces; 32 x 32 x 1024 7.1, 15.3, 8.5 by tiles; but 512 x 8 x 1024 8.3 and 6.6).  Twice as many where sequences are longer than kSteps.
+constexpr int64_t kSingles = 1 << 17;
+constexpr int kSteps = 16;
 constexpr int kApart = 32;                         // words from one chain's counter to the next: a line takes an atomic operation in 11 ns
 constexpr int64_t kMaxGrid = 1 << 23;
 constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
@@ -138,10 +142,10 @@ template <bool kDecay> __device__ inline Gate coefs_of(float packed) {
 template <bool kDecay> __device__ inline float step(float h, float x, Gate c) { return __builtin_fmaf(c.a, h, kDecay ? x : c.keep * x); }
 
 // ---- one thread a channel ----------------------------------------------------------------
-// A server's step, or its drafts: few tokens of many sequences.  The state may be written where it is read.
-template <class T, int L, bool kDecay>
+// A server's step, or its drafts: few tokens of many sequences.  The state may be written where it is read.  Bound by the launch (32 x 1 x 4096 bf16
+// 2.7 us replayed), then by the chain of a wavefront's tokens (8: 4.0), then memory (1024 x 8 x 4096 39 us, 6 TB/s).
+template <class T, int L, bool kDecay, int U>
 __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces, int64_t first) {
-    constexpr int U = 4;
     using raw_t = typename T::raw;
     const int64_t i = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int64_t b = i / pieces;
@@ -159,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
         Span<T, L> xs[U], gs[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t t = min(t0 + u, length - 1);
+            const int64_t t = min((int64_t)t0 + u, max(len, (int64_t)1) - 1);
             xs[u].load(x + t * a.x_step);
             gs[u].load(g + t * a.g_step);
         }
@@ -923,7 +927,9 @@ int run_short(const ScanArgs& a, hipStream_t s) {
     const int pieces = (a.dim + L - 1) / L;
     const int64_t threads = a.rows * pieces, most = kMaxGrid * kThreads;
     for (int64_t first = 0; first < threads; first += most) {
-        short_kernel<T, L, kDecay><<<(uint32_t)((std::min(most, threads - first) + kThreads - 1) / kThreads), kThreads, 0, s>>>(a, pieces, first);
+        const uint32_t grid = (uint32_t)((std::min(most, threads - first) + kThreads - 1) / kThreads);
+        if (a.length > 4) short_kernel<T, L, kDecay, 8><<<grid, kThreads, 0, s>>>(a, pieces, first);
+        else short_kernel<T, L, kDecay, 4><<<grid, kThreads, 0, s>>>(a, pieces, first);
         DCIH_HIP(hipGetLastError());
     }
     return 0;
@@ -931,7 +937,10 @@ int run_short(const ScanArgs& a, hipStream_t s) {
 
 template <class T, int L>
 int by_gates(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
-    if (!gradient && scan_is_short(a, dtype)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
+    if (!gradient && scan_is_short(a, dtype)) {
+        if (L > 1 && a.rows * a.dim > kSingles * (a.length > kSteps ? 2 : 1)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
+        return a.decay ? run_short<T, 1, true>(a, s) : run_short<T, 1, false>(a, s);
+    }
     if (a.decay) return a.shared ? run<T, L, true, true>(a, dtype, gradient, s) : run<T, L, true, false>(a, dtype, gradient, s);
     return a.shared ? run<T, L, false, true>(a, dtype, gradient, s) : run<T, L, false, false>(a, dtype, gradient, s);
 }
@@ -983,7 +992,7 @@ int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype) {
 bool scan_is_short(const ScanArgs& a, int dtype) {
     if (a.form != kRows || a.length > kShortOfMany) return false;
     const int len = span_len(a.dim, dtype);
-    return a.length <= kShort || a.rows * ((a.dim + len - 1) / len) >= kManyThreads * a.length;
+    return a.length <= kShort || a.rows * ((a.dim + len - 1) / len) >= kManyPieces * a.length;
 }
 
 int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a, dtype) ? a : flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, false, s); }

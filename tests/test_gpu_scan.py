@@ -268,6 +268,26 @@ def test_state_in_place(gpu, size, with_lengths):
     assert last2 is kept and kept._version > version and torch.equal(kept, last) and torch.equal(h2, h)
 
 
+MANY = [(140, 1, 1023), (140, 5, 1023), (130, 20, 1023), (260, 17, 1023), (400, 33, 1023)]      # by channels and by pieces of them, whose last two overlap
+
+
+@pytest.mark.parametrize("size", MANY, ids=str)
+@pytest.mark.parametrize("dtype, decay, view", [("f32", False, "time first"), ("f16", True, "part of wider tokens"), ("bf16", False, "every second token")])
+def test_many_channels(gpu, size, dtype, decay, view):
+    lengths = [(7 * i) % (size[1] + 1) for i in range(size[0])]
+    check(gpu, *size, dtype, decay, view=VIEWS[view], lengths=lengths if decay else None, grad=size[0] == 400 and not decay)
+
+
+@pytest.mark.parametrize("size", MANY, ids=str)
+def test_many_states_in_place(gpu, size):
+    x, gates, s, _, _ = (t.cuda() for t in inputs(*size, "bf16", False, False))
+    lengths = torch.arange(size[0], device="cuda") % (size[1] + 1)
+    h, last = gpu.gated_scan(x, gates, s, lengths=lengths)
+    kept = s.clone()
+    h2, _ = gpu.gated_scan(x, gates, kept, lengths=lengths, last=kept)
+    assert torch.equal(kept, last) and torch.equal(h2, h)
+
+
 def test_steps_are_the_sequence(gpu):
     """A server's steps, one by one, some drafts at a time, and the prompt in one call: the same within roundings."""
     x, gates, s, _, _ = (t.cuda() for t in inputs(4, 60, 40, "f32", False, False))
