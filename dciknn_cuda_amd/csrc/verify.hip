@@ -106,15 +106,20 @@ __global__ __launch_bounds__(kThreads, kSumWaves) void sums_kernel(VerifyArgs a,
     using P = Piece<T>;
     constexpr int U = kChunk / kWave / P::kLen;
     __shared__ u32x2 s_table[kParts];
-    fill_table(s_table);
-    __syncthreads();
     const int splits = (chunks + per - 1) / per, lane = lane_id();
     const int64_t item = first + (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = item / splits, b = row / (a.drafts + 1);
+    const int i = b < a.n ? (int)(row - b * (a.drafts + 1)) : 0, from = (int)(item - row * splits) * per, to = min(chunks, from + per);
+    int64_t draft = lane < i ? id_at(a.ids, a.wide_ids, b * a.drafts + lane) : 0;
+    fill_table(s_table);
+    __syncthreads();
     if (b >= a.n) return;
-    const int i = (int)(row - b * (a.drafts + 1)), from = (int)(item - row * splits) * per, to = min(chunks, from + per);
-    for (int j = lane; __any(j < i); j += kWave)
-        if (__any(j < i && id_at(a.ids, a.wide_ids, b * a.drafts + j) < 0)) return;
+    for (int j = lane;;) {
+        if (__any(draft < 0)) return;
+        j += kWave;
+        if (!__any(j < i)) break;
+        draft = j < i ? id_at(a.ids, a.wide_ids, b * a.drafts + j) : 0;
+    }
     const Row<T> r(a.z, row, a.stride, a.vocab);
     const double scale = a.c2 * kParts;
     const double deepest = -1000.0 / a.c2;                 // weights of less than 2^-1000 are that
@@ -187,6 +192,13 @@ __device__ inline double scan_threads(double v, double* s_part) {
     return before + v;
 }
 
+// The largest thread that says yes and what it brings, which grows with the threads.  (By the last lane of each wavefront: an atomic operation of 64
+// lanes takes them one by one, 1.5 us.)
+__device__ inline void last_that(bool yes, int value, int* s_last) {
+    const unsigned long long lanes = __ballot(yes);
+    if (lanes && lane_id() == kWave - 1 - __builtin_clzll(lanes)) atomicMax(s_last, value);
+}
+
 __device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
     switch (a.teacher_dtype) {
         case DCIH_F32: return ((const float*)a.teacher)[i];
@@ -198,7 +210,8 @@ __device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
 constexpr int kSlots = 1024, kNearChunks = 256;      // chunks whose amounts are added up beside the slots
 constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.693147180559945309417;
 
-// 15 us of 64 sequences with 7 drafts of 64 slots each, 11 of 4 with 4 drafts for certain: a chain of a dozen loads that wait for one another.
+// 11 us of 64 sequences with 7 drafts of 64 slots each, 7.4 of 4 with 4 drafts for certain: a chain of loads, exponentials and joined sums that wait
+// for one another.
 // One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
 // from the row that it comes from, by chunks, then among the entries of one.
 template <class T>
@@ -206,7 +219,7 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     constexpr int kPer = kChunk / kChoosers;
     __shared__ double s_total[kMaxDrafts + 1], s_part[kChooserWaves], s_weight[kChunk], s_gone[kSlots], s_target;
     __shared__ unsigned long long s_fixed[kSlots], s_taken[kNearChunks];
-    __shared__ float s_max[kMaxDrafts + 1], s_logp[kMaxDrafts];
+    __shared__ float s_max[kMaxDrafts + 1], s_z[kMaxDrafts + 1];
     __shared__ int s_kept[kMaxDrafts], s_id[kSlots], s_chunk_of[kSlots], s_chunk, s_token, s_last, s_slots;
     const int64_t b = first + blockIdx.x;
     const int k = a.drafts, lane = lane_id(), wave = threadIdx.x / kWave, tid = threadIdx.x;
@@ -214,6 +227,21 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     const double c2 = a.c2;
     const typename T::raw* logits = (const typename T::raw*)a.z + b * (k + 1) * a.stride;
     auto draft_at = [&](int i) { return id_at(a.ids, a.wide_ids, b * k + i); };
+    // what a row takes from memory, for the first one of a wavefront before it is known whether there is such a draft
+    struct Asked { Sum part; int64_t draft, id; float number, teacher; };
+    auto ask = [&](int i) {
+        Asked r{Sum{0.0, kNoLogit, 0.f}, -1, -1, 0.f, kNoLogit};
+        if (i <= k && lane < chunks) r.part = sums[(b * (k + 1) + i) * chunks + lane];
+        if (i >= k) return r;
+        r.draft = draft_at(i);
+        r.number = a.uniforms[b * (k + 1) + i];
+        if (a.slot_ids && lane < a.slots) {
+            r.id = id_at(a.slot_ids, a.wide_slots, (b * k + i) * a.slots + lane);
+            r.teacher = teacher_at(a, (b * k + i) * a.slots + lane);
+        }
+        return r;
+    };
+    Asked r = ask(wave);
     // how many drafts there are
     if (tid == 0) {
         s_slots = k;                                  // (for the moment)
@@ -224,50 +252,45 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
         if (draft_at(i) < 0) atomicMin(&s_slots, i);
     __syncthreads();
     const int given = s_slots;
-    for (int i = wave; i <= given; i += kChooserWaves) {
+    for (int i = wave; i <= given; i += kChooserWaves, r = ask(i)) {
+        const float z = i < given && r.draft < a.vocab ? (float)logits[i * a.stride + r.draft] : kNoLogit;
         const Sum* part = sums + (b * (k + 1) + i) * chunks;
-        float m = kNoLogit;
-        for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, part[c].m);
+        float m = r.part.m;
+        for (int c = lane + kWave; c < chunks; c += kWave) m = fmaxf(m, part[c].m);
         m = max_of_lanes(m);
         const double base = base_of(m);
-        double s = 0.0;
-        for (int c = lane; c < chunks; c += kWave) {
-            const Sum p = part[c];
-            s += p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
-        }
+        auto share_of = [&](const Sum& p) { return p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base); };
+        double s = share_of(r.part);
+        for (int c = lane + kWave; c < chunks; c += kWave) s += share_of(part[c]);
         s = lanes_sum(s);
         if (lane == 0) {
             s_total[i] = s;
             s_max[i] = m;
+            s_z[i] = z;
         }
         if (i == given) continue;
-        const int64_t t = draft_at(i);
-        // the probability that it was drawn with
-        double q = 1.0;
+        // the probability that it was drawn with: its / all
+        double its = 1.0, all = 1.0;
         if (a.slot_ids) {
             const int64_t at = (b * k + i) * a.slots;
-            float top = kNoLogit;
-            for (int j = lane; j < a.slots; j += kWave)
+            float top = r.id >= 0 ? r.teacher : kNoLogit;
+            for (int j = lane + kWave; j < a.slots; j += kWave)
                 if (id_at(a.slot_ids, a.wide_slots, at + j) >= 0) top = fmaxf(top, teacher_at(a, at + j));
             top = max_of_lanes(top);
             const double top_base = base_of(top);
-            double all = 0.0, its = 0.0;
-            for (int j = lane; j < a.slots; j += kWave) {
+            all = r.id < 0 ? 0.0 : weight_of(r.teacher, kLog2eWide, top_base);
+            its = r.id == r.draft ? all : 0.0;
+            for (int j = lane + kWave; j < a.slots; j += kWave) {
                 const int64_t id = id_at(a.slot_ids, a.wide_slots, at + j);
                 const double w = id < 0 ? 0.0 : weight_of(teacher_at(a, at + j), kLog2eWide, top_base);
                 all += w;
-                its += id == t ? w : 0.0;
+                its += id == r.draft ? w : 0.0;
             }
             all = lanes_sum(all);
             its = lanes_sum(its);
-            q = all == 0.0 ? 0.0 : its / all;
         }
-        if (lane == 0) {
-            const float z = t < a.vocab ? (float)logits[i * a.stride + t] : kNoLogit;
-            const double p = weight_of(z, c2, base);
-            s_kept[i] = p > 0.0 && (double)a.uniforms[b * (k + 1) + i] * q * s < p;
-            s_logp[i] = (float)(((double)z - base) * c2 * kLn2Wide - log(s));
-        }
+        const double p = weight_of(z, c2, base);
+        if (lane == 0) s_kept[i] = p > 0.0 && (all == 0.0 || (double)r.number * its * s < p * all);
     }
     __syncthreads();
     int kept = 0;
@@ -391,7 +414,7 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     }
     if (fine) {
         const double target = min(max((double)u, 0.0), 1.0) * all;
-        if (own > 0.0 && before - own <= target) atomicMax(&s_last, tid);      // (the last thread with weights below the target)
+        last_that(own > 0.0 && before - own <= target, tid, &s_last);      // (with weights below the target)
         __syncthreads();
         if (tid == s_last) {
             double sum = before - own;
@@ -437,7 +460,7 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
                 if (w[e] > 0.0 && sum <= s_target) found = tid * kPer + e;
                 sum += w[e];
             }
-            if (found >= 0) atomicMax(&s_last, found);
+            last_that(found >= 0, found, &s_last);
             __syncthreads();
             if (tid == 0 && s_last >= 0) s_token = from + s_last;
         }
@@ -446,8 +469,11 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     const int token = s_token;
     for (int i = tid; i <= k; i += kChoosers) {
         const int64_t t = i < kept ? draft_at(i) : i == kept ? token : -1;
-        float logp = i < kept ? s_logp[i] : 0.f;
-        if (i == kept) logp = t >= 0 ? (float)(((double)(float)row[t] - base) * c2 * kLn2Wide - log(total)) : __builtin_nanf("");
+        float logp = 0.f;
+        if (i <= kept) {
+            const float z = i < kept ? s_z[i] : t >= 0 ? (float)row[t] : __builtin_nanf("");
+            logp = (float)(((double)z - base_of(s_max[i])) * c2 * kLn2Wide - log(s_total[i]));
+        }
         a.tokens[b * (k + 1) + i] = (int32_t)t;
         a.logprobs[b * (k + 1) + i] = logp;
     }
