@@ -487,6 +487,10 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gates, cons
     states_of(into, s, x, "last");
     if (wants_grad(*into)) bad_value("last must not require a gradient");
     if (into->is_alias_of(x) || into->is_alias_of(gates)) bad_value("last must not share the memory of x or gates");
+    if (state.defined() && into->numel()) {
+        const char *a = (const char*)state.data_ptr(), *b = (const char*)into->data_ptr();
+        if (a != b && a < b + into->nbytes() && b < a + state.nbytes()) bad_value("last must be state, or share no memory with it");
+    }
     into->unsafeGetTensorImpl()->bump_version();
     const auto got = scan_forward(s, x, gates, state, *into, false);
     return {got[0], *into};

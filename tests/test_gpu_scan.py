@@ -398,6 +398,15 @@ def test_offsets_beyond_31_bits(gpu):
     assert torch.equal(h[:300], gpu.gated_scan(x[:384], gates[:384])[0][:300])
 
 
+def test_last_states_that_overlap_the_first(gpu):
+    pool, x = torch.ones(5, 8, device="cuda"), torch.zeros(3, 40, 8, device="cuda")
+    with pytest.raises(ValueError, match="last"):
+        gpu.gated_scan(x, x.clone(), pool[:3], last=pool[1:4])
+    h, last = gpu.gated_scan(x, x.clone(), pool[:3], last=pool[:3])              # in its place, by another view of it
+    assert (last == 2.0 ** -40).all() and torch.equal(pool[:3], last) and (pool[3:] == 1).all() and (h[:, 0] == 0.5).all()
+    gpu.gated_scan(x[:2], x[:2].clone(), pool[3:], last=pool[:2])
+
+
 def test_refusals(gpu):
     z = lambda *shape, dtype=torch.float32: torch.zeros(*shape, device="cuda", dtype=dtype)          # noqa: E731
     x, g, s = z(2, 5, 8), z(2, 5, 8), z(2, 8)
