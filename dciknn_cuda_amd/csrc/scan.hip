@@ -37,6 +37,10 @@ constexpr int64_t kManyPieces = 1280;
 // 8.7 by pieces; 32 x 32 x 1024 7.1, 15.3, 8.5 by tiles; but 512 x 8 x 1024 8.3 and 6.6).  Twice as many where sequences are longer than kSteps.
 constexpr int64_t kSingles = 1 << 17;
 constexpr int kSteps = 16;
+// Up to so many chains of so many tiles or more each are joined by a launch of their own (see link_kernel): 1 x 262144 x 64 bf16 81 us, with gradients 178,
+// chained 201 and 402; x 256 171 and 429, 226 and 444; x 384 241 and 582, 247 and 531; 1 x 16384 x 64 18 and 21, with gradients 73 and 68, the host's two
+// launches more.
+constexpr int kFewChains = 4, kManyTiles = 192;
 constexpr int kApart = 32;                         // words from one chain's counter to the next: a line takes an atomic operation in 11 ns
 constexpr int64_t kMaxGrid = 1 << 23;
 constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
@@ -204,6 +208,7 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
 // ---- tiles -------------------------------------------------------------------------------
 // A chain is a strip of kLanes pieces of one row of tokens; its tiles follow one another.  Workgroups take tiles by counters, those of a
 // chain in order: what a tile waits for was taken before it, by a workgroup that waits for nothing taken later.
+enum Phase { kChained, kMaps, kApply };              // all at once; or maps alone, then (behind link_kernel) what they lead to
 struct Chains {
     int pieces, strips, slots;         // pieces of a row; strips of them; channels of a strip, those beyond the row included
     int64_t tiles, count;              // tiles of a chain, chains
@@ -214,6 +219,7 @@ struct Chains {
     uint32_t* states;                  // [count][tiles][slots] the state behind a tile
     int32_t* from;                     // (kPacked) [tiles] the last sequence that begins before a tile
     float* sums;                       // [count][tiles][slots] (gradient of shared gates)
+    Phase phase;
 };
 
 int span_len(int dim, int dtype) {
@@ -303,7 +309,7 @@ __device__ inline uint32_t word_of(float v) {
 // few of its cache's channels only (65536 x 4096 bf16 packed 351 us, 403 so).  Strips that share lines with their neighbours stand 8
 // items from them, so that most of them are on one XCD and close in time (30011 x 1023 f16 with gradients 202 us, 239 apart; with
 // rows of whole lines 375 and 351 of the first case).  By one thread; returns chain * tiles + place.
-__device__ inline int64_t take_tile(const Chains& c, int64_t i) {
+__device__ inline int64_t take_tile(const Chains& c, Phase phase, int64_t i) {
     if (c.tiles == 1) return i;
     const int64_t round = i / c.count, at = i - round * c.count, row = at / c.strips;
     int strip = (int)(at - row * c.strips);
@@ -312,6 +318,7 @@ __device__ inline int64_t take_tile(const Chains& c, int64_t i) {
         strip = xcd * (c.strips / 8) + min(xcd, rest) + strip / 8;
     }
     const int64_t chain = row * c.strips + (strip + round) % c.strips;
+    if (phase != kChained) return chain * c.tiles + round;
     return chain * c.tiles + (atomicAdd(&c.tickets[chain * kApart], 1u) - kUnset);        // the counter begins at kUnset
 }
 
@@ -362,7 +369,7 @@ __device__ float carry_of(const Chains& c, int64_t chain, int64_t at, int slot) 
 // A channel's groups joined, by one thread: map (A, B) of each in the direction of the scan, `resets` those whose result does not
 // depend on what enters.  Leaves in B what enters each group.
 template <int kGroups, bool kBack>
-__device__ void join_groups(const Chains& c, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
+__device__ void join_groups(const Chains& c, Phase phase, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
     auto place = [&](int g) { return (kBack ? kGroups - 1 - g : g) * c.slots + slot; };
     float in = 0.f;
     if (c.tiles > 1) {
@@ -375,7 +382,11 @@ __device__ void join_groups(const Chains& c, int64_t chain, int64_t at, int slot
             A *= ga;
         }
         const int64_t cell = chain * c.tiles + at, word = cell * c.slots + slot;
-        const bool follows = at + 1 < c.tiles;
+        const bool follows = at + 1 < c.tiles && phase == kChained;
+        if (phase == kMaps) {
+            c.maps[word] = (uint64_t)word_of(B) << 32 | (resets ? kUnset : word_of(A));
+            return;
+        }
         if (resets) {
             if (follows) post(c.states + word, word_of(B));
             if (follows && slot == 0) post(c.flags + cell, kStateSet);
@@ -383,7 +394,7 @@ __device__ void join_groups(const Chains& c, int64_t chain, int64_t at, int slot
             post(c.maps + word, (uint64_t)word_of(B) << 32 | word_of(A));
             if (slot == 0) post(c.flags + cell, kMapSet);
         }
-        if (at) in = carry_of(c, chain, at, slot);
+        if (at) in = phase == kApply ? __builtin_bit_cast(float, c.states[word - c.slots]) : carry_of(c, chain, at, slot);
         if (!resets && follows) {
             post(c.states + word, word_of(__builtin_fmaf(A, in, B)));
             if (slot == 0) post(c.flags + cell, kStateSet);
@@ -449,19 +460,21 @@ __device__ inline int64_t row_end(const ScanArgs& a, int64_t row) {
 
 // A tile behind the end of a row's sequence: zeros, without a look at the tokens.  What enters the next tile is zero too.
 template <class T, int L>
-__device__ inline void write_zeros(const Chains& c, int64_t item, int64_t at, typename T::raw* out, int64_t step, int64_t tokens, bool live) {
+__device__ inline void write_zeros(const Chains& c, Phase phase, int64_t item, int64_t at, typename T::raw* out, int64_t step, int64_t tokens, bool live) {
     float zeros[L];
 #pragma unroll
     for (int k = 0; k < L; k++) zeros[k] = 0.f;
     if (out && live)
         for (int64_t u = 0; u < tokens; u++) Span<T, L>::store(out + u * step, zeros);
-    if (at + 1 < c.tiles && threadIdx.x < c.slots) {
-        post(c.states + (item - item % c.tiles + at) * c.slots + threadIdx.x, 0u);
-        if (threadIdx.x == 0) post(c.flags + item - item % c.tiles + at, kStateSet);
+    if (at >= c.tiles || threadIdx.x >= c.slots) return;
+    const int64_t cell = item - item % c.tiles + at, word = cell * c.slots + threadIdx.x;
+    if (phase == kMaps) c.maps[word] = kUnset;
+    if (phase == kChained && at + 1 < c.tiles) {
+        post(c.states + word, 0u);
+        if (threadIdx.x == 0) post(c.flags + cell, kStateSet);
     }
 }
 
-// By all threads; `s_first`, `s_end` and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
 // What finds the sequences of a tile (kPacked): the first of them that may begin or end there, and each thread's bounds, asked for ahead
 // of the tokens (what the vector memory answers comes in order).
 struct Found {
@@ -480,6 +493,7 @@ struct Found {
         hi = cut(a, id_at(a.bounds, a.wide_bounds, mine + 1));
     }
 };
+// By all threads; `s_first`, `s_end` and `s_marked` (a bit for each `per` tokens) are ready behind the next barrier.
 template <int kTokens>
 __device__ inline void find_marks(const ScanArgs& a, Found f, Marks& m, int per, int (&s_first)[kTokens], int (&s_end)[kTokens], uint32_t& s_marked) {
     m.lo = 0;
@@ -551,11 +565,12 @@ template <class Body> __device__ __forceinline__ void by_marks(bool any, Body bo
 // A tile, read and written once: bound by memory (65536 x 4096 bf16 355 us, 1.61 GB at 4.5 TB/s; 8 x 4096 x 2048 88 us) where chains are many or long,
 // by the wait for the tile before where one short row is all there is (20000 x 64 f32, 79 tiles: 18 us).  Without that wait the
 // second took 92 us of 113 at the time, without the gates' arithmetic 106.
-template <class T, int L, bool kDecay, bool kShared>
+template <class T, int L, bool kDecay, bool kShared, bool kPhased>
 __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
     constexpr int kTile = tile_of(L, kShared), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32, "a bit for each group");
     using raw_t = typename T::raw;
+    const Phase phase = kPhased ? c.phase : kChained;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
     __shared__ uint32_t s_marked, s_resets;
@@ -564,7 +579,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
     if (threadIdx.x == 0) {
         s_resets = 0;
-        s_item = take_tile(c, first + blockIdx.x);
+        s_item = take_tile(c, phase, first + blockIdx.x);
     }
     __syncthreads();
     const int64_t item = uniform(s_item), chain = item / c.tiles, at = item - chain * c.tiles, row = chain / c.strips;
@@ -573,7 +588,7 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     const int piece = (int)(chain - row * c.strips) * kLanes + lane, c0 = min(min(piece, c.pieces - 1) * L, a.dim - L);
     const bool live = piece < c.pieces;
     if (a.form == kRows && a.bounds && t0 >= row_end(a, row))
-        return write_zeros<T, L>(c, item, at, (raw_t*)a.h + (row * a.length + t) * a.dim + c0, a.dim, min((int64_t)U, m.length - t), live);
+        return write_zeros<T, L>(c, phase, item, at, phase == kMaps ? nullptr : (raw_t*)a.h + (row * a.length + t) * a.dim + c0, a.dim, min((int64_t)U, m.length - t), live);
     const raw_t* x = (const raw_t*)a.x + row * a.x_row + c0;
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
     const Found found(a, c, at, t0);
@@ -640,9 +655,10 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; }
     __syncthreads();
     if (threadIdx.x < kSlots) {
-        join_groups<kGroups, false>(c, chain, at, threadIdx.x, s_resets, s_a, s_b);
-        if (a.states) a.states[item * kSlots + threadIdx.x] = s_b[threadIdx.x];
+        join_groups<kGroups, false>(c, phase, chain, at, threadIdx.x, s_resets, s_a, s_b);
+        if (a.states && phase != kMaps) a.states[item * kSlots + threadIdx.x] = s_b[threadIdx.x];
     }
+    if (phase == kMaps) return;
     __syncthreads();
     if (!live) return;
     float h[L];
@@ -666,11 +682,12 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
 
 // The gradient of a tile: 8 x 4096 x 2048 bf16 155 us (671 MB at 4.3 TB/s; 133 with neither waits nor sums).  The states go forward from the one kept, the gradient that reaches them goes back from the tile
 // behind: its maps are s -> A s + Q of the same A.
-template <class T, int L, bool kDecay, bool kShared>
+template <class T, int L, bool kDecay, bool kShared, bool kPhased>
 __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArgs a, Chains c, int64_t first, int64_t empty) {
     constexpr int kTile = tile_of(L, kShared), kGroups = kThreads / kLanes, U = kTile / kGroups, kSlots = kLanes * L;
     static_assert(kGroups <= 32 && 2 * kSlots <= kThreads, "a bit for each group, threads for both directions");
     using raw_t = typename T::raw;
+    const Phase phase = kPhased ? c.phase : kChained;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
     __shared__ uint32_t s_marked, s_resets, s_back_resets;
@@ -679,7 +696,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
     if (threadIdx.x == 0) {
         s_resets = s_back_resets = 0;
-        s_item = take_tile(c, first + blockIdx.x);
+        s_item = take_tile(c, phase, first + blockIdx.x);
     }
     __syncthreads();
     const int64_t item = uniform(s_item), chain = item / c.tiles, at = item - chain * c.tiles, row = chain / c.strips;
@@ -692,13 +709,15 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     const raw_t* g = (const raw_t*)a.gates + (kShared ? 0 : row * a.g_row) + c0;
     if (a.form == kRows && a.bounds && t0 >= row_end(a, row)) {
         const int64_t place = (row * a.length + t) * a.dim + c0, own = min((int64_t)U, m.length - t);
-        write_zeros<T, L>(c, item, at, a.dx ? (raw_t*)a.dx + place : nullptr, a.dim, own, live);
-        if (!kShared && a.dgates) write_zeros<T, L>(c, item, c.tiles, (raw_t*)a.dgates + place, a.dim, own, live);
+        write_zeros<T, L>(c, phase, item, at, a.dx && phase != kMaps ? (raw_t*)a.dx + place : nullptr, a.dim, own, live);
+        if (phase == kMaps) return;
+        if (!kShared && a.dgates) write_zeros<T, L>(c, phase, item, c.tiles, (raw_t*)a.dgates + place, a.dim, own, live);
         if (kShared && a.dgates && threadIdx.x < kSlots) c.sums[(chain * c.tiles + tile) * kSlots + threadIdx.x] = 0.f;
         return;
     }
     const raw_t* dh = a.dh ? (const raw_t*)a.dh + row * a.length * a.dim + c0 : x;
-    const int64_t dh_step = a.dh ? a.dim : a.x_step;
+    const int64_t dh_step = a.dh ? a.dim : a.x_step, x_step = phase == kMaps ? dh_step : a.x_step;
+    if (phase == kMaps) x = dh;            // (the maps of what goes back take nothing of x)
     const Found found(a, c, tile, t0);
     Span<T, L> xs[U], gs[kShared ? 1 : U], ds[U];
     if (kShared) gs[0].load(g);
@@ -706,7 +725,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t from = min(t + u, m.length - 1);
-            xs[u].load_once(x + from * a.x_step);
+            xs[u].load_once(x + from * x_step);
             if (!kShared) gs[kShared ? 0 : u].load_once(g + from * a.g_step);
             ds[u].load_once(dh + from * dh_step);
         }
@@ -714,7 +733,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int64_t from = min(t + u, m.length - 1);
-            xs[u].load(x + from * a.x_step);
+            xs[u].load(x + from * x_step);
             if (!kShared) gs[kShared ? 0 : u].load(g + from * a.g_step);
             ds[u].load(dh + from * dh_step);
         }
@@ -792,8 +811,10 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; s_q[mine + k] = Q[k]; }
     __syncthreads();
     // the states by some wavefronts, the gradients by others
+    if (phase == kMaps && threadIdx.x >= kSlots) return;
     if (threadIdx.x < kSlots) {
-        join_groups<kGroups, true>(c, chain, at, threadIdx.x, s_back_resets, s_a, s_q);
+        join_groups<kGroups, true>(c, phase, chain, at, threadIdx.x, s_back_resets, s_a, s_q);
+        if (phase == kMaps) return;
     } else if (threadIdx.x < 2 * kSlots) {
         const int own = threadIdx.x - kSlots;
         float h = tile ? a.states[(chain * c.tiles + tile) * kSlots + own] : 0.f;      // (a row begins with a sequence, or with tokens of none)
@@ -861,6 +882,69 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     }
 }
 
+// Few chains of many tiles: a chain's wait from tile to tile, 0.1 us, is longer than their tokens take.  So their maps are formed by a launch of their own,
+// joined here, and the tokens read again.  One wavefront goes from map to map, in the order and by the steps of tiles that wait for one another: equal
+// bits.  What it reads comes by all of them, a round ahead, and leaves by all of them, a round behind (by that one alone stores wait for stores); a
+// workgroup has 16 channels (2048 tiles of 64 channels 43 us; with all of them 51, of which one CU reads and writes 30).
+constexpr int kLinkers = 1024, kLinkWords = 8, kLinkRound = kLinkers * kLinkWords;
+constexpr int link_width(int slots) { return slots < 16 ? slots : 16; }
+template <int kSlots>
+__global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
+    constexpr int U = 8, kWidth = link_width(kSlots), kParts = kSlots / kWidth;
+    __shared__ uint64_t s_maps[2][kLinkRound + U * kWidth];
+    const int64_t words = c.tiles * kWidth, own = (int64_t)(blockIdx.x / kParts) * c.tiles * kSlots + blockIdx.x % kParts * kWidth;
+    const uint64_t* maps = c.maps + own;
+    uint32_t* states = c.states + own;
+    auto place = [](int64_t word) { return word / kWidth * kSlots + word % kWidth; };
+    uint64_t m[kLinkWords];
+    auto load = [&](int64_t from) {
+#pragma unroll
+        for (int i = 0; i < kLinkWords; i++) m[i] = maps[place(min(from + i * kLinkers + (int)threadIdx.x, words - 1))];
+    };
+    auto leave = [&](int64_t from, int half) {
+#pragma unroll
+        for (int i = 0; i < kLinkWords; i++) {
+            const int at = i * kLinkers + threadIdx.x;
+            if (from + at < words) states[place(from + at)] = word_of(__builtin_bit_cast(float, (uint32_t)s_maps[half][at]));
+        }
+    };
+    load(0);
+    float h = 0.f;
+    int half = 0;
+    for (int64_t from = 0; from < words; from += kLinkRound, half ^= 1) {
+        // (each thread's own places, whose states it has taken away before)
+#pragma unroll
+        for (int i = 0; i < kLinkWords; i++) s_maps[half][i * kLinkers + threadIdx.x] = m[i];
+        __syncthreads();
+        if (from) leave(from - kLinkRound, half ^ 1);
+        if (from + kLinkRound < words) load(from + kLinkRound);
+        if (threadIdx.x >= kWidth) continue;
+        // (behind the last tile maps of no use are joined, whose states go nowhere)
+        const int tiles = (int)(min((int64_t)kLinkRound, words - from) / kWidth);
+        uint64_t *at = s_maps[half] + threadIdx.x, next[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) next[u] = at[u * kWidth];
+#pragma unroll 2
+        for (int i = 0; i < tiles; i += U, at += U * kWidth) {
+            uint64_t map[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                map[u] = next[u];
+                next[u] = at[(U + u) * kWidth];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const float b = __builtin_bit_cast(float, (uint32_t)(map[u] >> 32));
+                h = (uint32_t)map[u] == kUnset ? b : __builtin_fmaf(__builtin_bit_cast(float, (uint32_t)map[u]), h, b);
+                *(float*)(at + u * kWidth) = h;
+            }
+        }
+    }
+    __syncthreads();
+    const int64_t from = (words - 1) / kLinkRound * kLinkRound;
+    leave(from, (int)(from / kLinkRound % 2));
+}
+
 // The tiles' sums of a shared gate's gradient, in 64 bits and one order.
 constexpr int kSumChannels = 16;
 template <class T>
@@ -889,8 +973,9 @@ __global__ __launch_bounds__(1024) void sum_kernel(ScanArgs a, Chains c, int len
 // ---- launches ----------------------------------------------------------------------------
 int fill(const ScanArgs& a, const Chains& c, int tokens, hipStream_t s) {
     if (c.tiles <= 1) return 0;
-    const int64_t words = ((char*)c.from - (char*)c.tickets) / 16, blocks = (words + kThreads - 1) / kThreads;
+    const int64_t words = c.phase == kChained ? ((char*)c.from - (char*)c.tickets) / 16 : 0, blocks = (words + kThreads - 1) / kThreads;
     const int64_t more = a.form == kPacked ? (c.tiles + kThreads - 1) / kThreads : 0;
+    if (!(blocks + more)) return 0;
     fill_kernel<<<(uint32_t)(blocks + more), kThreads, 0, s>>>((u32x4*)c.tickets, words, blocks, a, c.from, c.tiles, tokens);
     DCIH_HIP(hipGetLastError());
     return 0;
@@ -905,15 +990,29 @@ int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     // what the caches hold is read through them: 30011 x 1024 f16 with gradients 164 us, 171 past them; what they do not, past them
     // (65536 x 4096 bf16 packed 351 us, 366)
     c.once = c.apart && a.rows * a.length * a.dim * kSize * (kShared ? 1 : 2) > (int64_t)256 << 20;
+    c.phase = c.count <= kFewChains && c.tiles >= kManyTiles ? kMaps : kChained;
     if (int rc = fill(a, c, tile_of(L, kShared), s)) return rc;
+    const int64_t tiles = c.count * c.tiles;
+    auto launch = [&](auto phased, int64_t empty) {
+        constexpr bool kPhased = decltype(phased)::value;
+        for (int64_t first = 0; first < tiles + empty; first += kMaxGrid) {
+            const uint32_t grid = (uint32_t)std::min(kMaxGrid, tiles + empty - first);
+            if (gradient) scan_grad_kernel<T, L, kDecay, kShared, kPhased><<<grid, kThreads, 0, s>>>(a, c, first, empty);
+            else scan_kernel<T, L, kDecay, kShared, kPhased><<<grid, kThreads, 0, s>>>(a, c, first, empty);
+            DCIH_HIP(hipGetLastError());
+        }
+        return 0;
+    };
     // (workgroups that pass on the states of sequences without tokens)
     const int64_t empty = a.bounds && (gradient ? a.dstate : a.last) ? std::min((a.sequences + kEmpty - 1) / kEmpty, kEmptyGrid) : 0;
-    const int64_t tiles = c.count * c.tiles;
-    for (int64_t first = 0; first < tiles + empty; first += kMaxGrid) {
-        const uint32_t grid = (uint32_t)std::min(kMaxGrid, tiles + empty - first);
-        if (gradient) scan_grad_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first, empty);
-        else scan_kernel<T, L, kDecay, kShared><<<grid, kThreads, 0, s>>>(a, c, first, empty);
+    if (c.phase == kMaps) {
+        if (int rc = launch(std::true_type{}, 0)) return rc;
+        link_kernel<kLanes * L><<<(uint32_t)(c.count * (kLanes * L / link_width(kLanes * L))), kLinkers, 0, s>>>(c);
         DCIH_HIP(hipGetLastError());
+        c.phase = kApply;
+        if (int rc = launch(std::true_type{}, empty)) return rc;
+    } else if (int rc = launch(std::false_type{}, empty)) {
+        return rc;
     }
     if (gradient && kShared && a.dgates) {
         sum_kernel<T><<<(uint32_t)((a.dim + kSumChannels - 1) / kSumChannels), 1024, 0, s>>>(a, c, L);

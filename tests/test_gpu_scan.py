@@ -323,6 +323,44 @@ def test_same_bits_every_time(gpu):
         assert all(torch.equal(a, b) for a, b in zip(got, first))
 
 
+LONG = [("bf16", False, False, 33_000, 40), ("f16", False, True, 66_100, 72), ("f32", True, False, 33_100, 32), ("f32", False, True, 65_700, 20), ("bf16", True, True, 65_600, 5)]
+
+
+@pytest.mark.parametrize("dtype, decay, shared, length, dim", LONG)
+def test_a_long_sequence_alone_and_among_others(gpu, dtype, decay, shared, length, dim):
+    """Equal bits, whether its tiles wait for one another or not, to the end of the row or not; and as several, one behind the other."""
+    x, gates, s, dh, dlast = (t.cuda() for t in inputs(1, length, dim, dtype, decay, shared, seed=5))
+
+    def run(x, gates, s, dh, dlast, **kw):
+        leaves = [t.detach().requires_grad_() for t in (x, gates, s)]
+        out = gpu.gated_scan(*leaves, decay=decay, **kw)
+        return list(out) + list(torch.autograd.grad(out, leaves, (dh, dlast)))
+
+    others = [t if t.dim() < 2 else torch.cat([t] + [0.5 * t] * 5) for t in (x, gates, s, dh, dlast)]
+    for lengths in (None, [length], [length - 5000], [129], [0]):
+        few = run(x, gates, s, dh, dlast, lengths=None if lengths is None else torch.tensor(lengths, device="cuda"))
+        many = run(*others, lengths=None if lengths is None else torch.tensor(lengths * 6, device="cuda"))
+        for i, (a, b) in enumerate(zip(few, many)):
+            assert i == 3 and shared or torch.equal(a, b[:1]), i
+    # short ones, a long one, one without tokens, tokens of none
+    cuts = [7, 100, 100, 128, 5000, length - 300, length - 256, length - 3]
+    n = len(cuts) - 1
+    states, dstates = torch.randn(n, dim, device="cuda"), torch.randn(n, dim, device="cuda")
+    flat = lambda t: t if t.dim() < 2 else t[0]                     # noqa: E731
+    got = run(flat(x), flat(gates), states, flat(dh), dstates, offsets=torch.tensor(cuts, device="cuda"))
+    covered = torch.zeros(length, 1, dtype=torch.bool, device="cuda")
+    for i, (lo, hi) in enumerate(zip(cuts[:-1], cuts[1:])):
+        cut = lambda t: t if t.dim() < 2 else t[:, lo:hi]           # noqa: E731
+        one = run(cut(x), cut(gates), states[i:i + 1], cut(dh).contiguous(), dstates[i:i + 1])
+        covered[lo:hi] = True
+        # (tiles begin elsewhere: other roundings, of up to 64 half steps of the largest, and one to the type)
+        for mine, want in ((got[0][lo:hi], one[0][0]), (got[1][i], one[1][0]), (got[2][lo:hi], one[2][0]), (got[4][i], one[4][0])):
+            if want.numel():
+                steps = 64 * O.STEP + (0 if want.dtype == torch.float32 else torch.finfo(want.dtype).eps)
+                assert (mine.float() - want.float()).abs().max() <= steps * want.float().abs().max().clamp(min=1), i
+    assert not got[0].float()[~covered.expand(-1, dim)].any() and not got[2].float()[~covered.expand(-1, dim)].any()
+
+
 def test_shapes_without_tokens(gpu):
     s = torch.randn(3, 8, device="cuda")
     h, last = gpu.gated_scan(torch.zeros(3, 0, 8, device="cuda"), torch.zeros(3, 0, 8, device="cuda"), s)
