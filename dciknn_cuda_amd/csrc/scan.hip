@@ -33,7 +33,7 @@ constexpr int kWaves = 4, kBackWaves = 3;
 // 128 x 48 x 1024 23 and 13).
 constexpr int kShort = 32, kShortOfMany = 64;
 constexpr int64_t kManyPieces = 1280;
-// Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 5.2 us,
+// Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 4.5 us,
 // 8.7 by pieces; 32 x 32 x 1024 7.1, 15.3, 8.5 by tiles; but 512 x 8 x 1024 8.3 and 6.6).  Twice as many where sequences are longer than kSteps.
 constexpr int64_t kSingles = 1 << 17;
 constexpr int kSteps = 16;
