@@ -361,6 +361,24 @@ def test_a_long_sequence_alone_and_among_others(gpu, dtype, decay, shared, lengt
     assert not got[0].float()[~covered.expand(-1, dim)].any() and not got[2].float()[~covered.expand(-1, dim)].any()
 
 
+def test_a_long_sequence_recorded(gpu):
+    x, gates, s, _, _ = (t.cuda() for t in inputs(1, 33_000, 40, "bf16", False, False, seed=6))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gpu.gated_scan(x, gates, s)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, last = gpu.gated_scan(x, gates, s, last=s)
+    for turn in range(4):
+        x.mul_(0.5).add_(turn)
+        s.fill_(float(turn))
+        want, state = gpu.gated_scan(x, gates, s)
+        graph.replay()
+        assert torch.equal(h, want) and torch.equal(last, state) and last.data_ptr() == s.data_ptr()
+
+
 def test_shapes_without_tokens(gpu):
     s = torch.randn(3, 8, device="cuda")
     h, last = gpu.gated_scan(torch.zeros(3, 0, 8, device="cuda"), torch.zeros(3, 0, 8, device="cuda"), s)
