@@ -29,10 +29,11 @@ constexpr int tile_of(int len, bool shared) { return len == 8 || (len == 4 && !s
 // Wavefronts of a SIMD: registers enough for a tile, tiles enough to hide one another's waits (one more each way spills: 8 x 4096 x 2048
 // with gradients 262 us instead of 238; one less is as fast).
 constexpr int kWaves = 4, kBackWaves = 3;
-// Tokens that one thread takes.  More where channels are many, for each token (512 x 40 x 2048 bf16 42 us, 58 by tiles; 512 x 48 x 1024 28 and 43,
-// 128 x 48 x 1024 23 and 13).
-constexpr int kShort = 32, kShortOfMany = 64;
-constexpr int64_t kManyPieces = 1280;
+// Tokens that one thread takes in any case.  Of longer rows it takes all where pieces are many, kManyPieces for each token up to kEnoughPieces: 512 x 40 x
+// 2048 bf16 42 us, 58 by tiles; 512 x 48 x 1024 28 and 43, 128 x 48 x 1024 23 and 13; 256 x 130 x 2048 87 and 158, 256 x 300 x 2048 202 and 247, 64 x 300 x
+// 2048 69 and 61.  But not where a tile is full to 7/8 or more and has no other to wait for (f32 256 x 116 x 1024 78 and 62).
+constexpr int kShort = 32;
+constexpr int64_t kManyPieces = 1280, kEnoughPieces = 1 << 16;
 // Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 4.5 us,
 // 8.7 by pieces; 32 x 32 x 1024 7.1, 15.3, 8.5 by tiles; but 512 x 8 x 1024 8.3 and 6.6).  Twice as many where sequences are longer than kSteps.
 constexpr int64_t kSingles = 1 << 17;
@@ -146,10 +147,12 @@ template <bool kDecay> __device__ inline Gate coefs_of(float packed) {
 template <bool kDecay> __device__ inline float step(float h, float x, Gate c) { return __builtin_fmaf(c.a, h, kDecay ? x : c.keep * x); }
 
 // ---- one thread a channel ----------------------------------------------------------------
-// A server's step, or its drafts: few tokens of many sequences.  The state may be written where it is read.  Bound by the launch (32 x 1 x 4096 bf16
+// A server's step, or its drafts, few tokens of many sequences; rows of any length where they are many.  The state may be written where it is read.  Bound by the launch (32 x 1 x 4096 bf16
 // 2.7 us replayed), then by the chain of a wavefront's tokens (8: 4.0), then memory (1024 x 8 x 4096 39 us, 6 TB/s).
-template <class T, int L, bool kDecay, int U>
+template <class T, int L, bool kDecay, int U, int kTile>
 __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces, int64_t first) {
+    constexpr bool kStates = kTile > 0;
+    const int64_t strips = (pieces + kLanes - 1) / kLanes, tiles = kStates ? (a.length + kTile - 1) / max(kTile, 1) : 0;
     using raw_t = typename T::raw;
     const int64_t i = first + (int64_t)blockIdx.x * kThreads + threadIdx.x;
     const int64_t b = i / pieces;
@@ -163,11 +166,14 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
 #pragma unroll
     for (int k = 0; k < L; k++) h[k] = 0.f;
     if (a.state) load_floats<L>(a.state + b * a.dim + c0, h);
-    for (int t0 = 0; t0 < length; t0 += U) {
+    int64_t t0 = 0;
+    for (; t0 < len; t0 += U) {
+        // what the gradient takes for the state before a tile
+        if (kStates && t0 % kTile == 0) store_floats<L>(a.states + ((b * strips + piece / kLanes) * tiles + t0 / kTile) * (kLanes * L) + piece % kLanes * L, h);
         Span<T, L> xs[U], gs[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int64_t t = min((int64_t)t0 + u, max(len, (int64_t)1) - 1);
+            const int64_t t = min(t0 + u, len - 1);
             xs[u].load(x + t * a.x_step);
             gs[u].load(g + t * a.g_step);
         }
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
                 h[k] = in ? next : h[k];
                 y[k] = in ? next : 0.f;
             }
-            raw_t* to = out + (int64_t)(t0 + u) * a.dim;
+            raw_t* to = out + (t0 + u) * a.dim;
             if (c0 == own) {
                 Span<T, L>::store(to, y);
             } else {           // the row's last piece: what it shares with the one before is that one's, whose state may be written already
@@ -194,6 +200,10 @@ __global__ __launch_bounds__(kThreads) void short_kernel(ScanArgs a, int pieces,
             }
         }
     }
+    float none[L];
+#pragma unroll
+    for (int k = 0; k < L; k++) none[k] = 0.f;
+    for (; t0 < length; t0++) Span<T, L>::store(out + t0 * a.dim, none);
     if (!a.last) return;
     float* last = a.last + b * a.dim + c0;
     if (c0 == own) {
@@ -1027,8 +1037,14 @@ int run_short(const ScanArgs& a, hipStream_t s) {
     const int64_t threads = a.rows * pieces, most = kMaxGrid * kThreads;
     for (int64_t first = 0; first < threads; first += most) {
         const uint32_t grid = (uint32_t)((std::min(most, threads - first) + kThreads - 1) / kThreads);
-        if (a.length > 4) short_kernel<T, L, kDecay, 8><<<grid, kThreads, 0, s>>>(a, pieces, first);
-        else short_kernel<T, L, kDecay, 4><<<grid, kThreads, 0, s>>>(a, pieces, first);
+        if (a.states && a.length > tile_of(L, a.shared)) {
+            if (tile_of(L, a.shared) == 128) short_kernel<T, L, kDecay, 8, 128><<<grid, kThreads, 0, s>>>(a, pieces, first);
+            else short_kernel<T, L, kDecay, 8, 256><<<grid, kThreads, 0, s>>>(a, pieces, first);
+        } else if (a.length > 4) {
+            short_kernel<T, L, kDecay, 8, 0><<<grid, kThreads, 0, s>>>(a, pieces, first);
+        } else {
+            short_kernel<T, L, kDecay, 4, 0><<<grid, kThreads, 0, s>>>(a, pieces, first);
+        }
         DCIH_HIP(hipGetLastError());
     }
     return 0;
@@ -1037,7 +1053,7 @@ int run_short(const ScanArgs& a, hipStream_t s) {
 template <class T, int L>
 int by_gates(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     if (!gradient && scan_is_short(a, dtype)) {
-        if (L > 1 && a.rows * a.dim > kSingles * (a.length > kSteps ? 2 : 1)) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
+        if (L > 1 && (a.length > kShort || a.rows * a.dim > kSingles * (a.length > kSteps ? 2 : 1))) return a.decay ? run_short<T, L, true>(a, s) : run_short<T, L, false>(a, s);
         return a.decay ? run_short<T, 1, true>(a, s) : run_short<T, 1, false>(a, s);
     }
     if (a.decay) return a.shared ? run<T, L, true, true>(a, dtype, gradient, s) : run<T, L, true, false>(a, dtype, gradient, s);
@@ -1089,9 +1105,10 @@ int64_t scan_work_bytes(int64_t rows, int64_t length, int dim, int dtype) {
 }
 
 bool scan_is_short(const ScanArgs& a, int dtype) {
-    if (a.form != kRows || a.length > kShortOfMany) return false;
-    const int len = span_len(a.dim, dtype);
-    return a.length <= kShort || a.rows * ((a.dim + len - 1) / len) >= kManyPieces * a.length;
+    if (a.form != kRows || a.length <= kShort) return a.form == kRows;
+    const int len = span_len(a.dim, dtype), tile = tile_of(len, a.shared);
+    if (a.length <= tile && 8 * a.length >= 7 * tile) return false;
+    return a.rows * ((a.dim + len - 1) / len) >= std::min(kManyPieces * a.length, kEnoughPieces);
 }
 
 int scan(const ScanArgs& a, int dtype, hipStream_t s) { return dispatch(scan_is_short(a, dtype) ? a : flattened(a, tile_of(span_len(a.dim, dtype), a.shared)), dtype, false, s); }

@@ -278,6 +278,37 @@ def test_many_channels(gpu, size, dtype, decay, view):
     check(gpu, *size, dtype, decay, view=VIEWS[view], lengths=lengths if decay else None, grad=size[0] == 400 and not decay)
 
 
+WIDE = [("bf16", False, (64, 300, 8192)), ("f32", False, (32, 70, 8192)), ("f32", True, (260, 260, 1021)), ("f16", False, (300, 129, 1771)), ("f32", False, (16384, 130, 16)), ("bf16", True, (66000, 40, 5))]
+
+
+@pytest.mark.parametrize("dtype, shared, size", WIDE, ids=str)
+@pytest.mark.parametrize("with_lengths", [False, True])
+def test_many_long_rows(gpu, dtype, shared, size, with_lengths):
+    """Rows that one thread takes from first to last, with the states that the gradient asks for, against the same rows in parts that tiles take."""
+    rows, length, dim = size
+    g = torch.Generator(device="cuda").manual_seed(length)
+    draw = lambda *shape: torch.randn(*shape, generator=g, device="cuda")       # noqa: E731
+    x, gates, s = draw(*size).to(TYPES[dtype]), (1.0 + 3.0 * draw(dim) if shared else 1.0 + 3.0 * draw(*size)).to(TYPES[dtype]), draw(rows, dim)
+    dh, dlast = draw(*size).to(TYPES[dtype]), draw(rows, dim)
+    lengths = torch.arange(rows, device="cuda") * 37 % (length + 1) if with_lengths else None
+
+    def run(rows):
+        leaves = [t.detach().requires_grad_() for t in (x[rows], gates if shared else gates[rows], s[rows])]
+        out = gpu.gated_scan(*leaves, lengths=lengths[rows] if with_lengths else None)
+        return list(out) + list(torch.autograd.grad(out, leaves, (dh[rows], dlast[rows])))
+
+    whole = run(slice(0, rows))
+    with torch.no_grad():
+        assert torch.equal(gpu.gated_scan(x, gates, s, lengths=lengths)[0], whole[0])
+    for part in (slice(0, 3), slice(rows - 3, rows)):
+        for i, (a, b) in enumerate(zip(whole, run(part))):
+            if i == 3 and shared:
+                continue
+            # (tiles join their maps: other roundings, of up to 64 half steps of the largest, and one to the type)
+            steps = 64 * O.STEP + (0 if a.dtype == torch.float32 else torch.finfo(a.dtype).eps)
+            assert (a[part].float() - b.float()).abs().max() <= steps * b.float().abs().max().clamp(min=1), i
+
+
 @pytest.mark.parametrize("size", MANY, ids=str)
 def test_many_states_in_place(gpu, size):
     x, gates, s, _, _ = (t.cuda() for t in inputs(*size, "bf16", False, False))
