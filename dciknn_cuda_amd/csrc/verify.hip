@@ -5,6 +5,8 @@
 //
 // A token is right or wrong: everything that decides on one is in 64 bits, exponentials included, so that a random number has to
 // be within 1e-13 of a border to be taken to its wrong side (in 32 bits the borders of 131072 tokens cover some hundredths of [0, 1)).
+// Behind a refused draft borders are parts of what is left of the row: a border there is 1e-13 of the row off while a thousandth or more is
+// left, 1e-14 of it where less is (see choose_kernel).  Taking off leaves nothing of an entry where it leaves as little as those roundings.
 #include "../../include/dci_hip.h"
 #include "verify.h"
 
@@ -215,7 +217,7 @@ constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.6931471805599
 // One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
 // from the row that it comes from, by chunks, then among the entries of one.
 template <class T>
-__global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const Sum* sums, int chunks, int64_t first) {
+__global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, Sum* sums, int chunks, int64_t first) {
     constexpr int kPer = kChunk / kChoosers;
     __shared__ double s_total[kMaxDrafts + 1], s_part[kChooserWaves], s_weight[kChunk], s_gone[kSlots], s_target;
     __shared__ unsigned long long s_fixed[kSlots], s_taken[kNearChunks];
@@ -298,9 +300,9 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
     // row `kept` names the next token
     const double total = s_total[kept], base = base_of(s_max[kept]);
     const typename T::raw* row = logits + kept * a.stride;
-    const Sum* part = sums + (b * (k + 1) + kept) * chunks;
+    Sum* part = sums + (b * (k + 1) + kept) * chunks;
     bool fine = total > 0.0 && total < __builtin_huge_val();
-    // what is taken off its weights: ids and amounts, each id once.  (Amounts that several threads add up are whole numbers of 2^-52 of
+    // what is taken off its weights: ids and amounts, each id once.  (What several threads add up are whole numbers of 2^-52 of
     // the largest, or of 2^-60 of the total: their order does not matter.)
     const int each = (chunks + kChoosers - 1) / kChoosers, begin = min(chunks, tid * each), end = min(chunks, begin + each);
     Sum mine{};
@@ -345,9 +347,11 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
             for (int w = 0; w < kChooserWaves; w++) top = fmaxf(top, (float)s_part[w]);
             const double top_base = base_of(top);
             bool bad = false;
+            double amount[E];
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const int j = tid + e * kChoosers;
+                amount[e] = 0.0;
                 if (id[e] < 0) continue;
                 const double w = weight_of(z[e], kLog2eWide, top_base);
                 bad |= !(w <= 1.0);
@@ -359,13 +363,17 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
                     for (int i = 7; i >= 0; i--) found = s_id[o + i] == id[e] && o + i < j ? o + i : found;
                     lead = found < lead ? found : lead;
                 }
-                if (!bad) atomicAdd(&s_fixed[lead], (unsigned long long)(w * 0x1p52));
+                if (lead == j) amount[e] = w;
+                else if (!bad) atomicAdd(&s_fixed[lead], (unsigned long long)(w * 0x1p52));
             }
             fine = !__syncthreads_or(bad);
-            unsigned long long sum = 0;
+            double all = 0.0;
 #pragma unroll
-            for (int e = 0; e < E; e++) sum += s_fixed[tid + e * kChoosers];
-            double all = lanes_sum((double)sum);
+            for (int e = 0; e < E; e++) {
+                amount[e] += (double)s_fixed[tid + e * kChoosers] * 0x1p-52;
+                all += amount[e];
+            }
+            all = lanes_sum(all);
             __syncthreads();
             if (lane == 0) s_part[wave] = all;
             __syncthreads();
@@ -375,44 +383,126 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const int j = tid + e * kChoosers;
-                s_gone[j] = (double)s_fixed[j] * share;
-                if (id[e] == a.vocab || s_fixed[j] == 0) s_id[j] = -1;
+                s_gone[j] = amount[e] * share;
+                if (id[e] == a.vocab || amount[e] == 0.0) s_id[j] = -1;
             }
         }
     }
     __syncthreads();
+    // What is left of an entry, nothing where that is within the roundings of what is taken off.
+    double rounding = 1e-13;
+    auto left_of = [&](double w, double gone) {
+        const double left = w - gone;
+        return left > gone * rounding ? left : 0.0;
+    };
     const double to_fixed = 0x1p60 / total;
     for (int j = tid; j < (slots + 7) / 8 * 8; j += kChoosers) {           // what entry s_id[j] weighs less than in p
         const int id = j < slots ? s_id[j] : -1;
-        const double w = id >= 0 ? weight_of((float)row[id], c2, base) : 0.0, less = id >= 0 ? w - max(w - s_gone[j], 0.0) : 0.0;
+        const double w = id >= 0 ? weight_of((float)row[id], c2, base) : 0.0, less = id >= 0 ? w - left_of(w, s_gone[j]) : 0.0;
         s_fixed[j] = (unsigned long long)(less * to_fixed);
         s_chunk_of[j] = id >= 0 ? id / kChunk : -1;
         if (id >= 0 && id / kChunk < kNearChunks) atomicAdd(&s_taken[id / kChunk], s_fixed[j]);
     }
     __syncthreads();
     fine = fine && u == u;
+    // The weights of a chunk's entries, less what is taken off; to be read behind the next barrier.  (Between the last read of others and this stands
+    // a barrier in each place: that of the sum or of the scan over them.)
+    auto weigh = [&](int from, bool all_of_them) {
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            const int i = e * kChoosers + tid;
+            s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, base) : 0.0;
+        }
+        if (all_of_them) return;
+        __syncthreads();
+        for (int j = tid; j < slots; j += kChoosers)
+            if (s_id[j] >= from && s_id[j] < from + kChunk) s_weight[s_id[j] - from] = left_of(s_weight[s_id[j] - from], s_gone[j]);
+    };
+    auto sum_of_weights = [&] {
+        __syncthreads();
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) sum += s_weight[tid * kPer + e];
+        scan_threads(sum, s_part);
+        sum = 0.0;
+        for (int w = 0; w < kChooserWaves; w++) sum += s_part[w];
+        return sum;
+    };
     // the chunk: a run of chunks for each thread
+    bool settled = false;                // what is left of a chunk stands in the place of its sum
     auto chunk_sum = [&](int c) -> double {
         const Sum p = c == begin ? mine : part[c];
         const double s = p.s == 0.0 ? 0.0 : p.s * weight_of(p.m, c2, base);
         unsigned long long taken = 0;
-        if (!slots) return s;
+        if (!slots || settled) return s;
         if (c < kNearChunks) taken = s_taken[c];
         else
             for (int o = 0; o < slots; o++) taken += s_chunk_of[o] == c ? s_fixed[o] : 0;
         return __builtin_fmax(s - (double)taken * (total * 0x1p-60), 0.0);
     };
     double all = 0.0, before = 0.0, own = 0.0;
-    for (int turn = 0; fine && turn < 2; turn++) {
+    auto sum_up = [&] {
         own = 0.0;
         for (int c = begin; c < end; c++) own += chunk_sum(c);
         before = scan_threads(own, s_part);
         all = 0.0;
         for (int w = 0; w < kChooserWaves; w++) all += s_part[w];
-        if (all > 0.0) break;
-        slots = 0;                       // nothing is left of p but roundings: drawn from p itself
+    };
+    auto put = [&](int c, double sum) {
+        if (tid == 0) part[c] = Sum{sum, s_max[kept], 0.f};
+    };
+    auto put_done = [&] {
+        __syncthreads();
+        if (begin < end) mine = part[begin];
+    };
+    if (fine) sum_up();
+    // Sums are 2.5e-14 off, each entry 1e-15.  Where little is left that is not small beside it: chunks that something is taken off are formed again
+    // from their entries, so that what is left is as near as 1e-14 of the row.
+    if (__builtin_expect(fine && slots && !(all >= total * 0x1p-10), 0)) {
+        rounding = 1e-14;
+        bool leads[kSlots / kChoosers];
+#pragma unroll
+        for (int e = 0; e < kSlots / kChoosers; e++) {
+            const int j = tid + e * kChoosers;
+            leads[e] = j < slots && s_chunk_of[j] >= 0;
+            for (int o = 0; leads[e] && o < j; o++) leads[e] = s_chunk_of[o] != s_chunk_of[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kSlots / kChoosers; e++)
+            if (tid + e * kChoosers < slots && !leads[e]) s_chunk_of[tid + e * kChoosers] = -1;
+        __syncthreads();
+        settled = true;
+        for (int j = 0; j < slots; j++) {
+            const int c = s_chunk_of[j];
+            if (c < 0) continue;
+            weigh(c * kChunk, true);
+            const double sum = sum_of_weights();
+            if (tid == 0) s_fixed[j] = __builtin_bit_cast(unsigned long long, sum);
+            put(c, sum);
+        }
+        put_done();
+        sum_up();
+        const double more = all / total;
+        for (int j = tid; j < slots; j += kChoosers) s_gone[j] *= more;
+        for (int j = 0; j < slots; j++) {
+            const int c = s_chunk_of[j];
+            if (c < 0) continue;
+            weigh(c * kChunk, false);
+            put(c, sum_of_weights());
+        }
+        put_done();
+        sum_up();
+        if (!(all > 0.0)) {              // nothing is left: drawn from p itself
+            for (int j = 0; j < slots; j++)
+                if (s_chunk_of[j] >= 0) put(s_chunk_of[j], __builtin_bit_cast(double, s_fixed[j]));
+            put_done();
+            slots = 0;
+            sum_up();
+        }
     }
-    if (fine) {
+    // (a chunk of which there is a sum, of roundings, and no entry counts as nothing: the next one is looked for)
+    while (fine && all > 0.0) {
         const double target = min(max((double)u, 0.0), 1.0) * all;
         last_that(own > 0.0 && before - own <= target, tid, &s_last);      // (with weights below the target)
         __syncthreads();
@@ -435,35 +525,34 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, const S
         __syncthreads();
         // the entry
         const int chunk = s_chunk, from = chunk * kChunk;
-        if (chunk >= 0) {
+        if (chunk < 0) break;
+        weigh(from, false);
+        if (tid == 0) s_last = -1;
+        __syncthreads();
+        double w[kPer], sum = 0.0;
 #pragma unroll
-            for (int e = 0; e < kPer; e++) {
-                const int i = e * kChoosers + tid;
-                s_weight[i] = from + i < a.vocab ? weight_of((float)row[from + i], c2, base) : 0.0;
-            }
-            __syncthreads();
-            for (int j = tid; j < slots; j += kChoosers)
-                if (s_id[j] >= from && s_id[j] < from + kChunk) s_weight[s_id[j] - from] = max(s_weight[s_id[j] - from] - s_gone[j], 0.0);
-            if (tid == 0) s_last = -1;
-            __syncthreads();
-            double w[kPer];
-            own = 0.0;
-#pragma unroll
-            for (int e = 0; e < kPer; e++) {
-                w[e] = s_weight[tid * kPer + e];
-                own += w[e];
-            }
-            double sum = scan_threads(own, s_part) - own;
-            int found = -1;
-#pragma unroll
-            for (int e = 0; e < kPer; e++) {
-                if (w[e] > 0.0 && sum <= s_target) found = tid * kPer + e;
-                sum += w[e];
-            }
-            last_that(found >= 0, found, &s_last);
-            __syncthreads();
-            if (tid == 0 && s_last >= 0) s_token = from + s_last;
+        for (int e = 0; e < kPer; e++) {
+            w[e] = s_weight[tid * kPer + e];
+            sum += w[e];
         }
+        sum = scan_threads(sum, s_part) - sum;
+        int found = -1;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            if (w[e] > 0.0 && sum <= s_target) found = tid * kPer + e;
+            sum += w[e];
+        }
+        last_that(found >= 0, found, &s_last);
+        __syncthreads();
+        if (s_last >= 0) {
+            if (tid == 0) s_token = from + s_last;
+            break;
+        }
+        put(chunk, 0.0);
+        put_done();
+        sum_up();
+        if (tid == 0) s_last = -1;
+        __syncthreads();
     }
     __syncthreads();
     const int token = s_token;
@@ -494,7 +583,7 @@ int run(const VerifyArgs& a, hipStream_t s) {
         DCIH_HIP(hipGetLastError());
     }
     for (int64_t first = 0; first < a.n; first += kMaxGrid) {
-        choose_kernel<T><<<(uint32_t)std::min(kMaxGrid, a.n - first), kChoosers, 0, s>>>(a, (const Sum*)a.work, chunks, first);
+        choose_kernel<T><<<(uint32_t)std::min(kMaxGrid, a.n - first), kChoosers, 0, s>>>(a, (Sum*)a.work, chunks, first);
         DCIH_HIP(hipGetLastError());
     }
     return 0;
