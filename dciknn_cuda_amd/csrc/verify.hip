@@ -292,7 +292,8 @@ __global__ __launch_bounds__(kChoosers) void choose_kernel(VerifyArgs a, Sum* su
             its = lanes_sum(its);
         }
         const double p = weight_of(z, c2, base);
-        if (lane == 0) s_kept[i] = p > 0.0 && (all == 0.0 || (double)r.number * its * s < p * all);
+        // (without slots it is none of what was drawn from: 0 < p, if the row has probabilities and the number is one)
+        if (lane == 0) s_kept[i] = p > 0.0 && (double)r.number * its * s < p * (all == 0.0 ? 1.0 : all);
     }
     __syncthreads();
     int kept = 0;

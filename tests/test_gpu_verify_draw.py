@@ -111,3 +111,20 @@ def test_large_vocabulary(gpu, lead):
         u[:, 1] = number
         check(gpu, z, drafts, u, on_border=True)
         check(gpu, z, drafts, u, *by_slots(drafts), on_border=True)
+
+
+def test_rows_that_say_nothing_beside_drafts_without_slots(gpu):
+    """A draft without filled slots stands where the model holds it for possible: not in a row without probabilities, nor with a number that is none."""
+    g = torch.Generator().manual_seed(6)
+    z = torch.randn(7, 3, 5000, generator=g)
+    drafts = torch.randint(0, 5000, (7, 2), generator=g)
+    u = torch.rand(7, 3, generator=g)
+    z[0, 0, 4999 - int(drafts[0, 0] == 4999)] = math.nan
+    z[1, 1, 77 + int(drafts[1, 1] == 77)] = math.nan
+    z[2, 0, 78 + int(drafts[2, 0] == 78)] = math.inf
+    z[3, 0] = -math.inf
+    u[4, 0], u[5, 1], u[6, 2] = math.nan, math.nan, math.nan
+    ids = torch.full((7, 2, 3), -1)
+    got = check(gpu, z, drafts, u, ids, torch.randn(7, 2, 3, generator=g), on_border=True)
+    assert got[1].tolist() == [0, 1, 0, 0, 0, 1, 2]
+    check(gpu, z, drafts, u, ids.clamp(min=5), torch.full((7, 2, 3), -math.inf), on_border=True)
