@@ -109,5 +109,7 @@ def verify_drafts(logits, drafts, uniforms, ids=None, teacher=None, temperature=
     The tokens are distributed as if drawn from the model one by one.
 
     tokens [batch, k + 1] int32: the accepted [batch] drafts, the next token, -1 behind it; logprobs float32: their log p,
-    0 behind them.  A row without probabilities (NaN, +inf, nothing but -inf) gives -1 with NaN.  Decided in 64 bits."""
+    0 behind them.  A row without probabilities (NaN, +inf, nothing but -inf) gives -1 with NaN.  Decided in 64 bits, at the temperature
+    rounded to 32 as everywhere here; what is left of a token within 1e-13 of what q takes off is nothing, and where nothing is left p is
+    drawn from."""
     return _ext._verify_drafts(logits, drafts, uniforms, ids, teacher, temperature)

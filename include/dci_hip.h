@@ -463,7 +463,9 @@ int dcih_clip(const dcih_span* spans, int64_t num_spans, double max_norm, double
  * nothing), behind the last one from p: the first with u_drafts * (sum of all weights) < (sum of the weights up to it).
  * d_accepted [num_sequences]: how many stand; d_tokens, d_logprobs [num_sequences][drafts + 1]: these, the next token and
  * -1, and their log p_i (0 for -1).  A draft beyond the vocabulary does not stand.  A row that holds NaN or +inf or nothing but
- * -inf, or whose slots do or whose random number is NaN, gives no token: -1 with a log probability of NaN.  What decides is formed in 64 bits.
+ * -inf, or whose slots hold NaN or +inf, gives no token, nor does a u_drafts that is NaN: -1 with a log probability of NaN.  (With another u_i
+ * that is NaN draft i does not stand.)  What decides is formed in 64 bits, from logits, numbers and a temperature as they are given: a border is off by up to 1e-13 of the row's
+ * weights, or 1e-14 where less than a thousandth of them is left to be drawn from; of an entry of which q_i leaves as little as that of itself nothing is left.
  */
 #define DCIH_MAX_DRAFTS 256
 int64_t dcih_verify_work(int64_t num_sequences, int drafts, int vocab, int dtype);
