@@ -177,6 +177,27 @@ const char* check_clip(const dcih_span* spans, int64_t n, bool written, double s
     return aligned(work, 16) ? nullptr : "workspace not aligned to 16 bytes";
 }
 
+// What a call reads or writes; null where nothing was given.
+struct Range {
+    const void* p;
+    int64_t bytes;
+    bool meets(const Range& o) const { return p && o.p && bytes > 0 && o.bytes > 0 && overlap(p, bytes, o.p, o.bytes); }
+};
+
+// Whether something that is written lies over something that is read, or over something else that is written.  (Workgroups, and lanes that share a
+// row's last piece, read what others have written by then.)
+bool any_meets(std::initializer_list<Range> written, std::initializer_list<Range> read) {
+    for (const Range* w = written.begin(); w != written.end(); w++) {
+        for (const Range& r : read)
+            if (w->meets(r)) return true;
+        for (const Range* o = w + 1; o != written.end(); o++)
+            if (w->meets(*o)) return true;
+    }
+    return false;
+}
+
+Range bounds_range(const ScanArgs& a) { return {a.bounds, (a.sequences + (a.form == kPacked)) * (a.wide_bounds ? 8 : 4)}; }
+
 // States in their own place: where one thread does not have a channel from first to last, the new ones wait in the workspace.
 int64_t last_bytes(int64_t sequences, int dim) { return (sequences * dim * 4 + 255) / 256 * 256; }
 
@@ -377,6 +398,10 @@ int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim,
     if (d_last && (overlap(d_last, states * 4, d_h, h_bytes) || overlap(d_last, states * 4, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
                    overlap(d_last, states * 4, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b)))
         return refuse(who, "the last states overlap x, the gates or h");
+    const Range first{d_state, states * 4}, bounds = bounds_range(a), kept{d_states, scan_state_floats(rows, length, dim, dtype) * 4};
+    if (any_meets({{d_h, h_bytes}, kept}, {first, bounds, {d_x, scan_extent(rows, length, dim, x_row, x_step) * b}, {d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b}}) ||
+        any_meets({{d_last, states * 4}}, {bounds, kept}))
+        return refuse(who, "something that is written overlaps something else");
     const int64_t own = scan_work_bytes(rows, length, dim, dtype);
     if (work_bytes < own + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
@@ -403,15 +428,22 @@ int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int
     if (!aligned(d_dh, type_bytes(dtype)) || !aligned(d_dx, type_bytes(dtype)) || !aligned(d_dgates, type_bytes(dtype)))
         return refuse(who, "gradients not aligned to their elements");
     const int64_t b = type_bytes(dtype), states = a.sequences * dim, cells = rows * length * dim * b;
+    if (any_meets({{d_dstate, states * 4}}, {{d_dlast, states * 4}, {d_state, states * 4}, bounds_range(a)}))
+        return refuse(who, "the gradient by the first states overlaps what it is formed from");
     if (!rows || !length) {
         if (a.shared && d_dgates) return refuse(who, "no tokens to sum a shared gate's gradient over");
         return d_dstate && states ? scan_copy(d_dlast, d_dstate, states, s) : DCIH_OK;
     }
     if (!d_states) return refuse(who, "null array");
-    for (const void* out : {(const void*)d_dx, a.shared ? nullptr : (const void*)d_dgates})
-        if (out && (overlap(out, cells, d_x, scan_extent(rows, length, dim, x_row, x_step) * b) ||
-                    overlap(out, cells, d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b) || (d_dh && overlap(out, cells, d_dh, cells))))
-            return refuse(who, "a gradient overlaps what it is formed from");
+    if (any_meets({{d_dx, cells}, {d_dgates, a.shared ? dim * b : cells}, {d_dstate, states * 4}},
+                  {{d_x, scan_extent(rows, length, dim, x_row, x_step) * b},
+                   {d_gates, scan_extent(rows, length, dim, a.g_row, a.g_step) * b},
+                   {d_dh, cells},
+                   {d_dlast, states * 4},
+                   {d_state, states * 4},
+                   {d_states, scan_state_floats(rows, length, dim, dtype) * 4},
+                   bounds_range(a)}))
+        return refuse(who, "a gradient overlaps another one, or what it is formed from");
     if (work_bytes < scan_work_bytes(rows, length, dim, dtype) + last_bytes(a.sequences, dim) || !d_work) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     a.states = const_cast<float*>(d_states);

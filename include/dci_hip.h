@@ -407,14 +407,14 @@ int dcih_distill_grad(const void* d_logits, int dtype, int64_t num_rows, int voc
  *   gates:                a_t = 1 / (1 + exp(-gates_t)),  h_t = a_t h_(t-1) + (1 - a_t) x_t
  *   DCIH_SCAN_DECAYS:     a_t = gates_t,                  h_t = a_t h_(t-1) + x_t
  * Token t of row b of x is at d_x + b * x_row + t * x_step (elements), its channels next to one another; the same for
- * the gates, or with DCIH_SCAN_SHARED one [dim] for all tokens.  d_h is [rows][length][dim] and may overlap neither.
+ * the gates, or with DCIH_SCAN_SHARED one [dim] for all tokens.  d_h is [rows][length][dim].
  * packed_sequences = 0: a row is a sequence; d_bounds is NULL or [rows] lengths (ids of id_bytes): tokens from there
  * on are not looked at, their h is 0.  packed_sequences = n > 0: rows is 1 and d_bounds are [n + 1] ascending offsets, sequence i
  * is tokens offsets[i] to offsets[i + 1] - 1; tokens of no sequence have h = 0.  Lengths and offsets are cut to [0, length].
  * d_state: NULL (zeros) or [sequences][dim] states before the first tokens; d_last: NULL or where the states behind the
  * last tokens go, also d_state itself (a sequence without tokens keeps its own).  A state that is not finite
  * leaves none finite behind it in its sequence.  d_states: NULL, or
- * dcih_scan_states floats that dcih_scan_grad takes.
+ * dcih_scan_states floats that dcih_scan_grad takes.  What is written overlaps nothing else of the call (but d_last = d_state): that is refused.
  */
 enum { DCIH_SCAN_DECAYS = 1, DCIH_SCAN_SHARED = 2 };
 int64_t dcih_scan_states(int64_t rows, int64_t length, int dim, int dtype);
@@ -427,7 +427,7 @@ int dcih_scan(const void* d_x, int dtype, int64_t rows, int64_t length, int dim,
 /*
  * The gradient of sum(d_dh * h) + sum(d_dlast * last), either of them NULL for zeros: by x and by the gates, contiguous and in their
  * type ([dim] for shared gates), and by the first states, [sequences][dim]; each NULL where it is not asked for.  The other arguments are those
- * of the call of dcih_scan that filled d_states.  Sums are in 32 bits (64 over the tiles of a shared gate), in one order.
+ * of the call of dcih_scan that filled d_states.  What is written overlaps nothing else of the call, d_dlast included.  Sums are in 32 bits (64 over the tiles of a shared gate), in one order.
  */
 int dcih_scan_grad(const void* d_x, int dtype, int64_t rows, int64_t length, int dim, int64_t x_row, int64_t x_step, const void* d_gates,
                    int64_t g_row, int64_t g_step, int flags, const float* d_state, const void* d_bounds, int id_bytes,
