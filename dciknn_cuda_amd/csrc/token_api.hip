@@ -495,6 +495,16 @@ int dcih_verify(const void* d_logits, int dtype, int64_t num_sequences, int draf
         if (const char* why = check_teacher(d_teacher, teacher_dtype, slots, d_slot_ids, slot_id_bytes)) return refuse(who, why);
     if (!d_uniforms || !d_tokens || !d_accepted || !d_logprobs) return refuse(who, "null array");
     if (!all_aligned({d_uniforms, d_tokens, d_accepted, d_logprobs})) return refuse(who, "arrays not aligned to their elements");
+    // (a sequence's random numbers are read before its log probabilities are written, by the same workgroup)
+    const int64_t rows = num_sequences * (drafts + 1), slot_count = drafts && d_slot_ids ? num_sequences * drafts * slots : 0;
+    if (any_meets({{d_tokens, rows * 4}, {d_accepted, num_sequences * 4}, {d_logprobs, rows * 4}},
+                  {{d_logits, ((rows - 1) * row_stride + vocab) * type_bytes(dtype)},
+                   {d_drafts, num_sequences * drafts * id_bytes},
+                   {d_uniforms, (const void*)d_uniforms == d_logprobs ? 0 : rows * 4},
+                   {d_slot_ids, slot_count * slot_id_bytes},
+                   {d_teacher, slot_count * type_bytes(teacher_dtype)}}) ||
+        any_meets({{d_tokens, rows * 4}, {d_accepted, num_sequences * 4}}, {{d_uniforms, rows * 4}}))
+        return refuse(who, "something that is written overlaps something else");
     if (!d_work || work_bytes < verify_work_bytes(num_sequences * (drafts + 1), vocab, dtype)) return refuse(who, "workspace too small");
     if (!aligned(d_work, 16)) return refuse(who, "workspace not aligned to 16 bytes");
     VerifyArgs a{};

@@ -466,6 +466,7 @@ int dcih_clip(const dcih_span* spans, int64_t num_spans, double max_norm, double
  * -inf, or whose slots hold NaN or +inf, gives no token, nor does a u_drafts that is NaN: -1 with a log probability of NaN.  (With another u_i
  * that is NaN draft i does not stand.)  What decides is formed in 64 bits, from logits, numbers and a temperature as they are given: a border is off by up to 1e-13 of the row's
  * weights, or 1e-14 where less than a thousandth of them is left to be drawn from; of an entry of which q_i leaves as little as that of itself nothing is left.
+ * What is written overlaps nothing else of the call (but d_logprobs = d_uniforms): that is refused.
  */
 #define DCIH_MAX_DRAFTS 256
 int64_t dcih_verify_work(int64_t num_sequences, int drafts, int vocab, int dtype);

@@ -44,3 +44,19 @@ GRAD = [dict(ds=L + (1 << 22)), dict(ds=S), dict(ds=S + STATES - 4), dict(ds=B +
 def test_scan_grad(lib, bad):
     assert scan_grad(lib, **bad) == -1
     assert b"overlap" in lib.dcih_last_error()
+
+
+def verify(lib, tokens=H, accepted=K, logprobs=L, drafts=X, uniforms=G, ids=S, teacher=B):
+    return lib.dcih_verify(W, BF16, 4, 3, 9000, 9000, drafts, 8, uniforms, ids, 4, teacher, BF16, 5, 1.0, tokens, accepted, logprobs, 9 << 24, 1 << 30, None)
+
+
+ROW = 4 * 4 * 4           # bytes of what has a number for each row of logits
+
+
+@pytest.mark.parametrize("bad", [
+    dict(tokens=X), dict(tokens=X + 4 * 3 * 8 - 4), dict(tokens=G), dict(tokens=S + 4 * 3 * 5 * 4 - 4), dict(tokens=B), dict(tokens=B + 4 * 3 * 5 * 2 - 4), dict(tokens=L), dict(tokens=K + 12),
+    dict(tokens=W + 16 * 9000 * 2 - 4), dict(accepted=X), dict(accepted=G + ROW - 4), dict(accepted=L + 8), dict(accepted=S), dict(accepted=W), dict(logprobs=G + 4), dict(logprobs=X),
+    dict(logprobs=S + 16), dict(logprobs=B), dict(logprobs=W + 1000), dict(logprobs=H, tokens=H + ROW - 4), dict(logprobs=G, tokens=G), dict(logprobs=G, accepted=G)], ids=str)
+def test_verify(lib, bad):
+    assert verify(lib, **bad) == -1
+    assert b"overlap" in lib.dcih_last_error()
