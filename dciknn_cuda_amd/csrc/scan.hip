@@ -901,7 +901,8 @@ constexpr int link_width(int slots) { return slots < 16 ? slots : 16; }
 template <int kSlots>
 __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
     constexpr int U = 8, kWidth = link_width(kSlots), kParts = kSlots / kWidth;
-    __shared__ uint64_t s_maps[2][kLinkRound + U * kWidth];
+    struct alignas(8) Map { uint32_t a, b; };         // a's place is the state's once it is joined
+    __shared__ Map s_maps[2][kLinkRound + U * kWidth];
     const int64_t words = c.tiles * kWidth, own = (int64_t)(blockIdx.x / kParts) * c.tiles * kSlots + blockIdx.x % kParts * kWidth;
     const uint64_t* maps = c.maps + own;
     uint32_t* states = c.states + own;
@@ -915,7 +916,7 @@ __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
 #pragma unroll
         for (int i = 0; i < kLinkWords; i++) {
             const int at = i * kLinkers + threadIdx.x;
-            if (from + at < words) states[place(from + at)] = word_of(__builtin_bit_cast(float, (uint32_t)s_maps[half][at]));
+            if (from + at < words) states[place(from + at)] = word_of(__builtin_bit_cast(float, s_maps[half][at].a));
         }
     };
     load(0);
@@ -924,19 +925,23 @@ __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
     for (int64_t from = 0; from < words; from += kLinkRound, half ^= 1) {
         // (each thread's own places, whose states it has taken away before)
 #pragma unroll
-        for (int i = 0; i < kLinkWords; i++) s_maps[half][i * kLinkers + threadIdx.x] = m[i];
+        for (int i = 0; i < kLinkWords; i++) s_maps[half][i * kLinkers + threadIdx.x] = Map{(uint32_t)m[i], (uint32_t)(m[i] >> 32)};
         __syncthreads();
         if (from) leave(from - kLinkRound, half ^ 1);
         if (from + kLinkRound < words) load(from + kLinkRound);
         if (threadIdx.x >= kWidth) continue;
         // (behind the last tile maps of no use are joined, whose states go nowhere)
         const int tiles = (int)(min((int64_t)kLinkRound, words - from) / kWidth);
-        uint64_t *at = s_maps[half] + threadIdx.x, next[U];
+        Map *at = s_maps[half] + threadIdx.x, next[U];
+        // (in this order: in another the loop's first wait is for all that is under way, and those of a round are for each other)
 #pragma unroll
-        for (int u = 0; u < U; u++) next[u] = at[u * kWidth];
+        for (int u = 0; u < U; u++) {
+            next[u] = at[u * kWidth];
+            if (u % 2) __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll 2
         for (int i = 0; i < tiles; i += U, at += U * kWidth) {
-            uint64_t map[U];
+            Map map[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 map[u] = next[u];
@@ -944,9 +949,9 @@ __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const float b = __builtin_bit_cast(float, (uint32_t)(map[u] >> 32));
-                h = (uint32_t)map[u] == kUnset ? b : __builtin_fmaf(__builtin_bit_cast(float, (uint32_t)map[u]), h, b);
-                *(float*)(at + u * kWidth) = h;
+                const float b = __builtin_bit_cast(float, map[u].b);
+                h = map[u].a == kUnset ? b : __builtin_fmaf(__builtin_bit_cast(float, map[u].a), h, b);
+                at[u * kWidth].a = __builtin_bit_cast(uint32_t, h);
             }
         }
     }
