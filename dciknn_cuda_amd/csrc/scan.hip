@@ -46,6 +46,11 @@ constexpr int kApart = 32;                         // words from one chain's cou
 constexpr int64_t kMaxGrid = 1 << 23;
 constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is filled with; no value that is published has these bits
 constexpr uint32_t kMapSet = 1, kStateSet = 2;
+// Decays beyond 1: where those of a tile could make something 2^100 times as large the product of all of them says too little in 32 bits (it may overflow
+// in front of a state of 0, which stays 0), and the tile's tokens are gone through one after the other by a thread a channel, 24 us a tile of a chain
+// (20000 x 64 f32 of nothing but such 3.8 ms, else 26 us; in a chain that is joined at once 55).  Below that a product may lose 2^-149 of what the state was, 2^-49 where that grows as much again.  In units of 2^(1 / kFine).
+constexpr int kFine = 256, kSteep = 100 * kFine;
+constexpr uint32_t kSteepMap = 0xfffffffeu;        // (in a map's A) no map: the tile's tokens say what is behind it
 
 typedef uint32_t u32x4_float __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -311,7 +316,7 @@ __device__ inline int64_t uniform(int64_t v) {
 }
 __device__ inline uint32_t word_of(float v) {
     const uint32_t w = __builtin_bit_cast(uint32_t, v);
-    return w == kUnset ? 0x7fc00000u : w;
+    return w >= kSteepMap ? 0x7fc00000u : w;           // (NaN for NaN)
 }
 
 // Item i of all is the next tile of a chain, in the direction of the scan, and each chain has as many items as tiles.  Neighbouring
@@ -376,12 +381,47 @@ __device__ float carry_of(const Chains& c, int64_t chain, int64_t at, int slot) 
     return h;
 }
 
+// How much a thread's decays may make of something, at most in any of its channels, is counted.  Whole numbers: the order does not matter.
+template <int R, int L> __device__ __forceinline__ void count_growth(const float (&as)[R][L], int times, int& s_growth, uint32_t& s_steep) {
+    float most = 0.f;
+#pragma unroll
+    for (int u = 0; u < R; u++)
+#pragma unroll
+        for (int k = 0; k < L; k++) most = fmaxf(most, __builtin_fabsf(as[u][k]));
+    if (!(most > 1.f)) return;
+    most = 1.f;
+#pragma unroll
+    for (int k = 0; k < L; k++) {
+        float grows = 1.f;
+#pragma unroll
+        for (int u = 0; u < R; u++) grows *= fmaxf(__builtin_fabsf(as[u][k]), 1.f);
+        most = fmaxf(most, grows);
+    }
+    const int by = (int)fminf(log2_fast(most) * kFine + 1.f, 1e6f) * times;
+    if (atomicAdd(&s_growth, by) + by > kSteep) s_steep = 1;
+}
+
 // A channel's groups joined, by one thread: map (A, B) of each in the direction of the scan, `resets` those whose result does not
-// depend on what enters.  Leaves in B what enters each group.
-template <int kGroups, bool kBack>
-__device__ void join_groups(const Chains& c, Phase phase, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b) {
+// depend on what enters.  Leaves in B what enters each group.  Where a tile is steep, `go` goes through the tokens of a group without such.
+template <int kGroups, bool kBack, class Go>
+__device__ void join_groups(const Chains& c, Phase phase, int64_t chain, int64_t at, int slot, uint32_t resets, const float* s_a, float* s_b, bool steep, Go go) {
     auto place = [&](int g) { return (kBack ? kGroups - 1 - g : g) * c.slots + slot; };
     float in = 0.f;
+    if (steep) {
+        const int64_t cell = chain * c.tiles + at, word = cell * c.slots + slot;
+        const bool follows = at + 1 < c.tiles && phase == kChained;
+        if (at && phase != kMaps) in = phase == kApply ? __builtin_bit_cast(float, c.states[word - c.slots]) : carry_of(c, chain, at, slot);
+        for (int i = 0; i < kGroups; i++) {
+            const int g = kBack ? kGroups - 1 - i : i;
+            const float gb = s_b[place(i)];
+            s_b[place(i)] = in;
+            in = resets >> g & 1 ? gb : go(g, slot, in);
+        }
+        if (phase == kMaps) c.maps[word] = (uint64_t)word_of(in) << 32 | (resets ? kUnset : kSteepMap);
+        if (follows) post(c.states + word, word_of(in));
+        if (follows && slot == 0) post(c.flags + cell, kStateSet);
+        return;
+    }
     if (c.tiles > 1) {
         float A = 1.f, B = 0.f;
 #pragma unroll 8
@@ -566,6 +606,33 @@ struct Bits {
     __device__ bool stops_any(int per) const { return (end | ~in) & ((1u << per) - 1); }
 };
 
+// A kernel's first argument, read again for what is hardly ever done: kept for that, its fields would take the scalar registers that the tiles need
+// (by which the gradient had 31 of them in vector registers).
+__device__ inline const ScanArgs& args_again() {
+    const ScanArgs* a = (const ScanArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return *a;
+}
+// The channel of a slot of a strip.
+template <int L> __device__ inline int channel_of(const ScanArgs& a, int strip, int slot) {
+    return min(min(strip * kLanes + slot / L, (a.dim - 1) / L) * L, a.dim - L) + slot % L;
+}
+// Tokens [t, t + n) of a row's channel one after the other, all of them in the middle of a sequence, by decays; or back through them.
+template <class T, int kUnroll> __device__ inline float go_forward(const ScanArgs& a, int64_t row, int channel, int64_t t, int n, float h) {
+    using raw_t = typename T::raw;
+    const raw_t *x = (const raw_t*)a.x + row * a.x_row + channel, *g = (const raw_t*)a.gates + (a.shared ? 0 : row * a.g_row) + channel;
+#pragma unroll kUnroll
+    for (int64_t i = t; i < t + n; i++) h = __builtin_fmaf((float)g[a.shared ? 0 : i * a.g_step], h, (float)x[i * a.x_step]);
+    return h;
+}
+template <class T, int kUnroll> __device__ inline float go_back(const ScanArgs& a, int64_t row, int channel, int64_t t, int n, float l) {
+    using raw_t = typename T::raw;
+    const raw_t *dh = (const raw_t*)a.dh + row * a.length * a.dim + channel, *g = (const raw_t*)a.gates + (a.shared ? 0 : row * a.g_row) + channel;
+#pragma unroll kUnroll
+    for (int64_t i = t + n - 1; i >= t; i--) l = (float)g[a.shared ? 0 : i * a.g_step] * ((a.dh ? (float)dh[i * a.dim] : 0.f) + l);
+    return l;
+}
+
 // Runs `body` as the wavefront has marks or not: without them there is no branch about a token.
 template <class Body> __device__ __forceinline__ void by_marks(bool any, Body body) {
     if (any) body(std::true_type{});
@@ -583,12 +650,14 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
     const Phase phase = kPhased ? c.phase : kChained;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
-    __shared__ uint32_t s_marked, s_resets;
+    __shared__ uint32_t s_marked, s_resets, s_steep;
+    __shared__ int s_growth[kLanes];
     __shared__ int64_t s_item;
     if (first + blockIdx.x >= c.count * c.tiles) return pass_empty(a, first + blockIdx.x - c.count * c.tiles, empty, a.state, a.last);
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    if (kDecay && threadIdx.x < kLanes) s_growth[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
-        s_resets = 0;
+        s_resets = s_steep = 0;
         s_item = take_tile(c, phase, first + blockIdx.x);
     }
     __syncthreads();
@@ -660,12 +729,16 @@ __global__ __launch_bounds__(kThreads, kWaves) void scan_kernel(ScanArgs a, Chai
         }
     });
     if (lane == 0 && bits.starts_any(U)) atomicOr(&s_resets, 1u << group);
+    if (kDecay) count_growth(as, kShared ? U : 1, s_growth[lane], s_steep);
     const int slot = lane * L, mine = group * kSlots + slot;
 #pragma unroll
     for (int k = 0; k < L; k++) { s_a[mine + k] = A[k]; s_b[mine + k] = B[k]; }
     __syncthreads();
     if (threadIdx.x < kSlots) {
-        join_groups<kGroups, false>(c, phase, chain, at, threadIdx.x, s_resets, s_a, s_b);
+        join_groups<kGroups, false>(c, phase, chain, at, threadIdx.x, s_resets, s_a, s_b, kDecay && s_steep, [&](int g, int own, float h) {
+            const ScanArgs& args = args_again();
+            return go_forward<T, 1>(args, row, channel_of<L>(args, (int)(chain - row * c.strips), own), t0 + g * U, U, h);
+        });
         if (a.states && phase != kMaps) a.states[item * kSlots + threadIdx.x] = s_b[threadIdx.x];
     }
     if (phase == kMaps) return;
@@ -700,12 +773,14 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     const Phase phase = kPhased ? c.phase : kChained;
     __shared__ float s_a[kGroups * kSlots], s_b[kGroups * kSlots], s_q[kGroups * kSlots];
     __shared__ int s_first[kTile], s_end[kTile];
-    __shared__ uint32_t s_marked, s_resets, s_back_resets;
+    __shared__ uint32_t s_marked, s_resets, s_back_resets, s_steep;
+    __shared__ int s_growth[kLanes];
     __shared__ int64_t s_item;
     if (first + blockIdx.x >= c.count * c.tiles) return pass_empty(a, first + blockIdx.x - c.count * c.tiles, empty, a.dlast, a.dstate);
     const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+    if (kDecay && threadIdx.x < kLanes) s_growth[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
-        s_resets = s_back_resets = 0;
+        s_resets = s_back_resets = s_steep = 0;
         s_item = take_tile(c, phase, first + blockIdx.x);
     }
     __syncthreads();
@@ -791,6 +866,7 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
 #pragma unroll
         for (int k = 0; k < L; k++) cs[u][k] = packed_of<T, kDecay>(cs[u][k]);
     }
+    if (kDecay) count_growth(cs, kShared ? U : 1, s_growth[lane], s_steep);
     again();
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -823,16 +899,28 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
     // the states by some wavefronts, the gradients by others
     if (phase == kMaps && threadIdx.x >= kSlots) return;
     if (threadIdx.x < kSlots) {
-        join_groups<kGroups, true>(c, phase, chain, at, threadIdx.x, s_back_resets, s_a, s_q);
+        join_groups<kGroups, true>(c, phase, chain, at, threadIdx.x, s_back_resets, s_a, s_q, kDecay && s_steep, [&](int g, int own, float l) {
+            const ScanArgs& args = args_again();
+            return go_back<T, 1>(args, row, channel_of<L>(args, strip, own), t0 + g * U, U, l);
+        });
         if (phase == kMaps) return;
     } else if (threadIdx.x < 2 * kSlots) {
         const int own = threadIdx.x - kSlots;
         float h = tile ? a.states[(chain * c.tiles + tile) * kSlots + own] : 0.f;      // (a row begins with a sequence, or with tokens of none)
+        if (kDecay && s_steep) {
+            const ScanArgs& args = args_again();
+            for (int i = 0; i < kGroups; i++) {
+                const float gb = s_b[i * kSlots + own];
+                s_b[i * kSlots + own] = h;
+                h = s_resets >> i & 1 ? gb : go_forward<T, 1>(args, row, channel_of<L>(args, strip, own), t0 + i * U, U, h);
+            }
+        } else {
 #pragma unroll 8
-        for (int i = 0; i < kGroups; i++) {
-            const float ga = s_a[i * kSlots + own], gb = s_b[i * kSlots + own];
-            s_b[i * kSlots + own] = h;
-            h = s_resets >> i & 1 ? gb : __builtin_fmaf(ga, h, gb);
+            for (int i = 0; i < kGroups; i++) {
+                const float ga = s_a[i * kSlots + own], gb = s_b[i * kSlots + own];
+                s_b[i * kSlots + own] = h;
+                h = s_resets >> i & 1 ? gb : __builtin_fmaf(ga, h, gb);
+            }
         }
     }
     __syncthreads();
@@ -898,11 +986,12 @@ __global__ __launch_bounds__(kThreads, kBackWaves) void scan_grad_kernel(ScanArg
 // workgroup has 16 channels (2048 tiles of 64 channels 43 us; with all of them 51, of which one CU reads and writes 30).
 constexpr int kLinkers = 1024, kLinkWords = 8, kLinkRound = kLinkers * kLinkWords;
 constexpr int link_width(int slots) { return slots < 16 ? slots : 16; }
-template <int kSlots>
-__global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
+template <class T, int kSlots, bool kDecay>
+__global__ __launch_bounds__(kLinkers) void link_kernel(Chains c, ScanArgs a, bool gradient, int tokens) {
     constexpr int U = 8, kWidth = link_width(kSlots), kParts = kSlots / kWidth;
     struct alignas(8) Map { uint32_t a, b; };         // a's place is the state's once it is joined
     __shared__ Map s_maps[2][kLinkRound + U * kWidth];
+    __shared__ uint32_t s_steep;
     const int64_t words = c.tiles * kWidth, own = (int64_t)(blockIdx.x / kParts) * c.tiles * kSlots + blockIdx.x % kParts * kWidth;
     const uint64_t* maps = c.maps + own;
     uint32_t* states = c.states + own;
@@ -919,13 +1008,28 @@ __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
             if (from + at < words) states[place(from + at)] = word_of(__builtin_bit_cast(float, s_maps[half][at].a));
         }
     };
+    // What is behind a tile without a map, whose tokens are all of one sequence.
+    auto go_through = [&](int64_t at, float h) {
+        const int64_t chain = blockIdx.x / kParts, row = chain / c.strips;
+        const int channel = channel_of<kSlots / kLanes>(a, (int)(chain - row * c.strips), blockIdx.x % kParts * kWidth + threadIdx.x);
+        return gradient ? go_back<T, 4>(a, row, channel, (c.tiles - 1 - at) * tokens, tokens, h) : go_forward<T, 4>(a, row, channel, at * tokens, tokens, h);
+    };
     load(0);
+    if (kDecay) {
+        if (threadIdx.x == 0) s_steep = 0;
+        __syncthreads();
+    }
     float h = 0.f;
     int half = 0;
     for (int64_t from = 0; from < words; from += kLinkRound, half ^= 1) {
         // (each thread's own places, whose states it has taken away before)
+        bool steep = false;
 #pragma unroll
-        for (int i = 0; i < kLinkWords; i++) s_maps[half][i * kLinkers + threadIdx.x] = Map{(uint32_t)m[i], (uint32_t)(m[i] >> 32)};
+        for (int i = 0; i < kLinkWords; i++) {
+            s_maps[half][i * kLinkers + threadIdx.x] = Map{(uint32_t)m[i], (uint32_t)(m[i] >> 32)};
+            steep |= kDecay && (uint32_t)m[i] == kSteepMap;
+        }
+        if (steep) s_steep = 1;
         __syncthreads();
         if (from) leave(from - kLinkRound, half ^ 1);
         if (from + kLinkRound < words) load(from + kLinkRound);
@@ -933,6 +1037,15 @@ __global__ __launch_bounds__(kLinkers) void link_kernel(Chains c) {
         // (behind the last tile maps of no use are joined, whose states go nowhere)
         const int tiles = (int)(min((int64_t)kLinkRound, words - from) / kWidth);
         Map *at = s_maps[half] + threadIdx.x, next[U];
+        if (kDecay && __builtin_expect(s_steep != 0, 0)) {
+            for (int i = 0; i < tiles; i++, at += kWidth) {
+                const float b = __builtin_bit_cast(float, at->b);
+                if (at->a == kSteepMap) h = go_through(from / kWidth + i, h);
+                else h = at->a == kUnset ? b : __builtin_fmaf(__builtin_bit_cast(float, at->a), h, b);
+                at->a = __builtin_bit_cast(uint32_t, h);
+            }
+            continue;
+        }
         // (in this order: in another the loop's first wait is for all that is under way, and those of a round are for each other)
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -1022,7 +1135,7 @@ int run(const ScanArgs& a, int dtype, bool gradient, hipStream_t s) {
     const int64_t empty = a.bounds && (gradient ? a.dstate : a.last) ? std::min((a.sequences + kEmpty - 1) / kEmpty, kEmptyGrid) : 0;
     if (c.phase == kMaps) {
         if (int rc = launch(std::true_type{}, 0)) return rc;
-        link_kernel<kLanes * L><<<(uint32_t)(c.count * (kLanes * L / link_width(kLanes * L))), kLinkers, 0, s>>>(c);
+        link_kernel<T, kLanes * L, kDecay><<<(uint32_t)(c.count * (kLanes * L / link_width(kLanes * L))), kLinkers, 0, s>>>(c, a, gradient, tile_of(L, kShared));
         DCIH_HIP(hipGetLastError());
         c.phase = kApply;
         if (int rc = launch(std::true_type{}, empty)) return rc;

@@ -76,7 +76,7 @@ def gated_scan(x, gates, state=None, *, decay=False, lengths=None, offsets=None,
     x's shape, or [dim] for all tokens; state [sequences, dim] float32 is what stands before the first tokens, zeros if not given.  h is of x's
     shape and type, last [sequences, dim] float32 the state behind the last tokens.  The channels of a token are next to one another, tokens and
     rows at any distances.  A server's step is a length of 1, with `last=state` in place.  States are in 32 bits; one that is not finite
-    leaves none finite behind it in its sequence.  Differentiable by x, gates and state, not with `last`."""
+    leaves none finite behind it in its sequence.  Decays may be of any size; stretches of a hundred tokens that may grow 2**100 times are slow.  Differentiable by x, gates and state, not with `last`."""
     return _ext._gated_scan(x, gates, state, decay, lengths, offsets, last)
 
 

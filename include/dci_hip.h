@@ -413,7 +413,8 @@ int dcih_distill_grad(const void* d_logits, int dtype, int64_t num_rows, int voc
  * is tokens offsets[i] to offsets[i + 1] - 1; tokens of no sequence have h = 0.  Lengths and offsets are cut to [0, length].
  * d_state: NULL (zeros) or [sequences][dim] states before the first tokens; d_last: NULL or where the states behind the
  * last tokens go, also d_state itself (a sequence without tokens keeps its own).  A state that is not finite
- * leaves none finite behind it in its sequence.  d_states: NULL, or
+ * leaves none finite behind it in its sequence.  Decays may be of any size: the result is that of the tokens one after the other also where the decays'
+ * product is beyond 32 bits (slowly: where 128 tokens, or 256, may grow 2^100 times).  d_states: NULL, or
  * dcih_scan_states floats that dcih_scan_grad takes.  What is written overlaps nothing else of the call (but d_last = d_state): that is refused.
  */
 enum { DCIH_SCAN_DECAYS = 1, DCIH_SCAN_SHARED = 2 };
