@@ -9,8 +9,9 @@
 //
 // Both directions are compositions of maps s -> A s + B, which are associative: a tile of 128 or 256 tokens by kLanes pieces
 // of 16 bytes is one workgroup's, in registers; each group of lanes composes its few tokens, the groups are joined in
-// shared memory, and a tile's map is joined to that of the tiles before it while these still run (see carry_of).  So every
-// element is read and written once.  The gradient forms h_(t-1) again, from x, g and the state before each tile, which
+// shared memory, and a tile's map is joined to that of the tiles before it while these still run (see carry_of; a scan in a single pass, with a
+// look back).  So every element is read and written once, but for few long chains, whose tokens are read a second time when their maps are joined
+// (see link_kernel; in the gradient dh and the gates).  The gradient forms h_(t-1) again, from x, g and the state before each tile, which
 // the forward call keeps in 32 bits: less to read than h itself, and not rounded.
 #include "../../include/dci_hip.h"
 #include "scan.h"
@@ -48,7 +49,8 @@ constexpr uint32_t kUnset = 0xffffffffu;           // what the workspace is fill
 constexpr uint32_t kMapSet = 1, kStateSet = 2;
 // Decays beyond 1: where those of a tile could make something 2^100 times as large the product of all of them says too little in 32 bits (it may overflow
 // in front of a state of 0, which stays 0), and the tile's tokens are gone through one after the other by a thread a channel, 24 us a tile of a chain
-// (20000 x 64 f32 of nothing but such 3.8 ms, else 26 us; in a chain that is joined at once 55).  Below that a product may lose 2^-149 of what the state was, 2^-49 where that grows as much again.  In units of 2^(1 / kFine).
+// (20000 x 64 f32 of nothing but such 3.8 ms, else 26 us; in a chain that is joined at once 55).  Below that a product may lose 2^-149 of
+// what the state was, 2^-49 where that grows as much again.  In units of 2^(1 / kFine).
 constexpr int kFine = 256, kSteep = 100 * kFine;
 constexpr uint32_t kSteepMap = 0xfffffffeu;        // (in a map's A) no map: the tile's tokens say what is behind it
 
@@ -639,7 +641,7 @@ template <class Body> __device__ __forceinline__ void by_marks(bool any, Body bo
     else body(std::false_type{});
 }
 
-// A tile, read and written once: bound by memory (65536 x 4096 bf16 355 us, 1.61 GB at 4.5 TB/s; 8 x 4096 x 2048 88 us) where chains are many or long,
+// A tile, read and written once (twice read in the chains of link_kernel): bound by memory (65536 x 4096 bf16 355 us, 1.61 GB at 4.5 TB/s; 8 x 4096 x 2048 88 us) where chains are many or long,
 // by the wait for the tile before where one short row is all there is (20000 x 64 f32, 79 tiles: 18 us).  Without that wait the
 // second took 92 us of 113 at the time, without the gates' arithmetic 106.
 template <class T, int L, bool kDecay, bool kShared, bool kPhased>
