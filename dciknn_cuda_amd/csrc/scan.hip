@@ -31,16 +31,17 @@ constexpr int tile_of(int len, bool shared) { return len == 8 || (len == 4 && !s
 // with gradients 262 us instead of 238; one less is as fast).
 constexpr int kWaves = 4, kBackWaves = 3;
 // Tokens that one thread takes in any case.  Of longer rows it takes all where pieces are many, kManyPieces for each token up to kEnoughPieces: 512 x 40 x
-// 2048 bf16 42 us, 58 by tiles; 512 x 48 x 1024 28 and 43, 128 x 48 x 1024 23 and 13; 256 x 130 x 2048 87 and 158, 256 x 300 x 2048 202 and 247, 64 x 300 x
-// 2048 69 and 61.  But not where a tile is full to 7/8 or more and has no other to wait for (f32 256 x 116 x 1024 78 and 62).
+// 2048 bf16 42 us, 53 by tiles; 512 x 48 x 1024 29 and 40, 128 x 48 x 1024 24 and 12; 256 x 130 x 2048 85 and 154, 256 x 300 x 2048 206 and 241, 64 x 300 x
+// 2048 132 and 58.  But not where a tile is full to 7/8 or more and has no other to wait for: there either is within a tenth of the other (bf16 512 x 128 x
+// 1024 80 and 72, 512 x 128 x 2048 159 and 167, f32 256 x 116 x 1024 59 and 58).
 constexpr int kShort = 32;
 constexpr int64_t kManyPieces = 1280, kEnoughPieces = 1 << 16;
-// Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 4.5 us,
-// 8.7 by pieces; 32 x 32 x 1024 7.1, 15.3, 8.5 by tiles; but 512 x 8 x 1024 8.3 and 6.6).  Twice as many where sequences are longer than kSteps.
+// Up to so many channels each has a thread, not a piece of them: a wavefront's arithmetic for 8 channels takes 0.4 us a token (32 x 16 x 1024 bf16 4.7 us,
+// 9.2 by pieces; 32 x 32 x 1024 7.4 and 16.3; but 512 x 8 x 1024 8.7 and 6.5).  Twice as many where sequences are longer than kSteps.
 constexpr int64_t kSingles = 1 << 17;
 constexpr int kSteps = 16;
 // Up to so many chains of so many tiles or more each are joined by a launch of their own (see link_kernel): 1 x 262144 x 64 bf16 81 us, with gradients 178,
-// chained 201 and 402; x 256 171 and 429, 226 and 444; x 384 241 and 582, 247 and 531; 1 x 16384 x 64 18 and 21, with gradients 73 and 68, the host's two
+// chained 200 and 398; x 256 171 and 427, 221 and 453; x 384 237 and 582, 245 and 525; 1 x 16384 x 64 19 and 21, with gradients 69 and 63, the host's two
 // launches more.
 constexpr int kFewChains = 4, kManyTiles = 192;
 constexpr int kApart = 32;                         // words from one chain's counter to the next: a line takes an atomic operation in 11 ns
