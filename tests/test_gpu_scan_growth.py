@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import recurrent_oracles as O
-from test_gpu_scan import TYPES, near
+from test_gpu_scan import TYPES, VIEWS, near
 
 pytestmark = pytest.mark.gpu
 
@@ -157,6 +157,27 @@ def test_many_rows_as_few(gpu, rows):
     x, state, dh, dlast = scaled(rng, level, O.sequences_of(2, length))
     many = lambda v: np.concatenate([v] * (rows // 2))                               # noqa: E731
     check(gpu, many(x), many(a), many(state), many(dh), many(dlast), "bf16", only=slice(0, 2))
+
+
+@pytest.mark.parametrize("view", VIEWS)
+@pytest.mark.parametrize("size", [(3, 300, 18), (2, 26_000, 16)], ids=str)
+@pytest.mark.parametrize("shared", [False, True])
+def test_strides(gpu, size, shared, view):
+    """Where tokens stand changes no bit."""
+    rng = np.random.default_rng(14)
+    a, level = wandering(*size, 40.0, [3.0 if t % 5000 < 200 else 0.01 for t in range(size[1])], 15)
+    x, state, dh, dlast = (torch.from_numpy(v).float().cuda() for v in scaled(rng, level, O.sequences_of(size[0], size[1])))
+    a = torch.from_numpy(a).float().cuda()
+    if shared:
+        a = torch.full((size[2],), 1.8, device="cuda")
+        x[:, :-20], dh[:, 20:], state, dlast = 0.0, 0.0, None, torch.zeros_like(dlast)
+    results = []
+    for of in (lambda t: t, VIEWS[view]):
+        leaves = [of(x).detach().requires_grad_(), (a if shared else of(a)).detach().requires_grad_()] + ([] if shared else [state.detach().requires_grad_()])
+        out = gpu.gated_scan(leaves[0], leaves[1], None if shared else leaves[2], decay=True)
+        results.append(list(out) + list(torch.autograd.grad(out, leaves, (of(dh), dlast))))
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+    assert all(bool(p.isfinite().all()) for p in results[0])
 
 
 def test_decays_that_are_not_finite(gpu):
