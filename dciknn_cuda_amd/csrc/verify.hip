@@ -212,7 +212,7 @@ __device__ inline float teacher_at(const VerifyArgs& a, int64_t i) {
 constexpr int kSlots = 1024, kNearChunks = 256;      // chunks whose amounts are added up beside the slots
 constexpr double kLog2eWide = 1.44269504088896340736, kLn2Wide = 0.693147180559945309417;
 
-// 11 us of 64 sequences with 7 drafts of 64 slots each, 7.4 of 4 with 4 drafts for certain: a chain of loads, exponentials and joined sums that wait
+// 11.3 us of 64 sequences with 7 drafts of 64 slots each, 7.6 of 4 with 4 drafts for certain: a chain of loads, exponentials and joined sums that wait
 // for one another.
 // One workgroup a sequence: a wavefront a row joins its sums and says whether the draft stands; then all of them draw the next token
 // from the row that it comes from, by chunks, then among the entries of one.
